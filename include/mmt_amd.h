@@ -598,6 +598,68 @@ int mmt_lane_gather(const double *table, const double *lanes, const int64_t *row
                     int n_lanes, int n_points, double scale, float *lane_input, float *lane_label, uint8_t *lane_mask,
                     void *stream);
 
+/* ---- attention over long rows (no counterpart in the reference: its rows are one agent's history or horizon) ------------------
+ * Beside mmt_attention_fwd / _bwd (rows of at most 32 keys, fp32, probabilities stored): rows of any length, bf16 / fp16 / fp32,
+ * nothing of the size Lq x Lk in memory.  For query i of batch row b, which stands at position p = n - Lq + i of a row of n keys
+ * (n = kv_len[b] clamped to 0..Lk, or Lk), and key j < n:
+ *   s = scale q_i . k_j;  u = softcap > 0 ? softcap tanh(s / softcap) : s;
+ *   u += -slopes[h] |p - j| + rel_bias[h][rel_buckets[clamp(j - p, -reach, reach) + reach]]
+ *   visible: equal ids in q_doc / k_doc, neither negative, and (not causal, or j <= p, or j < prefix[b])
+ *   out_i = sum_j softmax(u)_j v_j over the visible keys;  lse_i = log sum exp u.  A row that sees nothing: out 0, lse -inf,
+ *   gradients 0.  An entry of -inf in rel_bias hides its bucket like a mask.
+ * Heads: query head h reads key head h / (H / Hk).  q / k / v rows (head slices) are dh contiguous elements at any batch / token /
+ * head stride (elements) that keeps them at multiples of 16 bytes; a stride of 0 broadcasts.  out (B,Lq,H,dh) and lse (B,H,Lq; may
+ * be NULL) contiguous.  Keys at j >= n and keys and queries with a negative id are never multiplied with anything: they may hold
+ * NaN.  Bucket numbers are clamped to 0..n_buckets-1, lengths to 0..Lk.  Limits: dh a multiple of 8 up to 128, n_buckets <= 64,
+ * reach <= 4096, (H / Hk) n_buckets <= 8192.  Sums, statistics and the products' accumulators are fp32; the probabilities and the
+ * score gradients are rounded to the element type where they enter the second product.
+ * bwd: `out` and `lse` are the forward's, dout rows like q, dlse (B,H,Lq) may be NULL; dq (B,Lq,H,dh), dk, dv (B,Lk,Hk,dh)
+ * contiguous, drel_bias (H,n_buckets) fp32 (with rel_bias only); all written, every sum in a fixed order (the same bits every call).
+ * workspace: mmt_long_attention_workspace_bytes(a, backward) bytes, 16-byte aligned, no initialisation needed, not shared by calls
+ * that may overlap.  Both calls can be captured into a graph. */
+#define MMT_F32 0
+#define MMT_BF16 1
+#define MMT_F16 2
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_bs, q_rs, q_hs, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs;
+  int32_t dtype, B, Lq, Lk, H, Hk, dh, causal;
+  float scale, softcap;
+  const int32_t *prefix, *kv_len;        /* (B) or NULL */
+  const int32_t *q_doc, *k_doc;          /* (B,Lq), (B,Lk) or NULL */
+  const float *slopes;                   /* (H) or NULL */
+  const float *rel_bias;                 /* (H,n_buckets) or NULL */
+  const int32_t *rel_buckets;            /* (2*reach+1) or NULL */
+  int32_t n_buckets, reach;
+} mmt_long_attention;
+size_t mmt_long_attention_workspace_bytes(const mmt_long_attention *a, int backward);
+int mmt_long_attention_fwd(const mmt_long_attention *a, void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
+int mmt_long_attention_bwd(const mmt_long_attention *a, const void *out, const float *lse, const void *dout, int64_t do_bs, int64_t do_rs,
+                           int64_t do_hs, const float *dlse, void *dq, void *dk, void *dv, float *drel_bias, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
+/* ---- norm of queries and keys per head with the rotation of their positions in the same pass (no counterpart in the reference, whose
+ * positions are a table added to the input: Transformer_model.py:112-129).  For each token and head, x of dh elements:
+ *   n = x w / sqrt(mean(x^2) + eps);  pair m = (a, b) of n turned by the angle position * inv_freq[m]:
+ *   y_a = n_a cos - n_b sin, y_b = n_b cos + n_a sin;  (a, b) = (m, m + rot/2), or (2m, 2m + 1) with interleaved; elements >= rot stay n
+ * Angles are formed and reduced in 64 bits (positions (B,L) int64, or NULL: 0..L-1), the rest in fp32, one rounding at the end.
+ * q (B,L,H,dh), k (B,L,Hk,dh): rows like the rows of mmt_long_attention; weights (dh) in the same type (w_dtype = dtype) or fp32
+ * (w_dtype = MMT_F32); outputs contiguous.  bwd: gradients of the outputs dqo / dko (rows at any such strides) -> dq, dk contiguous,
+ * dq_weight, dk_weight (dh) in w_dtype; every sum in a fixed order.  Limits: dh a multiple of 8 up to 256, rot even, <= dh. */
+typedef struct {
+  const void *q, *k, *q_weight, *k_weight;
+  int64_t q_bs, q_rs, q_hs, k_bs, k_rs, k_hs;
+  const double *inv_freq;                /* (rot/2) */
+  const int64_t *positions;
+  int32_t dtype, w_dtype, B, L, H, Hk, dh, rot, interleaved;
+  float eps;
+} mmt_qk_norm_rope;
+int mmt_qk_norm_rope_fwd(const mmt_qk_norm_rope *a, void *q_out, void *k_out, void *stream);
+size_t mmt_qk_norm_rope_workspace_bytes(const mmt_qk_norm_rope *a);
+int mmt_qk_norm_rope_bwd(const mmt_qk_norm_rope *a, const void *dqo, int64_t dq_bs, int64_t dq_rs, int64_t dq_hs, const void *dko,
+                         int64_t dk_bs, int64_t dk_rs, int64_t dk_hs, void *dq, void *dk, void *dq_weight, void *dk_weight,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

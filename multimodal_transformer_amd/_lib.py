@@ -145,6 +145,27 @@ class AdamwTensor(C.Structure):
                 ("lr_scale", C.c_float), ("pad_", C.c_int32)]
 
 
+MMT_F32, MMT_BF16, MMT_F16 = 0, 1, 2
+
+
+class LongAttention(C.Structure):
+    """mmt_long_attention (include/mmt_amd.h)."""
+    _fields_ = [(n, fptr) for n in ("q", "k", "v")] + \
+               [(n, C.c_int64) for n in ("q_bs", "q_rs", "q_hs", "k_bs", "k_rs", "k_hs", "v_bs", "v_rs", "v_hs")] + \
+               [(n, C.c_int32) for n in ("dtype", "B", "Lq", "Lk", "H", "Hk", "dh", "causal")] + \
+               [("scale", C.c_float), ("softcap", C.c_float)] + \
+               [(n, fptr) for n in ("prefix", "kv_len", "q_doc", "k_doc", "slopes", "rel_bias", "rel_buckets")] + \
+               [("n_buckets", C.c_int32), ("reach", C.c_int32)]
+
+
+class QkNormRope(C.Structure):
+    """mmt_qk_norm_rope (include/mmt_amd.h)."""
+    _fields_ = [(n, fptr) for n in ("q", "k", "q_weight", "k_weight")] + \
+               [(n, C.c_int64) for n in ("q_bs", "q_rs", "q_hs", "k_bs", "k_rs", "k_hs")] + \
+               [("inv_freq", fptr), ("positions", fptr)] + \
+               [(n, C.c_int32) for n in ("dtype", "w_dtype", "B", "L", "H", "Hk", "dh", "rot", "interleaved")] + [("eps", C.c_float)]
+
+
 # symbol -> (restype, argtypes); tests check that the library exports exactly these
 SIGNATURES = {
     "mmt_last_error": (C.c_char_p, []),
@@ -230,6 +251,14 @@ SIGNATURES = {
     "mmt_gmm2d_mode": (C.c_int, [fptr, fptr, fptr, fptr, fptr, fptr, C.c_long, C.c_int, fptr, C.c_void_p]),
     "mmt_gmm2d_from_cov": (C.c_int, [fptr, C.c_long, fptr, fptr, C.c_void_p]),
     "mmt_map_crop": (C.c_int, [fptr, fptr, C.c_int, fptr, fptr, fptr, C.POINTER(C.c_int32), C.c_int, fptr, C.c_void_p]),
+    "mmt_long_attention_workspace_bytes": (C.c_size_t, [C.POINTER(LongAttention), C.c_int]),
+    "mmt_long_attention_fwd": (C.c_int, [C.POINTER(LongAttention), fptr, fptr, fptr, C.c_size_t, C.c_void_p]),
+    "mmt_long_attention_bwd": (C.c_int, [C.POINTER(LongAttention), fptr, fptr, fptr, C.c_int64, C.c_int64, C.c_int64, fptr, fptr, fptr,
+                                         fptr, fptr, fptr, C.c_size_t, C.c_void_p]),
+    "mmt_qk_norm_rope_fwd": (C.c_int, [C.POINTER(QkNormRope), fptr, fptr, C.c_void_p]),
+    "mmt_qk_norm_rope_workspace_bytes": (C.c_size_t, [C.POINTER(QkNormRope)]),
+    "mmt_qk_norm_rope_bwd": (C.c_int, [C.POINTER(QkNormRope), fptr, C.c_int64, C.c_int64, C.c_int64, fptr, C.c_int64, C.c_int64, C.c_int64,
+                                       fptr, fptr, fptr, fptr, fptr, C.c_size_t, C.c_void_p]),
     "mmt_finalize": (C.c_int, [fptr, fptr, fptr, C.c_int, C.c_int, C.c_int, fptr, fptr, fptr, fptr, C.c_void_p]),
 }
 

@@ -1,0 +1,285 @@
+// Device code shared by the long-sequence attention kernels (long_attention.hip): element types, LDS tiles, score transform.
+//
+// Mathematics.  For query i of a row of n keys (position p = n - Lq + i) and key j:
+//   s = scale q_i . k_j;   u = cap tanh(s / cap);   u += -slope_h |p - j| + table[h][bucket(j - p)]
+//   visible: j < n, equal documents, and (not causal, or j <= p, or j < prefix)   <=>   j < hi_i  and equal documents
+//   P = softmax of u over the visible keys (0 where there is none);   o = P v
+// Everything runs on v_mfma_f32_32x32x16 (16-bit types) or chains of v_mfma_f32_32x32x2 (fp32) with the SCORES TRANSPOSED: the
+// key is the row and the query the column of the 32 x 32 accumulator, so that a lane owns ONE query (lane % 32) and 16 of 32 keys:
+// row maximum and sum stay in the lane but for one exchange between the wave's halves, the rescaling factor is a lane's own scalar,
+// and the 16 probabilities of a lane are, eight at a time, exactly the B operand of the next product (o^T += v^T P^T) when its
+// reduction index runs over the keys in the accumulator's order.  P never leaves the registers.
+//   C layout of a 32 x 32 tile: column = lane % 32, register i -> row 8 (i / 4) + 4 (lane / 32) + i % 4
+//   A / B operands of a 16-deep step: row / column = lane % 32, element e of lane half h -> reduction index 8 h + e; any one-to-one
+//   relabelling of that index is allowed as long as A and B share it: the second product uses
+//   index (h, e) -> key 16 c + 4 h + e % 4 + 8 (e / 4), the order in which accumulator registers 8 c .. 8 c + 7 hold the keys.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/mmt_amd.h"
+
+namespace la {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS = 32 * WAVES;   // a workgroup: 4 waves of 32 rows each
+
+// ---- element types --------------------------------------------------------------------------------------------------------
+// BK: keys (queries, in the key-gradient kernel) per LDS tile; fp32 elements are twice as large, so half as many.
+// PSHIFT: probabilities are multiplied by 2^PSHIFT before they are rounded to the element type (and the sums with them): fp16 has
+// 5 exponent bits, so that without it every probability under 2^-14 would lose digits and every one under 2^-25 vanish.
+template <typename T> struct Elem;
+template <> struct Elem<__bf16> {
+  typedef bf16x8 V8;
+  typedef bf16x4 V4;
+  static constexpr int BK = 64;
+  static constexpr float PSHIFT = 0.f;
+  static __device__ __forceinline__ f32x16 mma(const V8 &a, const V8 &b, const f32x16 &c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Elem<_Float16> {
+  typedef f16x8 V8;
+  typedef f16x4 V4;
+  static constexpr int BK = 64;
+  static constexpr float PSHIFT = 14.f;
+  static __device__ __forceinline__ f32x16 mma(const V8 &a, const V8 &b, const f32x16 &c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Elem<float> {
+  typedef f32x8 V8;
+  typedef f32x4 V4;
+  static constexpr int BK = 32;
+  static constexpr float PSHIFT = 0.f;
+  // eight 2-deep steps; step e pairs element e of the two lane halves, which is what the 16-bit instruction sums too
+  static __device__ __forceinline__ f32x16 mma(const V8 &a, const V8 &b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <typename T> __device__ __forceinline__ typename Elem<T>::V8 round8(const float *x) {   // round to nearest even
+  typename Elem<T>::V8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = (T)x[e];
+  return r;
+}
+
+// ---- LDS tiles ------------------------------------------------------------------------------------------------------------
+// BK rows of D elements in 16-byte slots, NS slots per row (a power of two, so that a slot's place is an exclusive or).  A row
+// operand reads one slot of 32 different rows, a transposed read (ds_read_b64_tr_b16: four rows x 16 columns per 16 lanes) four
+// consecutive rows x four consecutive slots: the exclusive or spreads both over the 64 banks (16 slots).
+template <typename T, int D> struct Tile {
+  static constexpr int EPS = 16 / (int)sizeof(T);                 // elements per slot
+  static constexpr int DS = D <= 32 ? 32 : D <= 64 ? 64 : 128;
+  static constexpr int NS = DS / EPS;
+  static constexpr int BK = Elem<T>::BK;
+  static constexpr int BYTES = BK * NS * 16;
+  static constexpr int NLD = BK * NS / THREADS;                   // 16-byte loads per thread and tile
+  static __device__ __forceinline__ int swz(int row, int slot) {
+    if constexpr (sizeof(T) == 4) {
+      return slot ^ (NS >= 16 ? (row & 15) : ((row >> 1) & 7));
+    } else {
+      if constexpr (NS == 16) return slot ^ (((row & 3) << 2) | ((row >> 2) & 3));
+      else if constexpr (NS == 8) return slot ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
+      else return slot ^ ((row >> 2) & 3);
+    }
+  }
+};
+static_assert(Tile<__bf16, 32>::NLD == 1 && Tile<float, 32>::NLD == 1, "every tile is a whole number of 16-byte loads per thread");
+
+// row operand: elements 16 c + 8 h .. + 7 of row `row`
+template <typename T, int D> __device__ __forceinline__ typename Elem<T>::V8 row_frag(const char *t, int row, int c, int h) {
+  typedef Tile<T, D> L;
+  if constexpr (sizeof(T) == 2) {
+    return *(const typename Elem<T>::V8 *)(t + (row * L::NS + L::swz(row, 2 * c + h)) * 16);
+  } else {
+    const f32x4 a = *(const f32x4 *)(t + (row * L::NS + L::swz(row, 4 * c + 2 * h)) * 16);
+    const f32x4 b = *(const f32x4 *)(t + (row * L::NS + L::swz(row, 4 * c + 2 * h + 1)) * 16);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// transposed operand: column 32 dt + lane % 32 of rows r0 + 4 h + {0..3} and r0 + 8 + 4 h + {0..3}
+template <typename T, int D> __device__ __forceinline__ typename Elem<T>::V8 col_frag(const char *t, int r0, int dt, int lane) {
+  typedef Tile<T, D> L;
+  const int h = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    // lane i of a group of 16 hands in row i / 4, columns 4 (i % 4) .. + 3 and receives column i of the four rows
+    const int i = lane & 15, col = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+    s16x4 p[2];
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const int row = r0 + 8 * part + 4 * h + (i >> 2);
+      const char *a = t + (row * L::NS + L::swz(row, col >> 3)) * 16 + (col & 7) * 2;
+      p[part] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)a);
+    }
+    return __builtin_bit_cast(typename Elem<T>::V8, __builtin_shufflevector(p[0], p[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  } else {
+    const int col = 32 * dt + (lane & 31);
+    f32x8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int row = r0 + 8 * (e >> 2) + 4 * h + (e & 3);
+      r[e] = *(const float *)(t + (row * L::NS + L::swz(row, col >> 2)) * 16 + (col & 3) * 4);
+    }
+    return r;
+  }
+}
+
+// row operand straight from memory (the tile that stays in registers); elements at and beyond dh, and dead rows, are zero
+template <typename T> __device__ __forceinline__ typename Elem<T>::V8 mem_frag(const T *row, int c, int h, int dh, bool live) {
+  typedef typename Elem<T>::V8 V8;
+  V8 r = {};
+  const int d = 16 * c + 8 * h;
+  if (live && d < dh) r = *(const V8 *)(row + d);
+  return r;
+}
+
+// A tile on its way from memory to LDS through registers.  Rows that are not `live` become zeros whatever memory holds there (the
+// tail of a cache, padding): 0 x NaN would reach every other row of the tile.
+template <typename T, int D> struct Stage {
+  typedef Tile<T, D> L;
+  u32x4 r[L::NLD];
+  // rows r0 .. r0 + BK - 1 of a (rows, dh) matrix with `rs` elements between rows; rows >= n_rows are not read
+  __device__ __forceinline__ void load(const T *base, int64_t rs, int r0, int n_rows, int dh) {
+#pragma unroll
+    for (int n = 0; n < L::NLD; ++n) {
+      const int idx = threadIdx.x + n * THREADS, row = idx / L::NS, slot = L::swz(row, idx % L::NS);
+      u32x4 v = {};
+      if (r0 + row < n_rows && slot * L::EPS < dh) v = *(const u32x4 *)(base + (int64_t)(r0 + row) * rs + slot * L::EPS);
+      r[n] = v;
+    }
+  }
+  // rows at r0 + row >= end, or whose document id is negative, are written as zeros
+  __device__ __forceinline__ void store(char *lds, int r0, int end, const int *doc) {
+#pragma unroll
+    for (int n = 0; n < L::NLD; ++n) {
+      const int idx = threadIdx.x + n * THREADS, row = idx / L::NS;
+      u32x4 v = r[n];
+      const bool dead = r0 + row >= end || (doc && doc[r0 + row] < 0);
+      if (dead) v = u32x4{};
+      *(u32x4 *)(lds + idx * 16) = v;
+    }
+  }
+};
+
+// ---- lanes ----------------------------------------------------------------------------------------------------------------
+// the two halves of the wave hold complementary parts of a row: v[lane] op v[lane ^ 32]
+// (s_nop: the distance from a VALU write to the lane swap, which the compiler does not see inside asm)
+__device__ __forceinline__ float half_max(float v) {
+  float a = v, b = v;
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_sum(float v) {
+  float a = v, b = v;
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+  return a + b;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  return v;
+}
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v = min(v, __shfl_xor(v, m));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v = max(v, __shfl_xor(v, m));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
+// ---- score transform ------------------------------------------------------------------------------------------------------
+// tanh without cancellation.  |y| <= 3/8: odd series to y^11, remainder < 21844/6081075 y^13 = 3e-8 of y.  Beyond: 1 - 2 / (1 + e^2y),
+// whose absolute error of an ulp of 1 is then below 2e-7 of the value.
+__device__ __forceinline__ float tanh_series(float y) {
+  const float z = y * y;
+  float p = fmaf(z, -8.86323552990219657e-3f, 2.18694885361552028e-2f);
+  p = fmaf(z, p, -5.39682539682539683e-2f);
+  p = fmaf(z, p, 1.33333333333333333e-1f);
+  p = fmaf(z, p, -3.33333333333333333e-1f);
+  return fmaf(y * z, p, y);
+}
+__device__ __forceinline__ float tanh_any(float y) {
+  const float e = ex2(y * (2.f * LOG2E));
+  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e);
+  return fabsf(y) <= 0.375f ? tanh_series(y) : big;
+}
+// x -> tanh(x * f) for N scores of a lane; most tiles of a trained model stay inside the series' range: one wave-uniform branch
+template <int N> __device__ __forceinline__ void tanh_scores(float *x, float f) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x[i] *= f;
+    m = fmaxf(m, fabsf(x[i]));
+  }
+  if (__any(!(m <= 0.375f))) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = tanh_any(x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = tanh_series(x[i]);
+  }
+}
+
+// ---- work distribution ----------------------------------------------------------------------------------------------------
+// Workgroups go round-robin over the 8 XCDs, each with its own L2: consecutive items (which share keys and values) are dealt to one
+// XCD in one piece.  The grid is 8 * ceil(n / 8); surplus workgroups return -1.
+__device__ __forceinline__ int xcd_item(int n) {
+  const int per = (n + 7) >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  return item < n ? item : -1;
+}
+
+// Smallest / largest live document id of each tile of keys (or queries); live = id >= 0.
+struct DocRange {
+  int lo, hi, dead, pad;
+};
+
+// tiles t0 <= t < t1 whose documents overlap [lo, hi], in order; 64 tiles are looked up at a time
+struct TileIter {
+  const DocRange *rng;
+  int lo, hi, base, end;
+  unsigned long long mask;
+  __device__ __forceinline__ void start(const DocRange *r, int l, int h, int t0, int t1) {
+    rng = r, lo = l, hi = h, base = t0, end = t1, mask = 0;
+    fill();
+  }
+  __device__ __forceinline__ void fill() {
+    const int t = base + (threadIdx.x & 63);
+    bool ok = t < end;
+    if (ok && rng) ok = rng[t].lo <= hi && rng[t].hi >= lo;
+    mask = __ballot(ok);
+  }
+  __device__ __forceinline__ int next() {            // -1 when there is none left
+    while (mask == 0) {
+      base += 64;
+      if (base >= end) return -1;
+      fill();
+    }
+    const int n = __builtin_ctzll(mask);
+    mask &= mask - 1;
+    return __builtin_amdgcn_readfirstlane(base + n);
+  }
+};
+
+}  // namespace la

@@ -43,6 +43,14 @@ _lib.define("vit_map_fwd(Tensor maps, int handle, bool input_affine) -> Tensor")
 _lib.define("lane_enc_fwd(Tensor lanes, int handle) -> Tensor")
 _lib.define("unstandardize(Tensor pred_st, Tensor node_pos) -> Tensor")
 _lib.define("ade_fde(Tensor pred, Tensor gt) -> (Tensor, Tensor)")
+_ATTN = ("float? scale, bool causal, Tensor? prefix, Tensor? q_doc, Tensor? k_doc, Tensor? kv_len, float softcap, Tensor? slopes, "
+         "Tensor? rel_bias, Tensor? rel_buckets")
+_ROPE = "Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor inv_freq, Tensor? positions, float eps, bool interleaved"
+_lib.define(f"long_attention(Tensor q, Tensor k, Tensor v, {_ATTN}) -> (Tensor, Tensor)")
+_lib.define(f"long_attention_bwd(Tensor dout, Tensor? dlse, Tensor out, Tensor lse, Tensor q, Tensor k, Tensor v, {_ATTN}) "
+            "-> (Tensor, Tensor, Tensor, Tensor)")
+_lib.define(f"qk_norm_rope({_ROPE}) -> (Tensor, Tensor)")
+_lib.define(f"qk_norm_rope_bwd(Tensor dq_out, Tensor dk_out, {_ROPE}) -> (Tensor, Tensor, Tensor, Tensor)")
 
 
 def _encoder_fwd(x_st, handle):
@@ -100,7 +108,36 @@ def _ade_fde(pred, gt):
     return ade, fde
 
 
+# ---- attention over long rows, norm + rotation: differentiable ------------------------------------------------------------------
+def _long_attention_bwd(*args):
+    dq, dk, dv, dbias = ops.long_attention_backward(*args)
+    return dq, dk, dv, dbias if dbias is not None else dq.new_empty(0, dtype=torch.float32)
+
+
+def _long_attention_meta(q, k, v, *rest):
+    B, Lq, H, _ = q.shape
+    return q.new_empty(q.shape), q.new_empty((B, H, Lq), dtype=torch.float32)
+
+
+def _long_attention_bwd_meta(dout, dlse, out, lse, q, k, v, *rest):
+    table = rest[-2]
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), \
+        q.new_empty(table.shape if table is not None else 0, dtype=torch.float32)
+
+
+def _qk_norm_rope_meta(q, k, *rest):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+def _qk_norm_rope_bwd_meta(dqo, dko, q, k, q_weight, k_weight, *rest):
+    return q.new_empty(q.shape), k.new_empty(k.shape), q_weight.new_empty(q_weight.shape), k_weight.new_empty(k_weight.shape)
+
+
 for _name, _fn, _meta in (
+        ("long_attention", ops.long_attention, _long_attention_meta),
+        ("long_attention_bwd", _long_attention_bwd, _long_attention_bwd_meta),
+        ("qk_norm_rope", ops.qk_norm_rope, _qk_norm_rope_meta),
+        ("qk_norm_rope_bwd", ops.qk_norm_rope_backward, _qk_norm_rope_bwd_meta),
         ("encoder_fwd", _encoder_fwd, _encoder_fwd_meta),
         ("decoder_ar_fwd", _decoder_ar_fwd, _decoder_ar_fwd_meta),
         ("decoder_tf_fwd", _decoder_tf_fwd, _decoder_tf_fwd_meta),
@@ -111,6 +148,53 @@ for _name, _fn, _meta in (
         ("ade_fde", _ade_fde, lambda p, g: (p.new_empty(p.shape[0]), p.new_empty(p.shape[0])))):
     _lib.impl(_name, _fn, "CUDA")
     _lib.impl(_name, _meta, "Meta")
+
+
+def _long_attention_ctx(ctx, inputs, output):
+    q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets = inputs
+    if slopes is not None and slopes.requires_grad:
+        raise MmtError("long_attention: the slopes of the distance bias are constants, they get no gradient")
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(q, k, v, *output, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets)
+    ctx.plain = scale, causal, softcap
+
+
+def _long_attention_grad(ctx, dout, dlse):
+    q, k, v, out, lse, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets = ctx.saved_tensors
+    scale, causal, softcap = ctx.plain
+    if dout is None and dlse is None:
+        return (None,) * 13
+    if dout is None:
+        dout = torch.zeros_like(out)
+    dq, dk, dv, dbias = torch.ops.mmt.long_attention_bwd(dout, dlse, out, lse, q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len,
+                                                         softcap, slopes, rel_bias, rel_buckets)
+    return (dq, dk, dv) + (None,) * 8 + (dbias if rel_bias is not None else None, None)
+
+
+def _qk_norm_rope_ctx(ctx, inputs, output):
+    q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved = inputs
+    if inv_freq.requires_grad:
+        raise MmtError("qk_norm_rope: the frequencies are constants, they get no gradient")
+    ctx.save_for_backward(q, k, q_weight, k_weight, inv_freq, positions)
+    ctx.plain = eps, interleaved
+
+
+def _qk_norm_rope_grad(ctx, dqo, dko):
+    q, k, q_weight, k_weight, inv_freq, positions = ctx.saved_tensors
+    grads = torch.ops.mmt.qk_norm_rope_bwd(dqo, dko, q, k, q_weight, k_weight, inv_freq, positions, *ctx.plain)
+    return tuple(grads) + (None,) * 4
+
+
+def _no_second(name):
+    def refuse(ctx, *grads):
+        raise MmtError(f"{name}: there is no second derivative")
+    return refuse
+
+
+torch.library.register_autograd("mmt::long_attention", _long_attention_grad, setup_context=_long_attention_ctx, lib=_lib)
+torch.library.register_autograd("mmt::qk_norm_rope", _qk_norm_rope_grad, setup_context=_qk_norm_rope_ctx, lib=_lib)
+torch.library.register_autograd("mmt::long_attention_bwd", _no_second("long_attention"), lib=_lib)
+torch.library.register_autograd("mmt::qk_norm_rope_bwd", _no_second("qk_norm_rope"), lib=_lib)
 
 
 # ---- what the module classes call: the same ops through the dispatcher, with this package's error for host tensors ------------
@@ -153,3 +237,30 @@ def lane_enc_fwd(packed, lanes):
 def unstandardize(pred_st, node_pos):
     _dev(pred_st, node_pos)
     return torch.ops.mmt.unstandardize(pred_st, node_pos)
+
+
+def long_attention(q, k, v, *, scale=None, causal=False, prefix=None, q_doc=None, k_doc=None, kv_len=None, softcap=0.0, slopes=None,
+                   rel_bias=None, rel_buckets=None, return_lse=False):
+    """Attention over rows of any length, differentiable in q, k, v and rel_bias.  q (B,Lq,H,dh), k and v (B,Lk,Hk,dh) in bfloat16,
+    float16 or float32, H a multiple of Hk; query i of batch row b stands at position ``kv_len[b] - Lq + i`` (``Lk - Lq + i`` without
+    cache lengths), so the same call serves training (Lq = Lk), a chunk of new tokens and a single one over a cache.
+
+    scale      factor of the products, dh^-1/2 by default          softcap   > 0: scores become softcap * tanh(score / softcap)
+    causal     keys behind the query's position are hidden ...     prefix    (B) int32: ... but the first prefix[b] are not
+    kv_len     (B) int32: keys at and beyond it do not exist       q_doc, k_doc  (B,Lq), (B,Lk) int32: only equal ids see each other;
+                                                                             negative: padding, sees and is seen by nothing
+    slopes     (H) float32: -slopes[h] * distance is added         rel_bias  (H,n) float32, learned, at rel_buckets (2 reach + 1) int32 of
+                                                                             the clamped distance (``ops.relative_buckets``)
+    Rows that see nothing give zeros (and an lse of -inf).  Returns out (B,Lq,H,dh), with ``return_lse`` also the log-sums (B,H,Lq)."""
+    _dev(q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets)
+    out, lse = torch.ops.mmt.long_attention(q, k, v, scale, bool(causal), prefix, q_doc, k_doc, kv_len, float(softcap), slopes, rel_bias,
+                                            rel_buckets)
+    return (out, lse) if return_lse else out
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps=1e-6, interleaved=False):
+    """RMS norm of queries (B,L,H,dh) and keys (B,L,Hk,dh) per head, times the weights (dh), and the rotation of their first
+    2 * len(inv_freq) elements by position * inv_freq (float64, ``ops.rotary_frequencies``) in the same pass; differentiable in q, k
+    and the weights.  ``positions`` (B,L) int64, None: 0..L-1.  Pairs are (m, m + rot/2), with ``interleaved`` (2m, 2m + 1)."""
+    _dev(q, k, q_weight, k_weight, inv_freq, positions)
+    return torch.ops.mmt.qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, float(eps), bool(interleaved))
