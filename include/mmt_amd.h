@@ -608,12 +608,14 @@ int mmt_lane_gather(const double *table, const double *lanes, const int64_t *row
  *   out_i = sum_j softmax(u)_j v_j over the visible keys;  lse_i = log sum exp u.  A row that sees nothing: out 0, lse -inf,
  *   gradients 0.  An entry of -inf in rel_bias hides its bucket like a mask.
  * Heads: query head h reads key head h / (H / Hk).  q / k / v rows (head slices) are dh contiguous elements at any batch / token /
- * head stride (elements) that keeps them at multiples of 16 bytes; a stride of 0 broadcasts.  out (B,Lq,H,dh) and lse (B,H,Lq; may
+ * head stride (elements) that keeps them at multiples of 16 bytes, token strides below 2^24; a stride of 0 broadcasts.  out (B,Lq,H,dh) and lse (B,H,Lq; may
  * be NULL) contiguous.  Keys at j >= n and keys and queries with a negative id are never multiplied with anything: they may hold
  * NaN.  Bucket numbers are clamped to 0..n_buckets-1, lengths to 0..Lk.  Limits: dh a multiple of 8 up to 128, n_buckets <= 64,
  * reach <= 4096, (H / Hk) n_buckets <= 8192.  Sums, statistics and the products' accumulators are fp32; the probabilities and the
  * score gradients are rounded to the element type where they enter the second product.
- * bwd: `out` and `lse` are the forward's, dout rows like q, dlse (B,H,Lq) may be NULL; dq (B,Lq,H,dh), dk, dv (B,Lk,Hk,dh)
+ * fwd: out_low (like out, may be NULL) receives what rounding took from out, rounded to the element type itself: with it the
+ * backward forms rowsum(dout out) to twice the digits, which rows that see few keys need.
+ * bwd: `out`, `out_low` (may be NULL) and `lse` are the forward's, dout rows like q, dlse (B,H,Lq) may be NULL; dq (B,Lq,H,dh), dk, dv (B,Lk,Hk,dh)
  * contiguous, drel_bias (H,n_buckets) fp32 (with rel_bias only); all written, every sum in a fixed order (the same bits every call).
  * workspace: mmt_long_attention_workspace_bytes(a, backward) bytes, 16-byte aligned, no initialisation needed, not shared by calls
  * that may overlap.  Both calls can be captured into a graph. */
@@ -633,9 +635,10 @@ typedef struct {
   int32_t n_buckets, reach;
 } mmt_long_attention;
 size_t mmt_long_attention_workspace_bytes(const mmt_long_attention *a, int backward);
-int mmt_long_attention_fwd(const mmt_long_attention *a, void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
-int mmt_long_attention_bwd(const mmt_long_attention *a, const void *out, const float *lse, const void *dout, int64_t do_bs, int64_t do_rs,
-                           int64_t do_hs, const float *dlse, void *dq, void *dk, void *dv, float *drel_bias, void *workspace,
+int mmt_long_attention_fwd(const mmt_long_attention *a, void *out, void *out_low, float *lse, void *workspace, size_t workspace_bytes,
+                           void *stream);
+int mmt_long_attention_bwd(const mmt_long_attention *a, const void *out, const void *out_low, const float *lse, const void *dout,
+                           int64_t do_bs, int64_t do_rs, int64_t do_hs, const float *dlse, void *dq, void *dk, void *dv, float *drel_bias, void *workspace,
                            size_t workspace_bytes, void *stream);
 
 /* ---- norm of queries and keys per head with the rotation of their positions in the same pass (no counterpart in the reference, whose

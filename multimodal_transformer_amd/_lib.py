@@ -252,8 +252,8 @@ SIGNATURES = {
     "mmt_gmm2d_from_cov": (C.c_int, [fptr, C.c_long, fptr, fptr, C.c_void_p]),
     "mmt_map_crop": (C.c_int, [fptr, fptr, C.c_int, fptr, fptr, fptr, C.POINTER(C.c_int32), C.c_int, fptr, C.c_void_p]),
     "mmt_long_attention_workspace_bytes": (C.c_size_t, [C.POINTER(LongAttention), C.c_int]),
-    "mmt_long_attention_fwd": (C.c_int, [C.POINTER(LongAttention), fptr, fptr, fptr, C.c_size_t, C.c_void_p]),
-    "mmt_long_attention_bwd": (C.c_int, [C.POINTER(LongAttention), fptr, fptr, fptr, C.c_int64, C.c_int64, C.c_int64, fptr, fptr, fptr,
+    "mmt_long_attention_fwd": (C.c_int, [C.POINTER(LongAttention), fptr, fptr, fptr, fptr, C.c_size_t, C.c_void_p]),
+    "mmt_long_attention_bwd": (C.c_int, [C.POINTER(LongAttention), fptr, fptr, fptr, fptr, C.c_int64, C.c_int64, C.c_int64, fptr, fptr, fptr,
                                          fptr, fptr, fptr, C.c_size_t, C.c_void_p]),
     "mmt_qk_norm_rope_fwd": (C.c_int, [C.POINTER(QkNormRope), fptr, fptr, C.c_void_p]),
     "mmt_qk_norm_rope_workspace_bytes": (C.c_size_t, [C.POINTER(QkNormRope)]),

@@ -18,11 +18,10 @@
 #include <math.h>
 #include <stdint.h>
 
-#include "../../include/mmt_amd.h"
+#include "long_attention_args.cuh"
 
 namespace la {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -34,7 +33,6 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS = 32 * WAVES;   // a workgroup: 4 waves of 32 rows each
 
 // ---- element types --------------------------------------------------------------------------------------------------------
 // BK: keys (queries, in the key-gradient kernel) per LDS tile; fp32 elements are twice as large, so half as many.
@@ -150,33 +148,59 @@ template <typename T> __device__ __forceinline__ typename Elem<T>::V8 mem_frag(c
   return r;
 }
 
-// A tile on its way from memory to LDS through registers.  Rows that are not `live` become zeros whatever memory holds there (the
-// tail of a cache, padding): 0 x NaN would reach every other row of the tile.
-template <typename T, int D> struct Stage {
+// One 16-byte piece per lane straight from memory into LDS (no registers in between): lane l's piece lands at lds + 16 l.
+// Untracked by the compiler: dma_wait() before the barrier that publishes the tile.  M0 holds the LDS address (below 64 KiB).
+__device__ __forceinline__ void dma16(const void *base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+__device__ __forceinline__ unsigned lds_address(const void *p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char *)p;
+}
+
+// Tiles of a (rows, dh) matrix on their way to LDS.  A lane's byte offset inside a tile is the same for every tile; the tile's own
+// part is a scalar.  Slots at and beyond dh repeat slot 0 and rows at and beyond n_rows the last row (nothing outside the tensor is
+// read); the operands these elements meet are zero, or results nobody stores.
+template <typename T, int D> struct Dma {
   typedef Tile<T, D> L;
-  u32x4 r[L::NLD];
-  // rows r0 .. r0 + BK - 1 of a (rows, dh) matrix with `rs` elements between rows; rows >= n_rows are not read
-  __device__ __forceinline__ void load(const T *base, int64_t rs, int r0, int n_rows, int dh) {
+  const char *base;
+  int64_t rs;                        // bytes between rows; 64 rows stay below 2^31 bytes
+  int n_rows;
+  unsigned off[L::NLD];
+  __device__ __forceinline__ void init(const T *p, int64_t row_stride, int rows, int dh) {
+    base = (const char *)p, rs = row_stride * (int64_t)sizeof(T), n_rows = rows;
 #pragma unroll
     for (int n = 0; n < L::NLD; ++n) {
       const int idx = threadIdx.x + n * THREADS, row = idx / L::NS, slot = L::swz(row, idx % L::NS);
-      u32x4 v = {};
-      if (r0 + row < n_rows && slot * L::EPS < dh) v = *(const u32x4 *)(base + (int64_t)(r0 + row) * rs + slot * L::EPS);
-      r[n] = v;
+      off[n] = (unsigned)(row * rs) + (slot * L::EPS < dh ? slot * 16 : 0);
     }
   }
-  // rows at r0 + row >= end, or whose document id is negative, are written as zeros
-  __device__ __forceinline__ void store(char *lds, int r0, int end, const int *doc) {
+  __device__ __forceinline__ void load(unsigned lds, int r0) const {
+    const char *b = base + r0 * rs;
+    const unsigned mine = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+    if (r0 + L::BK <= n_rows) {
 #pragma unroll
-    for (int n = 0; n < L::NLD; ++n) {
-      const int idx = threadIdx.x + n * THREADS, row = idx / L::NS;
-      u32x4 v = r[n];
-      const bool dead = r0 + row >= end || (doc && doc[r0 + row] < 0);
-      if (dead) v = u32x4{};
-      *(u32x4 *)(lds + idx * 16) = v;
+      for (int n = 0; n < L::NLD; ++n) dma16(b, off[n], mine + n * THREADS * 16);
+    } else {
+#pragma unroll
+      for (int n = 0; n < L::NLD; ++n) {
+        const int row = (int)(threadIdx.x + n * THREADS) / L::NS, over = max(0, r0 + row - (n_rows - 1));
+        dma16(b, off[n] - (unsigned)(over * rs), mine + n * THREADS * 16);
+      }
     }
   }
 };
+
+// Rows of a tile that must not take part become zeros (whatever they hold: 0 x NaN would reach every other row): at and beyond `end`
+// (tile row), or with a negative document id
+template <typename T, int D> __device__ __forceinline__ void zero_rows(char *lds, int end, const int *doc) {
+  typedef Tile<T, D> L;
+#pragma unroll
+  for (int n = 0; n < L::NLD; ++n) {
+    const int idx = threadIdx.x + n * THREADS, row = idx / L::NS;
+    if (row >= end || (doc && doc[row] < 0)) *(u32x4 *)(lds + idx * 16) = u32x4{};
+  }
+}
 
 // ---- lanes ----------------------------------------------------------------------------------------------------------------
 // the two halves of the wave hold complementary parts of a row: v[lane] op v[lane ^ 32]
@@ -243,31 +267,30 @@ template <int N> __device__ __forceinline__ void tanh_scores(float *x, float f) 
 }
 
 // ---- work distribution ----------------------------------------------------------------------------------------------------
-// Workgroups go round-robin over the 8 XCDs, each with its own L2: consecutive items (which share keys and values) are dealt to one
-// XCD in one piece.  The grid is 8 * ceil(n / 8); surplus workgroups return -1.
-__device__ __forceinline__ int xcd_item(int n) {
-  const int per = (n + 7) >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  return item < n ? item : -1;
-}
+// Workgroups go round-robin over the 8 XCDs, each with its own L2.  Item n belongs to group n % groups (the workgroups that read the
+// same keys and values): with a multiple of 8 groups each stays on one XCD, and within all groups the items come in the order
+// n / groups, the longest first.
 
-// Smallest / largest live document id of each tile of keys (or queries); live = id >= 0.
-struct DocRange {
-  int lo, hi, dead, pad;
-};
-
-// tiles t0 <= t < t1 whose documents overlap [lo, hi], in order; 64 tiles are looked up at a time
+// tiles t0 <= t < t1 whose documents overlap [lo, hi], in order; 64 tiles are looked up at a time, one per lane
 struct TileIter {
   const DocRange *rng;
   int lo, hi, base, end;
   unsigned long long mask;
+  DocRange mine;
+  int cur_lo, cur_hi, cur_dead;                      // of the tile that next() returned
   __device__ __forceinline__ void start(const DocRange *r, int l, int h, int t0, int t1) {
-    rng = r, lo = l, hi = h, base = t0, end = t1, mask = 0;
+    rng = r, lo = l, hi = h, base = t0, end = t1;
+    mine = DocRange{0, 0, 0, 0};
+    cur_lo = cur_hi = cur_dead = 0;
     fill();
   }
   __device__ __forceinline__ void fill() {
     const int t = base + (threadIdx.x & 63);
     bool ok = t < end;
-    if (ok && rng) ok = rng[t].lo <= hi && rng[t].hi >= lo;
+    if (ok && rng) {
+      mine = rng[t];
+      ok = mine.lo <= hi && mine.hi >= lo;
+    }
     mask = __ballot(ok);
   }
   __device__ __forceinline__ int next() {            // -1 when there is none left
@@ -278,8 +301,15 @@ struct TileIter {
     }
     const int n = __builtin_ctzll(mask);
     mask &= mask - 1;
+    if (rng) {
+      cur_lo = __builtin_amdgcn_readlane(mine.lo, n);
+      cur_hi = __builtin_amdgcn_readlane(mine.hi, n);
+      cur_dead = __builtin_amdgcn_readlane(mine.dead, n);
+    }
     return __builtin_amdgcn_readfirstlane(base + n);
   }
+  // not a single document that all rows of [lo, hi] share: masks are needed
+  __device__ __forceinline__ bool mixed() const { return rng && !(cur_dead == 0 && cur_lo == cur_hi && lo == hi && lo == cur_lo); }
 };
 
 }  // namespace la

@@ -1,0 +1,1026 @@
+// The kernels of attention over long rows and their launchers, included by one translation unit per element type
+// (long_attention_{bf16,fp16,fp32}.hip); the entry points are in long_attention.hip.
+#pragma once
+#include "long_attention.cuh"
+#include "long_attention_args.cuh"
+
+namespace la {
+
+// what a lane knows about its query row
+struct Row {
+  bool valid, live;                // a row of this call; and not padding
+  int i, h, p, hi, doc;            // query, head, position, first invisible key (before documents), document
+  float slope;                     // slope times log2 e
+};
+
+template <typename A> __device__ __forceinline__ int row_len(const A &a, int b) {
+  return a.kv_len ? max(0, min(a.kv_len[b], a.Lk)) : a.Lk;
+}
+
+__device__ __forceinline__ Row make_row(const Args &g, int b, int head0, int r, int len) {
+  const mmt_long_attention &a = g.a;
+  Row w;
+  w.i = r / g.pack;
+  w.h = head0 + r % g.pack;
+  w.valid = w.i < a.Lq;
+  w.p = len - a.Lq + w.i;
+  w.doc = 0;
+  if (a.q_doc && w.valid) w.doc = a.q_doc[(int64_t)b * a.Lq + w.i];
+  w.live = w.valid && w.doc >= 0;
+  w.hi = len;
+  if (a.causal) w.hi = min(len, max(w.p + 1, a.prefix ? a.prefix[b] : 0));
+  w.slope = a.slopes && w.valid ? a.slopes[w.h] * LOG2E : 0.f;
+  return w;
+}
+
+// bounds over the live rows of a wave, then of the workgroup
+struct Bounds {
+  int hi_min, hi_max, p_min, p_max, d_min, d_max;
+};
+__device__ __forceinline__ Bounds wave_bounds(const Row &w) {
+  Bounds b;
+  b.hi_min = wave_min(w.live ? w.hi : 0x7fffffff);
+  b.hi_max = wave_max(w.live ? w.hi : 0);
+  b.p_min = wave_min(w.live ? w.p : 0x7fffffff);
+  b.p_max = wave_max(w.live ? w.p : -0x7fffffff);
+  b.d_min = wave_min(w.live ? w.doc : 0x7fffffff);
+  b.d_max = wave_max(w.live ? w.doc : -1);
+  return b;
+}
+__device__ __forceinline__ Bounds group_bounds(const Bounds &w, int *s, int wave) {      // s: 6 * WAVES ints of LDS
+  if ((threadIdx.x & 63) == 0) {
+    s[wave * 6 + 0] = w.hi_min, s[wave * 6 + 1] = w.hi_max, s[wave * 6 + 2] = w.p_min;
+    s[wave * 6 + 3] = w.p_max, s[wave * 6 + 4] = w.d_min, s[wave * 6 + 5] = w.d_max;
+  }
+  __syncthreads();
+  Bounds b = {0x7fffffff, 0, 0x7fffffff, -0x7fffffff, 0x7fffffff, -1};
+  for (int v = 0; v < WAVES; ++v) {
+    b.hi_min = min(b.hi_min, s[v * 6 + 0]), b.hi_max = max(b.hi_max, s[v * 6 + 1]), b.p_min = min(b.p_min, s[v * 6 + 2]);
+    b.p_max = max(b.p_max, s[v * 6 + 3]), b.d_min = min(b.d_min, s[v * 6 + 4]), b.d_max = max(b.d_max, s[v * 6 + 5]);
+  }
+  b.hi_min = __builtin_amdgcn_readfirstlane(b.hi_min), b.hi_max = __builtin_amdgcn_readfirstlane(b.hi_max);
+  b.p_min = __builtin_amdgcn_readfirstlane(b.p_min), b.p_max = __builtin_amdgcn_readfirstlane(b.p_max);
+  b.d_min = __builtin_amdgcn_readfirstlane(b.d_min), b.d_max = __builtin_amdgcn_readfirstlane(b.d_max);
+  return b;
+}
+
+// The learned bias in LDS: the table rows of the workgroup's heads (in units of log 2) and the bucket of each clamped distance.
+// Bucket numbers outside the table are clamped into it.  An entry at or below -2^100 (the lowest value of a type, used as a mask) is
+// taken for -inf: next to it a score vanishes in rounding, and the saved log-sum of a row of such entries could not tell them apart.
+struct BiasLds {
+  float *table;             // [pack][nb]
+  unsigned char *bucket;    // [2 reach + 1]
+  __device__ __forceinline__ void fill(const mmt_long_attention &a, int head0, int pack) {
+    for (int n = threadIdx.x; n < pack * a.n_buckets; n += THREADS) {
+      const float v = a.rel_bias[(int64_t)(head0 + n / a.n_buckets) * a.n_buckets + n % a.n_buckets];
+      table[n] = v <= -0x1p100f ? -INFINITY : v * LOG2E;
+    }
+    for (int n = threadIdx.x; n < 2 * a.reach + 1; n += THREADS)
+      bucket[n] = (unsigned char)max(0, min(a.rel_buckets[n], a.n_buckets - 1));
+  }
+};
+static inline __host__ __device__ int bias_lds_bytes(const mmt_long_attention &a, int pack) {
+  return a.rel_bias ? pack * a.n_buckets * 4 + ((2 * a.reach + 1 + 15) & ~15) : 0;
+}
+
+// Raw products -> modified scores in units of log 2; `t` receives tanh(s / cap) when the scores are capped and the caller needs it.
+struct ScoreCtx {
+  float c_scale, cap_in, cap_out;  // scale log2 e; scale / cap; cap log2 e
+  bool capped, rel;
+};
+__device__ __forceinline__ ScoreCtx score_ctx(const mmt_long_attention &a) {
+  ScoreCtx s;
+  s.c_scale = a.scale * LOG2E;
+  s.capped = a.softcap > 0.f;
+  s.cap_in = s.capped ? a.scale / a.softcap : 0.f;
+  s.cap_out = a.softcap * LOG2E;
+  s.rel = a.rel_bias != nullptr;
+  return s;
+}
+
+// x: N raw products of a lane, element i belongs to the distance d0 + step (8 (i / 4) + i % 4); far: the whole tile lies beyond the
+// reach on one side (-1 behind, 1 ahead): one bucket
+template <int N, bool KEEP>
+__device__ __forceinline__ void modify(const mmt_long_attention &a, const ScoreCtx &sc, float *x, float *t, int d0, int step, float slope,
+                                       const float *tab, const unsigned char *bucket, int far) {
+  if (sc.capped) {
+    tanh_scores<N>(x, sc.cap_in);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (KEEP) t[i] = x[i];
+      x[i] *= sc.cap_out;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= sc.c_scale;
+  }
+  if (a.slopes) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = fmaf(-slope, fabsf((float)(d0 + step * (8 * (i >> 2) + (i & 3)))), x[i]);
+  }
+  if (sc.rel) {
+    if (far != 0) {
+      const float v = tab[bucket[far < 0 ? 0 : 2 * a.reach]];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] += v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] += tab[bucket[max(-a.reach, min(a.reach, d0 + step * (8 * (i >> 2) + (i & 3)))) + a.reach]];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- forward
+// One workgroup = 128 rows (4 waves x 32) of one head - or of the `pack` heads that share a key head, when there are few queries -
+// against a range of key tiles.  K and V tiles go straight from memory to LDS, one tile ahead of the products (two buffers, one
+// barrier per tile).  MOD: the scores are capped or biased; without it they go from the product into the exponential as they are.
+template <typename T, int D, bool MOD>
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_fwd_kernel(const Args g) {
+  typedef Tile<T, D> L;
+  typedef typename Elem<T>::V8 V8;
+  constexpr int BK = L::BK, NK = BK / 32, NC = D / 16, ND = D / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const mmt_long_attention &a = g.a;
+  int *sDoc = (int *)(smem + 4 * L::BYTES), *sB = sDoc + BK;
+  BiasLds bias;
+  bias.table = (float *)(sB + 6 * WAVES);
+  const int ngroup = g.pack > 1 ? 1 : g.G, grp = blockIdx.x % g.groups;
+  int n = blockIdx.x / g.groups;
+  const int split = n % g.nsplit;
+  n /= g.nsplit;
+  const int gi = n % ngroup;
+  int qt = n / ngroup;
+  if (a.causal) qt = g.nqt - 1 - qt;                     // the tiles with the most keys first
+  const int kh = grp % a.Hk, b = grp / a.Hk;
+  const int head0 = kh * g.G + gi;
+  bias.bucket = (unsigned char *)(bias.table + (MOD && a.rel_bias ? g.pack * a.n_buckets : 0));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+  const int len = row_len(a, b);
+  const Row w = make_row(g, b, head0, qt * ROWS + wave * 32 + col, len);
+  const Bounds wb = wave_bounds(w);
+  const Bounds gb = group_bounds(wb, sB, wave);
+  if (MOD && a.rel_bias) bias.fill(a, head0, g.pack);
+  const float *tab = bias.table + (g.pack > 1 ? (w.h - head0) * a.n_buckets : 0);
+
+  const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)w.h * a.q_hs;
+  V8 fq[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+  const ScoreCtx sc = score_ctx(a);
+
+  const int tiles = (gb.hi_max + BK - 1) / BK, per = (tiles + g.nsplit - 1) / g.nsplit;
+  TileIter it;
+  it.start(g.krng ? g.krng + (int64_t)b * g.nkt : nullptr, gb.d_min, gb.d_max, split * per, min(tiles, (split + 1) * per));
+  const int *kdoc = a.k_doc ? a.k_doc + (int64_t)b * a.Lk : nullptr;
+  Dma<T, D> dk, dv;
+  dk.init((const T *)a.k + (int64_t)b * a.k_bs + (int64_t)kh * a.k_hs, a.k_rs, a.Lk, a.dh);
+  dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
+  const unsigned lds = lds_address(smem);
+  int t = it.next(), buf = 0;
+  if (t >= 0) {
+    dk.load(lds, t * BK);
+    dv.load(lds + L::BYTES, t * BK);
+  }
+  while (t >= 0) {
+    const int k0 = t * BK;
+    const bool mixed = it.mixed(), dead = it.cur_dead != 0;
+    char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
+    dma_wait();
+    __syncthreads();                                     // the tile is here, and nobody reads the other buffer any more
+    if (mixed) {
+      if (threadIdx.x < BK) sDoc[threadIdx.x] = k0 + (int)threadIdx.x < a.Lk ? kdoc[k0 + threadIdx.x] : -1;
+      __syncthreads();
+    }
+    if (k0 + BK > len || (mixed && dead)) {
+      zero_rows<T, D>(sK, len - k0, mixed ? sDoc : nullptr);
+      zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
+      __syncthreads();
+    }
+    const int tn = it.next();
+    if (tn >= 0) {
+      dk.load(lds + (buf ^ 1) * 2 * L::BYTES, tn * BK);
+      dv.load(lds + (buf ^ 1) * 2 * L::BYTES + L::BYTES, tn * BK);
+    }
+    if (k0 < wb.hi_max) {
+      const bool need_mask = k0 + BK > wb.hi_min || mixed;
+      float x[NK * 16];
+#pragma unroll
+      for (int kt = 0; kt < NK; ++kt) {
+        f32x16 s = {};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[16 * kt + i] = s[i];
+      }
+      float cf = sc.c_scale;
+      if constexpr (MOD) {
+        const int far = !a.rel_bias ? 0 : k0 + BK - 1 - wb.p_min <= -a.reach ? -1 : k0 - wb.p_max >= a.reach ? 1 : 0;
+#pragma unroll
+        for (int kt = 0; kt < NK; ++kt)
+          modify<16, false>(a, sc, x + 16 * kt, nullptr, k0 + 32 * kt + 4 * h - w.p, 1, w.slope, tab, bias.bucket, far);
+        cf = 1.f;
+      }
+      if (need_mask) {
+#pragma unroll
+        for (int i = 0; i < NK * 16; ++i) {
+          const int j = 32 * (i >> 4) + acc_row(i & 15, h);
+          bool see = k0 + j < w.hi;
+          if (mixed) see = see && sDoc[j] == w.doc;
+          if (!see) x[i] = -INFINITY;
+        }
+      }
+      float mx = x[0];
+#pragma unroll
+      for (int i = 1; i < NK * 16; ++i) mx = fmaxf(mx, x[i]);
+      const float m_new = fmaxf(m, half_max(mx) * cf);
+      const float ms = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = ex2(m - ms);
+      m = m_new;
+      const float off = Elem<T>::PSHIFT - ms;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < NK * 16; ++i) {
+        x[i] = ex2(fmaf(x[i], cf, off));
+        sum += x[i];
+      }
+      l = fmaf(l, alpha, sum);
+      if (__any(alpha != 1.f)) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+      }
+#pragma unroll
+      for (int c = 0; c < NK * 2; ++c) {
+        const V8 p = round8<T>(x + 8 * c);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] = Elem<T>::mma(col_frag<T, D>(sV, 16 * c, d, lane), p, acc[d]);
+      }
+    }
+    t = tn;
+    buf ^= 1;
+  }
+  l = half_sum(l);
+  if (!w.valid) return;
+  const int64_t r = ((int64_t)b * a.H + w.h) * a.Lq + w.i;
+  if (g.nsplit > 1) {
+    const int64_t rs = (int64_t)split * a.B * a.H * a.Lq + r;
+    if (h == 0) {
+      g.part_ml[2 * rs] = w.live ? m : -INFINITY;
+      g.part_ml[2 * rs + 1] = w.live ? l : 0.f;
+    }
+    float *o = g.part_o + rs * a.dh;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int dim = 32 * d + 8 * q + 4 * h;
+        if (dim < a.dh) *(f32x4 *)(o + dim) = f32x4{acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]};
+      }
+    return;
+  }
+  const bool some = w.live && l != 0.f;                   // (a NaN sum is "some")
+  const float inv = some ? 1.f / l : 0.f;
+  if (g.lse && h == 0) g.lse[r] = some ? (m + log2f(l) - Elem<T>::PSHIFT) * LN2 : -INFINITY;
+  const int64_t o = (((int64_t)b * a.Lq + w.i) * a.H + w.h) * a.dh;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int dim = 32 * d + 8 * q + 4 * h;
+      if (dim < a.dh) {
+        typename Elem<T>::V4 v, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = some ? acc[d][4 * q + e] * inv : 0.f;
+          v[e] = (T)y, lo[e] = (T)(y - (float)v[e]);
+        }
+        *(typename Elem<T>::V4 *)((T *)g.out + o + dim) = v;
+        if (g.low) *(typename Elem<T>::V4 *)((T *)g.low + o + dim) = lo;
+      }
+    }
+}
+
+// Joins the splits of a row: weights 2^(m_s - max m).  16 lanes per row, up to 8 elements per lane.
+template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_join_kernel(const Args g) {
+  const mmt_long_attention &a = g.a;
+  const int64_t rows = (int64_t)a.B * a.H * a.Lq, r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (r >= rows) return;
+  const int d0 = (threadIdx.x & 15) * 8;
+  float m = -INFINITY;
+  for (int s = 0; s < g.nsplit; ++s) m = fmaxf(m, g.part_ml[2 * (s * rows + r)]);
+  const float ms = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  f32x4 o[2] = {};
+  for (int s = 0; s < g.nsplit; ++s) {
+    const int64_t rs = s * rows + r;
+    const float ls = g.part_ml[2 * rs + 1], f = ls == 0.f ? 0.f : ex2(g.part_ml[2 * rs] - ms);
+    l = fmaf(ls, f, l);
+    if (d0 < a.dh && ls != 0.f) {
+      o[0] += *(const f32x4 *)(g.part_o + rs * a.dh + d0) * f;
+      o[1] += *(const f32x4 *)(g.part_o + rs * a.dh + d0 + 4) * f;
+    }
+  }
+  const bool some = l != 0.f;
+  const float inv = some ? 1.f / l : 0.f;
+  const int64_t i = r % a.Lq, bh = r / a.Lq, hd = bh % a.H, b = bh / a.H;
+  if (g.lse && (threadIdx.x & 15) == 0) g.lse[r] = some ? (m + log2f(l) - Elem<T>::PSHIFT) * LN2 : -INFINITY;
+  if (d0 < a.dh) {
+    typename Elem<T>::V8 v, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = some ? o[e >> 2][e & 3] * inv : 0.f;
+      v[e] = (T)y, lo[e] = (T)(y - (float)v[e]);
+    }
+    const int64_t at = ((b * a.Lq + i) * a.H + hd) * a.dh + d0;
+    *(typename Elem<T>::V8 *)((T *)g.out + at) = v;
+    if (g.low) *(typename Elem<T>::V8 *)((T *)g.low + at) = lo;
+  }
+}
+
+// document ids -> per tile of `bk`: smallest, largest live id, and whether any row of the tile is dead or missing.  Entries 0 .. nk - 1
+// are of the keys, the rest of the queries.
+template <typename T> __global__ void mmt_long_attn_docs_kernel(const Args g, int bk, int nk, int total, DocRange *out) {
+  int n = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, at = n;
+  if (n >= total) return;
+  const bool key = n < nk;
+  if (!key) n -= nk;
+  const int L = key ? g.a.Lk : g.a.Lq, nt = (L + bk - 1) / bk, t = n % nt, j = t * bk + lane;
+  const int *doc = key ? g.a.k_doc : g.a.q_doc;
+  const int id = lane < bk && j < L ? doc[(int64_t)(n / nt) * L + j] : -1;
+  const int lo = wave_min(id >= 0 ? id : 0x7fffffff), hi = wave_max(id);
+  const bool dead = __any(lane < bk && id < 0);
+  if (lane == 0) out[at] = DocRange{lo, hi, dead ? 1 : 0, 0};
+}
+
+// --------------------------------------------------------------------------------------------------------------- backward
+//   dV = P^T dO;   dP = dO V^T;   dU = P (dP - delta), delta_i = rowsum(dO o) - dlse_i;   dS = dU (1 - tanh^2)
+//   dQ = scale dS K;   dK = scale dS^T Q;   dtable[h][b] = sum of dU over the pairs of the bucket
+// Two kernels recompute the probabilities from the saved log-sum: one walks the keys of a query tile (dQ), the other the queries of
+// a key tile (dK, dV, summed over the query heads that share the key head).  Seven products instead of the five of a single pass,
+// but every sum has a fixed order and an owner: no atomics, the same bits every time.
+// delta is the small difference of large terms where a row sees few keys: it is formed from out and what rounding took from it
+// (`low`), which the forward keeps for this.
+
+// delta and the log-sum in units of log 2; 16 lanes per row.
+// fp16: the score gradients are rounded to 5 exponent bits, so they are first multiplied by a power of two that takes their bound
+// 2 max|do_i| max|v_j| + max|dlse| to at most 2^15; each workgroup leaves its part of the three maxima.
+template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_stat_kernel(const Args g, float2 *stat, f32x4 *maxima) {
+  const mmt_long_attention &a = g.a;
+  typedef typename Elem<T>::V8 V8;
+  const int64_t rows = (int64_t)a.B * a.H * a.Lq;
+  const int d0 = (threadIdx.x & 15) * 8;
+  float mx = 0.f, mv = 0.f, ml = 0.f;
+  for (int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); r < rows; r += (int64_t)gridDim.x * 16) {
+    // rows in the order of the tensors (b, i, h), the statistics in the order of the kernels that read them (b, h, i)
+    const int64_t hd = r % a.H, bi = r / a.H, i = bi % a.Lq, b = bi / a.Lq, w = (b * a.H + hd) * a.Lq + i;
+    const bool live = !(a.q_doc && a.q_doc[b * a.Lq + i] < 0);
+    float s = 0.f, nn = 0.f;
+    if (d0 < a.dh && live) {
+      const V8 o = *(const V8 *)((const T *)g.out + r * a.dh + d0);
+      const V8 d = *(const V8 *)((const T *)g.dout + b * g.do_bs + i * g.do_rs + hd * g.do_hs + d0);
+      V8 lo = {};
+      if (g.low) lo = *(const V8 *)((const T *)g.low + r * a.dh + d0);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s = fmaf((float)o[e] + (float)lo[e], (float)d[e], s);
+        nn = fmaf((float)d[e], (float)d[e], nn);
+      }
+    }
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) {
+      s += __shfl_xor(s, m);
+      nn += __shfl_xor(nn, m);
+    }
+    const float ls = g.lse[w], dl = g.dlse && live ? g.dlse[w] : 0.f;
+    if (isfinite(nn)) mx = fmaxf(mx, nn);
+    if (isfinite(dl)) ml = fmaxf(ml, fabsf(dl));
+    // a row without keys has probabilities 0: its log-sum is turned around
+    if ((threadIdx.x & 15) == 0) stat[w] = make_float2(ls == -INFINITY ? INFINITY : ls * LOG2E, s - dl);
+  }
+  if (!maxima) return;
+  const int64_t vrows = (int64_t)a.B * a.Lk * a.Hk;
+  for (int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); r < vrows; r += (int64_t)gridDim.x * 16) {
+    const int64_t hd = r % a.Hk, bj = r / a.Hk, j = bj % a.Lk, b = bj / a.Lk;
+    if (j >= row_len(a, (int)b) || (a.k_doc && a.k_doc[b * a.Lk + j] < 0)) continue;
+    float s = 0.f;
+    if (d0 < a.dh) {
+      const V8 v = *(const V8 *)((const T *)a.v + b * a.v_bs + j * a.v_rs + hd * a.v_hs + d0);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = fmaf((float)v[e], (float)v[e], s);
+    }
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) s += __shfl_xor(s, m);
+    if (isfinite(s)) mv = fmaxf(mv, s);
+  }
+#pragma unroll
+  for (int m = 16; m < 64; m <<= 1) {
+    mx = fmaxf(mx, __shfl_xor(mx, m));
+    mv = fmaxf(mv, __shfl_xor(mv, m));
+    ml = fmaxf(ml, __shfl_xor(ml, m));
+  }
+  __shared__ f32x4 part[4];
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = f32x4{mx, mv, ml, 0.f};
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    f32x4 v = part[0];
+    for (int w = 1; w < 4; ++w)
+      for (int e = 0; e < 3; ++e) v[e] = fmaxf(v[e], part[w][e]);
+    maxima[blockIdx.x] = v;
+  }
+}
+template <typename T> __global__ void __launch_bounds__(64) mmt_long_attn_dscale_kernel(const f32x4 *maxima, int parts, float *dscale) {
+  f32x4 v = {};
+  for (int n = threadIdx.x; n < parts; n += 64)
+    for (int e = 0; e < 3; ++e) v[e] = fmaxf(v[e], maxima[n][e]);
+  for (int m = 1; m < 64; m <<= 1)
+    for (int e = 0; e < 3; ++e) v[e] = fmaxf(v[e], __shfl_xor(v[e], m));
+  const float bound = 2.f * sqrtf(v[0]) * sqrtf(v[1]) + v[2];
+  int e = 0;
+  const bool known = bound > 0.f && isfinite(bound);
+  if (known) (void)frexpf(bound, &e);                                     // bound < 2^e
+  if (threadIdx.x == 0) dscale[0] = ldexpf(1.f, known ? max(-60, min(60, 15 - e)) : 0);
+}
+
+// dQ.  The forward's geometry; K is read twice from LDS (as rows for the scores, transposed for dQ^T += K^T dS^T), V once.
+// With a learned bias it also leaves, per row, the exact delta (see the table kernel) and the sums of dU over the tiles that lie wholly
+// beyond the reach on either side.
+template <typename T, int D, bool MOD>
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_dq_kernel(const Args g) {
+  typedef Tile<T, D> L;
+  typedef typename Elem<T>::V8 V8;
+  constexpr int BK = L::BK, NK = BK / 32, NC = D / 16, ND = D / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const mmt_long_attention &a = g.a;
+  int *sDoc = (int *)(smem + 4 * L::BYTES), *sB = sDoc + BK;
+  BiasLds bias;
+  bias.table = (float *)(sB + 6 * WAVES);
+  bias.bucket = (unsigned char *)(bias.table + (MOD && a.rel_bias ? a.n_buckets : 0));
+  const int grp = blockIdx.x % g.groups, n = blockIdx.x / g.groups, gi = n % g.G;
+  int qt = n / g.G;
+  if (a.causal) qt = g.nqt - 1 - qt;
+  const int kh = grp % a.Hk, b = grp / a.Hk, head = kh * g.G + gi;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+  const int len = row_len(a, b);
+  const Row w = make_row(g, b, head, qt * ROWS + wave * 32 + col, len);
+  const Bounds wb = wave_bounds(w);
+  const Bounds gb = group_bounds(wb, sB, wave);
+  if (MOD && a.rel_bias) bias.fill(a, head, 1);
+  const int64_t r = ((int64_t)b * a.H + head) * a.Lq + min(w.i, a.Lq - 1);
+  const float2 st = w.live ? g.stat[r] : make_float2(INFINITY, 0.f);
+
+  const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)head * a.q_hs;
+  const T *drow = (const T *)g.dout + (int64_t)b * g.do_bs + (int64_t)min(w.i, a.Lq - 1) * g.do_rs + (int64_t)head * g.do_hs;
+  V8 fq[NC], fd[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
+    fd[c] = mem_frag<T>(drow, c, h, a.dh, w.live);
+  }
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+  const ScoreCtx sc = score_ctx(a);
+  const float dscale = sizeof(T) == 2 && g.dscale ? g.dscale[0] : 1.f;
+  float all_u = 0.f, far_u[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f};
+
+  const int tiles = (gb.hi_max + BK - 1) / BK;
+  TileIter it;
+  it.start(g.krng ? g.krng + (int64_t)b * g.nkt : nullptr, gb.d_min, gb.d_max, 0, tiles);
+  const int *kdoc = a.k_doc ? a.k_doc + (int64_t)b * a.Lk : nullptr;
+  Dma<T, D> dk, dv;
+  dk.init((const T *)a.k + (int64_t)b * a.k_bs + (int64_t)kh * a.k_hs, a.k_rs, a.Lk, a.dh);
+  dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
+  const unsigned lds = lds_address(smem);
+  int t = it.next(), buf = 0;
+  if (t >= 0) {
+    dk.load(lds, t * BK);
+    dv.load(lds + L::BYTES, t * BK);
+  }
+  while (t >= 0) {
+    const int k0 = t * BK;
+    const bool mixed = it.mixed(), dead = it.cur_dead != 0;
+    char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
+    dma_wait();
+    __syncthreads();
+    if (mixed) {
+      if (threadIdx.x < BK) sDoc[threadIdx.x] = k0 + (int)threadIdx.x < a.Lk ? kdoc[k0 + threadIdx.x] : -1;
+      __syncthreads();
+    }
+    if (k0 + BK > len || (mixed && dead)) {
+      zero_rows<T, D>(sK, len - k0, mixed ? sDoc : nullptr);
+      zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
+      __syncthreads();
+    }
+    const int tn = it.next();
+    if (tn >= 0) {
+      dk.load(lds + (buf ^ 1) * 2 * L::BYTES, tn * BK);
+      dv.load(lds + (buf ^ 1) * 2 * L::BYTES + L::BYTES, tn * BK);
+    }
+    if (k0 < wb.hi_max) {
+      const bool need_mask = k0 + BK > wb.hi_min || mixed;
+      // by the whole workgroup's rows: the table kernel takes the tiles that are left with the same rule
+      const int far = !(MOD && a.rel_bias) ? 0 : k0 + BK - 1 - gb.p_min <= -a.reach ? -1 : k0 - gb.p_max >= a.reach ? 1 : 0;
+#pragma unroll
+      for (int kt = 0; kt < NK; ++kt) {
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s);
+          dp = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp);
+        }
+        float x[16], th[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = s[i];
+        float cf = sc.c_scale;
+        if constexpr (MOD) {
+          modify<16, true>(a, sc, x, th, k0 + 32 * kt + 4 * h - w.p, 1, w.slope, bias.table, bias.bucket, far);
+          cf = 1.f;
+        }
+        if (need_mask) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = 32 * kt + acc_row(i, h);
+            bool see = k0 + j < w.hi;
+            if (mixed) see = see && sDoc[j] == w.doc;
+            if (!see) x[i] = -INFINITY;
+          }
+        }
+        float su = 0.f, sp = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = ex2(fmaf(x[i], cf, -st.x));
+          x[i] = p * (dp[i] - st.y);
+          if (MOD) su += x[i], sp += p;
+        }
+        if (MOD && a.rel_bias) {
+          all_u += su;
+          if (far != 0) {
+            far_u[far > 0] += su;
+            far_p[far > 0] += sp;
+          }
+        }
+        if (MOD && sc.capped) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] *= fmaf(-th[i], th[i], 1.f);
+        }
+        if (sizeof(T) == 2 && Elem<T>::PSHIFT != 0.f) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] *= dscale;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const V8 ds = round8<T>(x + 8 * c);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) acc[d] = Elem<T>::mma(col_frag<T, D>(sK, 32 * kt + 16 * c, d, lane), ds, acc[d]);
+        }
+      }
+    }
+    t = tn;
+    buf ^= 1;
+  }
+  if (MOD && a.rel_bias) {
+    // the sum of dU over a row is dlse (0 without it) by definition: what is left is what the rounding of o has put into delta
+    all_u = half_sum(all_u) - (g.dlse && w.live ? g.dlse[r] : 0.f);
+    if (w.valid && h == 0) g.delta_fix[r] = st.y + (w.live ? all_u : 0.f);
+    if (!w.live) all_u = 0.f;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) far_u[s] = wave_sum(w.live ? far_u[s] - all_u * far_p[s] : 0.f);
+    __syncthreads();
+    float *sF = (float *)sB;
+    if (lane == 0) sF[2 * wave] = far_u[0], sF[2 * wave + 1] = far_u[1];
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      float v = 0.f;
+      for (int u = 0; u < WAVES; ++u) v += sF[2 * u + threadIdx.x];
+      // item order (b, qt, head) for the reduction, whatever order the workgroups ran in
+      g.far_part[(((int64_t)b * g.nqt + qt) * a.H + head) * 2 + threadIdx.x] = v;
+    }
+  }
+  if (!w.valid) return;
+  T *o = (T *)g.dq + (((int64_t)b * a.Lq + w.i) * a.H + head) * a.dh;
+  const float f = a.scale / dscale;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int dim = 32 * d + 8 * q + 4 * h;
+      if (dim < a.dh) {
+        typename Elem<T>::V4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(w.live ? acc[d][4 * q + e] * f : 0.f);
+        *(typename Elem<T>::V4 *)(o + dim) = v;
+      }
+    }
+}
+
+// dK, dV.  A wave owns 32 keys (the accumulator's columns; their rows of K and V stay in registers as operands), the queries of the
+// heads that share the key head go by in LDS tiles, as rows for S and dP and transposed for dV^T += dO^T P and dK^T += Q^T dS.
+// With few key tiles the query heads and the queries are dealt over zh x zq parts, which a second kernel adds up in order.
+// K, V, dK and dV of 32 keys take 192 registers at a head size of 128: one wave per SIMD there, its 512 registers against the latency.
+template <typename T, int D, bool MOD>
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt_long_attn_dkv_kernel(const Args g) {
+  typedef Tile<T, D> L;
+  typedef typename Elem<T>::V8 V8;
+  constexpr int BQ = L::BK, NQ = BQ / 32, NC = D / 16, ND = D / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const mmt_long_attention &a = g.a;
+  float2 *sStat2 = (float2 *)(smem + 4 * L::BYTES);       // [2][BQ]
+  int *sDoc2 = (int *)(sStat2 + 2 * BQ), *sB = sDoc2 + 2 * BQ;
+  BiasLds bias;
+  bias.table = (float *)(sB + 6 * WAVES);
+  const int grp = blockIdx.x % g.groups;
+  int n = blockIdx.x / g.groups;
+  const int z = n % (g.zh * g.zq), zh = z % g.zh, zq = z / g.zh;
+  const int kt = n / (g.zh * g.zq);                       // causal: the first keys are seen by the most queries
+  const int kh = grp % a.Hk, b = grp / a.Hk, head0 = kh * g.G;
+  const int g_per = (g.G + g.zh - 1) / g.zh, g0 = zh * g_per, g1 = min(g.G, g0 + g_per);
+  bias.bucket = (unsigned char *)(bias.table + (MOD && a.rel_bias ? g.G * a.n_buckets : 0));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+  const int len = row_len(a, b), off = len - a.Lq, prefix = a.prefix ? a.prefix[b] : 0;
+  const int j = kt * ROWS + wave * 32 + col;
+  const int kdoc = a.k_doc && j < a.Lk ? a.k_doc[(int64_t)b * a.Lk + j] : 0;
+  const bool live = j < len && kdoc >= 0;
+  const int j_lo = kt * ROWS + wave * 32;                 // first key of the wave
+  const int d_min = wave_min(live ? kdoc : 0x7fffffff), d_max = wave_max(live ? kdoc : -1);
+  const bool all_live = __all(live);
+  if (lane == 0) sB[2 * wave] = d_min, sB[2 * wave + 1] = d_max;
+  __syncthreads();
+  int gd_min = 0x7fffffff, gd_max = -1;
+  for (int v = 0; v < WAVES; ++v) gd_min = min(gd_min, sB[2 * v]), gd_max = max(gd_max, sB[2 * v + 1]);
+  gd_min = __builtin_amdgcn_readfirstlane(gd_min), gd_max = __builtin_amdgcn_readfirstlane(gd_max);
+  if (MOD && a.rel_bias) bias.fill(a, head0, g.G);
+
+  const T *krow = (const T *)a.k + (int64_t)b * a.k_bs + (int64_t)min(j, a.Lk - 1) * a.k_rs + (int64_t)kh * a.k_hs;
+  const T *vrow = (const T *)a.v + (int64_t)b * a.v_bs + (int64_t)min(j, a.Lk - 1) * a.v_rs + (int64_t)kh * a.v_hs;
+  V8 fk[NC], fv[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    fk[c] = mem_frag<T>(krow, c, h, a.dh, live);
+    fv[c] = mem_frag<T>(vrow, c, h, a.dh, live);
+  }
+  f32x16 acck[ND], accv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acck[d] = f32x16{}, accv[d] = f32x16{};
+  const ScoreCtx sc = score_ctx(a);
+  // fp16: P is rounded times 2^PSHIFT; the surplus is taken out of dS again together with its own scaling
+  const float dscale = sizeof(T) == 2 && g.dscale ? g.dscale[0] : 1.f;
+  const float ds_mul = dscale * ex2(-Elem<T>::PSHIFT);
+
+  // queries that may see a key of this workgroup: position >= its first key, unless the prefix reaches into it
+  const int i_first = a.causal && prefix <= kt * ROWS ? max(0, kt * ROWS - off) : 0;
+  const int all0 = min(i_first, a.Lq) / BQ, all1 = kt * ROWS < len ? (a.Lq + BQ - 1) / BQ : 0;
+  const int t_per = (max(0, all1 - all0) + g.zq - 1) / g.zq, t0 = all0 + zq * t_per, t1 = min(all1, t0 + t_per);
+  const DocRange *rng = g.qrng ? g.qrng + (int64_t)b * ((a.Lq + BQ - 1) / BQ) : nullptr;
+  const int *qdoc = a.q_doc ? a.q_doc + (int64_t)b * a.Lq : nullptr;
+  const unsigned lds = lds_address(smem);
+  Dma<T, D> dmq, dmo;
+  dmq.init((const T *)a.q + (int64_t)b * a.q_bs + (int64_t)head0 * a.q_hs, a.q_rs, a.Lq, a.dh);
+  dmo.init((const T *)g.dout + (int64_t)b * g.do_bs + (int64_t)head0 * g.do_hs, g.do_rs, a.Lq, a.dh);
+  const char *qbase = dmq.base, *obase = dmo.base;
+
+  // the tiles of all heads as one sequence, so that the next head's first tile is on its way during this head's last
+  TileIter it;
+  int gi = g0 - 1, t = -1, buf = 0;
+  const float2 *stat = nullptr;
+  float2 st_next = make_float2(INFINITY, 0.f);
+  int doc_next = -1;
+  auto advance = [&]() {                                  // next tile, over head ends; -1 at the end
+    int n = gi < g0 ? -1 : it.next();
+    while (n < 0 && ++gi < g1) {
+      stat = g.stat + ((int64_t)b * a.H + head0 + gi) * a.Lq;
+      dmq.base = qbase + (int64_t)gi * a.q_hs * (int64_t)sizeof(T);
+      dmo.base = obase + (int64_t)gi * g.do_hs * (int64_t)sizeof(T);
+      it.start(rng, gd_min, gd_max, t0, t1);
+      n = it.next();
+    }
+    return n;
+  };
+  auto fetch = [&](int tile, int to) {
+    dmq.load(lds + to * 2 * L::BYTES, tile * BQ);
+    dmo.load(lds + to * 2 * L::BYTES + L::BYTES, tile * BQ);
+    if (threadIdx.x < BQ) {
+      const int i = tile * BQ + threadIdx.x;
+      doc_next = i < a.Lq ? (qdoc ? qdoc[i] : 0) : -1;
+      st_next = doc_next >= 0 ? stat[i] : make_float2(INFINITY, 0.f);
+    }
+  };
+  t = advance();
+  if (t >= 0) fetch(t, 0);
+  while (t >= 0) {
+    const int q0 = t * BQ, head = head0 + gi;
+    char *sQ = smem + buf * 2 * L::BYTES, *sO = sQ + L::BYTES;
+    float2 *sStat = sStat2 + buf * BQ;
+    int *sDoc = sDoc2 + buf * BQ;
+    const bool mixed = it.mixed(), dead = it.cur_dead != 0;
+    const int cur_gi = gi;
+    if (threadIdx.x < BQ) {
+      sDoc[threadIdx.x] = doc_next;
+      sStat[threadIdx.x] = st_next;
+    }
+    dma_wait();
+    __syncthreads();
+    if (q0 + BQ > a.Lq || dead) {
+      zero_rows<T, D>(sQ, a.Lq - q0, sDoc);
+      zero_rows<T, D>(sO, a.Lq - q0, sDoc);
+      __syncthreads();
+    }
+    const int tn = advance();
+    if (tn >= 0) fetch(tn, buf ^ 1);
+    const int p0 = off + q0;
+    // the last row of the tile sees the most
+    if (!a.causal || max(p0 + BQ, prefix) > j_lo) {
+      const bool need_mask = mixed || !all_live || (a.causal && max(p0 + 1, prefix) < j_lo + 32);
+      const float slope = MOD && a.slopes ? a.slopes[head] * LOG2E : 0.f;
+      const float *tab = bias.table + cur_gi * a.n_buckets;
+#pragma unroll
+      for (int qt = 0; qt < NQ; ++qt) {
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          s = Elem<T>::mma(row_frag<T, D>(sQ, 32 * qt + col, c, h), fk[c], s);
+          dp = Elem<T>::mma(row_frag<T, D>(sO, 32 * qt + col, c, h), fv[c], dp);
+        }
+        float x[16], th[16], p[16];
+        float cf = sc.c_scale;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = s[i];
+        if constexpr (MOD) {
+          const int pq = p0 + 32 * qt;
+          const int far = !a.rel_bias ? 0 : j_lo + 31 - pq <= -a.reach ? -1 : j_lo - (pq + 31) >= a.reach ? 1 : 0;
+          modify<16, true>(a, sc, x, th, j - pq - 4 * h, -1, slope, tab, bias.bucket, far);
+          cf = 1.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int row = 32 * qt + acc_row(i, h);
+          const float2 st = sStat[row];
+          p[i] = ex2(fmaf(x[i], cf, Elem<T>::PSHIFT - st.x));
+          if (need_mask) {
+            bool see = live && (!a.causal || j < max(p0 + row + 1, prefix));
+            if (mixed) see = see && sDoc[row] == kdoc;
+            if (!see) p[i] = 0.f;
+          }
+          x[i] = p[i] * (dp[i] - st.y);
+        }
+        if (MOD && sc.capped) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] *= fmaf(-th[i], th[i], 1.f);
+        }
+        if (sizeof(T) == 2 && Elem<T>::PSHIFT != 0.f) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] *= ds_mul;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const V8 fp = round8<T>(p + 8 * c), fs = round8<T>(x + 8 * c);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            accv[d] = Elem<T>::mma(col_frag<T, D>(sO, 32 * qt + 16 * c, d, lane), fp, accv[d]);
+            acck[d] = Elem<T>::mma(col_frag<T, D>(sQ, 32 * qt + 16 * c, d, lane), fs, acck[d]);
+          }
+        }
+      }
+    }
+    t = tn;
+    buf ^= 1;
+  }
+  if (j >= a.Lk) return;
+  const int64_t o = (((int64_t)b * a.Lk + j) * a.Hk + kh) * a.dh, part = (int64_t)a.B * a.Lk * a.Hk * a.dh * z;
+  const float f_k = a.scale / dscale, f_v = ex2(-Elem<T>::PSHIFT);
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int dim = 32 * d + 8 * q + 4 * h;
+      if (dim >= a.dh) continue;
+      f32x4 vk, vv;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        vk[e] = live ? acck[d][4 * q + e] * f_k : 0.f;
+        vv[e] = live ? accv[d][4 * q + e] * f_v : 0.f;
+      }
+      if (g.part_dk) {
+        *(f32x4 *)(g.part_dk + part + o + dim) = vk;
+        *(f32x4 *)(g.part_dv + part + o + dim) = vv;
+      } else {
+        *(typename Elem<T>::V4 *)((T *)g.dk + o + dim) = __builtin_convertvector(vk, typename Elem<T>::V4);
+        *(typename Elem<T>::V4 *)((T *)g.dv + o + dim) = __builtin_convertvector(vv, typename Elem<T>::V4);
+      }
+    }
+}
+
+// the parts of dK and dV, in order
+template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_dkv_sum_kernel(const Args g) {
+  const int64_t n = (int64_t)g.a.B * g.a.Lk * g.a.Hk * g.a.dh, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 k = {}, v = {};
+  for (int z = 0; z < g.zh * g.zq; ++z) {
+    k += *(const f32x4 *)(g.part_dk + n * z + i);
+    v += *(const f32x4 *)(g.part_dv + n * z + i);
+  }
+  *(typename Elem<T>::V4 *)((T *)g.dk + i) = __builtin_convertvector(k, typename Elem<T>::V4);
+  *(typename Elem<T>::V4 *)((T *)g.dv + i) = __builtin_convertvector(v, typename Elem<T>::V4);
+}
+
+// The gradient of the learned bias over the tiles within the reach (the dQ kernel has summed the others).  Sums of millions of
+// signed terms that have to come out right to fp32: dU is recomputed with the exact delta of each row, and every lane adds into
+// a column of its own of a [bucket][lane] array in LDS, so that the order of the additions is the program's.
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1) mmt_long_attn_table_kernel(const Args g, float *part) {
+  typedef Tile<T, D> L;
+  typedef typename Elem<T>::V8 V8;
+  constexpr int BK = L::BK, NK = BK / 32, NC = D / 16;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const mmt_long_attention &a = g.a;
+  char *sK = smem, *sV = smem + L::BYTES;
+  int *sDoc = (int *)(smem + 2 * L::BYTES), *sB = sDoc + BK;
+  BiasLds bias;
+  bias.table = (float *)(sB + 6 * WAVES);
+  bias.bucket = (unsigned char *)(bias.table + a.n_buckets);
+  float *hist = (float *)(bias.bucket + ((2 * a.reach + 1 + 15) & ~15));
+  const int grp = blockIdx.x % g.groups, n = blockIdx.x / g.groups, gi = n % g.G, qt = n / g.G;
+  const int kh = grp % a.Hk, b = grp / a.Hk, head = kh * g.G + gi;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+  const int len = row_len(a, b);
+  const Row w = make_row(g, b, head, qt * ROWS + wave * 32 + col, len);
+  const Bounds wb = wave_bounds(w);
+  const Bounds gb = group_bounds(wb, sB, wave);
+  bias.fill(a, head, 1);
+  float *mine = hist + (int64_t)wave * a.n_buckets * 64 + lane;
+  for (int k = 0; k < a.n_buckets; ++k) mine[k * 64] = 0.f;
+  const int64_t r = ((int64_t)b * a.H + head) * a.Lq + min(w.i, a.Lq - 1);
+  const float lse2 = w.live ? g.stat[r].x : INFINITY, delta = w.live ? g.delta_fix[r] : 0.f;
+  const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)head * a.q_hs;
+  const T *drow = (const T *)g.dout + (int64_t)b * g.do_bs + (int64_t)min(w.i, a.Lq - 1) * g.do_rs + (int64_t)head * g.do_hs;
+  V8 fq[NC], fd[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
+    fd[c] = mem_frag<T>(drow, c, h, a.dh, w.live);
+  }
+  const ScoreCtx sc = score_ctx(a);
+  const int tiles = (gb.hi_max + BK - 1) / BK;
+  const DocRange *rng = g.krng ? g.krng + (int64_t)b * g.nkt : nullptr;
+  const unsigned lds = lds_address(smem);
+  Dma<T, D> dk, dv;
+  dk.init((const T *)a.k + (int64_t)b * a.k_bs + (int64_t)kh * a.k_hs, a.k_rs, a.Lk, a.dh);
+  dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
+  const int *kdoc = a.k_doc ? a.k_doc + (int64_t)b * a.Lk : nullptr;
+  // tiles with k0 + BK - 1 - p_min > -reach and k0 - p_max < reach
+  int t0 = 0, t1 = 0;
+  if (gb.hi_max > 0) {
+    t0 = max(0, (gb.p_min - a.reach - BK + 1) / BK);
+    while (t0 < tiles && t0 * BK + BK - 1 - gb.p_min <= -a.reach) ++t0;
+    t1 = min(tiles, max(0, gb.p_max + a.reach + BK) / BK + 1);
+    while (t1 > t0 && (t1 - 1) * BK - gb.p_max >= a.reach) --t1;
+  }
+  for (int t = t0; t < t1; ++t) {
+    if (rng && (rng[t].lo > gb.d_max || rng[t].hi < gb.d_min)) continue;
+    const int k0 = t * BK;
+    __syncthreads();
+    dk.load(lds, k0);
+    dv.load(lds + L::BYTES, k0);
+    if (kdoc && threadIdx.x < BK) sDoc[threadIdx.x] = k0 + (int)threadIdx.x < a.Lk ? kdoc[k0 + threadIdx.x] : -1;
+    dma_wait();
+    __syncthreads();
+    if (k0 + BK > len || kdoc) {
+      zero_rows<T, D>(sK, len - k0, kdoc ? sDoc : nullptr);
+      zero_rows<T, D>(sV, len - k0, kdoc ? sDoc : nullptr);
+      __syncthreads();
+    }
+    if (k0 >= wb.hi_max) continue;
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s);
+        dp = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp);
+      }
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = s[i];
+      modify<16, false>(a, sc, x, nullptr, k0 + 32 * kt + 4 * h - w.p, 1, w.slope, bias.table, bias.bucket, 0);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int j = 32 * kt + acc_row(i, h);
+        bool see = k0 + j < w.hi;
+        if (kdoc) see = see && sDoc[j] == w.doc;
+        if (!see) x[i] = -INFINITY;
+      }
+      const int d0 = k0 + 32 * kt + 4 * h - w.p;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = ex2(x[i] - lse2), u = p * (dp[i] - delta);
+        const int d = max(-a.reach, min(a.reach, d0 + 8 * (i >> 2) + (i & 3))) + a.reach;
+        mine[bias.bucket[d] * 64] += u;
+      }
+    }
+  }
+  __syncthreads();
+  // columns -> one value per bucket, in a fixed order: wave u takes buckets u, u + 4, ..
+  for (int k = wave; k < a.n_buckets; k += WAVES) {
+    float v = 0.f;
+    for (int u = 0; u < WAVES; ++u) v += hist[((int64_t)u * a.n_buckets + k) * 64 + lane];
+    v = wave_sum(v);
+    if (lane == 0) part[(((int64_t)b * g.nqt + qt) * a.H + head) * a.n_buckets + k] = v;
+  }
+}
+
+// the parts of all (batch row, query tile) pairs, in 64 bits and in order; one wave per (head, bucket)
+template <typename T> __global__ void mmt_long_attn_table_sum_kernel(const mmt_long_attention a, int64_t n, const float *part, const float *far_part, float *dtable) {
+  const int hd = blockIdx.x / a.n_buckets, k = blockIdx.x % a.n_buckets, lane = threadIdx.x;
+  const int left = max(0, min(a.rel_buckets[0], a.n_buckets - 1)), right = max(0, min(a.rel_buckets[2 * a.reach], a.n_buckets - 1));
+  double v = 0.;
+  for (int64_t i = lane; i < n; i += 64) {
+    v += part[(i * a.H + hd) * a.n_buckets + k];
+    if (k == left) v += far_part[(i * a.H + hd) * 2];
+    if (k == right) v += far_part[(i * a.H + hd) * 2 + 1];
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  if (lane == 0) dtable[(int64_t)hd * a.n_buckets + k] = (float)v;
+}
+
+// --------------------------------------------------------------------------------------------------------------- launchers
+template <typename K> static void launch(K kernel, int64_t grid, size_t lds, hipStream_t st, const Args &g) {
+  if (lds > 65536) (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(THREADS), lds, st, g);
+}
+
+static inline bool modified(const mmt_long_attention &a) { return a.softcap > 0.f || a.slopes || a.rel_bias; }
+
+template <typename T, int D> static void fwd_size(const Args &g, hipStream_t st) {
+  const size_t lds = 4 * Tile<T, D>::BYTES + 4 * Tile<T, D>::BK + 24 * WAVES + bias_lds_bytes(g.a, g.pack);
+  if (modified(g.a)) launch(mmt_long_attn_fwd_kernel<T, D, true>, g.items, lds, st, g);
+  else launch(mmt_long_attn_fwd_kernel<T, D, false>, g.items, lds, st, g);
+}
+
+template <typename T, int D> static void bwd_size(Args &g, hipStream_t st, float *table_part, float *dtable) {
+  typedef Tile<T, D> L;
+  const mmt_long_attention &a = g.a;
+  const bool mod = modified(a);
+  const size_t small = 24 * WAVES;
+  const int64_t qitems = (int64_t)a.B * a.H * g.nqt;
+  const size_t lds_q = 4 * L::BYTES + 4 * L::BK + small + bias_lds_bytes(a, 1);
+  if (mod) launch(mmt_long_attn_dq_kernel<T, D, true>, qitems, lds_q, st, g);
+  else launch(mmt_long_attn_dq_kernel<T, D, false>, qitems, lds_q, st, g);
+  if (a.rel_bias) {
+    const size_t lds = 2 * L::BYTES + 4 * L::BK + small + bias_lds_bytes(a, 1) + (size_t)WAVES * a.n_buckets * 256;
+    (void)hipFuncSetAttribute((const void *)mmt_long_attn_table_kernel<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    hipLaunchKernelGGL((mmt_long_attn_table_kernel<T, D>), dim3((unsigned)qitems), dim3(THREADS), lds, st, g, table_part);
+    hipLaunchKernelGGL(mmt_long_attn_table_sum_kernel<T>, dim3(a.H * a.n_buckets), dim3(64), 0, st, a, (int64_t)a.B * g.nqt, table_part,
+                       g.far_part, dtable);
+  }
+  const size_t lds_k = 4 * L::BYTES + 24 * L::BK + small + bias_lds_bytes(a, g.G);
+  const int64_t kitems = (int64_t)g.groups * ((a.Lk + ROWS - 1) / ROWS) * g.zh * g.zq;
+  if (mod) launch(mmt_long_attn_dkv_kernel<T, D, true>, kitems, lds_k, st, g);
+  else launch(mmt_long_attn_dkv_kernel<T, D, false>, kitems, lds_k, st, g);
+}
+
+template <typename T> static void docs(const Args &g, DocRange *out, bool queries, hipStream_t st) {
+  const int bk = Elem<T>::BK, nk = g.a.B * g.nkt, total = nk + (queries ? g.a.B * ((g.a.Lq + bk - 1) / bk) : 0);
+  hipLaunchKernelGGL(mmt_long_attn_docs_kernel<T>, dim3((total + 3) / 4), dim3(256), 0, st, g, bk, nk, total, out);
+}
+
+template <typename T> void forward(Args &g, DocRange *ranges, hipStream_t st) {
+  const mmt_long_attention &a = g.a;
+  if (ranges) docs<T>(g, ranges, false, st), g.krng = ranges;
+  if (a.dh <= 32) fwd_size<T, 32>(g, st);
+  else if (a.dh <= 64) fwd_size<T, 64>(g, st);
+  else if (a.dh <= 96) fwd_size<T, 96>(g, st);
+  else fwd_size<T, 128>(g, st);
+  if (g.nsplit > 1) {
+    const int64_t rows = (int64_t)a.B * a.H * a.Lq;
+    hipLaunchKernelGGL(mmt_long_attn_join_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, g);
+  }
+}
+
+template <typename T> void backward(Args &g, DocRange *ranges, float2 *stat, f32x4 *maxima, float *table_part, float *dtable, hipStream_t st) {
+  const mmt_long_attention &a = g.a;
+  if (ranges) docs<T>(g, ranges, true, st), g.krng = ranges, g.qrng = ranges + (int64_t)a.B * g.nkt;
+  const int64_t rows = (int64_t)a.B * a.Lq * a.H, blocks = (rows + 15) / 16;
+  const int parts = (int)(blocks < (maxima ? STAT_PARTS : 8192) ? blocks : (maxima ? STAT_PARTS : 8192));
+  hipLaunchKernelGGL(mmt_long_attn_stat_kernel<T>, dim3(parts), dim3(256), 0, st, g, stat, maxima);
+  if (maxima) {
+    g.dscale = (float *)(maxima + STAT_PARTS);
+    hipLaunchKernelGGL(mmt_long_attn_dscale_kernel<T>, dim3(1), dim3(64), 0, st, maxima, parts, (float *)(maxima + STAT_PARTS));
+  }
+  if (a.dh <= 32) bwd_size<T, 32>(g, st, table_part, dtable);
+  else if (a.dh <= 64) bwd_size<T, 64>(g, st, table_part, dtable);
+  else if (a.dh <= 96) bwd_size<T, 96>(g, st, table_part, dtable);
+  else bwd_size<T, 128>(g, st, table_part, dtable);
+  if (g.part_dk) {
+    const int64_t n = (int64_t)a.B * a.Lk * a.Hk * a.dh;
+    hipLaunchKernelGGL(mmt_long_attn_dkv_sum_kernel<T>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, g);
+  }
+}
+
+}  // namespace la

@@ -783,7 +783,7 @@ def _head_rows(t, name, shape=None, like=None):
     if like is not None and t.device != like.device:
         raise MmtError(f"{name}: tensor is on {t.device}, expected {like.device}")
     unit = 16 // t.element_size()
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(t.stride(i) % unit for i in range(3) if t.shape[i] > 1) or \
+    if t.stride(3) != 1 or t.stride(1) >= 1 << 24 or t.data_ptr() % 16 or any(t.stride(i) % unit for i in range(3) if t.shape[i] > 1) or \
             any(t.stride(i) < 0 for i in range(3)):
         t = t.contiguous()
         if t.data_ptr() % 16:          # contiguous all along, but cut out of a larger buffer at an odd place
@@ -935,29 +935,36 @@ def _attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softca
 
 
 def long_attention(q, k, v, scale=None, causal=False, prefix=None, q_doc=None, k_doc=None, kv_len=None, softcap=0.0, slopes=None,
-                   rel_bias=None, rel_buckets=None):
+                   rel_bias=None, rel_buckets=None, keep_low=False):
     """Attention of q (B,Lq,H,dh) over k, v (B,Lk,Hk,dh) of any length (``mmt_long_attention_fwd``; the header states the formula,
-    the masks and the limits) -> out (B,Lq,H,dh), lse (B,H,Lq) fp32.  Queries are the last Lq of ``kv_len[b]`` (or Lk) tokens."""
+    the masks and the limits) -> out (B,Lq,H,dh), lse (B,H,Lq) fp32 and, with
+    ``keep_low``, what rounding took from out (for the backward; None in fp32).  Queries are the last Lq of ``kv_len[b]`` (or Lk)
+    tokens."""
     a, q, k, v = _attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets)
     with torch.cuda.device(q.device):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        low = torch.empty_like(out) if keep_low and q.dtype != torch.float32 else None
         lse = torch.empty((a.B, a.H, a.Lq), dtype=torch.float32, device=q.device)
-        if not a.B * a.Lq:
-            return out, lse
         if not a.Lk:
-            return out.zero_(), lse.fill_(float("-inf"))
-        lib = _lib.load()
-        ws = _workspace(lib.mmt_long_attention_workspace_bytes(C.byref(a), 0), q.device)
-        _lib.check(lib.mmt_long_attention_fwd(C.byref(a), _ptr(out), _ptr(lse), _ptr(ws), ws.numel(), _stream()), "mmt_long_attention_fwd")
-    return out, lse
+            out.zero_(), lse.fill_(float("-inf"))
+            if low is not None:
+                low.zero_()
+        elif a.B * a.Lq:
+            lib = _lib.load()
+            ws = _workspace(lib.mmt_long_attention_workspace_bytes(C.byref(a), 0), q.device)
+            _lib.check(lib.mmt_long_attention_fwd(C.byref(a), _ptr(out), _ptr(low), _ptr(lse), _ptr(ws), ws.numel(), _stream()),
+                       "mmt_long_attention_fwd")
+    return (out, lse, low) if keep_low else (out, lse)
 
 
-def long_attention_backward(dout, dlse, out, lse, q, k, v, scale=None, causal=False, prefix=None, q_doc=None, k_doc=None, kv_len=None,
+def long_attention_backward(dout, dlse, out, lse, low, q, k, v, scale=None, causal=False, prefix=None, q_doc=None, k_doc=None, kv_len=None,
                             softcap=0.0, slopes=None, rel_bias=None, rel_buckets=None):
-    """Gradients of q, k, v and rel_bias (None without it) from those of ``long_attention``'s out and lse (``dlse`` may be None)."""
+    """Gradients of q, k, v and rel_bias (None without it) from those of ``long_attention``'s out and lse (``dlse`` may be None);
+    ``low`` is the forward's, or None."""
     a, q, k, v = _attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets)
     dout = _head_rows(dout, "dout", q.shape, q)
     out = _head_rows(out, "out", q.shape, q).contiguous()
+    low = _head_rows(low, "low", q.shape, q).contiguous() if low is not None else None
     _side(lse, "lse", (a.B, a.H, a.Lq), torch.float32, q)
     if dlse is not None:
         dlse = _side(dlse.contiguous(), "dlse", (a.B, a.H, a.Lq), torch.float32, q)
@@ -973,6 +980,6 @@ def long_attention_backward(dout, dlse, out, lse, q, k, v, scale=None, causal=Fa
             return dq, dk, dv, dbias
         lib = _lib.load()
         ws = _workspace(lib.mmt_long_attention_workspace_bytes(C.byref(a), 1), q.device)
-        _lib.check(lib.mmt_long_attention_bwd(C.byref(a), _ptr(out), _ptr(lse), _ptr(dout), *_strides(dout), _ptr(dlse), _ptr(dq), _ptr(dk),
+        _lib.check(lib.mmt_long_attention_bwd(C.byref(a), _ptr(out), _ptr(low), _ptr(lse), _ptr(dout), *_strides(dout), _ptr(dlse), _ptr(dq), _ptr(dk),
                                               _ptr(dv), _ptr(dbias), _ptr(ws), ws.numel(), _stream()), "mmt_long_attention_bwd")
     return dq, dk, dv, dbias

@@ -46,8 +46,8 @@ _lib.define("ade_fde(Tensor pred, Tensor gt) -> (Tensor, Tensor)")
 _ATTN = ("float? scale, bool causal, Tensor? prefix, Tensor? q_doc, Tensor? k_doc, Tensor? kv_len, float softcap, Tensor? slopes, "
          "Tensor? rel_bias, Tensor? rel_buckets")
 _ROPE = "Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor inv_freq, Tensor? positions, float eps, bool interleaved"
-_lib.define(f"long_attention(Tensor q, Tensor k, Tensor v, {_ATTN}) -> (Tensor, Tensor)")
-_lib.define(f"long_attention_bwd(Tensor dout, Tensor? dlse, Tensor out, Tensor lse, Tensor q, Tensor k, Tensor v, {_ATTN}) "
+_lib.define(f"long_attention(Tensor q, Tensor k, Tensor v, {_ATTN}) -> (Tensor out, Tensor lse, Tensor low)")
+_lib.define(f"long_attention_bwd(Tensor dout, Tensor? dlse, Tensor out, Tensor lse, Tensor? low, Tensor q, Tensor k, Tensor v, {_ATTN}) "
             "-> (Tensor, Tensor, Tensor, Tensor)")
 _lib.define(f"qk_norm_rope({_ROPE}) -> (Tensor, Tensor)")
 _lib.define(f"qk_norm_rope_bwd(Tensor dq_out, Tensor dk_out, {_ROPE}) -> (Tensor, Tensor, Tensor, Tensor)")
@@ -109,6 +109,11 @@ def _ade_fde(pred, gt):
 
 
 # ---- attention over long rows, norm + rotation: differentiable ------------------------------------------------------------------
+def _long_attention(*args):
+    out, lse, low = ops.long_attention(*args, keep_low=True)
+    return out, lse, low if low is not None else out.new_empty(0)
+
+
 def _long_attention_bwd(*args):
     dq, dk, dv, dbias = ops.long_attention_backward(*args)
     return dq, dk, dv, dbias if dbias is not None else dq.new_empty(0, dtype=torch.float32)
@@ -116,10 +121,10 @@ def _long_attention_bwd(*args):
 
 def _long_attention_meta(q, k, v, *rest):
     B, Lq, H, _ = q.shape
-    return q.new_empty(q.shape), q.new_empty((B, H, Lq), dtype=torch.float32)
+    return q.new_empty(q.shape), q.new_empty((B, H, Lq), dtype=torch.float32), q.new_empty(q.shape if q.dtype != torch.float32 else 0)
 
 
-def _long_attention_bwd_meta(dout, dlse, out, lse, q, k, v, *rest):
+def _long_attention_bwd_meta(dout, dlse, out, lse, low, q, k, v, *rest):
     table = rest[-2]
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), \
         q.new_empty(table.shape if table is not None else 0, dtype=torch.float32)
@@ -134,7 +139,7 @@ def _qk_norm_rope_bwd_meta(dqo, dko, q, k, q_weight, k_weight, *rest):
 
 
 for _name, _fn, _meta in (
-        ("long_attention", ops.long_attention, _long_attention_meta),
+        ("long_attention", _long_attention, _long_attention_meta),
         ("long_attention_bwd", _long_attention_bwd, _long_attention_bwd_meta),
         ("qk_norm_rope", ops.qk_norm_rope, _qk_norm_rope_meta),
         ("qk_norm_rope_bwd", ops.qk_norm_rope_backward, _qk_norm_rope_bwd_meta),
@@ -150,39 +155,75 @@ for _name, _fn, _meta in (
     _lib.impl(_name, _meta, "Meta")
 
 
-def _long_attention_ctx(ctx, inputs, output):
-    q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets = inputs
-    if slopes is not None and slopes.requires_grad:
-        raise MmtError("long_attention: the slopes of the distance bias are constants, they get no gradient")
-    ctx.set_materialize_grads(False)
-    ctx.save_for_backward(q, k, v, *output, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets)
-    ctx.plain = scale, causal, softcap
+class _LongAttention(torch.autograd.Function):
+    """Differentiable in q, k, v and rel_bias; the arguments of ``mmt::long_attention`` in order."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets):
+        _constant(slopes, "long_attention: the slopes of the distance bias")
+        out, lse, low = ops.long_attention(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets,
+                                           keep_low=True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(out, lse, low, q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets)
+        ctx.plain = scale, causal, softcap
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dlse):
+        return _long_attention_grads(ctx, dout, dlse, ops.long_attention_backward)
 
 
-def _long_attention_grad(ctx, dout, dlse):
-    q, k, v, out, lse, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets = ctx.saved_tensors
+def _constant(t, what):
+    if t is not None and t.requires_grad:
+        raise MmtError(f"{what} are constants, they get no gradient")
+
+
+def _long_attention_grads(ctx, dout, dlse, bwd):
+    out, lse, low, q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets = ctx.saved_tensors
     scale, causal, softcap = ctx.plain
     if dout is None and dlse is None:
         return (None,) * 13
     if dout is None:
         dout = torch.zeros_like(out)
-    dq, dk, dv, dbias = torch.ops.mmt.long_attention_bwd(dout, dlse, out, lse, q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len,
-                                                         softcap, slopes, rel_bias, rel_buckets)
+    dq, dk, dv, dbias = bwd(dout, dlse, out, lse, low, q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias,
+                            rel_buckets)
     return (dq, dk, dv) + (None,) * 8 + (dbias if rel_bias is not None else None, None)
+
+
+class _QkNormRope(torch.autograd.Function):
+    """Differentiable in q, k and the weights; the arguments of ``mmt::qk_norm_rope`` in order."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved):
+        _constant(inv_freq, "qk_norm_rope: the frequencies")
+        ctx.save_for_backward(q, k, q_weight, k_weight, inv_freq, positions)
+        ctx.plain = eps, interleaved
+        return ops.qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dqo, dko):
+        return ops.qk_norm_rope_backward(dqo, dko, *ctx.saved_tensors, *ctx.plain) + (None,) * 4
+
+
+# The same through the dispatcher, for callers of torch.ops.mmt.* and for tracing
+def _long_attention_ctx(ctx, inputs, output):
+    q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets = inputs
+    _constant(slopes, "long_attention: the slopes of the distance bias")
+    out, lse, low = output
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(low)
+    ctx.save_for_backward(out, lse, low if low.numel() == out.numel() else None, q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias,
+                          rel_buckets)
+    ctx.plain = scale, causal, softcap
 
 
 def _qk_norm_rope_ctx(ctx, inputs, output):
     q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved = inputs
-    if inv_freq.requires_grad:
-        raise MmtError("qk_norm_rope: the frequencies are constants, they get no gradient")
+    _constant(inv_freq, "qk_norm_rope: the frequencies")
     ctx.save_for_backward(q, k, q_weight, k_weight, inv_freq, positions)
     ctx.plain = eps, interleaved
-
-
-def _qk_norm_rope_grad(ctx, dqo, dko):
-    q, k, q_weight, k_weight, inv_freq, positions = ctx.saved_tensors
-    grads = torch.ops.mmt.qk_norm_rope_bwd(dqo, dko, q, k, q_weight, k_weight, inv_freq, positions, *ctx.plain)
-    return tuple(grads) + (None,) * 4
 
 
 def _no_second(name):
@@ -191,10 +232,18 @@ def _no_second(name):
     return refuse
 
 
-torch.library.register_autograd("mmt::long_attention", _long_attention_grad, setup_context=_long_attention_ctx, lib=_lib)
-torch.library.register_autograd("mmt::qk_norm_rope", _qk_norm_rope_grad, setup_context=_qk_norm_rope_ctx, lib=_lib)
+torch.library.register_autograd("mmt::long_attention", lambda ctx, dout, dlse, _: _long_attention_grads(
+    ctx, dout, dlse, torch.ops.mmt.long_attention_bwd), setup_context=_long_attention_ctx, lib=_lib)
+torch.library.register_autograd("mmt::qk_norm_rope", lambda ctx, dqo, dko: tuple(torch.ops.mmt.qk_norm_rope_bwd(
+    dqo, dko, *ctx.saved_tensors, *ctx.plain)) + (None,) * 4, setup_context=_qk_norm_rope_ctx, lib=_lib)
 torch.library.register_autograd("mmt::long_attention_bwd", _no_second("long_attention"), lib=_lib)
 torch.library.register_autograd("mmt::qk_norm_rope_bwd", _no_second("qk_norm_rope"), lib=_lib)
+
+
+def _traced(t):
+    """The call is being traced (fake tensors, a dispatch mode, torch.compile): it has to go through the dispatcher.  Otherwise the
+    wrappers below go straight to the kernels, which saves the dispatcher's way through Python (some 50 us per call)."""
+    return type(t) not in (torch.Tensor, torch.nn.Parameter) or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
 
 
 # ---- what the module classes call: the same ops through the dispatcher, with this package's error for host tensors ------------
@@ -252,9 +301,13 @@ def long_attention(q, k, v, *, scale=None, causal=False, prefix=None, q_doc=None
     slopes     (H) float32: -slopes[h] * distance is added         rel_bias  (H,n) float32, learned, at rel_buckets (2 reach + 1) int32 of
                                                                              the clamped distance (``ops.relative_buckets``)
     Rows that see nothing give zeros (and an lse of -inf).  Returns out (B,Lq,H,dh), with ``return_lse`` also the log-sums (B,H,Lq)."""
-    _dev(q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets)
-    out, lse = torch.ops.mmt.long_attention(q, k, v, scale, bool(causal), prefix, q_doc, k_doc, kv_len, float(softcap), slopes, rel_bias,
-                                            rel_buckets)
+    args = (q, k, v, scale, bool(causal), prefix, q_doc, k_doc, kv_len, float(softcap), slopes, rel_bias, rel_buckets)
+    if _traced(q):
+        out, lse = torch.ops.mmt.long_attention(*args)[:2]
+    elif torch.is_grad_enabled():
+        out, lse = _LongAttention.apply(*args)
+    else:
+        out, lse = ops.long_attention(*args)
     return (out, lse) if return_lse else out
 
 
@@ -262,5 +315,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps=1e-6
     """RMS norm of queries (B,L,H,dh) and keys (B,L,Hk,dh) per head, times the weights (dh), and the rotation of their first
     2 * len(inv_freq) elements by position * inv_freq (float64, ``ops.rotary_frequencies``) in the same pass; differentiable in q, k
     and the weights.  ``positions`` (B,L) int64, None: 0..L-1.  Pairs are (m, m + rot/2), with ``interleaved`` (2m, 2m + 1)."""
-    _dev(q, k, q_weight, k_weight, inv_freq, positions)
-    return torch.ops.mmt.qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, float(eps), bool(interleaved))
+    args = (q, k, q_weight, k_weight, inv_freq, positions, float(eps), bool(interleaved))
+    if _traced(q):
+        return torch.ops.mmt.qk_norm_rope(*args)
+    return _QkNormRope.apply(*args) if torch.is_grad_enabled() else ops.qk_norm_rope(*args)

@@ -44,9 +44,9 @@ def test_attention_refuses_on_the_host(bad, word):
     lib = _lib.load()
     a = _desc(**bad)
     assert lib.mmt_long_attention_workspace_bytes(ctypes.byref(a), 1) == 0
-    rc = lib.mmt_long_attention_fwd(ctypes.byref(a), 0x1000, None, 0x1000, 1 << 40, None)
+    rc = lib.mmt_long_attention_fwd(ctypes.byref(a), 0x1000, None, None, 0x1000, 1 << 40, None)
     assert rc == -1 and word in lib.mmt_last_error()
-    rc = lib.mmt_long_attention_bwd(ctypes.byref(a), 0x1000, 0x1000, 0x1000, 0, 0, 0, None, 0x1000, 0x1000, 0x1000, 0x1000, 0x1000, 1 << 40,
+    rc = lib.mmt_long_attention_bwd(ctypes.byref(a), 0x1000, None, 0x1000, 0x1000, 0, 0, 0, None, 0x1000, 0x1000, 0x1000, 0x1000, 0x1000, 1 << 40,
                                     None)
     assert rc == -1 and word in lib.mmt_last_error()
 
@@ -56,19 +56,19 @@ def test_attention_refuses_missing_outputs_and_small_workspaces():
     a = _desc(rel_bias=0x1000, rel_buckets=0x1000, n_buckets=8, reach=8)
     need = lib.mmt_long_attention_workspace_bytes(ctypes.byref(a), 1)
     assert need > 0
-    fwd = lambda out, ws, n: lib.mmt_long_attention_fwd(ctypes.byref(a), out, None, ws, n, None)
-    bwd = lambda dq, bias, ws, n, dout=0x1000: lib.mmt_long_attention_bwd(ctypes.byref(a), 0x1000, 0x1000, dout, 0, 0, 0, None, dq, 0x1000,
+    fwd = lambda out, ws, n: lib.mmt_long_attention_fwd(ctypes.byref(a), out, None, None, ws, n, None)
+    bwd = lambda dq, bias, ws, n, dout=0x1000: lib.mmt_long_attention_bwd(ctypes.byref(a), 0x1000, None, 0x1000, dout, 0, 0, 0, None, dq, 0x1000,
                                                                           0x1000, bias, ws, n, None)
     assert fwd(None, 0x1000, 1 << 40) == -1 and fwd(0x1004, 0x1000, 1 << 40) == -1
     assert bwd(None, 0x1000, 0x1000, need) == -1 and bwd(0x1000, None, 0x1000, need) == -1
     assert bwd(0x1000, 0x1000, 0x1000, need - 1) == -1 and b"workspace" in lib.mmt_last_error()
     assert bwd(0x1000, 0x1000, None, need) == -1 and bwd(0x1000, 0x1000, 0x1004, need) == -1
     assert bwd(0x1000, 0x1000, 0x1000, need, dout=0x1002) == -1
-    assert lib.mmt_long_attention_fwd(None, 0x1000, None, None, 0, None) == -1
+    assert lib.mmt_long_attention_fwd(None, 0x1000, None, None, None, 0, None) == -1
     long = _desc(Lq=1, Lk=4096, B=1)                      # split over the keys: needs somewhere to put the parts
     need = lib.mmt_long_attention_workspace_bytes(ctypes.byref(long), 0)
     assert need > 0
-    assert lib.mmt_long_attention_fwd(ctypes.byref(long), 0x1000, None, None, 0, None) == -1 and b"workspace" in lib.mmt_last_error()
+    assert lib.mmt_long_attention_fwd(ctypes.byref(long), 0x1000, None, None, None, 0, None) == -1 and b"workspace" in lib.mmt_last_error()
 
 
 @pytest.mark.parametrize("bad,word", [
@@ -103,8 +103,8 @@ def test_host_tensors_are_refused_and_shapes_propagate():
         torch.ops.mmt.long_attention(q, k, k, None, False, None, None, None, None, 0.0, None, None, None)
     with torch.device("meta"):
         q, k, w = torch.empty(2, 3, 4, 16, dtype=BF16), torch.empty(2, 5, 2, 16, dtype=BF16), torch.empty(16)
-        out, lse = torch.ops.mmt.long_attention(q, k, k, None, False, None, None, None, None, 0.0, None, None, None)
-        assert out.shape == q.shape and out.dtype == BF16 and lse.shape == (2, 4, 3) and lse.dtype == F32
+        out, lse, low = torch.ops.mmt.long_attention(q, k, k, None, False, None, None, None, None, 0.0, None, None, None)
+        assert low.shape == q.shape and out.shape == q.shape and out.dtype == BF16 and lse.shape == (2, 4, 3) and lse.dtype == F32
         a, b = torch.ops.mmt.qk_norm_rope(q, q[:, :, :2], w, w, torch.empty(8, dtype=torch.float64), None, 1e-6, False)
         assert a.shape == q.shape and b.shape == (2, 3, 2, 16)
 
@@ -379,9 +379,33 @@ def test_refusals_on_the_gpu():
             torch_ops.qk_norm_rope(*a)
     # no second derivative: an error, not a silent zero
     q = q.clone().requires_grad_()
-    g, = torch.autograd.grad(torch_ops.long_attention(q, k, v).float().sum(), q, create_graph=True)
-    with pytest.raises((MmtError, RuntimeError)):
-        g.float().sum().backward()
+    for fn in (lambda: torch_ops.long_attention(q, k, v), lambda: torch.ops.mmt.long_attention(q, k, v, None, False, None, None, None, None, 0.0, None, None, None)[0]):
+        g, = torch.autograd.grad(fn().float().sum(), q, create_graph=True)
+        with pytest.raises((MmtError, RuntimeError)):
+            g.float().sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_dispatcher_calls_equal_the_wrappers(dtype):
+    """torch.ops.mmt.* (what tracing sees) and the torch_ops wrappers (straight to the kernels): the same bits, gradients included."""
+    t, kw = _case(dtype, 2, 70, 70, 4, 2, 64, buckets=8, reach=16)
+    w, f = torch.ones(64, dtype=dtype, device=DEV), ops.rotary_frequencies(64, device=DEV)
+    res = []
+    for way in (0, 1):
+        q, k, v, b, ww = (x.clone().requires_grad_() for x in (t["q"], t["k"], t["v"], kw["rel_bias"], w))
+        if way:
+            x, y = torch.ops.mmt.qk_norm_rope(q, k, ww, w, f, None, 1e-6, False)
+            o, lse, _ = torch.ops.mmt.long_attention(x, y, v, None, True, None, None, None, None, 0.0, None, b, kw["rel_buckets"])
+        else:
+            x, y = torch_ops.qk_norm_rope(q, k, ww, w, f)
+            o, lse = torch_ops.long_attention(x, y, v, causal=True, rel_bias=b, rel_buckets=kw["rel_buckets"], return_lse=True)
+        res.append([o, lse] + list(torch.autograd.grad((o, lse), (q, k, v, b, ww), (t["go"], torch.ones_like(lse)))))
+    assert all(torch.equal(x, y) for x, y in zip(*res))
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():                                # tracing: shapes without a kernel
+        q = torch.empty(2, 5, 4, 64, dtype=dtype, device=DEV)
+        assert torch_ops.long_attention(q, q[:, :, :2], q[:, :, 2:]).shape == q.shape
 
 
 @pytest.mark.gpu
@@ -420,8 +444,8 @@ def test_captured_calls_replay(dtype):
 
     def train():
         a, b = ops.qk_norm_rope(t["q"], t["k"], w, w, f)
-        o, lse = ops.long_attention(a, b, t["v"], causal=True, **kw)
-        g = ops.long_attention_backward(t["go"], None, o, lse, a, b, t["v"], causal=True, **kw)
+        o, lse, low = ops.long_attention(a, b, t["v"], causal=True, keep_low=True, **kw)
+        g = ops.long_attention_backward(t["go"], None, o, lse, low, a, b, t["v"], causal=True, **kw)
         return (o, lse) + tuple(g) + tuple(ops.qk_norm_rope_backward(g[0], g[1], t["q"], t["k"], w, w, f))
 
     def serve():
