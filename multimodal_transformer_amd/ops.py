@@ -769,45 +769,61 @@ def finalize(pred_st, node_pos=None, gt=None, metres=True, want_pred=True, want_
 _ELEM = {torch.float32: _lib.MMT_F32, torch.bfloat16: _lib.MMT_BF16, torch.float16: _lib.MMT_F16}
 
 
-def _head_rows(t, name, shape=None, like=None):
+def _head_rows(t, name, shape, dtype, device):
     """A (B, L, heads, dh) tensor whose rows (head slices) the kernels can read where they are: contiguous elements, every row at a
-    multiple of 16 bytes; anything else (a transposed last axis, an odd offset) is copied once.  Strides of 0 (broadcast) are fine."""
+    multiple of 16 bytes; anything else (a transposed last axis, an odd offset) is copied once.  Strides of 0 (broadcast) are fine.
+    -> the tensor and its address, batch, token and head stride (0 for an axis of length 1, whose stride means nothing)."""
     if not isinstance(t, torch.Tensor):
         raise MmtError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
-    if not t.is_cuda:
-        raise MmtError(f"{name}: tensor is on {t.device}; the HIP kernels need device memory (no CPU fallback)")
-    if t.dim() != 4 or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise MmtError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape) if shape is not None else '(batch, tokens, heads, head size)'}")
-    if t.dtype not in _ELEM or (like is not None and t.dtype != like.dtype):
-        raise MmtError(f"{name}: dtype {t.dtype}, expected {like.dtype if like is not None else 'float32, bfloat16 or float16'}")
-    if like is not None and t.device != like.device:
-        raise MmtError(f"{name}: tensor is on {t.device}, expected {like.device}")
-    unit = 16 // t.element_size()
-    if t.stride(3) != 1 or t.stride(1) >= 1 << 24 or t.data_ptr() % 16 or any(t.stride(i) % unit for i in range(3) if t.shape[i] > 1) or \
-            any(t.stride(i) < 0 for i in range(3)):
-        t = t.contiguous()
-        if t.data_ptr() % 16:          # contiguous all along, but cut out of a larger buffer at an odd place
-            t = t.clone()
-    return t
+    if t.dtype is not dtype or not t.is_cuda or t.device != device or t.dim() != 4 or (shape is not None and t.shape != shape):
+        if not t.is_cuda:
+            raise MmtError(f"{name}: tensor is on {t.device}; the HIP kernels need device memory (no CPU fallback)")
+        if t.dim() != 4 or (shape is not None and t.shape != shape):
+            raise MmtError(f"{name}: shape {tuple(t.shape)}, expected "
+                           f"{tuple(shape) if shape is not None else '(batch, tokens, heads, head size)'}")
+        if t.dtype is not dtype:
+            raise MmtError(f"{name}: dtype {t.dtype}, expected {dtype}")
+        raise MmtError(f"{name}: tensor is on {t.device}, expected {device}")
+    b, r, h, one = t.stride()
+    p = t.data_ptr()
+    odd = 15 // t.element_size()
+    if one != 1 or (p & 15) or ((b | r | h) & odd) or r >= 1 << 24:
+        n0, n1, n2, n3 = t.shape
+        b, r, h = b if n0 > 1 else 0, r if n1 > 1 else 0, h if n2 > 1 else 0
+        if (one != 1 and n3 > 1) or (p & 15) or ((b | r | h) & odd) or r >= 1 << 24:
+            t = t.contiguous()
+            if t.data_ptr() & 15:          # contiguous all along, but cut out of a larger buffer at an odd place
+                t = t.clone()
+            b, r, h, _ = t.stride()
+            p = t.data_ptr()
+            if ((b | r | h) & odd) or r >= 1 << 24:      # head sizes and widths that the library refuses
+                b, r, h = b & ~odd, min(r & ~odd, (1 << 24) - 1 - odd), h & ~odd
+    return t, p, b, r, h
 
 
-def _strides(t):
-    """Batch, token and head stride; the stride of an axis of length 1 is never used and may be anything: 0."""
-    return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
-
-
-def _side(t, name, shape, dtype, like):
-    """An optional contiguous tensor beside q (a mask's numbers, a table) on q's device."""
+def _side(t, name, shape, dtype, device):
+    """The address of an optional contiguous tensor beside q (a mask's numbers, a table) on q's device."""
     if t is None:
         return None
-    _chk(t, name, shape, dtype)
-    if t.device != like.device:
-        raise MmtError(f"{name}: tensor is on {t.device}, expected {like.device}")
-    return t
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.device == device):
+        _chk(t, name, shape, dtype)
+        raise MmtError(f"{name}: tensor is on {t.device}, expected {device}")
+    return t.data_ptr()
 
 
-def _workspace(nbytes, device):
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+def _on_device(fn):
+    """Runs fn(first tensor, ...) with the tensor's device current (outputs, workspace and launches go to its current stream)."""
+    def call(first, *args, **kw):
+        if isinstance(first, torch.Tensor) and first.is_cuda and first.device.index != torch.cuda.current_device():
+            with torch.cuda.device(first.device):
+                return fn(first, *args, **kw)
+        return fn(first, *args, **kw)
+    call.__name__, call.__doc__ = fn.__name__, fn.__doc__
+    return call
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def rotary_frequencies(rot, base=10000.0, device=None):
@@ -842,144 +858,152 @@ def relative_buckets(n_buckets, reach, bidirectional, device=None):
 
 
 def _rope_args(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved):
-    q = _head_rows(q, "q")
+    elem, dev = _ELEM.get(getattr(q, "dtype", None)), getattr(q, "device", None)
+    if elem is None:
+        raise MmtError(f"q: expected a float32, bfloat16 or float16 tensor, got {getattr(q, 'dtype', type(q).__name__)}")
+    q, qp, qb, qr, qh = _head_rows(q, "q", None, q.dtype, dev)
+    k, kp, kb, kr, kh = _head_rows(k, "k", None, q.dtype, dev)
     B, L, H, dh = q.shape
-    k = _head_rows(k, "k", None, q)
     if k.shape[0] != B or k.shape[1] != L or k.shape[3] != dh or k.shape[2] < 1 or H < 1:
         raise MmtError(f"qk_norm_rope: q {tuple(q.shape)} and k {tuple(k.shape)} do not line up")
     if not isinstance(q_weight, torch.Tensor) or q_weight.dtype not in (q.dtype, torch.float32):
         raise MmtError(f"q_weight: expected a tensor of type {q.dtype} or torch.float32")
-    qw = _side(q_weight, "q_weight", (dh,), q_weight.dtype, q)
-    kw = _side(k_weight, "k_weight", (dh,), q_weight.dtype, q)
-    if kw is None or inv_freq is None:
-        raise MmtError("qk_norm_rope: k_weight and inv_freq are needed")
-    _side(inv_freq, "inv_freq", (None,), torch.float64, q)
-    _side(positions, "positions", (B, L), torch.int64, q)
-    a = _lib.QkNormRope()
-    a.q, a.k, a.q_weight, a.k_weight = q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr()
-    a.q_bs, a.q_rs, a.q_hs = _strides(q)
-    a.k_bs, a.k_rs, a.k_hs = _strides(k)
-    a.inv_freq, a.positions = inv_freq.data_ptr(), positions.data_ptr() if positions is not None else None
-    a.dtype, a.w_dtype = _ELEM[q.dtype], _ELEM[qw.dtype]
-    a.B, a.L, a.H, a.Hk, a.dh, a.rot = B, L, H, k.shape[2], dh, 2 * inv_freq.numel()
-    a.interleaved, a.eps = int(bool(interleaved)), float(eps)
+    if k_weight is None or not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
+        raise MmtError("qk_norm_rope: k_weight and inv_freq (one axis) are needed")
+    wt, pairs = q_weight.dtype, inv_freq.numel()
+    a = _lib.QkNormRope(qp, kp, _side(q_weight, "q_weight", (dh,), wt, dev), _side(k_weight, "k_weight", (dh,), wt, dev),
+                        qb, qr, qh, kb, kr, kh, _side(inv_freq, "inv_freq", (pairs,), torch.float64, dev),
+                        _side(positions, "positions", (B, L), torch.int64, dev), elem, _ELEM[wt], B, L, H, k.shape[2], dh, 2 * pairs,
+                        bool(interleaved), eps)
     return a, q, k
 
 
+@_on_device
 def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, eps=1e-6, interleaved=False):
     """RMS norm of every head of q (B,L,H,dh) and k (B,L,Hk,dh) with weights (dh), then the rotation of the pairs of its first
     2 * len(inv_freq) elements by position * inv_freq, in one pass (``mmt_qk_norm_rope_fwd``).  ``positions`` (B,L) int64, None:
     0..L-1.  Returns new contiguous tensors."""
     a, q, k = _rope_args(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
-    with torch.cuda.device(q.device):
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        if a.B * a.L:
-            lib = _lib.load()
-            _lib.check(lib.mmt_qk_norm_rope_fwd(C.byref(a), _ptr(qo), _ptr(ko), _stream()), "mmt_qk_norm_rope_fwd")
+    dev = q.device
+    qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    ko = torch.empty(k.shape, dtype=q.dtype, device=dev)
+    if a.B * a.L:
+        rc = _lib.load().mmt_qk_norm_rope_fwd(C.byref(a), qo.data_ptr(), ko.data_ptr(), _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "mmt_qk_norm_rope_fwd")
     return qo, ko
 
 
+@_on_device
 def qk_norm_rope_backward(dqo, dko, q, k, q_weight, k_weight, inv_freq, positions=None, eps=1e-6, interleaved=False):
     """Gradients of q, k, q_weight, k_weight from those of ``qk_norm_rope``'s outputs (``mmt_qk_norm_rope_bwd``)."""
     a, q, k = _rope_args(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
-    dqo, dko = _head_rows(dqo, "dq_out", q.shape, q), _head_rows(dko, "dk_out", k.shape, q)
-    with torch.cuda.device(q.device):
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dqw, dkw = torch.empty_like(q_weight), torch.empty_like(k_weight)
-        if not a.B * a.L:
-            return dq, dk, dqw.zero_(), dkw.zero_()
-        lib = _lib.load()
-        ws = _workspace(lib.mmt_qk_norm_rope_workspace_bytes(C.byref(a)), q.device)
-        _lib.check(lib.mmt_qk_norm_rope_bwd(C.byref(a), _ptr(dqo), *_strides(dqo), _ptr(dko), *_strides(dko), _ptr(dq), _ptr(dk),
-                                            _ptr(dqw), _ptr(dkw), _ptr(ws), ws.numel(), _stream()), "mmt_qk_norm_rope_bwd")
+    dev = q.device
+    dqo, dqp, dqb, dqr, dqh = _head_rows(dqo, "dq_out", q.shape, q.dtype, dev)
+    dko, dkp, dkb, dkr, dkh = _head_rows(dko, "dk_out", k.shape, q.dtype, dev)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=dev)
+    dqw, dkw = torch.empty_like(q_weight), torch.empty_like(k_weight)
+    if not a.B * a.L:
+        return dq, dk, dqw.zero_(), dkw.zero_()
+    lib = _lib.load()
+    nb = lib.mmt_qk_norm_rope_workspace_bytes(C.byref(a))
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    rc = lib.mmt_qk_norm_rope_bwd(C.byref(a), dqp, dqb, dqr, dqh, dkp, dkb, dkr, dkh, dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(),
+                                  dkw.data_ptr(), ws.data_ptr(), nb, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "mmt_qk_norm_rope_bwd")
     return dq, dk, dqw, dkw
 
 
 def _attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets):
-    q = _head_rows(q, "q")
+    elem, dev = _ELEM.get(getattr(q, "dtype", None)), getattr(q, "device", None)
+    if elem is None:
+        raise MmtError(f"q: expected a float32, bfloat16 or float16 tensor, got {getattr(q, 'dtype', type(q).__name__)}")
+    q, qp, qb, qr, qh = _head_rows(q, "q", None, q.dtype, dev)
+    k, kp, kb, kr, kh = _head_rows(k, "k", None, q.dtype, dev)
+    v, vp, vb, vr, vh = _head_rows(v, "v", k.shape, q.dtype, dev)
     B, Lq, H, dh = q.shape
-    k = _head_rows(k, "k", None, q)
-    v = _head_rows(v, "v", k.shape, q)
-    Lk, Hk = k.shape[1], k.shape[2]
-    if k.shape[0] != B or k.shape[3] != dh or Hk < 1 or H < 1 or H % Hk:
+    kB, Lk, Hk, kd = k.shape
+    if kB != B or kd != dh or Hk < 1 or H < 1 or H % Hk:
         raise MmtError(f"long_attention: q {tuple(q.shape)} and k {tuple(k.shape)} do not line up (batch, head size, heads a "
                        "multiple of the key heads)")
+    i32, f32, n, reach = torch.int32, torch.float32, 0, 0
     if prefix is not None and not causal:
         raise MmtError("long_attention: a prefix is an exception from the causal mask")
     if (q_doc is None) != (k_doc is None):
         raise MmtError("long_attention: documents need ids for the queries and the keys")
     if (rel_bias is None) != (rel_buckets is None):
         raise MmtError("long_attention: a learned bias needs its table and its buckets")
-    _side(prefix, "prefix", (B,), torch.int32, q), _side(kv_len, "kv_len", (B,), torch.int32, q)
-    _side(q_doc, "q_doc", (B, Lq), torch.int32, q), _side(k_doc, "k_doc", (B, Lk), torch.int32, q)
-    _side(slopes, "slopes", (H,), torch.float32, q), _side(rel_bias, "rel_bias", (H, None), torch.float32, q)
-    _side(rel_buckets, "rel_buckets", (None,), torch.int32, q)
-    if rel_buckets is not None and (rel_buckets.numel() < 3 or rel_buckets.numel() % 2 == 0):
-        raise MmtError(f"rel_buckets: {rel_buckets.numel()} entries, expected 2 reach + 1")
-    a = _lib.LongAttention()
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_bs, a.q_rs, a.q_hs = _strides(q)
-    a.k_bs, a.k_rs, a.k_hs = _strides(k)
-    a.v_bs, a.v_rs, a.v_hs = _strides(v)
-    a.dtype, a.B, a.Lq, a.Lk, a.H, a.Hk, a.dh, a.causal = _ELEM[q.dtype], B, Lq, Lk, H, Hk, dh, int(bool(causal))
-    a.scale, a.softcap = float(scale) if scale is not None else dh ** -0.5, float(softcap)
-    for name, t in (("prefix", prefix), ("kv_len", kv_len), ("q_doc", q_doc), ("k_doc", k_doc), ("slopes", slopes),
-                    ("rel_bias", rel_bias), ("rel_buckets", rel_buckets)):
-        if t is not None:
-            setattr(a, name, t.data_ptr())
     if rel_bias is not None:
-        a.n_buckets, a.reach = rel_bias.shape[1], rel_buckets.numel() // 2
+        if not isinstance(rel_bias, torch.Tensor) or rel_bias.dim() != 2:
+            raise MmtError("rel_bias: expected a (heads, buckets) tensor")
+        if not isinstance(rel_buckets, torch.Tensor) or rel_buckets.dim() != 1 or rel_buckets.numel() < 3 or rel_buckets.numel() % 2 == 0:
+            raise MmtError("rel_buckets: expected 2 reach + 1 entries")
+        n, reach = rel_bias.shape[1], rel_buckets.numel() // 2
+    a = _lib.LongAttention(qp, kp, vp, qb, qr, qh, kb, kr, kh, vb, vr, vh, elem, B, Lq, Lk, H, Hk, dh, bool(causal),
+                           dh ** -0.5 if scale is None else scale, softcap, _side(prefix, "prefix", (B,), i32, dev),
+                           _side(kv_len, "kv_len", (B,), i32, dev), _side(q_doc, "q_doc", (B, Lq), i32, dev),
+                           _side(k_doc, "k_doc", (B, Lk), i32, dev), _side(slopes, "slopes", (H,), f32, dev),
+                           _side(rel_bias, "rel_bias", (H, n), f32, dev), _side(rel_buckets, "rel_buckets", (2 * reach + 1,), i32, dev),
+                           n, reach)
     return a, q, k, v
 
 
+@_on_device
 def long_attention(q, k, v, scale=None, causal=False, prefix=None, q_doc=None, k_doc=None, kv_len=None, softcap=0.0, slopes=None,
                    rel_bias=None, rel_buckets=None, keep_low=False):
     """Attention of q (B,Lq,H,dh) over k, v (B,Lk,Hk,dh) of any length (``mmt_long_attention_fwd``; the header states the formula,
-    the masks and the limits) -> out (B,Lq,H,dh), lse (B,H,Lq) fp32 and, with
-    ``keep_low``, what rounding took from out (for the backward; None in fp32).  Queries are the last Lq of ``kv_len[b]`` (or Lk)
-    tokens."""
+    the masks and the limits) -> out (B,Lq,H,dh), lse (B,H,Lq) fp32 and, with ``keep_low``, what rounding took from out (for the
+    backward; None in fp32).  Queries are the last Lq of ``kv_len[b]`` (or Lk) tokens."""
     a, q, k, v = _attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets)
-    with torch.cuda.device(q.device):
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        low = torch.empty_like(out) if keep_low and q.dtype != torch.float32 else None
-        lse = torch.empty((a.B, a.H, a.Lq), dtype=torch.float32, device=q.device)
-        if not a.Lk:
-            out.zero_(), lse.fill_(float("-inf"))
-            if low is not None:
-                low.zero_()
-        elif a.B * a.Lq:
-            lib = _lib.load()
-            ws = _workspace(lib.mmt_long_attention_workspace_bytes(C.byref(a), 0), q.device)
-            _lib.check(lib.mmt_long_attention_fwd(C.byref(a), _ptr(out), _ptr(low), _ptr(lse), _ptr(ws), ws.numel(), _stream()),
-                       "mmt_long_attention_fwd")
+    dev = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    low = torch.empty(q.shape, dtype=q.dtype, device=dev) if keep_low and a.dtype != _lib.MMT_F32 else None
+    lse = torch.empty((a.B, a.H, a.Lq), dtype=torch.float32, device=dev)
+    if not a.Lk:
+        out.zero_(), lse.fill_(float("-inf"))
+        if low is not None:
+            low.zero_()
+    elif a.B * a.Lq:
+        lib = _lib.load()
+        nb = lib.mmt_long_attention_workspace_bytes(C.byref(a), 0)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        rc = lib.mmt_long_attention_fwd(C.byref(a), out.data_ptr(), low.data_ptr() if low is not None else None, lse.data_ptr(),
+                                        ws.data_ptr() if nb else None, nb, _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "mmt_long_attention_fwd")
     return (out, lse, low) if keep_low else (out, lse)
 
 
+@_on_device
 def long_attention_backward(dout, dlse, out, lse, low, q, k, v, scale=None, causal=False, prefix=None, q_doc=None, k_doc=None, kv_len=None,
                             softcap=0.0, slopes=None, rel_bias=None, rel_buckets=None):
     """Gradients of q, k, v and rel_bias (None without it) from those of ``long_attention``'s out and lse (``dlse`` may be None);
     ``low`` is the forward's, or None."""
     a, q, k, v = _attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets)
-    dout = _head_rows(dout, "dout", q.shape, q)
-    out = _head_rows(out, "out", q.shape, q).contiguous()
-    low = _head_rows(low, "low", q.shape, q).contiguous() if low is not None else None
-    _side(lse, "lse", (a.B, a.H, a.Lq), torch.float32, q)
+    dev, dt = q.device, q.dtype
+    dout, gp, gb, gr, gh = _head_rows(dout, "dout", q.shape, dt, dev)
+    stats = (a.B, a.H, a.Lq)
+    out_p, low_p = _side(out, "out", q.shape, dt, dev), _side(low, "low", q.shape, dt, dev)
+    lse_p = _side(lse, "lse", stats, torch.float32, dev)
     if dlse is not None:
-        dlse = _side(dlse.contiguous(), "dlse", (a.B, a.H, a.Lq), torch.float32, q)
-    with torch.cuda.device(q.device):
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dbias = torch.empty_like(rel_bias) if rel_bias is not None else None
-        if not a.B * a.Lq * a.Lk:
-            for t in (dq, dk, dv, dbias):
-                if t is not None:
-                    t.zero_()
-            return dq, dk, dv, dbias
-        lib = _lib.load()
-        ws = _workspace(lib.mmt_long_attention_workspace_bytes(C.byref(a), 1), q.device)
-        _lib.check(lib.mmt_long_attention_bwd(C.byref(a), _ptr(out), _ptr(low), _ptr(lse), _ptr(dout), *_strides(dout), _ptr(dlse), _ptr(dq), _ptr(dk),
-                                              _ptr(dv), _ptr(dbias), _ptr(ws), ws.numel(), _stream()), "mmt_long_attention_bwd")
+        dlse = dlse.contiguous()
+    dlse_p = _side(dlse, "dlse", stats, torch.float32, dev)
+    dq = torch.empty(q.shape, dtype=dt, device=dev)
+    dk = torch.empty(k.shape, dtype=dt, device=dev)
+    dv = torch.empty(k.shape, dtype=dt, device=dev)
+    dbias = torch.empty(rel_bias.shape, dtype=torch.float32, device=dev) if rel_bias is not None else None
+    if not a.B * a.Lq * a.Lk:
+        for t in (dq, dk, dv, dbias):
+            if t is not None:
+                t.zero_()
+        return dq, dk, dv, dbias
+    lib = _lib.load()
+    nb = lib.mmt_long_attention_workspace_bytes(C.byref(a), 1)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    rc = lib.mmt_long_attention_bwd(C.byref(a), out_p, low_p, lse_p, gp, gb, gr, gh, dlse_p, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                    dbias.data_ptr() if dbias is not None else None, ws.data_ptr(), nb, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "mmt_long_attention_bwd")
     return dq, dk, dv, dbias
