@@ -87,7 +87,6 @@ template <typename T, int D> struct Tile {
   static constexpr int NS = DS / EPS;
   static constexpr int BK = Elem<T>::BK;
   static constexpr int BYTES = BK * NS * 16;
-  static constexpr int NLD = BK * NS / THREADS;                   // 16-byte loads per thread and tile
   static __device__ __forceinline__ int swz(int row, int slot) {
     if constexpr (sizeof(T) == 4) {
       return slot ^ (NS >= 16 ? (row & 15) : ((row >> 1) & 7));
@@ -98,8 +97,6 @@ template <typename T, int D> struct Tile {
     }
   }
 };
-static_assert(Tile<__bf16, 32>::NLD == 1 && Tile<float, 32>::NLD == 1, "every tile is a whole number of 16-byte loads per thread");
-
 // row operand: elements 16 c + 8 h .. + 7 of row `row`
 template <typename T, int D> __device__ __forceinline__ typename Elem<T>::V8 row_frag(const char *t, int row, int c, int h) {
   typedef Tile<T, D> L;
@@ -149,11 +146,19 @@ template <typename T> __device__ __forceinline__ typename Elem<T>::V8 mem_frag(c
 }
 
 // One 16-byte piece per lane straight from memory into LDS (no registers in between): lane l's piece lands at lds + 16 l.
-// Untracked by the compiler: dma_wait() before the barrier that publishes the tile.  M0 holds the LDS address (below 64 KiB).
+// Untracked by the compiler: dma_wait before the barrier that publishes the tile.  M0 holds the LDS address.
 __device__ __forceinline__ void dma16(const void *base, unsigned off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(lds) : "memory");
 }
-__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+// all but the newest N requests of the wave have arrived (requests of the compiler's own in between only make this stricter)
+template <int N> __device__ __forceinline__ void dma_wait() {
+  static_assert(N == 0 || N == 2 || N == 4 || N == 8 || N == 16, "one of the tiles' request counts");
+  if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+  else if constexpr (N == 2) asm volatile("s_waitcnt vmcnt(2)" : : : "memory");
+  else if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" : : : "memory");
+  else if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" : : : "memory");
+  else asm volatile("s_waitcnt vmcnt(16)" : : : "memory");
+}
 __device__ __forceinline__ unsigned lds_address(const void *p) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char *)p;
 }
@@ -161,31 +166,34 @@ __device__ __forceinline__ unsigned lds_address(const void *p) {
 // Tiles of a (rows, dh) matrix on their way to LDS.  A lane's byte offset inside a tile is the same for every tile; the tile's own
 // part is a scalar.  Slots at and beyond dh repeat slot 0 and rows at and beyond n_rows the last row (nothing outside the tensor is
 // read); the operands these elements meet are zero, or results nobody stores.
-template <typename T, int D> struct Dma {
+// NT threads (the workgroup, or one wave) move tiles of R rows.
+template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS> struct Dma {
   typedef Tile<T, D> L;
+  static constexpr int N = R * L::NS / NT;
+  static_assert(N * NT == R * L::NS, "a tile is a whole number of 16-byte loads per thread");
   const char *base;
   int64_t rs;                        // bytes between rows; 64 rows stay below 2^31 bytes
   int n_rows;
-  unsigned off[L::NLD];
+  unsigned off[N];
   __device__ __forceinline__ void init(const T *p, int64_t row_stride, int rows, int dh) {
     base = (const char *)p, rs = row_stride * (int64_t)sizeof(T), n_rows = rows;
 #pragma unroll
-    for (int n = 0; n < L::NLD; ++n) {
-      const int idx = threadIdx.x + n * THREADS, row = idx / L::NS, slot = L::swz(row, idx % L::NS);
+    for (int n = 0; n < N; ++n) {
+      const int idx = threadIdx.x % NT + n * NT, row = idx / L::NS, slot = L::swz(row, idx % L::NS);
       off[n] = (unsigned)(row * rs) + (slot * L::EPS < dh ? slot * 16 : 0);
     }
   }
   __device__ __forceinline__ void load(unsigned lds, int r0) const {
     const char *b = base + r0 * rs;
-    const unsigned mine = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
-    if (r0 + L::BK <= n_rows) {
+    const unsigned mine = __builtin_amdgcn_readfirstlane(lds + ((threadIdx.x % NT) >> 6) * 1024);
+    if (r0 + R <= n_rows) {
 #pragma unroll
-      for (int n = 0; n < L::NLD; ++n) dma16(b, off[n], mine + n * THREADS * 16);
+      for (int n = 0; n < N; ++n) dma16(b, off[n], mine + n * NT * 16);
     } else {
 #pragma unroll
-      for (int n = 0; n < L::NLD; ++n) {
-        const int row = (int)(threadIdx.x + n * THREADS) / L::NS, over = max(0, r0 + row - (n_rows - 1));
-        dma16(b, off[n] - (unsigned)(over * rs), mine + n * THREADS * 16);
+      for (int n = 0; n < N; ++n) {
+        const int row = (int)(threadIdx.x % NT + n * NT) / L::NS, over = max(0, r0 + row - (n_rows - 1));
+        dma16(b, off[n] - (unsigned)(over * rs), mine + n * NT * 16);
       }
     }
   }
@@ -193,11 +201,12 @@ template <typename T, int D> struct Dma {
 
 // Rows of a tile that must not take part become zeros (whatever they hold: 0 x NaN would reach every other row): at and beyond `end`
 // (tile row), or with a negative document id
-template <typename T, int D> __device__ __forceinline__ void zero_rows(char *lds, int end, const int *doc) {
+template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS>
+__device__ __forceinline__ void zero_rows(char *lds, int end, const int *doc) {
   typedef Tile<T, D> L;
 #pragma unroll
-  for (int n = 0; n < L::NLD; ++n) {
-    const int idx = threadIdx.x + n * THREADS, row = idx / L::NS;
+  for (int n = 0; n < R * L::NS / NT; ++n) {
+    const int idx = threadIdx.x % NT + n * NT, row = idx / L::NS;
     if (row >= end || (doc && doc[row] < 0)) *(u32x4 *)(lds + idx * 16) = u32x4{};
   }
 }
@@ -230,6 +239,8 @@ __device__ __forceinline__ int wave_max(int v) {
   for (int m = 1; m < 64; m <<= 1) v = max(v, __shfl_xor(v, m));
   return __builtin_amdgcn_readfirstlane(v);
 }
+// what the wave has read from and written to LDS so far is done before what follows, requests straight into LDS among it
+__device__ __forceinline__ void wave_sync() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 

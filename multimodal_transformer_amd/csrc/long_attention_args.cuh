@@ -20,7 +20,8 @@ struct DocRange {
 
 struct Args {                      // mmt_long_attention plus what the launcher derives
   mmt_long_attention a;
-  int G, pack;                     // query heads per key head; heads sharing a workgroup's rows (1 or G)
+  int G, pack;                     // query heads per key head; heads whose rows share a tile (1 or G)
+  int few;                         // all rows of a key head fit into 32: the waves split the keys instead
   int nqt, nkt, nsplit, items;     // row tiles, key tiles, splits of the keys, workgroups
   int groups;                      // workgroups n, n + groups, .. share keys and values
   int zh, zq;                      // dK / dV: parts over the query heads of a key head, over the queries

@@ -131,46 +131,162 @@ __device__ __forceinline__ void modify(const mmt_long_attention &a, const ScoreC
 }
 
 // ---------------------------------------------------------------------------------------------------------------- forward
-// One workgroup = 128 rows (4 waves x 32) of one head - or of the `pack` heads that share a key head, when there are few queries -
-// against a range of key tiles.  K and V tiles go straight from memory to LDS, one tile ahead of the products (two buffers, one
-// barrier per tile).  MOD: the scores are capped or biased; without it they go from the product into the exponential as they are.
+// One wave's 32 rows against NK x 32 keys of a tile in LDS: products, modification, masks, running maximum and sum, o^T += v^T P^T.
+// The running maximum is kept in units of log 2.
+template <typename T, int D> struct FwdState {
+  f32x16 acc[D / 32];
+  float m, l;
+};
+template <typename T, int D, int NK>
+__device__ __forceinline__ void fwd_products(float *x, const typename Elem<T>::V8 *fq, const char *sK, int lane) {
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt) {
+    f32x16 s = {};
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + (lane & 31), c, lane >> 5), fq[c], s);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[16 * kt + i] = s[i];
+  }
+}
+// products -> probabilities (not yet divided by their sum)
+template <typename T, int D, bool MOD, int NK>
+__device__ __forceinline__ void fwd_softmax(FwdState<T, D> &st, float *x, int key0, const Row &w, const mmt_long_attention &a, const ScoreCtx &sc,
+                                            const float *tab, const unsigned char *bucket, int far, bool need_mask, const int *sDoc, int h) {
+  constexpr int ND = D / 32;
+  float cf = sc.c_scale;
+  if constexpr (MOD) {
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt)
+      modify<16, false>(a, sc, x + 16 * kt, nullptr, key0 + 32 * kt + 4 * h - w.p, 1, w.slope, tab, bucket, far);
+    cf = 1.f;
+  }
+  if (need_mask) {
+#pragma unroll
+    for (int i = 0; i < NK * 16; ++i) {
+      const int j = 32 * (i >> 4) + acc_row(i & 15, h);
+      bool see = key0 + j < w.hi;
+      if (sDoc) see = see && sDoc[j] == w.doc;
+      if (!see) x[i] = -INFINITY;
+    }
+  }
+  float mx = x[0];
+#pragma unroll
+  for (int i = 1; i < NK * 16; ++i) mx = fmaxf(mx, x[i]);
+  const float m_new = fmaxf(st.m, half_max(mx) * cf);
+  const float ms = m_new == -INFINITY ? 0.f : m_new;
+  const float alpha = ex2(st.m - ms);
+  st.m = m_new;
+  const float off = Elem<T>::PSHIFT - ms;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < NK * 16; ++i) {
+    x[i] = ex2(fmaf(x[i], cf, off));
+    sum += x[i];
+  }
+  st.l = fmaf(st.l, alpha, sum);
+  if (__any(alpha != 1.f)) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.acc[d][i] *= alpha;
+  }
+}
+template <typename T, int D, int NK> __device__ __forceinline__ void fwd_values(FwdState<T, D> &st, const float *x, const char *sV, int lane) {
+  constexpr int ND = D / 32;
+#pragma unroll
+  for (int c = 0; c < NK * 2; ++c) {
+    const typename Elem<T>::V8 p = round8<T>(x + 8 * c);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) st.acc[d] = Elem<T>::mma(col_frag<T, D>(sV, 16 * c, d, lane), p, st.acc[d]);
+  }
+}
+
+// A row's result: o^T of the accumulator scaled, or this split's part of it
+template <typename T, int D>
+__device__ __forceinline__ void fwd_store(const Args &g, const FwdState<T, D> &st, const Row &w, int b, int split, int h) {
+  constexpr int ND = D / 32;
+  const mmt_long_attention &a = g.a;
+  const float l = half_sum(st.l);
+  if (!w.valid) return;
+  const int64_t r = ((int64_t)b * a.H + w.h) * a.Lq + w.i;
+  if (g.nsplit > 1) {
+    const int64_t rs = (int64_t)split * a.B * a.H * a.Lq + r;
+    if (h == 0) {
+      g.part_ml[2 * rs] = w.live ? st.m : -INFINITY;
+      g.part_ml[2 * rs + 1] = w.live ? l : 0.f;
+    }
+    float *o = g.part_o + rs * a.dh;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int dim = 32 * d + 8 * q + 4 * h;
+        if (dim < a.dh) *(f32x4 *)(o + dim) = f32x4{st.acc[d][4 * q], st.acc[d][4 * q + 1], st.acc[d][4 * q + 2], st.acc[d][4 * q + 3]};
+      }
+    return;
+  }
+  const bool some = w.live && l != 0.f;                   // (a NaN sum is "some")
+  const float inv = some ? 1.f / l : 0.f;
+  if (g.lse && h == 0) g.lse[r] = some ? (st.m + log2f(l) - Elem<T>::PSHIFT) * LN2 : -INFINITY;
+  const int64_t o = (((int64_t)b * a.Lq + w.i) * a.H + w.h) * a.dh;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int dim = 32 * d + 8 * q + 4 * h;
+      if (dim < a.dh) {
+        typename Elem<T>::V4 v, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = some ? st.acc[d][4 * q + e] * inv : 0.f;
+          v[e] = (T)y, lo[e] = (T)(y - (float)v[e]);
+        }
+        *(typename Elem<T>::V4 *)((T *)g.out + o + dim) = v;
+        if (g.low) *(typename Elem<T>::V4 *)((T *)g.low + o + dim) = lo;
+      }
+    }
+}
+
+// One workgroup = 128 rows (4 waves x 32) of one head against a range of key tiles.  K and V tiles go straight from memory to LDS, one
+// tile ahead of the products (two buffers, one barrier per tile).  MOD: the scores are capped or biased; without it they go from the
+// product into the exponential as they are.
 template <typename T, int D, bool MOD>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_fwd_kernel(const Args g) {
   typedef Tile<T, D> L;
   typedef typename Elem<T>::V8 V8;
-  constexpr int BK = L::BK, NK = BK / 32, NC = D / 16, ND = D / 32;
+  constexpr int BK = L::BK, NC = D / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
   int *sDoc = (int *)(smem + 4 * L::BYTES), *sB = sDoc + BK;
   BiasLds bias;
   bias.table = (float *)(sB + 6 * WAVES);
-  const int ngroup = g.pack > 1 ? 1 : g.G, grp = blockIdx.x % g.groups;
+  const int grp = blockIdx.x % g.groups;
   int n = blockIdx.x / g.groups;
   const int split = n % g.nsplit;
   n /= g.nsplit;
-  const int gi = n % ngroup;
-  int qt = n / ngroup;
+  const int gi = n % g.G;
+  int qt = n / g.G;
   if (a.causal) qt = g.nqt - 1 - qt;                     // the tiles with the most keys first
   const int kh = grp % a.Hk, b = grp / a.Hk;
   const int head0 = kh * g.G + gi;
-  bias.bucket = (unsigned char *)(bias.table + (MOD && a.rel_bias ? g.pack * a.n_buckets : 0));
+  bias.bucket = (unsigned char *)(bias.table + (MOD && a.rel_bias ? a.n_buckets : 0));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
   const int len = row_len(a, b);
   const Row w = make_row(g, b, head0, qt * ROWS + wave * 32 + col, len);
   const Bounds wb = wave_bounds(w);
   const Bounds gb = group_bounds(wb, sB, wave);
-  if (MOD && a.rel_bias) bias.fill(a, head0, g.pack);
-  const float *tab = bias.table + (g.pack > 1 ? (w.h - head0) * a.n_buckets : 0);
+  if (MOD && a.rel_bias) bias.fill(a, head0, 1);
+  const float *tab = bias.table;
 
   const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)w.h * a.q_hs;
   V8 fq[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
 
-  f32x16 acc[ND];
+  FwdState<T, D> st;
 #pragma unroll
-  for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
-  float m = -INFINITY, l = 0.f;
+  for (int d = 0; d < D / 32; ++d) st.acc[d] = f32x16{};
+  st.m = -INFINITY, st.l = 0.f;
   const ScoreCtx sc = score_ctx(a);
 
   const int tiles = (gb.hi_max + BK - 1) / BK, per = (tiles + g.nsplit - 1) / g.nsplit;
@@ -190,14 +306,13 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     const int k0 = t * BK;
     const bool mixed = it.mixed(), dead = it.cur_dead != 0;
     char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
-    dma_wait();
+    dma_wait<0>();
     __syncthreads();                                     // the tile is here, and nobody reads the other buffer any more
     if (mixed) {
       if (threadIdx.x < BK) sDoc[threadIdx.x] = k0 + (int)threadIdx.x < a.Lk ? kdoc[k0 + threadIdx.x] : -1;
       __syncthreads();
     }
-    if (k0 + BK > len || (mixed && dead)) {
-      zero_rows<T, D>(sK, len - k0, mixed ? sDoc : nullptr);
+    if (k0 + BK > len || (mixed && dead)) {              // (a key row only reaches scores that are masked: V alone)
       zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
       __syncthreads();
     }
@@ -208,102 +323,125 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     }
     if (k0 < wb.hi_max) {
       const bool need_mask = k0 + BK > wb.hi_min || mixed;
-      float x[NK * 16];
+      const int far = !(MOD && a.rel_bias) ? 0 : k0 + BK - 1 - wb.p_min <= -a.reach ? -1 : k0 - wb.p_max >= a.reach ? 1 : 0;
+      // modified scores: 32 keys at a time (the modification needs the registers); else all of the tile
+      constexpr int NK = MOD ? 1 : BK / 32;
 #pragma unroll
-      for (int kt = 0; kt < NK; ++kt) {
-        f32x16 s = {};
-#pragma unroll
-        for (int c = 0; c < NC; ++c) s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[16 * kt + i] = s[i];
-      }
-      float cf = sc.c_scale;
-      if constexpr (MOD) {
-        const int far = !a.rel_bias ? 0 : k0 + BK - 1 - wb.p_min <= -a.reach ? -1 : k0 - wb.p_max >= a.reach ? 1 : 0;
-#pragma unroll
-        for (int kt = 0; kt < NK; ++kt)
-          modify<16, false>(a, sc, x + 16 * kt, nullptr, k0 + 32 * kt + 4 * h - w.p, 1, w.slope, tab, bias.bucket, far);
-        cf = 1.f;
-      }
-      if (need_mask) {
-#pragma unroll
-        for (int i = 0; i < NK * 16; ++i) {
-          const int j = 32 * (i >> 4) + acc_row(i & 15, h);
-          bool see = k0 + j < w.hi;
-          if (mixed) see = see && sDoc[j] == w.doc;
-          if (!see) x[i] = -INFINITY;
-        }
-      }
-      float mx = x[0];
-#pragma unroll
-      for (int i = 1; i < NK * 16; ++i) mx = fmaxf(mx, x[i]);
-      const float m_new = fmaxf(m, half_max(mx) * cf);
-      const float ms = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = ex2(m - ms);
-      m = m_new;
-      const float off = Elem<T>::PSHIFT - ms;
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < NK * 16; ++i) {
-        x[i] = ex2(fmaf(x[i], cf, off));
-        sum += x[i];
-      }
-      l = fmaf(l, alpha, sum);
-      if (__any(alpha != 1.f)) {
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
-      }
-#pragma unroll
-      for (int c = 0; c < NK * 2; ++c) {
-        const V8 p = round8<T>(x + 8 * c);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = Elem<T>::mma(col_frag<T, D>(sV, 16 * c, d, lane), p, acc[d]);
+      for (int kt = 0; kt < BK / 32; kt += NK) {
+        float x[NK * 16];
+        fwd_products<T, D, NK>(x, fq, sK + kt * 32 * L::NS * 16, lane);
+        fwd_softmax<T, D, MOD, NK>(st, x, k0 + 32 * kt, w, a, sc, tab, bias.bucket, far, need_mask, mixed ? sDoc + 32 * kt : nullptr, h);
+        fwd_values<T, D, NK>(st, x, sV + kt * 32 * L::NS * 16, lane);
       }
     }
     t = tn;
     buf ^= 1;
   }
-  l = half_sum(l);
-  if (!w.valid) return;
-  const int64_t r = ((int64_t)b * a.H + w.h) * a.Lq + w.i;
-  if (g.nsplit > 1) {
-    const int64_t rs = (int64_t)split * a.B * a.H * a.Lq + r;
-    if (h == 0) {
-      g.part_ml[2 * rs] = w.live ? m : -INFINITY;
-      g.part_ml[2 * rs + 1] = w.live ? l : 0.f;
-    }
-    float *o = g.part_o + rs * a.dh;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int dim = 32 * d + 8 * q + 4 * h;
-        if (dim < a.dh) *(f32x4 *)(o + dim) = f32x4{acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]};
-      }
-    return;
+  fwd_store(g, st, w, b, split, h);
+}
+
+// Few queries (all rows that share a key head fit into 32): the rows are the same for all four waves, which deal the keys among
+// themselves, 32 at a time, and meet at the end, where their maxima, sums and accumulators are joined.  Each has one buffer for K and
+// one for V: the next keys are requested as soon as the products have been taken from the buffer, the next values after theirs, so
+// that up to 32 KiB per wave and, with two workgroups, 128 KiB per CU are on their way.  Bound by reading the cache.
+template <typename T, int D, bool MOD>
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_few_kernel(const Args g) {
+  typedef Tile<T, D> L;
+  typedef typename Elem<T>::V8 V8;
+  constexpr int BK = 32, NC = D / 16, ND = D / 32, TILE = BK * L::NS * 16;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const mmt_long_attention &a = g.a;
+  int *sDocs = (int *)(smem + 2 * WAVES * TILE);
+  BiasLds bias;
+  bias.table = (float *)(sDocs + BK * WAVES);
+  bias.bucket = (unsigned char *)(bias.table + (MOD && a.rel_bias ? g.pack * a.n_buckets : 0));
+  const int grp = blockIdx.x % g.groups, split = blockIdx.x / g.groups, kh = grp % a.Hk, b = grp / a.Hk, head0 = kh * g.G;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+  const int len = row_len(a, b);
+  const Row w = make_row(g, b, head0, col, len);
+  const Bounds wb = wave_bounds(w);
+  if (MOD && a.rel_bias) {
+    bias.fill(a, head0, g.pack);
+    __syncthreads();
   }
-  const bool some = w.live && l != 0.f;                   // (a NaN sum is "some")
-  const float inv = some ? 1.f / l : 0.f;
-  if (g.lse && h == 0) g.lse[r] = some ? (m + log2f(l) - Elem<T>::PSHIFT) * LN2 : -INFINITY;
-  const int64_t o = (((int64_t)b * a.Lq + w.i) * a.H + w.h) * a.dh;
+  const float *tab = bias.table + (w.valid ? w.h - head0 : 0) * a.n_buckets;
+  const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)w.h * a.q_hs;
+  V8 fq[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
+  FwdState<T, D> st;
+#pragma unroll
+  for (int d = 0; d < ND; ++d) st.acc[d] = f32x16{};
+  st.m = -INFINITY, st.l = 0.f;
+  const ScoreCtx sc = score_ctx(a);
+  const int tiles = (wb.hi_max + BK - 1) / BK, workers = g.nsplit * WAVES;
+  const int *kdoc = a.k_doc ? a.k_doc + (int64_t)b * a.Lk : nullptr;
+  Dma<T, D, BK, 64> dk, dv;
+  dk.init((const T *)a.k + (int64_t)b * a.k_bs + (int64_t)kh * a.k_hs, a.k_rs, a.Lk, a.dh);
+  dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
+  char *sK = smem + wave * 2 * TILE, *sV = sK + TILE;
+  int *sDoc = sDocs + wave * BK;
+  const unsigned lds = lds_address(sK);
+  int t = split * WAVES + wave;                           // neighbouring tiles go to neighbouring waves
+  if (t < tiles) {
+    dk.load(lds, t * BK);
+    dv.load(lds + TILE, t * BK);
+  }
+  while (t < tiles) {
+    const int k0 = t * BK, tn = t + workers;
+    const int doc = kdoc && lane < BK && k0 + lane < a.Lk ? kdoc[k0 + lane] : -1;
+    const int far = !(MOD && a.rel_bias) ? 0 : k0 + BK - 1 - wb.p_min <= -a.reach ? -1 : k0 - wb.p_max >= a.reach ? 1 : 0;
+    // requests complete in order: all but the newest tile (the values asked for after these keys, the keys asked for after these values)
+    dma_wait<dv.N>();
+    float x[16];
+    fwd_products<T, D, 1>(x, fq, sK, lane);
+    wave_sync();                                          // the keys have been read
+    if (tn < tiles) dk.load(lds, tn * BK);
+    if (kdoc) {
+      if (lane < BK) sDoc[lane] = doc;
+      wave_sync();
+    }
+    fwd_softmax<T, D, MOD, 1>(st, x, k0, w, a, sc, tab, bias.bucket, far, k0 + BK > wb.hi_min || kdoc, kdoc ? sDoc : nullptr, h);
+    if (tn < tiles) dma_wait<dk.N>();
+    else dma_wait<0>();
+    if (k0 + BK > len || kdoc) {
+      zero_rows<T, D, BK, 64>(sV, len - k0, kdoc ? sDoc : nullptr);
+      wave_sync();
+    }
+    fwd_values<T, D, 1>(st, x, sV, lane);
+    wave_sync();                                          // the values have been read
+    if (tn < tiles) dv.load(lds + TILE, tn * BK);
+    t = tn;
+  }
+  // join the waves: weights 2^(m_w - max m); accumulators through LDS (the tiles are done with)
+  __syncthreads();
+  float *sM = (float *)smem, *sL = sM + 64 * WAVES, *sA = sL + 64 * WAVES;       // [wave][lane], [wave][register][lane]
+  sM[wave * 64 + lane] = st.m;
+  __syncthreads();
+  float m = sM[lane];
+#pragma unroll
+  for (int u = 1; u < WAVES; ++u) m = fmaxf(m, sM[u * 64 + lane]);
+  const float f = m == -INFINITY ? 0.f : ex2(st.m - m);
+  st.m = m;
+  sL[wave * 64 + lane] = st.l * f;
+  // one block of 32 dimensions at a time; wave u adds the four waves' copies of block u and keeps the sum
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int dim = 32 * d + 8 * q + 4 * h;
-      if (dim < a.dh) {
-        typename Elem<T>::V4 v, lo;
+    for (int i = 0; i < 16; ++i) sA[((wave * ND + d) * 16 + i) * 64 + lane] = st.acc[d][i] * f;
+  __syncthreads();
+  st.l = sL[lane] + sL[64 + lane] + sL[128 + lane] + sL[192 + lane];
+  if (wave != 0) return;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y = some ? acc[d][4 * q + e] * inv : 0.f;
-          v[e] = (T)y, lo[e] = (T)(y - (float)v[e]);
-        }
-        *(typename Elem<T>::V4 *)((T *)g.out + o + dim) = v;
-        if (g.low) *(typename Elem<T>::V4 *)((T *)g.low + o + dim) = lo;
-      }
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float v = 0.f;
+#pragma unroll
+      for (int u = 0; u < WAVES; ++u) v += sA[((u * ND + d) * 16 + i) * 64 + lane];
+      st.acc[d][i] = v;
     }
+  fwd_store(g, st, w, b, split, h);
 }
 
 // Joins the splits of a row: weights 2^(m_s - max m).  16 lanes per row, up to 8 elements per lane.
@@ -507,7 +645,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     const int k0 = t * BK;
     const bool mixed = it.mixed(), dead = it.cur_dead != 0;
     char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
-    dma_wait();
+    dma_wait<0>();
     __syncthreads();
     if (mixed) {
       if (threadIdx.x < BK) sDoc[threadIdx.x] = k0 + (int)threadIdx.x < a.Lk ? kdoc[k0 + threadIdx.x] : -1;
@@ -724,7 +862,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
       sDoc[threadIdx.x] = doc_next;
       sStat[threadIdx.x] = st_next;
     }
-    dma_wait();
+    dma_wait<0>();
     __syncthreads();
     if (q0 + BQ > a.Lq || dead) {
       zero_rows<T, D>(sQ, a.Lq - q0, sDoc);
@@ -888,7 +1026,7 @@ __global__ void __launch_bounds__(THREADS, 1) mmt_long_attn_table_kernel(const A
     dk.load(lds, k0);
     dv.load(lds + L::BYTES, k0);
     if (kdoc && threadIdx.x < BK) sDoc[threadIdx.x] = k0 + (int)threadIdx.x < a.Lk ? kdoc[k0 + threadIdx.x] : -1;
-    dma_wait();
+    dma_wait<0>();
     __syncthreads();
     if (k0 + BK > len || kdoc) {
       zero_rows<T, D>(sK, len - k0, kdoc ? sDoc : nullptr);
@@ -958,7 +1096,14 @@ template <typename K> static void launch(K kernel, int64_t grid, size_t lds, hip
 static inline bool modified(const mmt_long_attention &a) { return a.softcap > 0.f || a.slopes || a.rel_bias; }
 
 template <typename T, int D> static void fwd_size(const Args &g, hipStream_t st) {
-  const size_t lds = 4 * Tile<T, D>::BYTES + 4 * Tile<T, D>::BK + 24 * WAVES + bias_lds_bytes(g.a, g.pack);
+  if (g.few) {
+    const size_t tiles = 2 * WAVES * 32 * Tile<T, D>::NS * 16 + 4 * 32 * WAVES + bias_lds_bytes(g.a, g.pack);
+    const size_t join = 4 * 64 * WAVES * (2 + D / 2), lds = tiles > join ? tiles : join;
+    if (modified(g.a)) launch(mmt_long_attn_few_kernel<T, D, true>, g.items, lds, st, g);
+    else launch(mmt_long_attn_few_kernel<T, D, false>, g.items, lds, st, g);
+    return;
+  }
+  const size_t lds = 4 * Tile<T, D>::BYTES + 4 * Tile<T, D>::BK + 24 * WAVES + bias_lds_bytes(g.a, 1);
   if (modified(g.a)) launch(mmt_long_attn_fwd_kernel<T, D, true>, g.items, lds, st, g);
   else launch(mmt_long_attn_fwd_kernel<T, D, false>, g.items, lds, st, g);
 }

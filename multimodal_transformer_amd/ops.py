@@ -796,8 +796,6 @@ def _head_rows(t, name, shape, dtype, device):
                 t = t.clone()
             b, r, h, _ = t.stride()
             p = t.data_ptr()
-            if ((b | r | h) & odd) or r >= 1 << 24:      # head sizes and widths that the library refuses
-                b, r, h = b & ~odd, min(r & ~odd, (1 << 24) - 1 - odd), h & ~odd
     return t, p, b, r, h
 
 
