@@ -611,7 +611,7 @@ int mmt_lane_gather(const double *table, const double *lanes, const int64_t *row
  * head stride (elements) that keeps them at multiples of 16 bytes, token strides below 2^24; a stride of 0 broadcasts.  out (B,Lq,H,dh) and lse (B,H,Lq; may
  * be NULL) contiguous.  Keys at j >= n and keys and queries with a negative id are never multiplied with anything: they may hold
  * NaN.  Bucket numbers are clamped to 0..n_buckets-1, lengths to 0..Lk.  Limits: dh a multiple of 8 up to 128, n_buckets <= 64,
- * reach <= 4096, (H / Hk) n_buckets <= 8192.  Sums, statistics and the products' accumulators are fp32; the probabilities and the
+ * reach <= 1024.  Sums, statistics and the products' accumulators are fp32; the probabilities and the
  * score gradients are rounded to the element type where they enter the second product.
  * fwd: out_low (like out, may be NULL) receives what rounding took from out, rounded to the element type itself: with it the
  * backward forms rowsum(dout out) to twice the digits, which rows that see few keys need.

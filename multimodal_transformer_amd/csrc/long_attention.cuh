@@ -87,9 +87,10 @@ template <typename T, int D> struct Tile {
   static constexpr int NS = DS / EPS;
   static constexpr int BK = Elem<T>::BK;
   static constexpr int BYTES = BK * NS * 16;
+  static constexpr int PERIOD = sizeof(T) == 4 ? (NS == 8 ? 16 : 8) : 16;     // swz depends on row % PERIOD
   static __device__ __forceinline__ int swz(int row, int slot) {
     if constexpr (sizeof(T) == 4) {
-      return slot ^ (NS >= 16 ? (row & 15) : ((row >> 1) & 7));
+      return slot ^ (NS >= 16 ? (row & 7) : ((row >> 1) & 7));
     } else {
       if constexpr (NS == 16) return slot ^ (((row & 3) << 2) | ((row >> 2) & 3));
       else if constexpr (NS == 8) return slot ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
@@ -166,21 +167,23 @@ __device__ __forceinline__ unsigned lds_address(const void *p) {
 // Tiles of a (rows, dh) matrix on their way to LDS.  A lane's byte offset inside a tile is the same for every tile; the tile's own
 // part is a scalar.  Slots at and beyond dh repeat slot 0 and rows at and beyond n_rows the last row (nothing outside the tensor is
 // read); the operands these elements meet are zero, or results nobody stores.
-// NT threads (the workgroup, or one wave) move tiles of R rows.
+// NT threads (the workgroup, or one wave) move tiles of R rows, NT / NS rows at a time; where the exclusive or of a row repeats after
+// as many rows, the steps differ by a scalar and one offset serves them all.
 template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS> struct Dma {
   typedef Tile<T, D> L;
-  static constexpr int N = R * L::NS / NT;
-  static_assert(N * NT == R * L::NS, "a tile is a whole number of 16-byte loads per thread");
+  static constexpr int N = R * L::NS / NT, STEP = NT / L::NS;
+  static constexpr bool ONE = STEP % L::PERIOD == 0;
+  static_assert(N * NT == R * L::NS && STEP * L::NS == NT, "a tile is a whole number of 16-byte loads per thread");
   const char *base;
   int64_t rs;                        // bytes between rows; 64 rows stay below 2^31 bytes
   int n_rows;
-  unsigned off[N];
+  unsigned off[ONE ? 1 : N];
   __device__ __forceinline__ void init(const T *p, int64_t row_stride, int rows, int dh) {
     base = (const char *)p, rs = row_stride * (int64_t)sizeof(T), n_rows = rows;
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
+    for (int n = 0; n < (ONE ? 1 : N); ++n) {
       const int idx = threadIdx.x % NT + n * NT, row = idx / L::NS, slot = L::swz(row, idx % L::NS);
-      off[n] = (unsigned)(row * rs) + (slot * L::EPS < dh ? slot * 16 : 0);
+      off[n] = (unsigned)((ONE ? row : row - n * STEP) * rs) + (slot * L::EPS < dh ? slot * 16 : 0);
     }
   }
   __device__ __forceinline__ void load(unsigned lds, int r0) const {
@@ -188,12 +191,13 @@ template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS> struct Dm
     const unsigned mine = __builtin_amdgcn_readfirstlane(lds + ((threadIdx.x % NT) >> 6) * 1024);
     if (r0 + R <= n_rows) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) dma16(b, off[n], mine + n * NT * 16);
+      for (int n = 0; n < N; ++n) dma16(b + n * STEP * rs, off[ONE ? 0 : n], mine + n * NT * 16);
     } else {
+      // the rows beyond the last one repeat it
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const int row = (int)(threadIdx.x % NT + n * NT) / L::NS, over = max(0, r0 + row - (n_rows - 1));
-        dma16(b, off[n] - (unsigned)(over * rs), mine + n * NT * 16);
+        const int row = (int)(threadIdx.x % NT) / L::NS + n * STEP, over = max(0, r0 + row - (n_rows - 1));
+        dma16(b, off[ONE ? 0 : n] + (unsigned)(n * STEP * rs) - (unsigned)(over * rs), mine + n * NT * 16);
       }
     }
   }

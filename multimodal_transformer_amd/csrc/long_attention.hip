@@ -27,10 +27,8 @@ static int check(const mmt_long_attention *a, const char *who) {
   if (a->prefix && !a->causal) return mmt_set_error(MMT_EINVAL, "%s: a prefix is an exception from the causal mask", who);
   if (!a->q_doc != !a->k_doc) return mmt_set_error(MMT_EINVAL, "%s: documents need ids for the queries and the keys", who);
   if (!a->rel_bias != !a->rel_buckets) return mmt_set_error(MMT_EINVAL, "%s: a learned bias needs its table and its buckets", who);
-  if (a->rel_bias && (a->n_buckets < 1 || a->n_buckets > 64 || a->reach < 1 || a->reach > 4096))
-    return mmt_set_error(MMT_EINVAL, "%s: need 1..64 buckets and a reach of 1..4096", who);
-  if (a->rel_bias && (int64_t)(a->H / a->Hk) * a->n_buckets > 8192)
-    return mmt_set_error(MMT_EINVAL, "%s: at most 8192 bias entries per key head", who);
+  if (a->rel_bias && (a->n_buckets < 1 || a->n_buckets > 64 || a->reach < 1 || a->reach > 1024))
+    return mmt_set_error(MMT_EINVAL, "%s: need 1..64 buckets and a reach of 1..1024", who);
   if (a->Lk > (1 << 30) || a->Lq > (1 << 30)) return mmt_set_error(MMT_EINVAL, "%s: at most 2^30 tokens per row", who);
   const int64_t unit = 16 / elem_size(a->dtype);
   if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & 15 ||

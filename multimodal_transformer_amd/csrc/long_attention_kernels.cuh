@@ -64,29 +64,46 @@ __device__ __forceinline__ Bounds group_bounds(const Bounds &w, int *s, int wave
   return b;
 }
 
-// The learned bias in LDS: the table rows of the workgroup's heads (in units of log 2) and the bucket of each clamped distance.
-// Bucket numbers outside the table are clamped into it.  An entry at or below -2^100 (the lowest value of a type, used as a mask) is
-// taken for -inf: next to it a score vanishes in rounding, and the saved log-sum of a row of such entries could not tell them apart.
-struct BiasLds {
-  float *table;             // [pack][nb]
-  unsigned char *bucket;    // [2 reach + 1]
-  __device__ __forceinline__ void fill(const mmt_long_attention &a, int head0, int pack) {
-    for (int n = threadIdx.x; n < pack * a.n_buckets; n += THREADS) {
-      const float v = a.rel_bias[(int64_t)(head0 + n / a.n_buckets) * a.n_buckets + n % a.n_buckets];
-      table[n] = v <= -0x1p100f ? -INFINITY : v * LOG2E;
+// The learned bias in LDS, in units of log 2.  Bucket numbers outside the table are clamped into it.  An entry at or below -2^100 (the
+// lowest value of a type, used as a mask) is taken for -inf: next to it a score vanishes in rounding, and the saved log-sum of a row
+// of such entries could not tell them apart.
+__device__ __forceinline__ float bias_entry(const mmt_long_attention &a, int head, int bucket) {
+  const float v = a.rel_bias[(int64_t)head * a.n_buckets + bucket];
+  return v <= -0x1p100f ? -INFINITY : v * LOG2E;
+}
+__device__ __forceinline__ int bias_bucket(const mmt_long_attention &a, int d) {
+  return max(0, min(a.rel_buckets[max(-a.reach, min(a.reach, d)) + a.reach], a.n_buckets - 1));
+}
+// One head: the bias of every distance from -reach - PAD to reach + PAD, so that a tile that is not wholly beyond the reach finds all
+// of its distances (128 rows x 64 keys span 190) at constant steps from one address.
+constexpr int PAD = 192;
+struct Lut {
+  float *mid;                      // of distance 0
+  static __host__ __device__ int floats(const mmt_long_attention &a) { return a.rel_bias ? (2 * (a.reach + PAD) + 4) & ~3 : 0; }
+  __device__ __forceinline__ void fill(const mmt_long_attention &a, int head) const {
+    for (int n = threadIdx.x; n < 2 * (a.reach + PAD) + 1; n += blockDim.x) {
+      const int d = n - a.reach - PAD;
+      mid[d] = bias_entry(a, head, bias_bucket(a, d));
     }
-    for (int n = threadIdx.x; n < 2 * a.reach + 1; n += THREADS)
-      bucket[n] = (unsigned char)max(0, min(a.rel_buckets[n], a.n_buckets - 1));
   }
 };
-static inline __host__ __device__ int bias_lds_bytes(const mmt_long_attention &a, int pack) {
-  return a.rel_bias ? pack * a.n_buckets * 4 + ((2 * a.reach + 1 + 15) & ~15) : 0;
-}
+// Several heads (few queries): their table rows, and the bucket of each clamped distance
+struct PackedBias {
+  float *table;                    // [pack][n_buckets]
+  unsigned char *bucket;           // [2 reach + 1]
+  static __host__ __device__ int bytes(const mmt_long_attention &a, int pack) {
+    return a.rel_bias ? pack * a.n_buckets * 4 + ((2 * a.reach + 1 + 15) & ~15) : 0;
+  }
+  __device__ __forceinline__ void fill(const mmt_long_attention &a, int head0, int pack) {
+    for (int n = threadIdx.x; n < pack * a.n_buckets; n += blockDim.x) table[n] = bias_entry(a, head0 + n / a.n_buckets, n % a.n_buckets);
+    for (int n = threadIdx.x; n < 2 * a.reach + 1; n += blockDim.x) bucket[n] = (unsigned char)bias_bucket(a, n - a.reach);
+  }
+};
 
 // Raw products -> modified scores in units of log 2; `t` receives tanh(s / cap) when the scores are capped and the caller needs it.
 struct ScoreCtx {
   float c_scale, cap_in, cap_out;  // scale log2 e; scale / cap; cap log2 e
-  bool capped, rel;
+  bool capped, rel, sloped;
 };
 __device__ __forceinline__ ScoreCtx score_ctx(const mmt_long_attention &a) {
   ScoreCtx s;
@@ -95,38 +112,76 @@ __device__ __forceinline__ ScoreCtx score_ctx(const mmt_long_attention &a) {
   s.cap_in = s.capped ? a.scale / a.softcap : 0.f;
   s.cap_out = a.softcap * LOG2E;
   s.rel = a.rel_bias != nullptr;
+  s.sloped = a.slopes != nullptr;
   return s;
 }
-
-// x: N raw products of a lane, element i belongs to the distance d0 + step (8 (i / 4) + i % 4); far: the whole tile lies beyond the
-// reach on one side (-1 behind, 1 ahead): one bucket
-template <int N, bool KEEP>
-__device__ __forceinline__ void modify(const mmt_long_attention &a, const ScoreCtx &sc, float *x, float *t, int d0, int step, float slope,
-                                       const float *tab, const unsigned char *bucket, int far) {
+// where a tile lies: d_lo .. d_hi is the range of its distances over the wave's rows
+struct Place {
+  int far;                         // wholly beyond the reach: -1 behind, 1 ahead; 0 within it
+  int side;                        // distances of one sign: -1 none positive, 1 none negative; 0 both
+};
+__device__ __forceinline__ Place place(const mmt_long_attention &a, int d_lo, int d_hi) {
+  Place p;
+  p.far = d_hi <= -a.reach ? -1 : d_lo >= a.reach ? 1 : 0;
+  p.side = d_hi <= 0 ? -1 : d_lo >= 0 ? 1 : 0;
+  return p;
+}
+// x: 16 raw products of a lane, element i belongs to the distance d0 + STEP (8 (i / 4) + i % 4), STEP 1 or -1.
+// One multiplication and addition takes up the scale, the bias of a tile beyond the reach and, with distances of one sign, the lane's
+// part of the slope; what is left of the slope is a constant per element.
+template <int STEP, bool KEEP, bool PACKED>
+__device__ __forceinline__ void modify(const mmt_long_attention &a, const ScoreCtx &sc, float *x, float *t, int d0, float slope, const float *lut,
+                                       const unsigned char *bucket, Place at) {
+  float mul = sc.c_scale, add = 0.f;
   if (sc.capped) {
-    tanh_scores<N>(x, sc.cap_in);
+    tanh_scores<16>(x, sc.cap_in);
+    if (KEEP) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (KEEP) t[i] = x[i];
-      x[i] *= sc.cap_out;
+      for (int i = 0; i < 16; ++i) t[i] = x[i];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] *= sc.c_scale;
+    mul = sc.cap_out;
   }
-  if (a.slopes) {
+  if (sc.rel && at.far != 0) add = PACKED ? lut[bucket[at.far < 0 ? 0 : 2 * a.reach]] : lut[at.far < 0 ? -a.reach : a.reach];
+  const float s1 = at.side < 0 ? slope : -slope;          // u += s1 * distance
+  if (sc.sloped && at.side != 0) add = fmaf(s1, (float)d0, add);
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = fmaf(-slope, fabsf((float)(d0 + step * (8 * (i >> 2) + (i & 3)))), x[i]);
-  }
-  if (sc.rel) {
-    if (far != 0) {
-      const float v = tab[bucket[far < 0 ? 0 : 2 * a.reach]];
+  for (int i = 0; i < 16; ++i) x[i] = fmaf(x[i], mul, add);
+  if (sc.sloped) {
+    if (at.side != 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] += v;
+      for (int i = 0; i < 16; ++i) x[i] = fmaf(s1, (float)(STEP * (8 * (i >> 2) + (i & 3))), x[i]);
     } else {
+      const float f0 = (float)d0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] += tab[bucket[max(-a.reach, min(a.reach, d0 + step * (8 * (i >> 2) + (i & 3)))) + a.reach]];
+      for (int i = 0; i < 16; ++i) x[i] = fmaf(-slope, fabsf(f0 + (float)(STEP * (8 * (i >> 2) + (i & 3)))), x[i]);
     }
+  }
+  if (sc.rel && at.far == 0) {
+    if constexpr (PACKED) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] += lut[bucket[max(-a.reach, min(a.reach, d0 + STEP * (8 * (i >> 2) + (i & 3)))) + a.reach]];
+    } else {
+      // (rows that are not live may stand anywhere: their address is held inside the table)
+      const int lo = max(-a.reach - PAD, min(a.reach + PAD - 27, STEP > 0 ? d0 : d0 - 27));
+      const float *p = lut + lo;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int e = 8 * (i >> 2) + (i & 3);
+        x[i] += p[STEP > 0 ? e : 27 - e];
+      }
+    }
+  }
+}
+// what a row does not see -> -inf; key j of the sub-tile is the accumulator's row
+__device__ __forceinline__ void mask_keys(float *x, int key0, int hi, const int *sDoc, int doc, int h) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = key0 + acc_row(i, h) < hi ? x[i] : -INFINITY;
+  if (sDoc) {
+    int id[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) id[i] = sDoc[acc_row(i, h)];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = id[i] == doc ? x[i] : -INFINITY;
   }
 }
 
@@ -149,25 +204,20 @@ __device__ __forceinline__ void fwd_products(float *x, const typename Elem<T>::V
   }
 }
 // products -> probabilities (not yet divided by their sum)
-template <typename T, int D, bool MOD, int NK>
+template <typename T, int D, bool MOD, bool PACKED, int NK>
 __device__ __forceinline__ void fwd_softmax(FwdState<T, D> &st, float *x, int key0, const Row &w, const mmt_long_attention &a, const ScoreCtx &sc,
-                                            const float *tab, const unsigned char *bucket, int far, bool need_mask, const int *sDoc, int h) {
+                                            const float *lut, const unsigned char *bucket, Place at, bool need_mask, const int *sDoc, int h) {
   constexpr int ND = D / 32;
   float cf = sc.c_scale;
   if constexpr (MOD) {
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt)
-      modify<16, false>(a, sc, x + 16 * kt, nullptr, key0 + 32 * kt + 4 * h - w.p, 1, w.slope, tab, bucket, far);
+      modify<1, false, PACKED>(a, sc, x + 16 * kt, nullptr, key0 + 32 * kt + 4 * h - w.p, w.slope, lut, bucket, at);
     cf = 1.f;
   }
   if (need_mask) {
 #pragma unroll
-    for (int i = 0; i < NK * 16; ++i) {
-      const int j = 32 * (i >> 4) + acc_row(i & 15, h);
-      bool see = key0 + j < w.hi;
-      if (sDoc) see = see && sDoc[j] == w.doc;
-      if (!see) x[i] = -INFINITY;
-    }
+    for (int kt = 0; kt < NK; ++kt) mask_keys(x + 16 * kt, key0 + 32 * kt, w.hi, sDoc ? sDoc + 32 * kt : nullptr, w.doc, h);
   }
   float mx = x[0];
 #pragma unroll
@@ -258,8 +308,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
   int *sDoc = (int *)(smem + 4 * L::BYTES), *sB = sDoc + BK;
-  BiasLds bias;
-  bias.table = (float *)(sB + 6 * WAVES);
+  const Lut lut = {(float *)(sB + 6 * WAVES) + a.reach + PAD};
   const int grp = blockIdx.x % g.groups;
   int n = blockIdx.x / g.groups;
   const int split = n % g.nsplit;
@@ -269,14 +318,12 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   if (a.causal) qt = g.nqt - 1 - qt;                     // the tiles with the most keys first
   const int kh = grp % a.Hk, b = grp / a.Hk;
   const int head0 = kh * g.G + gi;
-  bias.bucket = (unsigned char *)(bias.table + (MOD && a.rel_bias ? a.n_buckets : 0));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
   const int len = row_len(a, b);
   const Row w = make_row(g, b, head0, qt * ROWS + wave * 32 + col, len);
   const Bounds wb = wave_bounds(w);
   const Bounds gb = group_bounds(wb, sB, wave);
-  if (MOD && a.rel_bias) bias.fill(a, head0, 1);
-  const float *tab = bias.table;
+  if (MOD && a.rel_bias) lut.fill(a, head0);
 
   const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)w.h * a.q_hs;
   V8 fq[NC];
@@ -323,14 +370,14 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     }
     if (k0 < wb.hi_max) {
       const bool need_mask = k0 + BK > wb.hi_min || mixed;
-      const int far = !(MOD && a.rel_bias) ? 0 : k0 + BK - 1 - wb.p_min <= -a.reach ? -1 : k0 - wb.p_max >= a.reach ? 1 : 0;
+      const Place at = place(a, k0 - wb.p_max, k0 + BK - 1 - wb.p_min);
       // modified scores: 32 keys at a time (the modification needs the registers); else all of the tile
       constexpr int NK = MOD ? 1 : BK / 32;
 #pragma unroll
       for (int kt = 0; kt < BK / 32; kt += NK) {
         float x[NK * 16];
         fwd_products<T, D, NK>(x, fq, sK + kt * 32 * L::NS * 16, lane);
-        fwd_softmax<T, D, MOD, NK>(st, x, k0 + 32 * kt, w, a, sc, tab, bias.bucket, far, need_mask, mixed ? sDoc + 32 * kt : nullptr, h);
+        fwd_softmax<T, D, MOD, false, NK>(st, x, k0 + 32 * kt, w, a, sc, lut.mid, nullptr, at, need_mask, mixed ? sDoc + 32 * kt : nullptr, h);
         fwd_values<T, D, NK>(st, x, sV + kt * 32 * L::NS * 16, lane);
       }
     }
@@ -352,7 +399,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
   int *sDocs = (int *)(smem + 2 * WAVES * TILE);
-  BiasLds bias;
+  PackedBias bias;
   bias.table = (float *)(sDocs + BK * WAVES);
   bias.bucket = (unsigned char *)(bias.table + (MOD && a.rel_bias ? g.pack * a.n_buckets : 0));
   const int grp = blockIdx.x % g.groups, split = blockIdx.x / g.groups, kh = grp % a.Hk, b = grp / a.Hk, head0 = kh * g.G;
@@ -390,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   while (t < tiles) {
     const int k0 = t * BK, tn = t + workers;
     const int doc = kdoc && lane < BK && k0 + lane < a.Lk ? kdoc[k0 + lane] : -1;
-    const int far = !(MOD && a.rel_bias) ? 0 : k0 + BK - 1 - wb.p_min <= -a.reach ? -1 : k0 - wb.p_max >= a.reach ? 1 : 0;
+    const Place at = place(a, k0 - wb.p_max, k0 + BK - 1 - wb.p_min);
     // requests complete in order: all but the newest tile (the values asked for after these keys, the keys asked for after these values)
     dma_wait<dv.N>();
     float x[16];
@@ -401,7 +448,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
       if (lane < BK) sDoc[lane] = doc;
       wave_sync();
     }
-    fwd_softmax<T, D, MOD, 1>(st, x, k0, w, a, sc, tab, bias.bucket, far, k0 + BK > wb.hi_min || kdoc, kdoc ? sDoc : nullptr, h);
+    fwd_softmax<T, D, MOD, true, 1>(st, x, k0, w, a, sc, tab, bias.bucket, at, k0 + BK > wb.hi_min || kdoc, kdoc ? sDoc : nullptr, h);
     if (tn < tiles) dma_wait<dk.N>();
     else dma_wait<0>();
     if (k0 + BK > len || kdoc) {
@@ -597,9 +644,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
   int *sDoc = (int *)(smem + 4 * L::BYTES), *sB = sDoc + BK;
-  BiasLds bias;
-  bias.table = (float *)(sB + 6 * WAVES);
-  bias.bucket = (unsigned char *)(bias.table + (MOD && a.rel_bias ? a.n_buckets : 0));
+  const Lut lut = {(float *)(sB + 6 * WAVES) + a.reach + PAD};
   const int grp = blockIdx.x % g.groups, n = blockIdx.x / g.groups, gi = n % g.G;
   int qt = n / g.G;
   if (a.causal) qt = g.nqt - 1 - qt;
@@ -609,7 +654,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   const Row w = make_row(g, b, head, qt * ROWS + wave * 32 + col, len);
   const Bounds wb = wave_bounds(w);
   const Bounds gb = group_bounds(wb, sB, wave);
-  if (MOD && a.rel_bias) bias.fill(a, head, 1);
+  if (MOD && a.rel_bias) lut.fill(a, head);
   const int64_t r = ((int64_t)b * a.H + head) * a.Lq + min(w.i, a.Lq - 1);
   const float2 st = w.live ? g.stat[r] : make_float2(INFINITY, 0.f);
 
@@ -664,45 +709,38 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     if (k0 < wb.hi_max) {
       const bool need_mask = k0 + BK > wb.hi_min || mixed;
       // by the whole workgroup's rows: the table kernel takes the tiles that are left with the same rule
-      const int far = !(MOD && a.rel_bias) ? 0 : k0 + BK - 1 - gb.p_min <= -a.reach ? -1 : k0 - gb.p_max >= a.reach ? 1 : 0;
-#pragma unroll
+      const Place at = place(a, k0 - gb.p_max, k0 + BK - 1 - gb.p_min);
+#pragma unroll 1
       for (int kt = 0; kt < NK; ++kt) {
+        // (the two products one after the other where registers are short: what is live grows with how far the compiler pulls them together)
         f32x16 s = {}, dp = {};
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s);
-          dp = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp);
-        }
+        for (int c = 0; c < NC; ++c) s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s);
         float x[16], th[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = s[i];
         float cf = sc.c_scale;
         if constexpr (MOD) {
-          modify<16, true>(a, sc, x, th, k0 + 32 * kt + 4 * h - w.p, 1, w.slope, bias.table, bias.bucket, far);
+          modify<1, true, false>(a, sc, x, th, k0 + 32 * kt + 4 * h - w.p, w.slope, lut.mid, nullptr, at);
           cf = 1.f;
         }
-        if (need_mask) {
+        if (need_mask) mask_keys(x, k0 + 32 * kt, w.hi, mixed ? sDoc + 32 * kt : nullptr, w.doc, h);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = 32 * kt + acc_row(i, h);
-            bool see = k0 + j < w.hi;
-            if (mixed) see = see && sDoc[j] == w.doc;
-            if (!see) x[i] = -INFINITY;
-          }
-        }
+        for (int i = 0; i < 16; ++i) x[i] = ex2(fmaf(x[i], cf, -st.x));
+        if constexpr (D > 64) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) dp = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp);
         float su = 0.f, sp = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float p = ex2(fmaf(x[i], cf, -st.x));
-          x[i] = p * (dp[i] - st.y);
-          if (MOD) su += x[i], sp += p;
+          if (MOD) sp += x[i];
+          x[i] *= dp[i] - st.y;
+          if (MOD) su += x[i];
         }
         if (MOD && a.rel_bias) {
           all_u += su;
-          if (far != 0) {
-            far_u[far > 0] += su;
-            far_p[far > 0] += sp;
-          }
+          if (at.far < 0) far_u[0] += su, far_p[0] += sp;
+          if (at.far > 0) far_u[1] += su, far_p[1] += sp;
         }
         if (MOD && sc.capped) {
 #pragma unroll
@@ -712,6 +750,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] *= dscale;
         }
+        if constexpr (D > 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const V8 ds = round8<T>(x + 8 * c);
@@ -771,15 +810,13 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
   const mmt_long_attention &a = g.a;
   float2 *sStat2 = (float2 *)(smem + 4 * L::BYTES);       // [2][BQ]
   int *sDoc2 = (int *)(sStat2 + 2 * BQ), *sB = sDoc2 + 2 * BQ;
-  BiasLds bias;
-  bias.table = (float *)(sB + 6 * WAVES);
+  const Lut lut = {(float *)(sB + 6 * WAVES) + a.reach + PAD};
   const int grp = blockIdx.x % g.groups;
   int n = blockIdx.x / g.groups;
   const int z = n % (g.zh * g.zq), zh = z % g.zh, zq = z / g.zh;
   const int kt = n / (g.zh * g.zq);                       // causal: the first keys are seen by the most queries
   const int kh = grp % a.Hk, b = grp / a.Hk, head0 = kh * g.G;
   const int g_per = (g.G + g.zh - 1) / g.zh, g0 = zh * g_per, g1 = min(g.G, g0 + g_per);
-  bias.bucket = (unsigned char *)(bias.table + (MOD && a.rel_bias ? g.G * a.n_buckets : 0));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
   const int len = row_len(a, b), off = len - a.Lq, prefix = a.prefix ? a.prefix[b] : 0;
   const int j = kt * ROWS + wave * 32 + col;
@@ -793,7 +830,6 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
   int gd_min = 0x7fffffff, gd_max = -1;
   for (int v = 0; v < WAVES; ++v) gd_min = min(gd_min, sB[2 * v]), gd_max = max(gd_max, sB[2 * v + 1]);
   gd_min = __builtin_amdgcn_readfirstlane(gd_min), gd_max = __builtin_amdgcn_readfirstlane(gd_max);
-  if (MOD && a.rel_bias) bias.fill(a, head0, g.G);
 
   const T *krow = (const T *)a.k + (int64_t)b * a.k_bs + (int64_t)min(j, a.Lk - 1) * a.k_rs + (int64_t)kh * a.k_hs;
   const T *vrow = (const T *)a.v + (int64_t)b * a.v_bs + (int64_t)min(j, a.Lk - 1) * a.v_rs + (int64_t)kh * a.v_hs;
@@ -825,7 +861,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
 
   // the tiles of all heads as one sequence, so that the next head's first tile is on its way during this head's last
   TileIter it;
-  int gi = g0 - 1, t = -1, buf = 0;
+  int gi = g0 - 1, t = -1, buf = 0, lut_gi = -1;
   const float2 *stat = nullptr;
   float2 st_next = make_float2(INFINITY, 0.f);
   int doc_next = -1;
@@ -864,6 +900,11 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
     }
     dma_wait<0>();
     __syncthreads();
+    if (MOD && a.rel_bias && lut_gi != cur_gi) {          // another head's bias
+      lut.fill(a, head);
+      lut_gi = cur_gi;
+      __syncthreads();
+    }
     if (q0 + BQ > a.Lq || dead) {
       zero_rows<T, D>(sQ, a.Lq - q0, sDoc);
       zero_rows<T, D>(sO, a.Lq - q0, sDoc);
@@ -876,7 +917,6 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
     if (!a.causal || max(p0 + BQ, prefix) > j_lo) {
       const bool need_mask = mixed || !all_live || (a.causal && max(p0 + 1, prefix) < j_lo + 32);
       const float slope = MOD && a.slopes ? a.slopes[head] * LOG2E : 0.f;
-      const float *tab = bias.table + cur_gi * a.n_buckets;
 #pragma unroll
       for (int qt = 0; qt < NQ; ++qt) {
         f32x16 s = {}, dp = {};
@@ -891,22 +931,28 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
         for (int i = 0; i < 16; ++i) x[i] = s[i];
         if constexpr (MOD) {
           const int pq = p0 + 32 * qt;
-          const int far = !a.rel_bias ? 0 : j_lo + 31 - pq <= -a.reach ? -1 : j_lo - (pq + 31) >= a.reach ? 1 : 0;
-          modify<16, true>(a, sc, x, th, j - pq - 4 * h, -1, slope, tab, bias.bucket, far);
+          modify<-1, true, false>(a, sc, x, th, j - pq - 4 * h, slope, lut.mid, nullptr, place(a, j_lo - pq - 31, j_lo + 31 - pq));
           cf = 1.f;
         }
+        float2 st[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int row = 32 * qt + acc_row(i, h);
-          const float2 st = sStat[row];
-          p[i] = ex2(fmaf(x[i], cf, Elem<T>::PSHIFT - st.x));
-          if (need_mask) {
-            bool see = live && (!a.causal || j < max(p0 + row + 1, prefix));
-            if (mixed) see = see && sDoc[row] == kdoc;
-            if (!see) p[i] = 0.f;
+        for (int i = 0; i < 16; ++i) st[i] = sStat[32 * qt + acc_row(i, h)];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = ex2(fmaf(x[i], cf, Elem<T>::PSHIFT - st[i].x));
+        if (need_mask) {
+          const int lo = a.causal ? (j < prefix ? 0 : j - off - q0 - 32 * qt) : -(1 << 30);      // first row of the sub-tile that sees key j
+#pragma unroll
+          for (int i = 0; i < 16; ++i) p[i] = live & (acc_row(i, h) >= lo) ? p[i] : 0.f;
+          if (mixed) {
+            int id[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) id[i] = sDoc[32 * qt + acc_row(i, h)];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = id[i] == kdoc ? p[i] : 0.f;
           }
-          x[i] = p[i] * (dp[i] - st.y);
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = p[i] * (dp[i] - st[i].y);
         if (MOD && sc.capped) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] *= fmaf(-th[i], th[i], 1.f);
@@ -979,10 +1025,9 @@ __global__ void __launch_bounds__(THREADS, 1) mmt_long_attn_table_kernel(const A
   const mmt_long_attention &a = g.a;
   char *sK = smem, *sV = smem + L::BYTES;
   int *sDoc = (int *)(smem + 2 * L::BYTES), *sB = sDoc + BK;
-  BiasLds bias;
-  bias.table = (float *)(sB + 6 * WAVES);
-  bias.bucket = (unsigned char *)(bias.table + a.n_buckets);
-  float *hist = (float *)(bias.bucket + ((2 * a.reach + 1 + 15) & ~15));
+  const Lut lut = {(float *)(sB + 6 * WAVES) + a.reach + PAD};
+  unsigned char *bucket = (unsigned char *)((float *)(sB + 6 * WAVES) + Lut::floats(a)) + a.reach + PAD;   // of distance 0
+  float *hist = (float *)(sB + 6 * WAVES) + Lut::floats(a) + ((Lut::floats(a) + 15) & ~15) / 4;
   const int grp = blockIdx.x % g.groups, n = blockIdx.x / g.groups, gi = n % g.G, qt = n / g.G;
   const int kh = grp % a.Hk, b = grp / a.Hk, head = kh * g.G + gi;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
@@ -990,7 +1035,8 @@ __global__ void __launch_bounds__(THREADS, 1) mmt_long_attn_table_kernel(const A
   const Row w = make_row(g, b, head, qt * ROWS + wave * 32 + col, len);
   const Bounds wb = wave_bounds(w);
   const Bounds gb = group_bounds(wb, sB, wave);
-  bias.fill(a, head, 1);
+  lut.fill(a, head);
+  for (int n = threadIdx.x; n < 2 * (a.reach + PAD) + 1; n += THREADS) bucket[n - a.reach - PAD] = (unsigned char)bias_bucket(a, n - a.reach - PAD);
   float *mine = hist + (int64_t)wave * a.n_buckets * 64 + lane;
   for (int k = 0; k < a.n_buckets; ++k) mine[k * 64] = 0.f;
   const int64_t r = ((int64_t)b * a.H + head) * a.Lq + min(w.i, a.Lq - 1);
@@ -1045,20 +1091,13 @@ __global__ void __launch_bounds__(THREADS, 1) mmt_long_attn_table_kernel(const A
       float x[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = s[i];
-      modify<16, false>(a, sc, x, nullptr, k0 + 32 * kt + 4 * h - w.p, 1, w.slope, bias.table, bias.bucket, 0);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int j = 32 * kt + acc_row(i, h);
-        bool see = k0 + j < w.hi;
-        if (kdoc) see = see && sDoc[j] == w.doc;
-        if (!see) x[i] = -INFINITY;
-      }
-      const int d0 = k0 + 32 * kt + 4 * h - w.p;
+      modify<1, false, false>(a, sc, x, nullptr, k0 + 32 * kt + 4 * h - w.p, w.slope, lut.mid, nullptr, place(a, k0 - gb.p_max, k0 + BK - 1 - gb.p_min));
+      mask_keys(x, k0 + 32 * kt, w.hi, kdoc ? sDoc + 32 * kt : nullptr, w.doc, h);
+      const unsigned char *bk = bucket + max(-a.reach - PAD, min(a.reach + PAD - 27, k0 + 32 * kt + 4 * h - w.p));
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float p = ex2(x[i] - lse2), u = p * (dp[i] - delta);
-        const int d = max(-a.reach, min(a.reach, d0 + 8 * (i >> 2) + (i & 3))) + a.reach;
-        mine[bias.bucket[d] * 64] += u;
+        mine[bk[8 * (i >> 2) + (i & 3)] * 64] += u;
       }
     }
   }
@@ -1097,13 +1136,13 @@ static inline bool modified(const mmt_long_attention &a) { return a.softcap > 0.
 
 template <typename T, int D> static void fwd_size(const Args &g, hipStream_t st) {
   if (g.few) {
-    const size_t tiles = 2 * WAVES * 32 * Tile<T, D>::NS * 16 + 4 * 32 * WAVES + bias_lds_bytes(g.a, g.pack);
+    const size_t tiles = 2 * WAVES * 32 * Tile<T, D>::NS * 16 + 4 * 32 * WAVES + PackedBias::bytes(g.a, g.pack);
     const size_t join = 4 * 64 * WAVES * (2 + D / 2), lds = tiles > join ? tiles : join;
     if (modified(g.a)) launch(mmt_long_attn_few_kernel<T, D, true>, g.items, lds, st, g);
     else launch(mmt_long_attn_few_kernel<T, D, false>, g.items, lds, st, g);
     return;
   }
-  const size_t lds = 4 * Tile<T, D>::BYTES + 4 * Tile<T, D>::BK + 24 * WAVES + bias_lds_bytes(g.a, 1);
+  const size_t lds = 4 * Tile<T, D>::BYTES + 4 * Tile<T, D>::BK + 24 * WAVES + 4 * Lut::floats(g.a);
   if (modified(g.a)) launch(mmt_long_attn_fwd_kernel<T, D, true>, g.items, lds, st, g);
   else launch(mmt_long_attn_fwd_kernel<T, D, false>, g.items, lds, st, g);
 }
@@ -1114,17 +1153,17 @@ template <typename T, int D> static void bwd_size(Args &g, hipStream_t st, float
   const bool mod = modified(a);
   const size_t small = 24 * WAVES;
   const int64_t qitems = (int64_t)a.B * a.H * g.nqt;
-  const size_t lds_q = 4 * L::BYTES + 4 * L::BK + small + bias_lds_bytes(a, 1);
+  const size_t lds_q = 4 * L::BYTES + 4 * L::BK + small + 4 * Lut::floats(a);
   if (mod) launch(mmt_long_attn_dq_kernel<T, D, true>, qitems, lds_q, st, g);
   else launch(mmt_long_attn_dq_kernel<T, D, false>, qitems, lds_q, st, g);
   if (a.rel_bias) {
-    const size_t lds = 2 * L::BYTES + 4 * L::BK + small + bias_lds_bytes(a, 1) + (size_t)WAVES * a.n_buckets * 256;
+    const size_t lds = 2 * L::BYTES + 4 * L::BK + small + 4 * Lut::floats(a) + ((Lut::floats(a) + 15) & ~15) + (size_t)WAVES * a.n_buckets * 256;
     (void)hipFuncSetAttribute((const void *)mmt_long_attn_table_kernel<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     hipLaunchKernelGGL((mmt_long_attn_table_kernel<T, D>), dim3((unsigned)qitems), dim3(THREADS), lds, st, g, table_part);
     hipLaunchKernelGGL(mmt_long_attn_table_sum_kernel<T>, dim3(a.H * a.n_buckets), dim3(64), 0, st, a, (int64_t)a.B * g.nqt, table_part,
                        g.far_part, dtable);
   }
-  const size_t lds_k = 4 * L::BYTES + 24 * L::BK + small + bias_lds_bytes(a, g.G);
+  const size_t lds_k = 4 * L::BYTES + 24 * L::BK + small + 4 * Lut::floats(a);
   const int64_t kitems = (int64_t)g.groups * ((a.Lk + ROWS - 1) / ROWS) * g.zh * g.zq;
   if (mod) launch(mmt_long_attn_dkv_kernel<T, D, true>, kitems, lds_k, st, g);
   else launch(mmt_long_attn_dkv_kernel<T, D, false>, kitems, lds_k, st, g);

@@ -37,7 +37,7 @@ def _desc(**kw):
     (dict(prefix=0x1000), b"prefix"), (dict(q_doc=0x1000), b"documents"), (dict(rel_bias=0x1000), b"bias"),
     (dict(rel_bias=0x1000, rel_buckets=0x1000, n_buckets=65, reach=8), b"buckets"),
     (dict(rel_bias=0x1000, rel_buckets=0x1000, n_buckets=8, reach=0), b"reach"),
-    (dict(rel_bias=0x1000, rel_buckets=0x1000, n_buckets=64, reach=8, H=512, Hk=2), b"entries"),
+    (dict(rel_bias=0x1000, rel_buckets=0x1000, n_buckets=64, reach=1025), b"reach"),
     (dict(q=0x1008), b"16 bytes"), (dict(k_rs=129), b"16 bytes"), (dict(B=1 << 30, Lq=1 << 20), b"too many")])
 def test_attention_refuses_on_the_host(bad, word):
     """Every argument the kernels could not run with is an error of the call, before anything is launched."""
