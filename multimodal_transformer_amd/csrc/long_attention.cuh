@@ -247,6 +247,11 @@ __device__ __forceinline__ int wave_max(int v) {
 __device__ __forceinline__ void wave_sync() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+// a number per accumulator row of a lane, from 32 in LDS (16-byte aligned)
+__device__ __forceinline__ void acc_rows(f32x4 *v, const float *s, int h) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v[q] = *(const f32x4 *)(s + 8 * q + 4 * h);
+}
 
 // ---- score transform ------------------------------------------------------------------------------------------------------
 // tanh without cancellation.  |y| <= 3/8: odd series to y^11, remainder < 21844/6081075 y^13 = 3e-8 of y.  Beyond: 1 - 2 / (1 + e^2y),

@@ -808,8 +808,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
   constexpr int BQ = L::BK, NQ = BQ / 32, NC = D / 16, ND = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
-  float2 *sStat2 = (float2 *)(smem + 4 * L::BYTES);       // [2][BQ]
-  int *sDoc2 = (int *)(sStat2 + 2 * BQ), *sB = sDoc2 + 2 * BQ;
+  float *sStat2 = (float *)(smem + 4 * L::BYTES);         // [2][log-sum, delta][BQ]
+  int *sDoc2 = (int *)(sStat2 + 4 * BQ), *sB = sDoc2 + 2 * BQ;
   const Lut lut = {(float *)(sB + 6 * WAVES) + a.reach + PAD};
   const int grp = blockIdx.x % g.groups;
   int n = blockIdx.x / g.groups;
@@ -890,13 +890,13 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
   while (t >= 0) {
     const int q0 = t * BQ, head = head0 + gi;
     char *sQ = smem + buf * 2 * L::BYTES, *sO = sQ + L::BYTES;
-    float2 *sStat = sStat2 + buf * BQ;
+    float *sStat = sStat2 + buf * 2 * BQ;
     int *sDoc = sDoc2 + buf * BQ;
     const bool mixed = it.mixed(), dead = it.cur_dead != 0;
     const int cur_gi = gi;
     if (threadIdx.x < BQ) {
       sDoc[threadIdx.x] = doc_next;
-      sStat[threadIdx.x] = st_next;
+      sStat[threadIdx.x] = st_next.x, sStat[BQ + threadIdx.x] = st_next.y;
     }
     dma_wait<0>();
     __syncthreads();
@@ -934,11 +934,10 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
           modify<-1, true, false>(a, sc, x, th, j - pq - 4 * h, slope, lut.mid, nullptr, place(a, j_lo - pq - 31, j_lo + 31 - pq));
           cf = 1.f;
         }
-        float2 st[16];
+        f32x4 st[4];
+        acc_rows(st, sStat + 32 * qt, h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) st[i] = sStat[32 * qt + acc_row(i, h)];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = ex2(fmaf(x[i], cf, Elem<T>::PSHIFT - st[i].x));
+        for (int i = 0; i < 16; ++i) p[i] = ex2(fmaf(x[i], cf, Elem<T>::PSHIFT - st[i >> 2][i & 3]));
         if (need_mask) {
           const int lo = a.causal ? (j < prefix ? 0 : j - off - q0 - 32 * qt) : -(1 << 30);      // first row of the sub-tile that sees key j
 #pragma unroll
@@ -951,8 +950,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
             for (int i = 0; i < 16; ++i) p[i] = id[i] == kdoc ? p[i] : 0.f;
           }
         }
+        acc_rows(st, sStat + BQ + 32 * qt, h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = p[i] * (dp[i] - st[i].y);
+        for (int i = 0; i < 16; ++i) x[i] = p[i] * (dp[i] - st[i >> 2][i & 3]);
         if (MOD && sc.capped) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] *= fmaf(-th[i], th[i], 1.f);
@@ -998,6 +998,221 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
         *(typename Elem<T>::V4 *)((T *)g.dv + o + dim) = __builtin_convertvector(vv, typename Elem<T>::V4);
       }
     }
+}
+
+// dK, dV at head sizes above 64 in 16-bit types.  Keys, their gradients and the products of 32 keys do not fit into the 256 registers
+// that two waves per SIMD leave each; so the eight waves of a workgroup (128 keys) share the work in two steps per tile of 64 queries:
+//   1. wave w computes P and dS of 32 queries x 32 keys (its K and V rows stay in registers) and leaves them in LDS in the order of
+//      the accumulator, which is the order of the second step's operand: 16 bytes per lane, no rearrangement;
+//   2. wave w adds up one of the two outputs for KB x 32 keys and a part of the dimensions, with dO or Q read transposed.
+// Bound by LDS: about 290 KiB go through it per tile, at 128 bytes a cycle a little more than the tile's matrix instructions take.
+template <typename T, int D, bool MOD>
+__global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g) {
+  typedef Tile<T, D> L;
+  typedef typename Elem<T>::V8 V8;
+  constexpr int BQ = 64, NC = D / 16, ND = D / 32, KB = ND % 2 ? 1 : 2, NT = ND / KB;      // KB key blocks and NT dimension tiles per wave
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const mmt_long_attention &a = g.a;
+  char *sP = smem + 4 * L::BYTES, *sS = sP + 128 * BQ * 2;                 // [key block][16 queries][lane] x 16 bytes
+  float *sStat2 = (float *)(sS + 128 * BQ * 2);                             // [2][log-sum, delta][BQ]
+  int *sDoc2 = (int *)(sStat2 + 4 * BQ), *sB = sDoc2 + 2 * BQ;
+  const Lut lut = {(float *)(sB + 16) + a.reach + PAD};
+  const int grp = blockIdx.x % g.groups;
+  int n = blockIdx.x / g.groups;
+  const int z = n % (g.zh * g.zq), zh = z % g.zh, zq = z / g.zh;
+  const int kt = n / (g.zh * g.zq);                       // causal: the first keys are seen by the most queries
+  const int kh = grp % a.Hk, b = grp / a.Hk, head0 = kh * g.G;
+  const int g_per = (g.G + g.zh - 1) / g.zh, g0 = zh * g_per, g1 = min(g.G, g0 + g_per);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+  const int len = row_len(a, b), off = len - a.Lq, prefix = a.prefix ? a.prefix[b] : 0;
+  const int qh = wave & 1, kb = wave >> 1;                // first step: half of the queries, block of 32 keys
+  const int j_lo = kt * ROWS + kb * 32, j = j_lo + col;
+  const int kdoc = a.k_doc && j < a.Lk ? a.k_doc[(int64_t)b * a.Lk + j] : 0;
+  const bool live = j < len && kdoc >= 0;
+  const int d_min = wave_min(live ? kdoc : 0x7fffffff), d_max = wave_max(live ? kdoc : -1);
+  const bool all_live = __all(live);
+  if (lane == 0) sB[2 * wave] = d_min, sB[2 * wave + 1] = d_max;
+  __syncthreads();
+  int gd_min = 0x7fffffff, gd_max = -1;
+  for (int v = 0; v < 8; ++v) gd_min = min(gd_min, sB[2 * v]), gd_max = max(gd_max, sB[2 * v + 1]);
+  gd_min = __builtin_amdgcn_readfirstlane(gd_min), gd_max = __builtin_amdgcn_readfirstlane(gd_max);
+
+  const T *krow = (const T *)a.k + (int64_t)b * a.k_bs + (int64_t)min(j, a.Lk - 1) * a.k_rs + (int64_t)kh * a.k_hs;
+  const T *vrow = (const T *)a.v + (int64_t)b * a.v_bs + (int64_t)min(j, a.Lk - 1) * a.v_rs + (int64_t)kh * a.v_hs;
+  V8 fk[NC], fv[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    fk[c] = mem_frag<T>(krow, c, h, a.dh, live);
+    fv[c] = mem_frag<T>(vrow, c, h, a.dh, live);
+  }
+  // second step: which output, which keys (blocks kb2, kb2 + 1, ..), which dimension tiles (dt2, ..)
+  const bool to_k = wave & 1;
+  const int part = wave >> 1, kb2 = KB == 2 ? 2 * (part & 1) : part, dt2 = KB == 2 ? NT * (part >> 1) : 0;
+  f32x16 acc[KB][NT];
+#pragma unroll
+  for (int k = 0; k < KB; ++k)
+#pragma unroll
+    for (int d = 0; d < NT; ++d) acc[k][d] = f32x16{};
+  const ScoreCtx sc = score_ctx(a);
+  const float dscale = g.dscale ? g.dscale[0] : 1.f;
+  const float ds_mul = dscale * ex2(-Elem<T>::PSHIFT);
+
+  const int i_first = a.causal && prefix <= kt * ROWS ? max(0, kt * ROWS - off) : 0;
+  const int all0 = min(i_first, a.Lq) / BQ, all1 = kt * ROWS < len ? (a.Lq + BQ - 1) / BQ : 0;
+  const int t_per = (max(0, all1 - all0) + g.zq - 1) / g.zq, t0 = all0 + zq * t_per, t1 = min(all1, t0 + t_per);
+  const DocRange *rng = g.qrng ? g.qrng + (int64_t)b * ((a.Lq + BQ - 1) / BQ) : nullptr;
+  const int *qdoc = a.q_doc ? a.q_doc + (int64_t)b * a.Lq : nullptr;
+  const unsigned lds = lds_address(smem);
+  Dma<T, D, BQ, 512> dmq, dmo;
+  dmq.init((const T *)a.q + (int64_t)b * a.q_bs + (int64_t)head0 * a.q_hs, a.q_rs, a.Lq, a.dh);
+  dmo.init((const T *)g.dout + (int64_t)b * g.do_bs + (int64_t)head0 * g.do_hs, g.do_rs, a.Lq, a.dh);
+  const char *qbase = dmq.base, *obase = dmo.base;
+
+  // the tiles of all heads as one sequence, so that the next head's first tile is on its way during this head's last
+  TileIter it;
+  int gi = g0 - 1, t = -1, buf = 0, lut_gi = -1;
+  const float2 *stat = nullptr;
+  float2 st_next = make_float2(INFINITY, 0.f);
+  int doc_next = -1;
+  auto advance = [&]() {
+    int n = gi < g0 ? -1 : it.next();
+    while (n < 0 && ++gi < g1) {
+      stat = g.stat + ((int64_t)b * a.H + head0 + gi) * a.Lq;
+      dmq.base = qbase + (int64_t)gi * a.q_hs * (int64_t)sizeof(T);
+      dmo.base = obase + (int64_t)gi * g.do_hs * (int64_t)sizeof(T);
+      it.start(rng, gd_min, gd_max, t0, t1);
+      n = it.next();
+    }
+    return n;
+  };
+  auto fetch = [&](int tile, int to) {
+    dmq.load(lds + to * 2 * L::BYTES, tile * BQ);
+    dmo.load(lds + to * 2 * L::BYTES + L::BYTES, tile * BQ);
+    if (threadIdx.x < BQ) {
+      const int i = tile * BQ + threadIdx.x;
+      doc_next = i < a.Lq ? (qdoc ? qdoc[i] : 0) : -1;
+      st_next = doc_next >= 0 ? stat[i] : make_float2(INFINITY, 0.f);
+    }
+  };
+  t = advance();
+  if (t >= 0) fetch(t, 0);
+  while (t >= 0) {
+    const int q0 = t * BQ, head = head0 + gi, cur_gi = gi;
+    char *sQ = smem + buf * 2 * L::BYTES, *sO = sQ + L::BYTES;
+    float *sStat = sStat2 + buf * 2 * BQ;
+    int *sDoc = sDoc2 + buf * BQ;
+    const bool mixed = it.mixed(), dead = it.cur_dead != 0;
+    if (threadIdx.x < BQ) {
+      sDoc[threadIdx.x] = doc_next;
+      sStat[threadIdx.x] = st_next.x, sStat[BQ + threadIdx.x] = st_next.y;
+    }
+    dma_wait<0>();
+    __syncthreads();                                      // the tile is here; the last one's second step is done everywhere
+    if (MOD && a.rel_bias && lut_gi != cur_gi) {          // another head's bias
+      lut.fill(a, head);
+      lut_gi = cur_gi;
+      __syncthreads();
+    }
+    if (q0 + BQ > a.Lq || dead) {
+      zero_rows<T, D, BQ, 512>(sQ, a.Lq - q0, sDoc);
+      zero_rows<T, D, BQ, 512>(sO, a.Lq - q0, sDoc);
+      __syncthreads();
+    }
+    const int tn = advance();
+    if (tn >= 0) fetch(tn, buf ^ 1);
+    {
+      const int p0 = off + q0 + 32 * qh;                  // position of the first of this wave's queries
+      const bool need_mask = mixed || !all_live || (a.causal && max(p0 + 1, prefix) < j_lo + 32);
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s = Elem<T>::mma(row_frag<T, D>(sQ, 32 * qh + col, c, h), fk[c], s);
+      float x[16], th[16], p[16];
+      float cf = sc.c_scale;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = s[i];
+      if constexpr (MOD) {
+        const float slope = a.slopes ? a.slopes[head] * LOG2E : 0.f;
+        modify<-1, true, false>(a, sc, x, th, j - p0 - 4 * h, slope, lut.mid, nullptr, place(a, j_lo - p0 - 31, j_lo + 31 - p0));
+        cf = 1.f;
+      }
+      f32x4 st[4];
+      acc_rows(st, sStat + 32 * qh, h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = ex2(fmaf(x[i], cf, Elem<T>::PSHIFT - st[i >> 2][i & 3]));
+      if (need_mask) {
+        const int lo = a.causal ? (j < prefix ? 0 : j - p0) : -(1 << 30);      // first of the queries that sees key j
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = live & (acc_row(i, h) >= lo) ? p[i] : 0.f;
+        if (mixed) {
+          int id[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) id[i] = sDoc[32 * qh + acc_row(i, h)];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) p[i] = id[i] == kdoc ? p[i] : 0.f;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);                  // (keeps the registers of the second product out of the first one's reach)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) dp = Elem<T>::mma(row_frag<T, D>(sO, 32 * qh + col, c, h), fv[c], dp);
+      acc_rows(st, sStat + BQ + 32 * qh, h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = p[i] * (dp[i] - st[i >> 2][i & 3]);
+      if (MOD && sc.capped) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= fmaf(-th[i], th[i], 1.f);
+      }
+      if (Elem<T>::PSHIFT != 0.f) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= ds_mul;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int at = ((kb * 4 + qh * 2 + c) * 64 + lane) * 16;
+        *(V8 *)(sP + at) = round8<T>(p + 8 * c);
+        *(V8 *)(sS + at) = round8<T>(x + 8 * c);
+      }
+    }
+    __syncthreads();                                      // P and dS of the tile are complete
+    {
+      const char *tr = to_k ? sQ : sO, *op = to_k ? sS : sP;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        V8 fb[KB];
+#pragma unroll
+        for (int k = 0; k < KB; ++k) fb[k] = *(const V8 *)(op + (((kb2 + k) * 4 + c) * 64 + lane) * 16);
+#pragma unroll
+        for (int d = 0; d < NT; ++d) {
+          const V8 fa = col_frag<T, D>(tr, 16 * c, dt2 + d, lane);
+#pragma unroll
+          for (int k = 0; k < KB; ++k) acc[k][d] = Elem<T>::mma(fa, fb[k], acc[k][d]);
+        }
+      }
+    }
+    t = tn;
+    buf ^= 1;
+  }
+  const float f = to_k ? a.scale / dscale : ex2(-Elem<T>::PSHIFT);
+  float *part_out = to_k ? g.part_dk : g.part_dv;
+  T *out = (T *)(to_k ? g.dk : g.dv);
+#pragma unroll
+  for (int k = 0; k < KB; ++k) {
+    const int jj = kt * ROWS + (kb2 + k) * 32 + col;
+    if (jj >= a.Lk) continue;
+    const bool ok = jj < len && !(a.k_doc && a.k_doc[(int64_t)b * a.Lk + jj] < 0);
+    const int64_t o = (((int64_t)b * a.Lk + jj) * a.Hk + kh) * a.dh, at = (int64_t)a.B * a.Lk * a.Hk * a.dh * z + o;
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int dim = 32 * (dt2 + d) + 8 * q + 4 * h;
+        if (dim >= a.dh) continue;
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = ok ? acc[k][d][4 * q + e] * f : 0.f;
+        if (part_out) *(f32x4 *)(part_out + at + dim) = v;
+        else *(typename Elem<T>::V4 *)(out + o + dim) = __builtin_convertvector(v, typename Elem<T>::V4);
+      }
+  }
 }
 
 // the parts of dK and dV, in order
@@ -1127,9 +1342,9 @@ template <typename T> __global__ void mmt_long_attn_table_sum_kernel(const mmt_l
 }
 
 // --------------------------------------------------------------------------------------------------------------- launchers
-template <typename K> static void launch(K kernel, int64_t grid, size_t lds, hipStream_t st, const Args &g) {
+template <typename K> static void launch(K kernel, int64_t grid, size_t lds, hipStream_t st, const Args &g, int threads = THREADS) {
   if (lds > 65536) (void)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(THREADS), lds, st, g);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, st, g);
 }
 
 static inline bool modified(const mmt_long_attention &a) { return a.softcap > 0.f || a.slopes || a.rel_bias; }
@@ -1165,8 +1380,14 @@ template <typename T, int D> static void bwd_size(Args &g, hipStream_t st, float
   }
   const size_t lds_k = 4 * L::BYTES + 24 * L::BK + small + 4 * Lut::floats(a);
   const int64_t kitems = (int64_t)g.groups * ((a.Lk + ROWS - 1) / ROWS) * g.zh * g.zq;
-  if (mod) launch(mmt_long_attn_dkv_kernel<T, D, true>, kitems, lds_k, st, g);
-  else launch(mmt_long_attn_dkv_kernel<T, D, false>, kitems, lds_k, st, g);
+  if constexpr (sizeof(T) == 2 && D > 64) {
+    const size_t lds2 = 4 * L::BYTES + 2 * 128 * 64 * 2 + 24 * 64 + 64 + 4 * Lut::floats(a);
+    if (mod) launch(mmt_long_attn_dkv2_kernel<T, D, true>, kitems, lds2, st, g, 512);
+    else launch(mmt_long_attn_dkv2_kernel<T, D, false>, kitems, lds2, st, g, 512);
+  } else {
+    if (mod) launch(mmt_long_attn_dkv_kernel<T, D, true>, kitems, lds_k, st, g);
+    else launch(mmt_long_attn_dkv_kernel<T, D, false>, kitems, lds_k, st, g);
+  }
 }
 
 template <typename T> static void docs(const Args &g, DocRange *out, bool queries, hipStream_t st) {
