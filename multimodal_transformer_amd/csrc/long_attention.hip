@@ -70,7 +70,7 @@ static void plan(Args &g, bool backward) {
 static size_t align64(size_t n) { return (n + 63) & ~(size_t)63; }
 
 struct Workspace {                 // one piece after another, each a multiple of 64 bytes
-  size_t docs, part_o, part_ml, stat, maxima, fix, far, table, part_dk, part_dv, total;
+  size_t docs, part_o, part_ml, stat, maxima, far, table, part_dk, part_dv, total;
 };
 static Workspace layout(const Args &g, bool backward) {
   const mmt_long_attention &a = g.a;
@@ -88,7 +88,6 @@ static Workspace layout(const Args &g, bool backward) {
     if (a.dtype == MMT_F16) w.maxima = n, n += 16 * (STAT_PARTS + 4);
     if (a.rel_bias) {
       const size_t tiles = (size_t)a.B * g.nqt * a.H;
-      w.fix = n, n += align64(4 * rows);
       w.far = n, n += align64(8 * tiles);
       w.table = n, n += align64(4 * tiles * a.n_buckets);
     }
@@ -156,16 +155,15 @@ extern "C" int mmt_long_attention_bwd(const mmt_long_attention *a, const void *o
   g.out = const_cast<void *>(out), g.low = const_cast<void *>(out_low), g.lse = const_cast<float *>(lse);
   g.dout = dout, g.do_bs = do_bs, g.do_rs = do_rs, g.do_hs = do_hs;
   g.dq = dq, g.dk = dk, g.dv = dv, g.dlse = dlse;
-  float2 *stat = (float2 *)(ws + w.stat);
-  g.stat = stat;
-  if (a->rel_bias) g.delta_fix = (float *)(ws + w.fix), g.far_part = (float *)(ws + w.far);
+  g.stat = (float2 *)(ws + w.stat);
+  if (a->rel_bias) g.far_part = (float *)(ws + w.far);
   if (g.zh * g.zq > 1) g.part_dk = (float *)(ws + w.part_dk), g.part_dv = (float *)(ws + w.part_dv);
   DocRange *ranges = a->q_doc ? (DocRange *)(ws + w.docs) : nullptr;
   float *table = a->rel_bias ? (float *)(ws + w.table) : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  if (a->dtype == MMT_BF16) backward<__bf16>(g, ranges, stat, nullptr, table, drel_bias, st);
-  else if (a->dtype == MMT_F16) backward<_Float16>(g, ranges, stat, (f32x4 *)(ws + w.maxima), table, drel_bias, st);
-  else backward<float>(g, ranges, stat, nullptr, table, drel_bias, st);
+  if (a->dtype == MMT_BF16) backward<__bf16>(g, ranges, nullptr, table, drel_bias, st);
+  else if (a->dtype == MMT_F16) backward<_Float16>(g, ranges, (f32x4 *)(ws + w.maxima), table, drel_bias, st);
+  else backward<float>(g, ranges, nullptr, table, drel_bias, st);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MMT_OK : mmt_set_error(MMT_ELAUNCH, "mmt_long_attention_bwd: %s", hipGetErrorString(e));
 }

@@ -34,15 +34,14 @@ struct Args {                      // mmt_long_attention plus what the launcher 
   // backward
   const void *dout;
   int64_t do_bs, do_rs, do_hs;
-  const float2 *stat;              // (B, H, Lq): lse in units of log 2, rowsum(do o) - dlse
+  float2 *stat;                    // (B, H, Lq): lse in units of log 2, rowsum(P dP) - dlse
   const float *dscale;             // fp16: power of two the score gradients are multiplied by before they are rounded
   void *dq, *dk, *dv;              // (B, Lq, H, dh), (B, Lk, Hk, dh)
   const float *dlse;               // (B, H, Lq) gradient of the log-sum, or NULL
-  float *delta_fix;                // (B, H, Lq) delta with the exact rowsum(P dP), or NULL
   float *far_part;                 // (items, 2)
 };
 
 template <typename T> void forward(Args &g, DocRange *ranges, hipStream_t st);
-template <typename T> void backward(Args &g, DocRange *ranges, float2 *stat, f32x4 *maxima, float *table_part, float *dtable, hipStream_t st);
+template <typename T> void backward(Args &g, DocRange *ranges, f32x4 *maxima, float *table_part, float *dtable, hipStream_t st);
 
 }  // namespace la

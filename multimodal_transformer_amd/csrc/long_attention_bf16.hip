@@ -3,5 +3,5 @@
 
 namespace la {
 template void forward<__bf16>(Args &, DocRange *, hipStream_t);
-template void backward<__bf16>(Args &, DocRange *, float2 *, f32x4 *, float *, float *, hipStream_t);
+template void backward<__bf16>(Args &, DocRange *, f32x4 *, float *, float *, hipStream_t);
 }  // namespace la

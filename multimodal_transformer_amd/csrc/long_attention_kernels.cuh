@@ -550,68 +550,46 @@ template <typename T> __global__ void mmt_long_attn_docs_kernel(const Args g, in
 // Two kernels recompute the probabilities from the saved log-sum: one walks the keys of a query tile (dQ), the other the queries of
 // a key tile (dK, dV, summed over the query heads that share the key head).  Seven products instead of the five of a single pass,
 // but every sum has a fixed order and an owner: no atomics, the same bits every time.
-// delta is the small difference of large terms where a row sees few keys: it is formed from out and what rounding took from it
-// (`low`), which the forward keeps for this.
+// delta decides the sign and size of dU where a row sees few keys.  It starts from out and what rounding took from it (`low`, which the
+// forward keeps for this); P itself was rounded on its way into out, but the sum of dU over a row has to be dlse: what it is instead is
+// the error of delta, and the dQ kernel corrects it for everything that comes after.
 
-// delta and the log-sum in units of log 2; 16 lanes per row.
 // fp16: the score gradients are rounded to 5 exponent bits, so they are first multiplied by a power of two that takes their bound
-// 2 max|do_i| max|v_j| + max|dlse| to at most 2^15; each workgroup leaves its part of the three maxima.
-template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_stat_kernel(const Args g, float2 *stat, f32x4 *maxima) {
+// 2 max|do_i| max|v_j| + max|dlse| to at most 2^15; each workgroup leaves its part of the three maxima.  16 lanes per row.
+template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_maxima_kernel(const Args g, f32x4 *maxima) {
   const mmt_long_attention &a = g.a;
   typedef typename Elem<T>::V8 V8;
-  const int64_t rows = (int64_t)a.B * a.H * a.Lq;
+  const int64_t rows = (int64_t)a.B * a.H * a.Lq, vrows = (int64_t)a.B * a.Lk * a.Hk;
   const int d0 = (threadIdx.x & 15) * 8;
-  float mx = 0.f, mv = 0.f, ml = 0.f;
-  for (int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); r < rows; r += (int64_t)gridDim.x * 16) {
-    // rows in the order of the tensors (b, i, h), the statistics in the order of the kernels that read them (b, h, i)
-    const int64_t hd = r % a.H, bi = r / a.H, i = bi % a.Lq, b = bi / a.Lq, w = (b * a.H + hd) * a.Lq + i;
-    const bool live = !(a.q_doc && a.q_doc[b * a.Lq + i] < 0);
-    float s = 0.f, nn = 0.f;
-    if (d0 < a.dh && live) {
-      const V8 o = *(const V8 *)((const T *)g.out + r * a.dh + d0);
-      const V8 d = *(const V8 *)((const T *)g.dout + b * g.do_bs + i * g.do_rs + hd * g.do_hs + d0);
-      V8 lo = {};
-      if (g.low) lo = *(const V8 *)((const T *)g.low + r * a.dh + d0);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        s = fmaf((float)o[e] + (float)lo[e], (float)d[e], s);
-        nn = fmaf((float)d[e], (float)d[e], nn);
-      }
-    }
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) {
-      s += __shfl_xor(s, m);
-      nn += __shfl_xor(nn, m);
-    }
-    const float ls = g.lse[w], dl = g.dlse && live ? g.dlse[w] : 0.f;
-    if (isfinite(nn)) mx = fmaxf(mx, nn);
-    if (isfinite(dl)) ml = fmaxf(ml, fabsf(dl));
-    // a row without keys has probabilities 0: its log-sum is turned around
-    if ((threadIdx.x & 15) == 0) stat[w] = make_float2(ls == -INFINITY ? INFINITY : ls * LOG2E, s - dl);
-  }
-  if (!maxima) return;
-  const int64_t vrows = (int64_t)a.B * a.Lk * a.Hk;
-  for (int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); r < vrows; r += (int64_t)gridDim.x * 16) {
-    const int64_t hd = r % a.Hk, bj = r / a.Hk, j = bj % a.Lk, b = bj / a.Lk;
-    if (j >= row_len(a, (int)b) || (a.k_doc && a.k_doc[b * a.Lk + j] < 0)) continue;
+  float m[3] = {0.f, 0.f, 0.f};
+  auto square = [&](const T *row) {
     float s = 0.f;
     if (d0 < a.dh) {
-      const V8 v = *(const V8 *)((const T *)a.v + b * a.v_bs + j * a.v_rs + hd * a.v_hs + d0);
+      const V8 v = *(const V8 *)(row + d0);
 #pragma unroll
       for (int e = 0; e < 8; ++e) s = fmaf((float)v[e], (float)v[e], s);
     }
 #pragma unroll
-    for (int m = 1; m < 16; m <<= 1) s += __shfl_xor(s, m);
-    if (isfinite(s)) mv = fmaxf(mv, s);
+    for (int k = 1; k < 16; k <<= 1) s += __shfl_xor(s, k);
+    return isfinite(s) ? s : 0.f;
+  };
+  for (int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); r < rows; r += (int64_t)gridDim.x * 16) {
+    const int64_t hd = r % a.H, bi = r / a.H, i = bi % a.Lq, b = bi / a.Lq;
+    if (a.q_doc && a.q_doc[b * a.Lq + i] < 0) continue;
+    m[0] = fmaxf(m[0], square((const T *)g.dout + b * g.do_bs + i * g.do_rs + hd * g.do_hs));
+    const float dl = g.dlse ? fabsf(g.dlse[(b * a.H + hd) * a.Lq + i]) : 0.f;
+    if (isfinite(dl)) m[2] = fmaxf(m[2], dl);
+  }
+  for (int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); r < vrows; r += (int64_t)gridDim.x * 16) {
+    const int64_t hd = r % a.Hk, bj = r / a.Hk, j = bj % a.Lk, b = bj / a.Lk;
+    if (j >= row_len(a, (int)b) || (a.k_doc && a.k_doc[b * a.Lk + j] < 0)) continue;
+    m[1] = fmaxf(m[1], square((const T *)a.v + b * a.v_bs + j * a.v_rs + hd * a.v_hs));
   }
 #pragma unroll
-  for (int m = 16; m < 64; m <<= 1) {
-    mx = fmaxf(mx, __shfl_xor(mx, m));
-    mv = fmaxf(mv, __shfl_xor(mv, m));
-    ml = fmaxf(ml, __shfl_xor(ml, m));
-  }
+  for (int k = 16; k < 64; k <<= 1)
+    for (int e = 0; e < 3; ++e) m[e] = fmaxf(m[e], __shfl_xor(m[e], k));
   __shared__ f32x4 part[4];
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = f32x4{mx, mv, ml, 0.f};
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = f32x4{m[0], m[1], m[2], 0.f};
   __syncthreads();
   if (threadIdx.x == 0) {
     f32x4 v = part[0];
@@ -633,9 +611,12 @@ template <typename T> __global__ void __launch_bounds__(64) mmt_long_attn_dscale
   if (threadIdx.x == 0) dscale[0] = ldexpf(1.f, known ? max(-60, min(60, 15 - e)) : 0);
 }
 
-// dQ.  The forward's geometry; K is read twice from LDS (as rows for the scores, transposed for dQ^T += K^T dS^T), V once.
-// With a learned bias it also leaves, per row, the exact delta (see the table kernel) and the sums of dU over the tiles that lie wholly
-// beyond the reach on either side.
+// dQ, and the statistics of the rows for the other kernels: log-sum in units of log 2 (+inf for a row without keys: its probabilities
+// are 0) and the corrected delta.  The forward's geometry; K is read twice from LDS (as rows for the scores, transposed for
+// dQ^T += K^T dS^T), V once.  16-bit types with rows of at most TWICE keys go over them twice, the first time for delta alone: there a
+// probability's rounding does not average out, and such calls are short (8 us for 128 rows of 21 keys and 8 heads, with one pass 7).
+// With a learned bias the kernel also sums dU over the tiles that lie wholly beyond the reach on either side.
+constexpr int TWICE = 512;
 template <typename T, int D, bool MOD>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_dq_kernel(const Args g) {
   typedef Tile<T, D> L;
@@ -656,16 +637,25 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   const Bounds gb = group_bounds(wb, sB, wave);
   if (MOD && a.rel_bias) lut.fill(a, head);
   const int64_t r = ((int64_t)b * a.H + head) * a.Lq + min(w.i, a.Lq - 1);
-  const float2 st = w.live ? g.stat[r] : make_float2(INFINITY, 0.f);
-
   const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)head * a.q_hs;
   const T *drow = (const T *)g.dout + (int64_t)b * g.do_bs + (int64_t)min(w.i, a.Lq - 1) * g.do_rs + (int64_t)head * g.do_hs;
+  const int64_t orow = (((int64_t)b * a.Lq + min(w.i, a.Lq - 1)) * a.H + head) * a.dh;
   V8 fq[NC], fd[NC];
+  float delta = 0.f;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
     fd[c] = mem_frag<T>(drow, c, h, a.dh, w.live);
+    const V8 o = mem_frag<T>((const T *)g.out + orow, c, h, a.dh, w.live);
+    V8 lo = {};
+    if (g.low) lo = mem_frag<T>((const T *)g.low + orow, c, h, a.dh, w.live);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) delta = fmaf((float)o[e] + (float)lo[e], (float)fd[c][e], delta);
   }
+  const float dl = g.dlse && w.live ? g.dlse[r] : 0.f;
+  delta = half_sum(delta) - dl;
+  float lse = w.live ? g.lse[r] : -INFINITY;
+  lse = lse == -INFINITY ? INFINITY : lse * LOG2E;
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
@@ -674,99 +664,106 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   float all_u = 0.f, far_u[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f};
 
   const int tiles = (gb.hi_max + BK - 1) / BK;
-  TileIter it;
-  it.start(g.krng ? g.krng + (int64_t)b * g.nkt : nullptr, gb.d_min, gb.d_max, 0, tiles);
   const int *kdoc = a.k_doc ? a.k_doc + (int64_t)b * a.Lk : nullptr;
   Dma<T, D> dk, dv;
   dk.init((const T *)a.k + (int64_t)b * a.k_bs + (int64_t)kh * a.k_hs, a.k_rs, a.Lk, a.dh);
   dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
   const unsigned lds = lds_address(smem);
-  int t = it.next(), buf = 0;
-  if (t >= 0) {
-    dk.load(lds, t * BK);
-    dv.load(lds + L::BYTES, t * BK);
-  }
-  while (t >= 0) {
-    const int k0 = t * BK;
-    const bool mixed = it.mixed(), dead = it.cur_dead != 0;
-    char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
-    dma_wait<0>();
-    __syncthreads();
-    if (mixed) {
-      if (threadIdx.x < BK) sDoc[threadIdx.x] = k0 + (int)threadIdx.x < a.Lk ? kdoc[k0 + threadIdx.x] : -1;
+  for (int pass = sizeof(T) == 2 && a.Lk <= TWICE ? 0 : 1; pass < 2; ++pass) {
+    TileIter it;
+    it.start(g.krng ? g.krng + (int64_t)b * g.nkt : nullptr, gb.d_min, gb.d_max, 0, tiles);
+    int t = it.next(), buf = 0;
+    if (t >= 0) {
+      dk.load(lds, t * BK);
+      dv.load(lds + L::BYTES, t * BK);
+    }
+    while (t >= 0) {
+      const int k0 = t * BK;
+      const bool mixed = it.mixed(), dead = it.cur_dead != 0;
+      char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
+      dma_wait<0>();
       __syncthreads();
-    }
-    if (k0 + BK > len || (mixed && dead)) {
-      zero_rows<T, D>(sK, len - k0, mixed ? sDoc : nullptr);
-      zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
-      __syncthreads();
-    }
-    const int tn = it.next();
-    if (tn >= 0) {
-      dk.load(lds + (buf ^ 1) * 2 * L::BYTES, tn * BK);
-      dv.load(lds + (buf ^ 1) * 2 * L::BYTES + L::BYTES, tn * BK);
-    }
-    if (k0 < wb.hi_max) {
-      const bool need_mask = k0 + BK > wb.hi_min || mixed;
-      // by the whole workgroup's rows: the table kernel takes the tiles that are left with the same rule
-      const Place at = place(a, k0 - gb.p_max, k0 + BK - 1 - gb.p_min);
+      if (mixed) {
+        if (threadIdx.x < BK) sDoc[threadIdx.x] = k0 + (int)threadIdx.x < a.Lk ? kdoc[k0 + threadIdx.x] : -1;
+        __syncthreads();
+      }
+      if (k0 + BK > len || (mixed && dead)) {
+        zero_rows<T, D>(sK, len - k0, mixed ? sDoc : nullptr);
+        zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
+        __syncthreads();
+      }
+      const int tn = it.next();
+      if (tn >= 0) {
+        dk.load(lds + (buf ^ 1) * 2 * L::BYTES, tn * BK);
+        dv.load(lds + (buf ^ 1) * 2 * L::BYTES + L::BYTES, tn * BK);
+      }
+      if (k0 < wb.hi_max) {
+        const bool need_mask = k0 + BK > wb.hi_min || mixed;
+        // by the whole workgroup's rows: the table kernel takes the tiles that are left with the same rule
+        const Place at = place(a, k0 - gb.p_max, k0 + BK - 1 - gb.p_min);
 #pragma unroll 1
-      for (int kt = 0; kt < NK; ++kt) {
-        // (the two products one after the other where registers are short: what is live grows with how far the compiler pulls them together)
-        f32x16 s = {}, dp = {};
+        for (int kt = 0; kt < NK; ++kt) {
+          // (the two products one after the other where registers are short: what is live grows with how far the compiler pulls them together)
+          f32x16 s = {}, dp = {};
 #pragma unroll
-        for (int c = 0; c < NC; ++c) s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s);
-        float x[16], th[16];
+          for (int c = 0; c < NC; ++c) s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s);
+          float x[16], th[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = s[i];
-        float cf = sc.c_scale;
-        if constexpr (MOD) {
-          modify<1, true, false>(a, sc, x, th, k0 + 32 * kt + 4 * h - w.p, w.slope, lut.mid, nullptr, at);
-          cf = 1.f;
-        }
-        if (need_mask) mask_keys(x, k0 + 32 * kt, w.hi, mixed ? sDoc + 32 * kt : nullptr, w.doc, h);
+          for (int i = 0; i < 16; ++i) x[i] = s[i];
+          float cf = sc.c_scale;
+          if constexpr (MOD) {
+            modify<1, true, false>(a, sc, x, th, k0 + 32 * kt + 4 * h - w.p, w.slope, lut.mid, nullptr, at);
+            cf = 1.f;
+          }
+          if (need_mask) mask_keys(x, k0 + 32 * kt, w.hi, mixed ? sDoc + 32 * kt : nullptr, w.doc, h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = ex2(fmaf(x[i], cf, -st.x));
-        if constexpr (D > 64) __builtin_amdgcn_sched_barrier(0);
+          for (int i = 0; i < 16; ++i) x[i] = ex2(fmaf(x[i], cf, -lse));
+          if constexpr (D > 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) dp = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp);
-        float su = 0.f, sp = 0.f;
+          for (int c = 0; c < NC; ++c) dp = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp);
+          float su = 0.f, sp = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (MOD) sp += x[i];
-          x[i] *= dp[i] - st.y;
-          if (MOD) su += x[i];
-        }
-        if (MOD && a.rel_bias) {
+          for (int i = 0; i < 16; ++i) {
+            if (MOD) sp += x[i];
+            x[i] *= dp[i] - delta;
+            su += x[i];
+          }
           all_u += su;
-          if (at.far < 0) far_u[0] += su, far_p[0] += sp;
-          if (at.far > 0) far_u[1] += su, far_p[1] += sp;
-        }
-        if (MOD && sc.capped) {
+          if (pass == 0) continue;
+          if (MOD && a.rel_bias) {
+            if (at.far < 0) far_u[0] += su, far_p[0] += sp;
+            if (at.far > 0) far_u[1] += su, far_p[1] += sp;
+          }
+          if (MOD && sc.capped) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] *= fmaf(-th[i], th[i], 1.f);
-        }
-        if (sizeof(T) == 2 && Elem<T>::PSHIFT != 0.f) {
+            for (int i = 0; i < 16; ++i) x[i] *= fmaf(-th[i], th[i], 1.f);
+          }
+          if (sizeof(T) == 2 && Elem<T>::PSHIFT != 0.f) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] *= dscale;
-        }
-        if constexpr (D > 64) __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < 16; ++i) x[i] *= dscale;
+          }
+          if constexpr (D > 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const V8 ds = round8<T>(x + 8 * c);
+          for (int c = 0; c < 2; ++c) {
+            const V8 ds = round8<T>(x + 8 * c);
 #pragma unroll
-          for (int d = 0; d < ND; ++d) acc[d] = Elem<T>::mma(col_frag<T, D>(sK, 32 * kt + 16 * c, d, lane), ds, acc[d]);
+            for (int d = 0; d < ND; ++d) acc[d] = Elem<T>::mma(col_frag<T, D>(sK, 32 * kt + 16 * c, d, lane), ds, acc[d]);
+          }
         }
       }
+      t = tn;
+      buf ^= 1;
     }
-    t = tn;
-    buf ^= 1;
+    // the sum of dU over a row is dlse (0 without it) by definition: what it is instead is the error of delta
+    all_u = lse == INFINITY ? 0.f : half_sum(all_u) - dl;
+    if (pass == 0) {
+      delta += all_u;
+      all_u = 0.f;
+      __syncthreads();                                      // (the buffers are filled anew)
+    }
   }
+  if (w.valid && h == 0) g.stat[r] = make_float2(lse, delta + all_u);
   if (MOD && a.rel_bias) {
-    // the sum of dU over a row is dlse (0 without it) by definition: what is left is what the rounding of o has put into delta
-    all_u = half_sum(all_u) - (g.dlse && w.live ? g.dlse[r] : 0.f);
-    if (w.valid && h == 0) g.delta_fix[r] = st.y + (w.live ? all_u : 0.f);
-    if (!w.live) all_u = 0.f;
 #pragma unroll
     for (int s = 0; s < 2; ++s) far_u[s] = wave_sum(w.live ? far_u[s] - all_u * far_p[s] : 0.f);
     __syncthreads();
@@ -1255,7 +1252,8 @@ __global__ void __launch_bounds__(THREADS, 1) mmt_long_attn_table_kernel(const A
   float *mine = hist + (int64_t)wave * a.n_buckets * 64 + lane;
   for (int k = 0; k < a.n_buckets; ++k) mine[k * 64] = 0.f;
   const int64_t r = ((int64_t)b * a.H + head) * a.Lq + min(w.i, a.Lq - 1);
-  const float lse2 = w.live ? g.stat[r].x : INFINITY, delta = w.live ? g.delta_fix[r] : 0.f;
+  const float2 rs = w.live ? g.stat[r] : make_float2(INFINITY, 0.f);
+  const float lse2 = rs.x, delta = rs.y;
   const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)head * a.q_hs;
   const T *drow = (const T *)g.dout + (int64_t)b * g.do_bs + (int64_t)min(w.i, a.Lq - 1) * g.do_rs + (int64_t)head * g.do_hs;
   V8 fq[NC], fd[NC];
@@ -1408,14 +1406,14 @@ template <typename T> void forward(Args &g, DocRange *ranges, hipStream_t st) {
   }
 }
 
-template <typename T> void backward(Args &g, DocRange *ranges, float2 *stat, f32x4 *maxima, float *table_part, float *dtable, hipStream_t st) {
+template <typename T> void backward(Args &g, DocRange *ranges, f32x4 *maxima, float *table_part, float *dtable, hipStream_t st) {
   const mmt_long_attention &a = g.a;
   if (ranges) docs<T>(g, ranges, true, st), g.krng = ranges, g.qrng = ranges + (int64_t)a.B * g.nkt;
-  const int64_t rows = (int64_t)a.B * a.Lq * a.H, blocks = (rows + 15) / 16;
-  const int parts = (int)(blocks < (maxima ? STAT_PARTS : 8192) ? blocks : (maxima ? STAT_PARTS : 8192));
-  hipLaunchKernelGGL(mmt_long_attn_stat_kernel<T>, dim3(parts), dim3(256), 0, st, g, stat, maxima);
   if (maxima) {
+    const int64_t rows = (int64_t)a.B * (a.Lq * (int64_t)a.H > a.Lk * (int64_t)a.Hk ? a.Lq * (int64_t)a.H : a.Lk * (int64_t)a.Hk), blocks = (rows + 15) / 16;
+    const int parts = (int)(blocks < STAT_PARTS ? blocks : STAT_PARTS);
     g.dscale = (float *)(maxima + STAT_PARTS);
+    hipLaunchKernelGGL(mmt_long_attn_maxima_kernel<T>, dim3(parts), dim3(256), 0, st, g, maxima);
     hipLaunchKernelGGL(mmt_long_attn_dscale_kernel<T>, dim3(1), dim3(64), 0, st, maxima, parts, (float *)(maxima + STAT_PARTS));
   }
   if (a.dh <= 32) bwd_size<T, 32>(g, st, table_part, dtable);
