@@ -77,6 +77,14 @@ template <typename T> __device__ __forceinline__ typename Elem<T>::V8 round8(con
   return r;
 }
 
+// The thread index where nothing derived from it may be taken for loop invariant: in the paths that few tiles take (masks, ragged ends),
+// what the compiler computes ahead of the loop would occupy registers in all of it.
+__device__ __forceinline__ int rare_tid() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 // ---- LDS tiles ------------------------------------------------------------------------------------------------------------
 // BK rows of D elements in 16-byte slots, NS slots per row (a power of two, so that a slot's place is an exclusive or).  A row
 // operand reads one slot of 32 different rows, a transposed read (ds_read_b64_tr_b16: four rows x 16 columns per 16 lanes) four
@@ -194,9 +202,10 @@ template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS> struct Dm
       for (int n = 0; n < N; ++n) dma16(b + n * STEP * rs, off[ONE ? 0 : n], mine + n * NT * 16);
     } else {
       // the rows beyond the last one repeat it
+      const int first = (rare_tid() % NT) / L::NS;
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const int row = (int)(threadIdx.x % NT) / L::NS + n * STEP, over = max(0, r0 + row - (n_rows - 1));
+        const int row = first + n * STEP, over = max(0, r0 + row - (n_rows - 1));
         dma16(b, off[ONE ? 0 : n] + (unsigned)(n * STEP * rs) - (unsigned)(over * rs), mine + n * NT * 16);
       }
     }
@@ -208,9 +217,10 @@ template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS> struct Dm
 template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS>
 __device__ __forceinline__ void zero_rows(char *lds, int end, const int *doc) {
   typedef Tile<T, D> L;
+  const int tid = rare_tid() % NT;
 #pragma unroll
   for (int n = 0; n < R * L::NS / NT; ++n) {
-    const int idx = threadIdx.x % NT + n * NT, row = idx / L::NS;
+    const int idx = tid + n * NT, row = idx / L::NS;
     if (row >= end || (doc && doc[row] < 0)) *(u32x4 *)(lds + idx * 16) = u32x4{};
   }
 }

@@ -174,6 +174,7 @@ __device__ __forceinline__ void modify(const mmt_long_attention &a, const ScoreC
 }
 // what a row does not see -> -inf; key j of the sub-tile is the accumulator's row
 __device__ __forceinline__ void mask_keys(float *x, int key0, int hi, const int *sDoc, int doc, int h) {
+  asm volatile("" : "+v"(h));                             // (few tiles: see rare_tid)
 #pragma unroll
   for (int i = 0; i < 16; ++i) x[i] = key0 + acc_row(i, h) < hi ? x[i] : -INFINITY;
   if (sDoc) {
@@ -356,7 +357,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     dma_wait<0>();
     __syncthreads();                                     // the tile is here, and nobody reads the other buffer any more
     if (mixed) {
-      if (threadIdx.x < BK) sDoc[threadIdx.x] = k0 + (int)threadIdx.x < a.Lk ? kdoc[k0 + threadIdx.x] : -1;
+      const int tid = rare_tid();
+      if (tid < BK) sDoc[tid] = k0 + tid < a.Lk ? kdoc[k0 + tid] : -1;
       __syncthreads();
     }
     if (k0 + BK > len || (mixed && dead)) {              // (a key row only reaches scores that are masked: V alone)
@@ -684,7 +686,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
       dma_wait<0>();
       __syncthreads();
       if (mixed) {
-        if (threadIdx.x < BK) sDoc[threadIdx.x] = k0 + (int)threadIdx.x < a.Lk ? kdoc[k0 + threadIdx.x] : -1;
+        const int tid = rare_tid();
+        if (tid < BK) sDoc[tid] = k0 + tid < a.Lk ? kdoc[k0 + tid] : -1;
         __syncthreads();
       }
       if (k0 + BK > len || (mixed && dead)) {
