@@ -275,9 +275,11 @@ __device__ __forceinline__ float tanh_series(float y) {
   return fmaf(y * z, p, y);
 }
 __device__ __forceinline__ float tanh_any(float y) {
+  asm volatile("" : "+v"(y));                             // (or the series, common to both ways, is hoisted for all elements at once)
   const float e = ex2(y * (2.f * LOG2E));
-  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e);
-  return fabsf(y) <= 0.375f ? tanh_series(y) : big;
+  float big = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e), small = tanh_series(y);
+  asm volatile("" : "+v"(big), "+v"(small));              // (both are computed: a branch per element costs more)
+  return fabsf(y) <= 0.375f ? small : big;
 }
 // x -> tanh(x * f) for N scores of a lane; most tiles of a trained model stay inside the series' range: one wave-uniform branch
 template <int N> __device__ __forceinline__ void tanh_scores(float *x, float f) {
@@ -289,7 +291,10 @@ template <int N> __device__ __forceinline__ void tanh_scores(float *x, float f) 
   }
   if (__any(!(m <= 0.375f))) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = tanh_any(x[i]);
+    for (int i = 0; i < N; ++i) {
+      x[i] = tanh_any(x[i]);
+      if (i % 2) __builtin_amdgcn_sched_barrier(0);       // (two at a time: all at once would set the kernel's register count)
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = tanh_series(x[i]);

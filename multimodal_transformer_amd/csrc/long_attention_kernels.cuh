@@ -128,9 +128,13 @@ __device__ __forceinline__ Place place(const mmt_long_attention &a, int d_lo, in
 }
 // x: 16 raw products of a lane, element i belongs to the distance d0 + STEP (8 (i / 4) + i % 4), STEP 1 or -1.
 // One multiplication and addition takes up the scale, the bias of a tile beyond the reach and, with distances of one sign, the lane's
-// part of the slope; what is left of the slope is a constant per element.
+// part of the slope; what is left of the slope is a constant per element.  Where nothing else is left the scores stay as they are and
+// the multiplication and addition are returned, for the one in front of the exponential.
+struct Linear {
+  float mul, add;                  // score = x mul + add, mul > 0
+};
 template <int STEP, bool KEEP, bool PACKED>
-__device__ __forceinline__ void modify(const mmt_long_attention &a, const ScoreCtx &sc, float *x, float *t, int d0, float slope, const float *lut,
+__device__ __forceinline__ Linear modify(const mmt_long_attention &a, const ScoreCtx &sc, float *x, float *t, int d0, float slope, const float *lut,
                                        const unsigned char *bucket, Place at) {
   float mul = sc.c_scale, add = 0.f;
   if (sc.capped) {
@@ -143,6 +147,7 @@ __device__ __forceinline__ void modify(const mmt_long_attention &a, const ScoreC
   }
   if (sc.rel && at.far != 0) add = PACKED ? lut[bucket[at.far < 0 ? 0 : 2 * a.reach]] : lut[at.far < 0 ? -a.reach : a.reach];
   const float s1 = at.side < 0 ? slope : -slope;          // u += s1 * distance
+  if (!sc.sloped && !(sc.rel && at.far == 0)) return Linear{mul, add};
   if (sc.sloped && at.side != 0) add = fmaf(s1, (float)d0, add);
 #pragma unroll
   for (int i = 0; i < 16; ++i) x[i] = fmaf(x[i], mul, add);
@@ -171,6 +176,7 @@ __device__ __forceinline__ void modify(const mmt_long_attention &a, const ScoreC
       }
     }
   }
+  return Linear{1.f, 0.f};
 }
 // what a row does not see -> -inf; key j of the sub-tile is the accumulator's row
 __device__ __forceinline__ void mask_keys(float *x, int key0, int hi, const int *sDoc, int doc, int h) {
@@ -209,12 +215,10 @@ template <typename T, int D, bool MOD, bool PACKED, int NK>
 __device__ __forceinline__ void fwd_softmax(FwdState<T, D> &st, float *x, int key0, const Row &w, const mmt_long_attention &a, const ScoreCtx &sc,
                                             const float *lut, const unsigned char *bucket, Place at, bool need_mask, const int *sDoc, int h) {
   constexpr int ND = D / 32;
-  float cf = sc.c_scale;
+  Linear f = {sc.c_scale, 0.f};
   if constexpr (MOD) {
-#pragma unroll
-    for (int kt = 0; kt < NK; ++kt)
-      modify<1, false, PACKED>(a, sc, x + 16 * kt, nullptr, key0 + 32 * kt + 4 * h - w.p, w.slope, lut, bucket, at);
-    cf = 1.f;
+    static_assert(NK == 1, "modified scores come 32 keys at a time");
+    f = modify<1, false, PACKED>(a, sc, x, nullptr, key0 + 4 * h - w.p, w.slope, lut, bucket, at);
   }
   if (need_mask) {
 #pragma unroll
@@ -223,15 +227,15 @@ __device__ __forceinline__ void fwd_softmax(FwdState<T, D> &st, float *x, int ke
   float mx = x[0];
 #pragma unroll
   for (int i = 1; i < NK * 16; ++i) mx = fmaxf(mx, x[i]);
-  const float m_new = fmaxf(st.m, half_max(mx) * cf);
+  const float m_new = fmaxf(st.m, fmaf(half_max(mx), f.mul, f.add));
   const float ms = m_new == -INFINITY ? 0.f : m_new;
   const float alpha = ex2(st.m - ms);
   st.m = m_new;
-  const float off = Elem<T>::PSHIFT - ms;
+  const float off = Elem<T>::PSHIFT + (f.add - ms);
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < NK * 16; ++i) {
-    x[i] = ex2(fmaf(x[i], cf, off));
+    x[i] = ex2(fmaf(x[i], f.mul, off));
     sum += x[i];
   }
   st.l = fmaf(st.l, alpha, sum);
@@ -713,14 +717,11 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
           float x[16], th[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = s[i];
-          float cf = sc.c_scale;
-          if constexpr (MOD) {
-            modify<1, true, false>(a, sc, x, th, k0 + 32 * kt + 4 * h - w.p, w.slope, lut.mid, nullptr, at);
-            cf = 1.f;
-          }
+          Linear f = {sc.c_scale, 0.f};
+          if constexpr (MOD) f = modify<1, true, false>(a, sc, x, th, k0 + 32 * kt + 4 * h - w.p, w.slope, lut.mid, nullptr, at);
           if (need_mask) mask_keys(x, k0 + 32 * kt, w.hi, mixed ? sDoc + 32 * kt : nullptr, w.doc, h);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = ex2(fmaf(x[i], cf, -lse));
+          for (int i = 0; i < 16; ++i) x[i] = ex2(fmaf(x[i], f.mul, f.add - lse));
           if constexpr (D > 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int c = 0; c < NC; ++c) dp = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp);
@@ -926,18 +927,18 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
           dp = Elem<T>::mma(row_frag<T, D>(sO, 32 * qt + col, c, h), fv[c], dp);
         }
         float x[16], th[16], p[16];
-        float cf = sc.c_scale;
+        Linear f = {sc.c_scale, 0.f};
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = s[i];
         if constexpr (MOD) {
           const int pq = p0 + 32 * qt;
-          modify<-1, true, false>(a, sc, x, th, j - pq - 4 * h, slope, lut.mid, nullptr, place(a, j_lo - pq - 31, j_lo + 31 - pq));
-          cf = 1.f;
+          f = modify<-1, true, false>(a, sc, x, th, j - pq - 4 * h, slope, lut.mid, nullptr, place(a, j_lo - pq - 31, j_lo + 31 - pq));
         }
+        f.add += Elem<T>::PSHIFT;
         f32x4 st[4];
         acc_rows(st, sStat + 32 * qt, h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = ex2(fmaf(x[i], cf, Elem<T>::PSHIFT - st[i >> 2][i & 3]));
+        for (int i = 0; i < 16; ++i) p[i] = ex2(fmaf(x[i], f.mul, f.add - st[i >> 2][i & 3]));
         if (need_mask) {
           const int lo = a.causal ? (j < prefix ? 0 : j - off - q0 - 32 * qt) : -(1 << 30);      // first row of the sub-tile that sees key j
 #pragma unroll
@@ -1127,18 +1128,18 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
 #pragma unroll
       for (int c = 0; c < NC; ++c) s = Elem<T>::mma(row_frag<T, D>(sQ, 32 * qh + col, c, h), fk[c], s);
       float x[16], th[16], p[16];
-      float cf = sc.c_scale;
+      Linear f = {sc.c_scale, 0.f};
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = s[i];
       if constexpr (MOD) {
         const float slope = a.slopes ? a.slopes[head] * LOG2E : 0.f;
-        modify<-1, true, false>(a, sc, x, th, j - p0 - 4 * h, slope, lut.mid, nullptr, place(a, j_lo - p0 - 31, j_lo + 31 - p0));
-        cf = 1.f;
+        f = modify<-1, true, false>(a, sc, x, th, j - p0 - 4 * h, slope, lut.mid, nullptr, place(a, j_lo - p0 - 31, j_lo + 31 - p0));
       }
+      f.add += Elem<T>::PSHIFT;
       f32x4 st[4];
       acc_rows(st, sStat + 32 * qh, h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = ex2(fmaf(x[i], cf, Elem<T>::PSHIFT - st[i >> 2][i & 3]));
+      for (int i = 0; i < 16; ++i) p[i] = ex2(fmaf(x[i], f.mul, f.add - st[i >> 2][i & 3]));
       if (need_mask) {
         const int lo = a.causal ? (j < prefix ? 0 : j - p0) : -(1 << 30);      // first of the queries that sees key j
 #pragma unroll
