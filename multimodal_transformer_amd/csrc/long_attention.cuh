@@ -154,6 +154,10 @@ template <typename T> __device__ __forceinline__ typename Elem<T>::V8 mem_frag(c
   return r;
 }
 
+// What was loaded ahead of a loop has arrived here.  Otherwise the compiler waits for it at its first use inside the loop, every time
+// around - and with it, requests being counted in order, for the tile that has just been asked for.
+template <typename V> __device__ __forceinline__ void settle(V &v) { asm volatile("" : "+v"(v)); }
+
 // One 16-byte piece per lane straight from memory into LDS (no registers in between): lane l's piece lands at lds + 16 l.
 // Untracked by the compiler: dma_wait before the barrier that publishes the tile.  M0 holds the LDS address.
 __device__ __forceinline__ void dma16(const void *base, unsigned off, unsigned lds) {

@@ -30,6 +30,7 @@ __device__ __forceinline__ Row make_row(const Args &g, int b, int head0, int r, 
   w.hi = len;
   if (a.causal) w.hi = min(len, max(w.p + 1, a.prefix ? a.prefix[b] : 0));
   w.slope = a.slopes && w.valid ? a.slopes[w.h] * LOG2E : 0.f;
+  settle(w.slope);
   return w;
 }
 
@@ -334,6 +335,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   V8 fq[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) settle(fq[c]);
 
   FwdState<T, D> st;
 #pragma unroll
@@ -422,6 +425,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   V8 fq[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) settle(fq[c]);
   FwdState<T, D> st;
 #pragma unroll
   for (int d = 0; d < ND; ++d) st.acc[d] = f32x16{};
@@ -658,10 +663,13 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
 #pragma unroll
     for (int e = 0; e < 8; ++e) delta = fmaf((float)o[e] + (float)lo[e], (float)fd[c][e], delta);
   }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) settle(fq[c]), settle(fd[c]);
   const float dl = g.dlse && w.live ? g.dlse[r] : 0.f;
   delta = half_sum(delta) - dl;
   float lse = w.live ? g.lse[r] : -INFINITY;
   lse = lse == -INFINITY ? INFINITY : lse * LOG2E;
+  settle(lse);
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
@@ -840,6 +848,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
     fk[c] = mem_frag<T>(krow, c, h, a.dh, live);
     fv[c] = mem_frag<T>(vrow, c, h, a.dh, live);
   }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) settle(fk[c]), settle(fv[c]);
   f32x16 acck[ND], accv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acck[d] = f32x16{}, accv[d] = f32x16{};
@@ -865,6 +875,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
   int gi = g0 - 1, t = -1, buf = 0, lut_gi = -1;
   const float2 *stat = nullptr;
   float2 st_next = make_float2(INFINITY, 0.f);
+  float slope_next = 0.f;
   int doc_next = -1;
   auto advance = [&]() {                                  // next tile, over head ends; -1 at the end
     int n = gi < g0 ? -1 : it.next();
@@ -872,6 +883,10 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
       stat = g.stat + ((int64_t)b * a.H + head0 + gi) * a.Lq;
       dmq.base = qbase + (int64_t)gi * a.q_hs * (int64_t)sizeof(T);
       dmo.base = obase + (int64_t)gi * g.do_hs * (int64_t)sizeof(T);
+      if (MOD && a.slopes) {
+        slope_next = a.slopes[head0 + gi] * LOG2E;
+        settle(slope_next);
+      }
       it.start(rng, gd_min, gd_max, t0, t1);
       n = it.next();
     }
@@ -895,6 +910,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
     int *sDoc = sDoc2 + buf * BQ;
     const bool mixed = it.mixed(), dead = it.cur_dead != 0;
     const int cur_gi = gi;
+    const float slope = slope_next;
     if (threadIdx.x < BQ) {
       sDoc[threadIdx.x] = doc_next;
       sStat[threadIdx.x] = st_next.x, sStat[BQ + threadIdx.x] = st_next.y;
@@ -917,7 +933,6 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
     // the last row of the tile sees the most
     if (!a.causal || max(p0 + BQ, prefix) > j_lo) {
       const bool need_mask = mixed || !all_live || (a.causal && max(p0 + 1, prefix) < j_lo + 32);
-      const float slope = MOD && a.slopes ? a.slopes[head] * LOG2E : 0.f;
 #pragma unroll
       for (int qt = 0; qt < NQ; ++qt) {
         f32x16 s = {}, dp = {};
@@ -1046,6 +1061,8 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
     fk[c] = mem_frag<T>(krow, c, h, a.dh, live);
     fv[c] = mem_frag<T>(vrow, c, h, a.dh, live);
   }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) settle(fk[c]), settle(fv[c]);
   // second step: which output, which keys (blocks kb2, kb2 + 1, ..), which dimension tiles (dt2, ..)
   const bool to_k = wave & 1;
   const int part = wave >> 1, kb2 = KB == 2 ? 2 * (part & 1) : part, dt2 = KB == 2 ? NT * (part >> 1) : 0;
@@ -1074,6 +1091,7 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
   int gi = g0 - 1, t = -1, buf = 0, lut_gi = -1;
   const float2 *stat = nullptr;
   float2 st_next = make_float2(INFINITY, 0.f);
+  float slope_next = 0.f;
   int doc_next = -1;
   auto advance = [&]() {
     int n = gi < g0 ? -1 : it.next();
@@ -1081,6 +1099,10 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
       stat = g.stat + ((int64_t)b * a.H + head0 + gi) * a.Lq;
       dmq.base = qbase + (int64_t)gi * a.q_hs * (int64_t)sizeof(T);
       dmo.base = obase + (int64_t)gi * g.do_hs * (int64_t)sizeof(T);
+      if (MOD && a.slopes) {
+        slope_next = a.slopes[head0 + gi] * LOG2E;
+        settle(slope_next);
+      }
       it.start(rng, gd_min, gd_max, t0, t1);
       n = it.next();
     }
@@ -1103,6 +1125,7 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
     float *sStat = sStat2 + buf * 2 * BQ;
     int *sDoc = sDoc2 + buf * BQ;
     const bool mixed = it.mixed(), dead = it.cur_dead != 0;
+    const float slope = slope_next;
     if (threadIdx.x < BQ) {
       sDoc[threadIdx.x] = doc_next;
       sStat[threadIdx.x] = st_next.x, sStat[BQ + threadIdx.x] = st_next.y;
@@ -1132,7 +1155,6 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = s[i];
       if constexpr (MOD) {
-        const float slope = a.slopes ? a.slopes[head] * LOG2E : 0.f;
         f = modify<-1, true, false>(a, sc, x, th, j - p0 - 4 * h, slope, lut.mid, nullptr, place(a, j_lo - p0 - 31, j_lo + 31 - p0));
       }
       f.add += Elem<T>::PSHIFT;
@@ -1266,6 +1288,8 @@ __global__ void __launch_bounds__(THREADS, 1) mmt_long_attn_table_kernel(const A
     fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
     fd[c] = mem_frag<T>(drow, c, h, a.dh, w.live);
   }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) settle(fq[c]), settle(fd[c]);
   const ScoreCtx sc = score_ctx(a);
   const int tiles = (gb.hi_max + BK - 1) / BK;
   const DocRange *rng = g.krng ? g.krng + (int64_t)b * g.nkt : nullptr;
