@@ -34,6 +34,10 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
+template <int N> struct Const {
+  static constexpr int value = N;
+};
+
 // ---- element types --------------------------------------------------------------------------------------------------------
 // BK: keys (queries, in the key-gradient kernel) per LDS tile; fp32 elements are twice as large, so half as many.
 // PSHIFT: probabilities are multiplied by 2^PSHIFT before they are rounded to the element type (and the sums with them): fp16 has

@@ -352,12 +352,14 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   dk.init((const T *)a.k + (int64_t)b * a.k_bs + (int64_t)kh * a.k_hs, a.k_rs, a.Lk, a.dh);
   dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
   const unsigned lds = lds_address(smem);
-  int t = it.next(), buf = 0;
+  int t = it.next();
   if (t >= 0) {
     dk.load(lds, t * BK);
     dv.load(lds + L::BYTES, t * BK);
   }
-  while (t >= 0) {
+  // (the buffer is a constant of the step: every LDS address of the loop is one register and an immediate)
+  auto step = [&](auto buffer) {
+    constexpr int buf = decltype(buffer)::value;
     const int k0 = t * BK;
     const bool mixed = it.mixed(), dead = it.cur_dead != 0;
     char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
@@ -391,7 +393,11 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
       }
     }
     t = tn;
-    buf ^= 1;
+  };
+  while (t >= 0) {
+    step(Const<0>());
+    if (t < 0) break;
+    step(Const<1>());
   }
   fwd_store(g, st, w, b, split, h);
 }
@@ -686,12 +692,13 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   for (int pass = sizeof(T) == 2 && a.Lk <= TWICE ? 0 : 1; pass < 2; ++pass) {
     TileIter it;
     it.start(g.krng ? g.krng + (int64_t)b * g.nkt : nullptr, gb.d_min, gb.d_max, 0, tiles);
-    int t = it.next(), buf = 0;
+    int t = it.next();
     if (t >= 0) {
       dk.load(lds, t * BK);
       dv.load(lds + L::BYTES, t * BK);
     }
-    while (t >= 0) {
+    auto step = [&](auto buffer) {
+      constexpr int buf = decltype(buffer)::value;
       const int k0 = t * BK;
       const bool mixed = it.mixed(), dead = it.cur_dead != 0;
       char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
@@ -716,7 +723,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
         const bool need_mask = k0 + BK > wb.hi_min || mixed;
         // by the whole workgroup's rows: the table kernel takes the tiles that are left with the same rule
         const Place at = place(a, k0 - gb.p_max, k0 + BK - 1 - gb.p_min);
-#pragma unroll 1
+#pragma unroll(D > 64 ? 1 : NK)
         for (int kt = 0; kt < NK; ++kt) {
           // (the two products one after the other where registers are short: what is live grows with how far the compiler pulls them together)
           f32x16 s = {}, dp = {};
@@ -764,7 +771,11 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
         }
       }
       t = tn;
-      buf ^= 1;
+    };
+    while (t >= 0) {
+      step(Const<0>());
+      if (t < 0) break;
+      step(Const<1>());
     }
     // the sum of dU over a row is dlse (0 without it) by definition: what it is instead is the error of delta
     all_u = lse == INFINITY ? 0.f : half_sum(all_u) - dl;
@@ -872,7 +883,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
 
   // the tiles of all heads as one sequence, so that the next head's first tile is on its way during this head's last
   TileIter it;
-  int gi = g0 - 1, t = -1, buf = 0, lut_gi = -1;
+  int gi = g0 - 1, t = -1, lut_gi = -1;
   const float2 *stat = nullptr;
   float2 st_next = make_float2(INFINITY, 0.f);
   float slope_next = 0.f;
@@ -903,7 +914,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
   };
   t = advance();
   if (t >= 0) fetch(t, 0);
-  while (t >= 0) {
+  auto step = [&](auto buffer) {
+    constexpr int buf = decltype(buffer)::value;
     const int q0 = t * BQ, head = head0 + gi;
     char *sQ = smem + buf * 2 * L::BYTES, *sO = sQ + L::BYTES;
     float *sStat = sStat2 + buf * 2 * BQ;
@@ -989,7 +1001,11 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
       }
     }
     t = tn;
-    buf ^= 1;
+  };
+  while (t >= 0) {
+    step(Const<0>());
+    if (t < 0) break;
+    step(Const<1>());
   }
   if (j >= a.Lk) return;
   const int64_t o = (((int64_t)b * a.Lk + j) * a.Hk + kh) * a.dh, part = (int64_t)a.B * a.Lk * a.Hk * a.dh * z;
