@@ -50,13 +50,15 @@ static void plan(Args &g, bool backward) {
   g.G = a.H / a.Hk;
   // few queries: the rows of all heads that share a key head go into one tile of 32, which reads the cache once
   g.few = !backward && (int64_t)a.Lq * g.G <= 32;
-  g.pack = g.few ? g.G : 1;
+  // (else packed where rows of one head would leave more of the tiles of 128 empty; a learned bias is laid out for one head)
+  const bool fewer = ((int64_t)a.Lq * g.G + ROWS - 1) / ROWS < (int64_t)g.G * ((a.Lq + ROWS - 1) / ROWS);
+  g.pack = g.few || (!backward && !a.rel_bias && fewer) ? g.G : 1;
   g.nqt = (int)(((int64_t)a.Lq * g.pack + ROWS - 1) / ROWS);
   g.nkt = (a.Lk + bk - 1) / bk;
   g.groups = a.B * a.Hk;
   g.nsplit = g.zh = g.zq = 1;
   if (!backward) {
-    const int64_t base = (int64_t)g.groups * (g.few ? 1 : g.G) * g.nqt;
+    const int64_t base = (int64_t)g.groups * (g.G / g.pack) * g.nqt;
     const int64_t tiles = g.few ? (a.Lk + 127) / 128 : g.nkt;               // a step of all waves
     if (base < 256) g.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>((512 + base - 1) / base, tiles / 4));
     g.items = (int)(base * g.nsplit);

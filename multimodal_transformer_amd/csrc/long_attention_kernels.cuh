@@ -303,7 +303,8 @@ __device__ __forceinline__ void fwd_store(const Args &g, const FwdState<T, D> &s
     }
 }
 
-// One workgroup = 128 rows (4 waves x 32) of one head against a range of key tiles.  K and V tiles go straight from memory to LDS, one
+// One workgroup = 128 rows (4 waves x 32) of one head - or, without a learned bias and where that takes fewer tiles, of all heads that
+// share a key head - against a range of key tiles.  K and V tiles go straight from memory to LDS, one
 // tile ahead of the products (two buffers, one barrier per tile).  MOD: the scores are capped or biased; without it they go from the
 // product into the exponential as they are.
 template <typename T, int D, bool MOD>
@@ -319,8 +320,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   int n = blockIdx.x / g.groups;
   const int split = n % g.nsplit;
   n /= g.nsplit;
-  const int gi = n % g.G;
-  int qt = n / g.G;
+  const int ngroup = g.G / g.pack, gi = n % ngroup;
+  int qt = n / ngroup;
   if (a.causal) qt = g.nqt - 1 - qt;                     // the tiles with the most keys first
   const int kh = grp % a.Hk, b = grp / a.Hk;
   const int head0 = kh * g.G + gi;
@@ -508,31 +509,40 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   fwd_store(g, st, w, b, split, h);
 }
 
-// Joins the splits of a row: weights 2^(m_s - max m).  16 lanes per row, up to 8 elements per lane.
+// Joins the splits of a row: weights 2^(m_s - max m).  One wave per row: four groups of 16 lanes (8 elements each) take every fourth
+// split and are added in a fixed order.
 template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_join_kernel(const Args g) {
   const mmt_long_attention &a = g.a;
-  const int64_t rows = (int64_t)a.B * a.H * a.Lq, r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int64_t rows = (int64_t)a.B * a.H * a.Lq, r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= rows) return;
-  const int d0 = (threadIdx.x & 15) * 8;
+  const int lane = threadIdx.x & 63, sub = lane >> 4, d0 = (lane & 15) * 8;
   float m = -INFINITY;
-  for (int s = 0; s < g.nsplit; ++s) m = fmaxf(m, g.part_ml[2 * (s * rows + r)]);
+  for (int s = lane; s < g.nsplit; s += 64) m = fmaxf(m, g.part_ml[2 * (s * rows + r)]);
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
   const float ms = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   f32x4 o[2] = {};
-  for (int s = 0; s < g.nsplit; ++s) {
+#pragma unroll 4
+  for (int s = sub; s < g.nsplit; s += 4) {
     const int64_t rs = s * rows + r;
     const float ls = g.part_ml[2 * rs + 1], f = ls == 0.f ? 0.f : ex2(g.part_ml[2 * rs] - ms);
+    f32x4 p[2] = {};
+    if (d0 < a.dh) p[0] = *(const f32x4 *)(g.part_o + rs * a.dh + d0), p[1] = *(const f32x4 *)(g.part_o + rs * a.dh + d0 + 4);
     l = fmaf(ls, f, l);
-    if (d0 < a.dh && ls != 0.f) {
-      o[0] += *(const f32x4 *)(g.part_o + rs * a.dh + d0) * f;
-      o[1] += *(const f32x4 *)(g.part_o + rs * a.dh + d0 + 4) * f;
-    }
+    if (ls != 0.f) o[0] += p[0] * f, o[1] += p[1] * f;   // (a split without keys may hold anything)
+  }
+#pragma unroll
+  for (int k = 16; k < 64; k <<= 1) {
+    l += __shfl_xor(l, k);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e >> 2][e & 3] += __shfl_xor(o[e >> 2][e & 3], k);
   }
   const bool some = l != 0.f;
   const float inv = some ? 1.f / l : 0.f;
   const int64_t i = r % a.Lq, bh = r / a.Lq, hd = bh % a.H, b = bh / a.H;
-  if (g.lse && (threadIdx.x & 15) == 0) g.lse[r] = some ? (m + log2f(l) - Elem<T>::PSHIFT) * LN2 : -INFINITY;
-  if (d0 < a.dh) {
+  if (g.lse && lane == 0) g.lse[r] = some ? (m + log2f(l) - Elem<T>::PSHIFT) * LN2 : -INFINITY;
+  if (sub == 0 && d0 < a.dh) {
     typename Elem<T>::V8 v, lo;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -1446,7 +1456,7 @@ template <typename T> void forward(Args &g, DocRange *ranges, hipStream_t st) {
   else fwd_size<T, 128>(g, st);
   if (g.nsplit > 1) {
     const int64_t rows = (int64_t)a.B * a.H * a.Lq;
-    hipLaunchKernelGGL(mmt_long_attn_join_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, g);
+    hipLaunchKernelGGL(mmt_long_attn_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, g);
   }
 }
 

@@ -1,11 +1,12 @@
 // Norm of queries and keys per head + rotation of their positions in one pass over memory (mmt_qk_norm_rope_fwd / _bwd).
 //
 // A group of LPH lanes (the power of two at or above dh / 8) holds one head of one token, 8 elements per lane: the mean square and,
-// backwards, the dot product are butterflies inside the group, everything else stays in the lane; with the half-split pairing a
-// pair's other element comes from the lane rot / 16 further on.  The angles of a token are shared by all its heads: a workgroup
-// forms them once per token, in 64 bits (position * frequency reaches 10^6 turns, of which fp32 would keep 2 digits), reduces them to
-// a fraction of a turn and keeps cosine and sine in LDS.  Bound by memory: every element is read once and written once (backwards:
-// two read, one written).
+// backwards, the dot product are reductions inside the group, everything else stays in the lane; with the half-split pairing a
+// pair's other element comes from the lane rot / 16 further on.  Both go through the VALU's lane crossings (DPP), not through LDS.
+// The angles of a token are shared by all its heads: a workgroup forms them once per token, in 64 bits (position * frequency reaches
+// 10^6 turns, of which fp32 would keep 2 digits), reduces them to a fraction of a turn, and a lane keeps the cosines and sines of its 8
+// elements in registers while it walks over the token's heads.  Bound by memory: every element is read once and written once
+// (backwards: two read, one written).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -13,6 +14,7 @@
 #include <algorithm>
 
 #include "../../include/mmt_amd.h"
+#include "mmt_gfx950.cuh"
 
 int mmt_set_error(int code, const char *fmt, ...);   // transformer.hip
 
@@ -22,8 +24,7 @@ constexpr int NT = 256, MAX_PARTS = 1024;
 
 template <typename T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
 
-template <typename T> __device__ __forceinline__ void load8(const T *p, float *x) {
-  const typename Vec8<T>::type v = *(const typename Vec8<T>::type *)p;
+template <typename T> __device__ __forceinline__ void widen(const typename Vec8<T>::type &v, float *x) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
 }
@@ -57,20 +58,49 @@ __device__ __forceinline__ void angles(const mmt_qk_norm_rope &a, int64_t t0, in
   }
 }
 
-// the pair partners of a lane's 8 elements (half-split pairing): from the lanes that hold them, or element by element when a half is
-// no whole number of lanes.  v: this lane's elements; row / w: where to fetch them (value = row[d] * scale(d))
-template <int LPH> __device__ __forceinline__ void partners(const float *v, float *o, int lane_in, int half) {
-  const int base = (threadIdx.x & 63) - lane_in, step = half / 8;
-  const int src = base + ((lane_in < step ? lane_in + step : lane_in - step) & (LPH - 1));
+// sum over the LPH lanes of a group, in all of them
+template <int LPH> __device__ __forceinline__ float group_sum(float v) {
+  v += dpp_mov<0xB1>(v);                                // quad_perm: lane ^ 1, lane ^ 2
+  v += dpp_mov<0x4E>(v);
+  if (LPH >= 8) v += dpp_mov<0x141>(v);                 // row_half_mirror
+  if (LPH >= 16) v += dpp_mov<0x140>(v);                // row_mirror
+  if (LPH == 32) v += __shfl_xor(v, 16);
+  return v;
+}
+// v of lane ^ S
+template <int S> __device__ __forceinline__ float lane_xor(float v) {
+  if constexpr (S == 1) return dpp_mov<0xB1>(v);
+  else if constexpr (S == 2) return dpp_mov<0x4E>(v);
+  else if constexpr (S == 8) return dpp_mov<0x128>(v);  // row_ror:8
+  else if constexpr (S == 4) {                          // row_shl:4 into the lower four lanes of each eight, row_shr:4 into the upper
+    const int i = __builtin_bit_cast(int, v);
+    const int low = __builtin_amdgcn_update_dpp(0, i, 0x104, 0xF, 0x5, false);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(low, i, 0x114, 0xF, 0xA, false));
+  } else return __shfl_xor(v, S);
+}
+// the pair partners of a lane's 8 elements with the half-split pairing and halves of whole lanes (half / 8 of them)
+template <int LPH> __device__ __forceinline__ void partners(const float *v, float *o, int lane_in, int step) {
+#define MMT_PARTNERS(S)                                 \
+  if (LPH >= 2 * S && step == S) {                      \
+    _Pragma("unroll") for (int e = 0; e < 8; ++e) o[e] = lane_xor<S>(v[e]); \
+    return;                                             \
+  }
+  MMT_PARTNERS(1) MMT_PARTNERS(2) MMT_PARTNERS(4) MMT_PARTNERS(8) MMT_PARTNERS(16)
+#undef MMT_PARTNERS
+  const int src = (threadIdx.x & 63) - lane_in + ((lane_in < step ? lane_in + step : lane_in - step) & (LPH - 1));
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = __shfl(v[e], src);
 }
 
-template <typename T, int LPH, bool BWD> __global__ void __launch_bounds__(NT) mmt_qk_norm_rope_kernel(const mmt_qk_norm_rope a, const Grads g, void *q_out, void *k_out, int tok) {
+// tok tokens per step and workgroup, their heads dealt over split lane groups each (tok * split = groups of the workgroup)
+template <typename T, int LPH, bool BWD> __global__ void __launch_bounds__(NT) mmt_qk_norm_rope_kernel(const mmt_qk_norm_rope a, const Grads g, void *q_out, void *k_out, int split) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  typedef typename Vec8<T>::type V8;
+  constexpr int GROUPS = NT / LPH;
   float2 *cs = (float2 *)smem;
   const int lane_in = threadIdx.x % LPH, group = threadIdx.x / LPH, d0 = lane_in * 8, half = a.rot / 2, heads = a.H + a.Hk;
-  constexpr int GROUPS = NT / LPH;
+  const int tok = GROUPS / split, lt = group / split, h0 = group % split;
+  const float inv_dh = 1.f / (float)a.dh;
   const bool on = d0 < a.dh, by_lane = half % 8 == 0;
   const int64_t tokens = (int64_t)a.B * a.L;
   float wq[8], wk[8], sq[8] = {}, sk[8] = {};
@@ -81,78 +111,78 @@ template <typename T, int LPH, bool BWD> __global__ void __launch_bounds__(NT) m
   }
   for (int64_t t0 = (int64_t)blockIdx.x * tok; t0 < tokens; t0 += (int64_t)gridDim.x * tok) {
     const int nt = (int)min((int64_t)tok, tokens - t0);
+    const int64_t t = t0 + (lt < nt ? lt : 0), b = t / a.L, i = t - b * a.L;
+    const bool mine = lt < nt && on;
+    const T *qrow = (const T *)a.q + b * a.q_bs + i * a.q_rs, *krow = (const T *)a.k + b * a.k_bs + i * a.k_rs - a.H * a.k_hs;
+    const T *qgrad = BWD ? (const T *)g.dqo + b * g.q_bs + i * g.q_rs : nullptr, *kgrad = BWD ? (const T *)g.dko + b * g.k_bs + i * g.k_rs - a.H * g.k_hs : nullptr;
+    V8 next = {}, gnext = {};
+    auto fetch = [&](int hh) {                          // (one head ahead)
+      const bool is_k = hh >= a.H;
+      next = *(const V8 *)((is_k ? krow + hh * a.k_hs : qrow + hh * a.q_hs) + d0);
+      if (BWD) gnext = *(const V8 *)((is_k ? kgrad + hh * g.k_hs : qgrad + hh * g.q_hs) + d0);
+    };
+    if (mine && h0 < heads) fetch(h0);
     __syncthreads();
     angles(a, t0, nt, cs);
     __syncthreads();
-    for (int u0 = 0; u0 < nt * heads; u0 += GROUPS) {
-      const int u = u0 + group;
-      const bool live = u < nt * heads;
-      const int lt = live ? u / heads : 0, hh = live ? u % heads : 0;
+    float c[8], sn[8];                                  // y = v c + partner sn; elements that are not turned: 1, 0
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = d0 + e;
+      const bool first = a.interleaved ? !(d & 1) : d < half, turned = d < a.rot && lt < nt;
+      const float2 v = turned ? cs[lt * half + (a.interleaved ? d >> 1 : first ? d : d - half)] : make_float2(1.f, 0.f);
+      c[e] = v.x;
+      sn[e] = first != BWD ? -v.y : v.y;                // forward: (-, +) for (first, second); the gradient turns back
+    }
+    for (int hh = h0; hh < heads; hh += split) {
       const bool is_k = hh >= a.H;
-      const int hd = is_k ? hh - a.H : hh;
-      const int64_t t = t0 + lt, b = t / a.L, i = t % a.L;
-      const T *row = is_k ? (const T *)a.k + b * a.k_bs + i * a.k_rs + hd * a.k_hs : (const T *)a.q + b * a.q_bs + i * a.q_rs + hd * a.q_hs;
-      const int64_t oi = is_k ? (t * a.Hk + hd) * a.dh : (t * a.H + hd) * a.dh;
-      const void *wrow = is_k ? a.k_weight : a.q_weight;
-      float x[8] = {}, gy[8] = {};
-      if (live && on) load8(row + d0, x);
-      const T *grow = nullptr;
-      if (BWD) {
-        grow = is_k ? (const T *)g.dko + b * g.k_bs + i * g.k_rs + hd * g.k_hs : (const T *)g.dqo + b * g.q_bs + i * g.q_rs + hd * g.q_hs;
-        if (live && on) load8(grow + d0, gy);
-      }
+      float x[8], gy[8];
+      widen<T>(next, x);
+      if (BWD) widen<T>(gnext, gy);
+      if (mine && hh + split < heads) fetch(hh + split);
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-      for (int m = 1; m < LPH; m <<= 1) ss += __shfl_xor(ss, m);
-      const float r = 1.f / sqrtf(ss / (float)a.dh + a.eps);
-      float v[8], o[8];                       // what is turned (forward: the norm, backward: the gradient), and its partners
+      const float r = 1.f / sqrtf(group_sum<LPH>(ss) * inv_dh + a.eps);
+      float v[8], o[8];                                 // what is turned (forward: the norm, backward: the gradient), and its partners
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = BWD ? gy[e] : x[e] * r * (is_k ? wk[e] : wq[e]);
       if (a.interleaved) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = v[e ^ 1];
       } else if (by_lane) {
-        partners<LPH>(v, o, lane_in, half);
-      } else {
+        partners<LPH>(v, o, lane_in, half / 8);
+      } else {                                          // a half ends inside a lane: element by element from memory
+        const void *wrow = is_k ? a.k_weight : a.q_weight;
+        const T *row = BWD ? (is_k ? kgrad + hh * g.k_hs : qgrad + hh * g.q_hs) : (is_k ? krow + hh * a.k_hs : qrow + hh * a.q_hs);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int d = d0 + e, p = d < half ? d + half : d - half;
           o[e] = 0.f;
-          if (live && on && d < a.rot)
-            o[e] = BWD ? (float)grow[p] : (float)row[p] * r * weight_at<T>(wrow, a.w_dtype == MMT_F32, p);
+          if (mine && d < a.rot) o[e] = BWD ? (float)row[p] : (float)row[p] * r * weight_at<T>(wrow, a.w_dtype == MMT_F32, p);
         }
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = d0 + e;
-        if (d < a.rot) {
-          const bool first = a.interleaved ? !(d & 1) : d < half;
-          const float2 c = cs[lt * half + (a.interleaved ? d >> 1 : first ? d : d - half)];
-          const float s = first != BWD ? -c.y : c.y;         // forward: (-, +) for (first, second); the gradient turns back
-          v[e] = fmaf(o[e], s, v[e] * c.x);
-        }
-      }
+      for (int e = 0; e < 8; ++e) v[e] = d0 + e < a.rot ? fmaf(o[e], sn[e], v[e] * c[e]) : v[e];
+      T *out;
       if (!BWD) {
-        if (live && on) store8((T *)(is_k ? k_out : q_out) + oi + d0, v);
+        out = is_k ? (T *)k_out + (t * a.Hk + (hh - a.H)) * a.dh : (T *)q_out + (t * a.H + hh) * a.dh;
       } else {
+        out = is_k ? (T *)g.dk + (t * a.Hk + (hh - a.H)) * a.dh : (T *)g.dq + (t * a.H + hh) * a.dh;
         float dot = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float c = live ? v[e] * x[e] * r : 0.f;
-          if (is_k) sk[e] += c;
-          else sq[e] += c;
+          const float u = mine ? v[e] * x[e] * r : 0.f;
+          if (is_k) sk[e] += u;
+          else sq[e] += u;
           v[e] *= is_k ? wk[e] : wq[e];
           dot = fmaf(v[e], x[e], dot);
         }
-#pragma unroll
-        for (int m = 1; m < LPH; m <<= 1) dot += __shfl_xor(dot, m);
-        const float f = dot * r * r / (float)a.dh;
+        const float f = group_sum<LPH>(dot) * r * r * inv_dh;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = r * fmaf(-f, x[e], v[e]);
-        if (live && on) store8((T *)(is_k ? g.dk : g.dq) + oi + d0, v);
       }
+      if (mine) store8(out + d0, v);
     }
   }
   if (BWD) {
@@ -173,16 +203,20 @@ template <typename T, int LPH, bool BWD> __global__ void __launch_bounds__(NT) m
   }
 }
 
-// parts -> weight gradients, in 64 bits and in a fixed order: 16 threads per element
-template <typename T> __global__ void mmt_qk_weight_sum_kernel(const float *part, int parts, int dh, int w_f32, void *dqw, void *dkw) {
-  const int n = blockIdx.x * 16 + (threadIdx.x >> 4), s = threadIdx.x & 15;
-  const bool on = n < 2 * dh;
+// parts -> weight gradients, in 64 bits and in a fixed order: 64 threads per element, 16 neighbouring elements per workgroup
+template <typename T> __global__ void __launch_bounds__(1024) mmt_qk_weight_sum_kernel(const float *part, int parts, int dh, int w_f32, void *dqw, void *dkw) {
+  const int n = blockIdx.x * 16 + (threadIdx.x & 15), s = threadIdx.x >> 4;
   double v = 0.;
-  if (on)
-    for (int p = s; p < parts; p += 16) v += part[(int64_t)p * 2 * dh + n];
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) v += __shfl_xor(v, m);
-  if (!on || s) return;
+  if (n < 2 * dh) {
+#pragma unroll 8
+    for (int p = s; p < parts; p += 64) v += part[(int64_t)p * 2 * dh + n];
+  }
+  __shared__ double sum[64][17];
+  sum[s][threadIdx.x & 15] = v;
+  __syncthreads();
+  if (threadIdx.x >= 16 || n >= 2 * dh) return;
+  v = 0.;
+  for (int p = 0; p < 64; ++p) v += sum[p][threadIdx.x];
   void *w = n < dh ? dqw : dkw;
   const int d = n < dh ? n : n - dh;
   if (w_f32) ((float *)w)[d] = (float)v;
@@ -204,8 +238,15 @@ int check(const mmt_qk_norm_rope *a, const char *who) {
   return MMT_OK;
 }
 
-// tokens per workgroup and step: several share the angles' latency, but few tokens are spread over the chip
-int tokens_per_group(const mmt_qk_norm_rope *a) { return (int64_t)a->B * a->L < 4096 ? 1 : 4; }
+// lane groups per token: one, unless there are too few tokens for 2048 workgroups that way (more than there are heads is no use)
+int lanes_per_head(const mmt_qk_norm_rope *a) { return a->dh <= 32 ? 4 : a->dh <= 64 ? 8 : a->dh <= 128 ? 16 : 32; }
+int groups_per_token(const mmt_qk_norm_rope *a) {
+  const int groups = NT / lanes_per_head(a);
+  int split = 1;
+  while (split < groups && split < a->H + a->Hk && (int64_t)a->B * a->L * split < (int64_t)2048 * groups) split *= 2;
+  return split;
+}
+int tokens_per_group(const mmt_qk_norm_rope *a) { return NT / lanes_per_head(a) / groups_per_token(a); }
 int workgroups(const mmt_qk_norm_rope *a, bool bwd) {
   const int tok = tokens_per_group(a);
   const int64_t n = ((int64_t)a->B * a->L + tok - 1) / tok;
@@ -217,12 +258,13 @@ void go(const mmt_qk_norm_rope *a, const Grads &g, void *qo, void *ko, hipStream
   const int tok = tokens_per_group(a);
   size_t lds = (size_t)tok * (a->rot / 2) * sizeof(float2);
   if (BWD) lds = std::max(lds, (size_t)NT * 8 * sizeof(float));
-  hipLaunchKernelGGL((mmt_qk_norm_rope_kernel<T, LPH, BWD>), dim3(workgroups(a, BWD)), dim3(NT), lds, st, *a, g, qo, ko, tok);
+  hipLaunchKernelGGL((mmt_qk_norm_rope_kernel<T, LPH, BWD>), dim3(workgroups(a, BWD)), dim3(NT), lds, st, *a, g, qo, ko, groups_per_token(a));
 }
 template <typename T, bool BWD> void by_size(const mmt_qk_norm_rope *a, const Grads &g, void *qo, void *ko, hipStream_t st) {
-  if (a->dh <= 32) go<T, 4, BWD>(a, g, qo, ko, st);
-  else if (a->dh <= 64) go<T, 8, BWD>(a, g, qo, ko, st);
-  else if (a->dh <= 128) go<T, 16, BWD>(a, g, qo, ko, st);
+  const int lanes = lanes_per_head(a);
+  if (lanes == 4) go<T, 4, BWD>(a, g, qo, ko, st);
+  else if (lanes == 8) go<T, 8, BWD>(a, g, qo, ko, st);
+  else if (lanes == 16) go<T, 16, BWD>(a, g, qo, ko, st);
   else go<T, 32, BWD>(a, g, qo, ko, st);
 }
 template <bool BWD> void by_type(const mmt_qk_norm_rope *a, const Grads &g, void *qo, void *ko, hipStream_t st) {
@@ -266,8 +308,8 @@ extern "C" int mmt_qk_norm_rope_bwd(const mmt_qk_norm_rope *a, const void *dqo, 
   by_type<true>(a, g, nullptr, nullptr, st);
   const int parts = workgroups(a, true), w_f32 = a->w_dtype == MMT_F32;
   const dim3 grid((2 * a->dh + 15) / 16);
-  if (a->dtype == MMT_BF16) hipLaunchKernelGGL(mmt_qk_weight_sum_kernel<__bf16>, grid, dim3(256), 0, st, g.part, parts, a->dh, w_f32, dq_weight, dk_weight);
-  else if (a->dtype == MMT_F16) hipLaunchKernelGGL(mmt_qk_weight_sum_kernel<_Float16>, grid, dim3(256), 0, st, g.part, parts, a->dh, w_f32, dq_weight, dk_weight);
-  else hipLaunchKernelGGL(mmt_qk_weight_sum_kernel<float>, grid, dim3(256), 0, st, g.part, parts, a->dh, w_f32, dq_weight, dk_weight);
+  if (a->dtype == MMT_BF16) hipLaunchKernelGGL(mmt_qk_weight_sum_kernel<__bf16>, grid, dim3(1024), 0, st, g.part, parts, a->dh, w_f32, dq_weight, dk_weight);
+  else if (a->dtype == MMT_F16) hipLaunchKernelGGL(mmt_qk_weight_sum_kernel<_Float16>, grid, dim3(1024), 0, st, g.part, parts, a->dh, w_f32, dq_weight, dk_weight);
+  else hipLaunchKernelGGL(mmt_qk_weight_sum_kernel<float>, grid, dim3(1024), 0, st, g.part, parts, a->dh, w_f32, dq_weight, dk_weight);
   return status("mmt_qk_norm_rope_bwd");
 }
