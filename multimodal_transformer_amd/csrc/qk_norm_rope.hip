@@ -20,7 +20,7 @@ int mmt_set_error(int code, const char *fmt, ...);   // transformer.hip
 
 namespace {
 
-constexpr int NT = 256, MAX_PARTS = 1024;
+constexpr int NT = 256, MAX_PARTS = 2048;
 
 template <typename T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
 
