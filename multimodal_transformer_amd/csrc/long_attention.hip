@@ -65,7 +65,7 @@ static void plan(Args &g, bool backward) {
   } else {
     const int64_t base = (int64_t)g.groups * ((a.Lk + ROWS - 1) / ROWS), want = ((a.causal ? 1024 : 512) + base - 1) / base;
     g.zh = (int)std::min<int64_t>(g.G, want);
-    g.zq = (int)std::max<int64_t>(1, std::min<int64_t>(want / g.zh, (a.Lq + bk - 1) / bk / 4));
+    g.zq = (int)std::max<int64_t>(1, std::min<int64_t>(want / g.zh, (a.Lq + bk - 1) / bk / 8));
   }
 }
 

@@ -11,7 +11,7 @@ namespace la {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS = 32 * WAVES;   // a workgroup: 4 waves of 32 rows each
-constexpr int STAT_PARTS = 1024;                                    // fp16: at most so many workgroups share the maxima
+constexpr int STAT_PARTS = 256, STAT_THREADS = 1024, STAT_ROWS = STAT_THREADS / 16;   // fp16 maxima: workgroups at most, 16 lanes per row
 
 // Smallest / largest live document id of each tile of keys (or queries); live = id >= 0.
 struct DocRange {
@@ -35,7 +35,9 @@ struct Args {                      // mmt_long_attention plus what the launcher 
   const void *dout;
   int64_t do_bs, do_rs, do_hs;
   float2 *stat;                    // (B, H, Lq): lse in units of log 2, rowsum(P dP) - dlse
-  const float *dscale;             // fp16: power of two the score gradients are multiplied by before they are rounded
+  const f32x4 *maxima;             // fp16: the parts of what bounds the score gradients
+  int stat_parts;
+  float *dscale;                   // fp16: power of two the score gradients are multiplied by before they are rounded
   void *dq, *dk, *dv;              // (B, Lq, H, dh), (B, Lk, Hk, dh)
   const float *dlse;               // (B, H, Lq) gradient of the log-sum, or NULL
   float *far_part;                 // (items, 2)

@@ -81,10 +81,24 @@ constexpr int PAD = 192;
 struct Lut {
   float *mid;                      // of distance 0
   static __host__ __device__ int floats(const mmt_long_attention &a) { return a.rel_bias ? (2 * (a.reach + PAD) + 4) & ~3 : 0; }
-  __device__ __forceinline__ void fill(const mmt_long_attention &a, int head) const {
-    for (int n = threadIdx.x; n < 2 * (a.reach + PAD) + 1; n += blockDim.x) {
-      const int d = n - a.reach - PAD;
-      mid[d] = bias_entry(a, head, bias_bucket(a, d));
+  // `bucket` (of distance 0), where it is wanted, receives the bucket numbers too.  Every wave holds the table, one entry per lane, and
+  // asks for the buckets of several distances at once: two waits for memory, whatever the reach.
+  template <int THREADS_ = THREADS> __device__ __forceinline__ void fill(const mmt_long_attention &a, int head, unsigned char *bucket = nullptr) const {
+    constexpr int AT_ONCE = 1024 / THREADS_;
+    const float entry = bias_entry(a, head, min((int)(threadIdx.x & 63), a.n_buckets - 1));
+    const int first = -a.reach - PAD, last = a.reach + PAD;
+    for (int d0 = first; d0 <= last; d0 += 1024) {
+      int k[AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) k[u] = bias_bucket(a, d0 + u * THREADS_ + (int)threadIdx.x);
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int d = d0 + u * THREADS_ + (int)threadIdx.x;
+        const float v = __shfl(entry, k[u]);
+        if (d > last) continue;
+        mid[d] = v;
+        if (bucket) bucket[d] = (unsigned char)k[u];
+      }
     }
   }
 };
@@ -583,7 +597,7 @@ template <typename T> __global__ void mmt_long_attn_docs_kernel(const Args g, in
 
 // fp16: the score gradients are rounded to 5 exponent bits, so they are first multiplied by a power of two that takes their bound
 // 2 max|do_i| max|v_j| + max|dlse| to at most 2^15; each workgroup leaves its part of the three maxima.  16 lanes per row.
-template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_maxima_kernel(const Args g, f32x4 *maxima) {
+template <typename T> __global__ void __launch_bounds__(STAT_THREADS) mmt_long_attn_maxima_kernel(const Args g, f32x4 *maxima) {
   const mmt_long_attention &a = g.a;
   typedef typename Elem<T>::V8 V8;
   const int64_t rows = (int64_t)a.B * a.H * a.Lq, vrows = (int64_t)a.B * a.Lk * a.Hk;
@@ -600,14 +614,14 @@ template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_maxim
     for (int k = 1; k < 16; k <<= 1) s += __shfl_xor(s, k);
     return isfinite(s) ? s : 0.f;
   };
-  for (int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); r < rows; r += (int64_t)gridDim.x * 16) {
+  for (int64_t r = (int64_t)blockIdx.x * STAT_ROWS + (threadIdx.x >> 4); r < rows; r += (int64_t)gridDim.x * STAT_ROWS) {
     const int64_t hd = r % a.H, bi = r / a.H, i = bi % a.Lq, b = bi / a.Lq;
     if (a.q_doc && a.q_doc[b * a.Lq + i] < 0) continue;
     m[0] = fmaxf(m[0], square((const T *)g.dout + b * g.do_bs + i * g.do_rs + hd * g.do_hs));
     const float dl = g.dlse ? fabsf(g.dlse[(b * a.H + hd) * a.Lq + i]) : 0.f;
     if (isfinite(dl)) m[2] = fmaxf(m[2], dl);
   }
-  for (int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); r < vrows; r += (int64_t)gridDim.x * 16) {
+  for (int64_t r = (int64_t)blockIdx.x * STAT_ROWS + (threadIdx.x >> 4); r < vrows; r += (int64_t)gridDim.x * STAT_ROWS) {
     const int64_t hd = r % a.Hk, bj = r / a.Hk, j = bj % a.Lk, b = bj / a.Lk;
     if (j >= row_len(a, (int)b) || (a.k_doc && a.k_doc[b * a.Lk + j] < 0)) continue;
     m[1] = fmaxf(m[1], square((const T *)a.v + b * a.v_bs + j * a.v_rs + hd * a.v_hs));
@@ -615,27 +629,31 @@ template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_maxim
 #pragma unroll
   for (int k = 16; k < 64; k <<= 1)
     for (int e = 0; e < 3; ++e) m[e] = fmaxf(m[e], __shfl_xor(m[e], k));
-  __shared__ f32x4 part[4];
+  __shared__ f32x4 part[STAT_THREADS / 64];
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = f32x4{m[0], m[1], m[2], 0.f};
   __syncthreads();
   if (threadIdx.x == 0) {
     f32x4 v = part[0];
-    for (int w = 1; w < 4; ++w)
+    for (int w = 1; w < STAT_THREADS / 64; ++w)
       for (int e = 0; e < 3; ++e) v[e] = fmaxf(v[e], part[w][e]);
     maxima[blockIdx.x] = v;
   }
 }
-template <typename T> __global__ void __launch_bounds__(64) mmt_long_attn_dscale_kernel(const f32x4 *maxima, int parts, float *dscale) {
+// each wave of the dQ kernel reads them all (4 KiB; a kernel in between cost 6 us and a launch)
+__device__ __forceinline__ float score_grad_scale(const f32x4 *maxima, int parts) {
   f32x4 v = {};
-  for (int n = threadIdx.x; n < parts; n += 64)
-    for (int e = 0; e < 3; ++e) v[e] = fmaxf(v[e], maxima[n][e]);
+#pragma unroll
+  for (int n = 0; n < STAT_PARTS / 64; ++n) {
+    const f32x4 u = maxima[min(n * 64 + (int)(threadIdx.x & 63), parts - 1)];
+    for (int e = 0; e < 3; ++e) v[e] = fmaxf(v[e], u[e]);
+  }
   for (int m = 1; m < 64; m <<= 1)
     for (int e = 0; e < 3; ++e) v[e] = fmaxf(v[e], __shfl_xor(v[e], m));
   const float bound = 2.f * sqrtf(v[0]) * sqrtf(v[1]) + v[2];
   int e = 0;
   const bool known = bound > 0.f && isfinite(bound);
   if (known) (void)frexpf(bound, &e);                                     // bound < 2^e
-  if (threadIdx.x == 0) dscale[0] = ldexpf(1.f, known ? max(-60, min(60, 15 - e)) : 0);
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(ldexpf(1.f, known ? max(-60, min(60, 15 - e)) : 0))));
 }
 
 // dQ, and the statistics of the rows for the other kernels: log-sum in units of log 2 (+inf for a row without keys: its probabilities
@@ -690,7 +708,11 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
   const ScoreCtx sc = score_ctx(a);
-  const float dscale = sizeof(T) == 2 && g.dscale ? g.dscale[0] : 1.f;
+  float dscale = 1.f;
+  if constexpr (Elem<T>::PSHIFT != 0.f) {
+    dscale = score_grad_scale(g.maxima, g.stat_parts);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *g.dscale = dscale;
+  }
   float all_u = 0.f, far_u[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f};
 
   const int tiles = (gb.hi_max + BK - 1) / BK;
@@ -767,7 +789,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] *= fmaf(-th[i], th[i], 1.f);
           }
-          if (sizeof(T) == 2 && Elem<T>::PSHIFT != 0.f) {
+          if constexpr (Elem<T>::PSHIFT != 0.f) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] *= dscale;
           }
@@ -876,7 +898,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
   for (int d = 0; d < ND; ++d) acck[d] = f32x16{}, accv[d] = f32x16{};
   const ScoreCtx sc = score_ctx(a);
   // fp16: P is rounded times 2^PSHIFT; the surplus is taken out of dS again together with its own scaling
-  const float dscale = sizeof(T) == 2 && g.dscale ? g.dscale[0] : 1.f;
+  const float dscale = Elem<T>::PSHIFT != 0.f ? *g.dscale : 1.f;
   const float ds_mul = dscale * ex2(-Elem<T>::PSHIFT);
 
   // queries that may see a key of this workgroup: position >= its first key, unless the prefix reaches into it
@@ -995,7 +1017,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] *= fmaf(-th[i], th[i], 1.f);
         }
-        if (sizeof(T) == 2 && Elem<T>::PSHIFT != 0.f) {
+        if constexpr (Elem<T>::PSHIFT != 0.f) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] *= ds_mul;
         }
@@ -1098,7 +1120,7 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
 #pragma unroll
     for (int d = 0; d < NT; ++d) acc[k][d] = f32x16{};
   const ScoreCtx sc = score_ctx(a);
-  const float dscale = g.dscale ? g.dscale[0] : 1.f;
+  const float dscale = Elem<T>::PSHIFT != 0.f ? *g.dscale : 1.f;
   const float ds_mul = dscale * ex2(-Elem<T>::PSHIFT);
 
   const int i_first = a.causal && prefix <= kt * ROWS ? max(0, kt * ROWS - off) : 0;
@@ -1159,7 +1181,7 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
     dma_wait<0>();
     __syncthreads();                                      // the tile is here; the last one's second step is done everywhere
     if (MOD && a.rel_bias && lut_gi != cur_gi) {          // another head's bias
-      lut.fill(a, head);
+      lut.fill<512>(a, head);
       lut_gi = cur_gi;
       __syncthreads();
     }
@@ -1279,16 +1301,19 @@ template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_dkv_s
 
 // The gradient of the learned bias over the tiles within the reach (the dQ kernel has summed the others).  Sums of millions of
 // signed terms that have to come out right to fp32: dU is recomputed with the exact delta of each row, and every lane adds into
-// a column of its own of a [bucket][lane] array in LDS, so that the order of the additions is the program's.
+// a column of its own of a [bucket][lane] array in LDS, so that the order of the additions is the program's.  Bound by the latency of
+// these load - add - store chains (LDS additions that return nothing took four times as long): four elements at a time are loaded
+// together, each of the four then adds all those of its bucket, so that equal buckets store equal sums.  The next tile is on its way
+// meanwhile.
 template <typename T, int D>
-__global__ void __launch_bounds__(THREADS, 1) mmt_long_attn_table_kernel(const Args g, float *part) {
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_table_kernel(const Args g, float *part) {
   typedef Tile<T, D> L;
   typedef typename Elem<T>::V8 V8;
   constexpr int BK = L::BK, NK = BK / 32, NC = D / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
   char *sK = smem, *sV = smem + L::BYTES;
-  int *sDoc = (int *)(smem + 2 * L::BYTES), *sB = sDoc + BK;
+  int *sDoc = (int *)(smem + 2 * L::BYTES), *sB = sDoc + 2 * BK;
   const Lut lut = {(float *)(sB + 6 * WAVES) + a.reach + PAD};
   unsigned char *bucket = (unsigned char *)((float *)(sB + 6 * WAVES) + Lut::floats(a)) + a.reach + PAD;   // of distance 0
   float *hist = (float *)(sB + 6 * WAVES) + Lut::floats(a) + ((Lut::floats(a) + 15) & ~15) / 4;
@@ -1299,8 +1324,7 @@ __global__ void __launch_bounds__(THREADS, 1) mmt_long_attn_table_kernel(const A
   const Row w = make_row(g, b, head, qt * ROWS + wave * 32 + col, len);
   const Bounds wb = wave_bounds(w);
   const Bounds gb = group_bounds(wb, sB, wave);
-  lut.fill(a, head);
-  for (int n = threadIdx.x; n < 2 * (a.reach + PAD) + 1; n += THREADS) bucket[n - a.reach - PAD] = (unsigned char)bias_bucket(a, n - a.reach - PAD);
+  lut.fill(a, head, bucket);
   float *mine = hist + (int64_t)wave * a.n_buckets * 64 + lane;
   for (int k = 0; k < a.n_buckets; ++k) mine[k * 64] = 0.f;
   const int64_t r = ((int64_t)b * a.H + head) * a.Lq + min(w.i, a.Lq - 1);
@@ -1332,41 +1356,74 @@ __global__ void __launch_bounds__(THREADS, 1) mmt_long_attn_table_kernel(const A
     t1 = min(tiles, max(0, gb.p_max + a.reach + BK) / BK + 1);
     while (t1 > t0 && (t1 - 1) * BK - gb.p_max >= a.reach) --t1;
   }
-  for (int t = t0; t < t1; ++t) {
-    if (rng && (rng[t].lo > gb.d_max || rng[t].hi < gb.d_min)) continue;
+  auto next = [&](int t) {                                // the first tile from t on with documents of these rows
+    while (t < t1 && rng && (rng[t].lo > gb.d_max || rng[t].hi < gb.d_min)) ++t;
+    return t;
+  };
+  auto request = [&](int t, int *ids) {
+    dk.load(lds, t * BK);
+    dv.load(lds + L::BYTES, t * BK);
+    if (kdoc && threadIdx.x < BK) ids[threadIdx.x] = t * BK + (int)threadIdx.x < a.Lk ? kdoc[t * BK + threadIdx.x] : -1;
+  };
+  int t = next(t0);
+  int *ids = sDoc, *ids_next = sDoc + BK;
+  __syncthreads();                                        // (the tables are filled)
+  if (t < t1) request(t, ids);
+  while (t < t1) {
     const int k0 = t * BK;
-    __syncthreads();
-    dk.load(lds, k0);
-    dv.load(lds + L::BYTES, k0);
-    if (kdoc && threadIdx.x < BK) sDoc[threadIdx.x] = k0 + (int)threadIdx.x < a.Lk ? kdoc[k0 + threadIdx.x] : -1;
     dma_wait<0>();
     __syncthreads();
     if (k0 + BK > len || kdoc) {
-      zero_rows<T, D>(sK, len - k0, kdoc ? sDoc : nullptr);
-      zero_rows<T, D>(sV, len - k0, kdoc ? sDoc : nullptr);
+      zero_rows<T, D>(sK, len - k0, kdoc ? ids : nullptr);
+      zero_rows<T, D>(sV, len - k0, kdoc ? ids : nullptr);
       __syncthreads();
     }
-    if (k0 >= wb.hi_max) continue;
+    f32x16 s[NK], dp[NK];
 #pragma unroll
     for (int kt = 0; kt < NK; ++kt) {
-      f32x16 s = {}, dp = {};
+      s[kt] = f32x16{}, dp[kt] = f32x16{};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s);
-        dp = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp);
-      }
-      float x[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = s[i];
-      modify<1, false, false>(a, sc, x, nullptr, k0 + 32 * kt + 4 * h - w.p, w.slope, lut.mid, nullptr, place(a, k0 - gb.p_max, k0 + BK - 1 - gb.p_min));
-      mask_keys(x, k0 + 32 * kt, w.hi, kdoc ? sDoc + 32 * kt : nullptr, w.doc, h);
-      const unsigned char *bk = bucket + max(-a.reach - PAD, min(a.reach + PAD - 27, k0 + 32 * kt + 4 * h - w.p));
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = ex2(x[i] - lse2), u = p * (dp[i] - delta);
-        mine[bk[8 * (i >> 2) + (i & 3)] * 64] += u;
+        s[kt] = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s[kt]);
+        dp[kt] = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp[kt]);
       }
     }
+    __syncthreads();                                      // the products have been taken from the tile
+    t = next(t + 1);
+    if (t < t1) request(t, ids_next);
+    if (k0 < wb.hi_max) {
+      const Place at = place(a, k0 - gb.p_max, k0 + BK - 1 - gb.p_min);
+#pragma unroll
+      for (int kt = 0; kt < NK; ++kt) {
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = s[kt][i];
+        modify<1, false, false>(a, sc, x, nullptr, k0 + 32 * kt + 4 * h - w.p, w.slope, lut.mid, nullptr, at);
+        mask_keys(x, k0 + 32 * kt, w.hi, kdoc ? ids + 32 * kt : nullptr, w.doc, h);
+        const unsigned char *bk = bucket + max(-a.reach - PAD, min(a.reach + PAD - 27, k0 + 32 * kt + 4 * h - w.p));
+        int bucket_of[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bucket_of[i] = bk[8 * (i >> 2) + (i & 3)];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int *n = bucket_of + 4 * q;
+          float u[4], v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = mine[n[e] * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[e] = ex2(x[4 * q + e] - lse2) * (dp[kt][4 * q + e] - delta);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float sum = n[0] == n[e] ? u[0] : 0.f;
+#pragma unroll
+            for (int f = 1; f < 4; ++f) sum += n[f] == n[e] ? u[f] : 0.f;
+            mine[n[e] * 64] = v[e] + sum;
+          }
+        }
+      }
+    }
+    int *swap = ids;
+    ids = ids_next, ids_next = swap;
   }
   __syncthreads();
   // columns -> one value per bucket, in a fixed order: wave u takes buckets u, u + 4, ..
@@ -1424,7 +1481,7 @@ template <typename T, int D> static void bwd_size(Args &g, hipStream_t st, float
   if (mod) launch(mmt_long_attn_dq_kernel<T, D, true>, qitems, lds_q, st, g);
   else launch(mmt_long_attn_dq_kernel<T, D, false>, qitems, lds_q, st, g);
   if (a.rel_bias) {
-    const size_t lds = 2 * L::BYTES + 4 * L::BK + small + 4 * Lut::floats(a) + ((Lut::floats(a) + 15) & ~15) + (size_t)WAVES * a.n_buckets * 256;
+    const size_t lds = 2 * L::BYTES + 8 * L::BK + small + 4 * Lut::floats(a) + ((Lut::floats(a) + 15) & ~15) + (size_t)WAVES * a.n_buckets * 256;
     (void)hipFuncSetAttribute((const void *)mmt_long_attn_table_kernel<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     hipLaunchKernelGGL((mmt_long_attn_table_kernel<T, D>), dim3((unsigned)qitems), dim3(THREADS), lds, st, g, table_part);
     hipLaunchKernelGGL(mmt_long_attn_table_sum_kernel<T>, dim3(a.H * a.n_buckets), dim3(64), 0, st, a, (int64_t)a.B * g.nqt, table_part,
@@ -1464,11 +1521,11 @@ template <typename T> void backward(Args &g, DocRange *ranges, f32x4 *maxima, fl
   const mmt_long_attention &a = g.a;
   if (ranges) docs<T>(g, ranges, true, st), g.krng = ranges, g.qrng = ranges + (int64_t)a.B * g.nkt;
   if (maxima) {
-    const int64_t rows = (int64_t)a.B * (a.Lq * (int64_t)a.H > a.Lk * (int64_t)a.Hk ? a.Lq * (int64_t)a.H : a.Lk * (int64_t)a.Hk), blocks = (rows + 15) / 16;
-    const int parts = (int)(blocks < STAT_PARTS ? blocks : STAT_PARTS);
+    const int64_t rows = (int64_t)a.B * (a.Lq * (int64_t)a.H > a.Lk * (int64_t)a.Hk ? a.Lq * (int64_t)a.H : a.Lk * (int64_t)a.Hk), blocks = (rows + STAT_ROWS - 1) / STAT_ROWS;
+    g.stat_parts = (int)(blocks < STAT_PARTS ? blocks : STAT_PARTS);
+    g.maxima = maxima;
     g.dscale = (float *)(maxima + STAT_PARTS);
-    hipLaunchKernelGGL(mmt_long_attn_maxima_kernel<T>, dim3(parts), dim3(256), 0, st, g, maxima);
-    hipLaunchKernelGGL(mmt_long_attn_dscale_kernel<T>, dim3(1), dim3(64), 0, st, maxima, parts, (float *)(maxima + STAT_PARTS));
+    hipLaunchKernelGGL(mmt_long_attn_maxima_kernel<T>, dim3(g.stat_parts), dim3(STAT_THREADS), 0, st, g, maxima);
   }
   if (a.dh <= 32) bwd_size<T, 32>(g, st, table_part, dtable);
   else if (a.dh <= 64) bwd_size<T, 64>(g, st, table_part, dtable);
