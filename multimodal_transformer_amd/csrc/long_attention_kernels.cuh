@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   constexpr int BK = L::BK, NC = D / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
-  int *sDoc = (int *)(smem + 4 * L::BYTES), *sB = sDoc + BK;
+  int *sDoc2 = (int *)(smem + 4 * L::BYTES), *sB = sDoc2 + 2 * BK;
   const Lut lut = {(float *)(sB + 6 * WAVES) + a.reach + PAD};
   const int grp = blockIdx.x % g.groups;
   int n = blockIdx.x / g.groups;
@@ -368,9 +368,11 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
   const unsigned lds = lds_address(smem);
   int t = it.next();
+  int ids = 0;                                           // the document of the tile's key `lane`
   if (t >= 0) {
     dk.load(lds, t * BK);
     dv.load(lds + L::BYTES, t * BK);
+    if (kdoc) ids = kdoc[min(t * BK + lane, a.Lk - 1)];
   }
   // (the buffer is a constant of the step: every LDS address of the loop is one register and an immediate)
   auto step = [&](auto buffer) {
@@ -378,13 +380,10 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     const int k0 = t * BK;
     const bool mixed = it.mixed(), dead = it.cur_dead != 0;
     char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
+    int *sDoc = sDoc2 + buf * BK;
+    if (kdoc && wave == 0 && lane < BK) sDoc[lane] = ids;
     dma_wait<0>();
     __syncthreads();                                     // the tile is here, and nobody reads the other buffer any more
-    if (mixed) {
-      const int tid = rare_tid();
-      if (tid < BK) sDoc[tid] = k0 + tid < a.Lk ? kdoc[k0 + tid] : -1;
-      __syncthreads();
-    }
     if (k0 + BK > len || (mixed && dead)) {              // (a key row only reaches scores that are masked: V alone)
       zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
       __syncthreads();
@@ -393,6 +392,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     if (tn >= 0) {
       dk.load(lds + (buf ^ 1) * 2 * L::BYTES, tn * BK);
       dv.load(lds + (buf ^ 1) * 2 * L::BYTES + L::BYTES, tn * BK);
+      if (kdoc) ids = kdoc[min(tn * BK + lane, a.Lk - 1)];
     }
     if (k0 < wb.hi_max) {
       const bool need_mask = k0 + BK > wb.hi_min || mixed;
@@ -669,7 +669,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   constexpr int BK = L::BK, NK = BK / 32, NC = D / 16, ND = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
-  int *sDoc = (int *)(smem + 4 * L::BYTES), *sB = sDoc + BK;
+  int *sDoc2 = (int *)(smem + 4 * L::BYTES), *sB = sDoc2 + 2 * BK;
   const Lut lut = {(float *)(sB + 6 * WAVES) + a.reach + PAD};
   const int grp = blockIdx.x % g.groups, n = blockIdx.x / g.groups, gi = n % g.G;
   int qt = n / g.G;
@@ -725,22 +725,21 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     TileIter it;
     it.start(g.krng ? g.krng + (int64_t)b * g.nkt : nullptr, gb.d_min, gb.d_max, 0, tiles);
     int t = it.next();
+    int ids = 0;                                           // the document of the tile's key `lane`
     if (t >= 0) {
       dk.load(lds, t * BK);
       dv.load(lds + L::BYTES, t * BK);
+      if (kdoc) ids = kdoc[min(t * BK + lane, a.Lk - 1)];
     }
     auto step = [&](auto buffer) {
       constexpr int buf = decltype(buffer)::value;
       const int k0 = t * BK;
       const bool mixed = it.mixed(), dead = it.cur_dead != 0;
       char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
+      int *sDoc = sDoc2 + buf * BK;
+      if (kdoc && wave == 0 && lane < BK) sDoc[lane] = ids;
       dma_wait<0>();
       __syncthreads();
-      if (mixed) {
-        const int tid = rare_tid();
-        if (tid < BK) sDoc[tid] = k0 + tid < a.Lk ? kdoc[k0 + tid] : -1;
-        __syncthreads();
-      }
       if (k0 + BK > len || (mixed && dead)) {
         zero_rows<T, D>(sK, len - k0, mixed ? sDoc : nullptr);
         zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
@@ -750,6 +749,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
       if (tn >= 0) {
         dk.load(lds + (buf ^ 1) * 2 * L::BYTES, tn * BK);
         dv.load(lds + (buf ^ 1) * 2 * L::BYTES + L::BYTES, tn * BK);
+        if (kdoc) ids = kdoc[min(tn * BK + lane, a.Lk - 1)];
       }
       if (k0 < wb.hi_max) {
         const bool need_mask = k0 + BK > wb.hi_min || mixed;
@@ -939,9 +939,10 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
     dmq.load(lds + to * 2 * L::BYTES, tile * BQ);
     dmo.load(lds + to * 2 * L::BYTES + L::BYTES, tile * BQ);
     if (threadIdx.x < BQ) {
-      const int i = tile * BQ + threadIdx.x;
-      doc_next = i < a.Lq ? (qdoc ? qdoc[i] : 0) : -1;
-      st_next = doc_next >= 0 ? stat[i] : make_float2(INFINITY, 0.f);
+      // (neither waits for the other, or for the tile: rows that are missing or dead are sorted out when the tile is here)
+      const int i = min(tile * BQ + (int)threadIdx.x, a.Lq - 1);
+      doc_next = qdoc ? qdoc[i] : 0;
+      st_next = stat[i];
     }
   };
   t = advance();
@@ -956,8 +957,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
     const int cur_gi = gi;
     const float slope = slope_next;
     if (threadIdx.x < BQ) {
-      sDoc[threadIdx.x] = doc_next;
-      sStat[threadIdx.x] = st_next.x, sStat[BQ + threadIdx.x] = st_next.y;
+      const int doc = q0 + (int)threadIdx.x < a.Lq ? doc_next : -1;
+      sDoc[threadIdx.x] = doc;
+      sStat[threadIdx.x] = doc >= 0 ? st_next.x : INFINITY, sStat[BQ + threadIdx.x] = doc >= 0 ? st_next.y : 0.f;
     }
     dma_wait<0>();
     __syncthreads();
@@ -1160,9 +1162,10 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
     dmq.load(lds + to * 2 * L::BYTES, tile * BQ);
     dmo.load(lds + to * 2 * L::BYTES + L::BYTES, tile * BQ);
     if (threadIdx.x < BQ) {
-      const int i = tile * BQ + threadIdx.x;
-      doc_next = i < a.Lq ? (qdoc ? qdoc[i] : 0) : -1;
-      st_next = doc_next >= 0 ? stat[i] : make_float2(INFINITY, 0.f);
+      // (neither waits for the other, or for the tile: rows that are missing or dead are sorted out when the tile is here)
+      const int i = min(tile * BQ + (int)threadIdx.x, a.Lq - 1);
+      doc_next = qdoc ? qdoc[i] : 0;
+      st_next = stat[i];
     }
   };
   t = advance();
@@ -1175,8 +1178,9 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
     const bool mixed = it.mixed(), dead = it.cur_dead != 0;
     const float slope = slope_next;
     if (threadIdx.x < BQ) {
-      sDoc[threadIdx.x] = doc_next;
-      sStat[threadIdx.x] = st_next.x, sStat[BQ + threadIdx.x] = st_next.y;
+      const int doc = q0 + (int)threadIdx.x < a.Lq ? doc_next : -1;
+      sDoc[threadIdx.x] = doc;
+      sStat[threadIdx.x] = doc >= 0 ? st_next.x : INFINITY, sStat[BQ + threadIdx.x] = doc >= 0 ? st_next.y : 0.f;
     }
     dma_wait<0>();
     __syncthreads();                                      // the tile is here; the last one's second step is done everywhere
@@ -1466,7 +1470,7 @@ template <typename T, int D> static void fwd_size(const Args &g, hipStream_t st)
     else launch(mmt_long_attn_few_kernel<T, D, false>, g.items, lds, st, g);
     return;
   }
-  const size_t lds = 4 * Tile<T, D>::BYTES + 4 * Tile<T, D>::BK + 24 * WAVES + 4 * Lut::floats(g.a);
+  const size_t lds = 4 * Tile<T, D>::BYTES + 8 * Tile<T, D>::BK + 24 * WAVES + 4 * Lut::floats(g.a);
   if (modified(g.a)) launch(mmt_long_attn_fwd_kernel<T, D, true>, g.items, lds, st, g);
   else launch(mmt_long_attn_fwd_kernel<T, D, false>, g.items, lds, st, g);
 }
@@ -1477,7 +1481,7 @@ template <typename T, int D> static void bwd_size(Args &g, hipStream_t st, float
   const bool mod = modified(a);
   const size_t small = 24 * WAVES;
   const int64_t qitems = (int64_t)a.B * a.H * g.nqt;
-  const size_t lds_q = 4 * L::BYTES + 4 * L::BK + small + 4 * Lut::floats(a);
+  const size_t lds_q = 4 * L::BYTES + 8 * L::BK + small + 4 * Lut::floats(a);
   if (mod) launch(mmt_long_attn_dq_kernel<T, D, true>, qitems, lds_q, st, g);
   else launch(mmt_long_attn_dq_kernel<T, D, false>, qitems, lds_q, st, g);
   if (a.rel_bias) {
