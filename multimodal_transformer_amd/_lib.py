@@ -287,6 +287,27 @@ def load():
     return lib
 
 
+_native = None
+
+
+def native():
+    """_autograd.so: the autograd nodes of the operators that are bound by the host, in C++; raises when it is not built."""
+    global _native
+    if _native is None:
+        try:
+            from . import _autograd
+        except ImportError as e:
+            raise MmtError(f"{os.path.join(_HERE, '_autograd.so')} is not built for this torch ({e}): run "
+                           "`make -C multimodal_transformer_amd/csrc` (or __graft_entry__.build())") from None
+        lib = load()
+        _autograd.bind([C.cast(getattr(lib, n), C.c_void_p).value for n in (
+            "mmt_last_error", "mmt_long_attention_workspace_bytes", "mmt_long_attention_fwd", "mmt_long_attention_bwd",
+            "mmt_qk_norm_rope_fwd", "mmt_qk_norm_rope_workspace_bytes", "mmt_qk_norm_rope_bwd")],
+            (C.sizeof(LongAttention), C.sizeof(QkNormRope)), MmtError)
+        _native = _autograd
+    return _native
+
+
 def check(rc: int, what: str = ""):
     if rc != 0:
         msg = load().mmt_last_error()

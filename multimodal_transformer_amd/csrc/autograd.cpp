@@ -1,0 +1,256 @@
+// Autograd nodes of the operators whose training step is bound by the host: attention over long rows, norm + rotation of queries and
+// keys (no counterpart in the reference).  torch runs a node's backward on a thread of its own.  A Python function has to be entered
+// there, with the interpreter's lock handed over twice, and runs on a core that has not seen it: with 128 rows of 21 tokens and 8
+// heads (fp32) a step of forward and backward took 147 us, of which the kernels are busy for 46.  These nodes do the same without the
+// interpreter: 70 us, and 12 instead of 16 for a call without gradients.  Arguments are checked in Python (ops.py), which also fills the argument struct; the C entry points of libmmt_amd.so are
+// handed over as addresses, so that this file needs torch's headers and nothing of the library's.
+#include <ATen/FuncTorchTLS.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/extension.h>
+
+#include "../../include/mmt_amd.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+typedef std::optional<Tensor> Maybe;
+
+struct Entries {
+  decltype(&mmt_last_error) last_error;
+  decltype(&mmt_long_attention_workspace_bytes) attention_workspace;
+  decltype(&mmt_long_attention_fwd) attention_fwd;
+  decltype(&mmt_long_attention_bwd) attention_bwd;
+  decltype(&mmt_qk_norm_rope_fwd) rope_fwd;
+  decltype(&mmt_qk_norm_rope_workspace_bytes) rope_workspace;
+  decltype(&mmt_qk_norm_rope_bwd) rope_bwd;
+} lib;
+
+struct Failure : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+void check(int rc) {
+  if (rc) throw Failure(lib.last_error());
+}
+
+void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+Tensor like(const Tensor &t) { return at::empty(t.sizes(), at::TensorOptions().dtype(t.scalar_type()).device(t.device())); }
+Tensor bytes(size_t n, const Tensor &beside) { return at::empty({(int64_t)n}, at::TensorOptions().dtype(at::kByte).device(beside.device())); }
+template <typename T> const T *address(const Tensor &t) { return t.defined() ? (const T *)t.const_data_ptr() : nullptr; }
+
+// Row strides of a (B, L, heads, dh) tensor as the kernels read them where it lies, of a copy where they cannot (ops._head_rows)
+struct Rows {
+  const void *p;
+  int64_t b, r, h;
+};
+Rows rows(Tensor &t) {
+  for (int copies = 0;; ++copies) {
+    const int64_t odd = 15 / t.element_size();
+    const Rows s = {t.const_data_ptr(), t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0, t.size(2) > 1 ? t.stride(2) : 0};
+    if (!(t.stride(3) != 1 && t.size(3) > 1) && !((uintptr_t)s.p & 15) && !((s.b | s.r | s.h) & odd) && s.r < (1 << 24)) return s;
+    TORCH_CHECK(copies < 2, "rows cannot be laid out for the kernels");
+    t = copies ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
+  }
+}
+
+// what these nodes do not support has to be an error, as with any other function of torch that does not
+void supported(std::initializer_list<Tensor> inputs) {
+  const auto &functorch = at::functorch::functorchTLSAccessor();
+  if (functorch) functorch->checkSupportsCppAutogradFunction();
+  for (const Tensor &t : inputs)
+    if (t.defined() && t._fw_grad(0).defined()) throw Failure("forward-mode gradients are not supported");
+}
+
+// the gradients have no history of their own: a second derivative is an error, not a silent zero
+variable_list final_grads(variable_list &&g, const char *what) {
+  if (!at::GradMode::is_enabled()) return std::move(g);
+  for (Tensor &t : g)
+    if (t.defined()) t.set_requires_grad(true);
+  return torch::autograd::DelayedError(std::string(what) + ": there is no second derivative", (int64_t)g.size()).apply(std::move(g));
+}
+
+template <typename N> std::shared_ptr<N> node_for(std::initializer_list<Tensor> inputs) {
+  std::shared_ptr<N> n(new N(), torch::autograd::deleteNode);
+  torch::autograd::edge_list edges;
+  for (const Tensor &t : inputs) edges.push_back(t.defined() ? torch::autograd::impl::gradient_edge(t) : torch::autograd::Edge());
+  n->set_next_edges(std::move(edges));
+  return n;
+}
+
+// ---- attention over long rows ----------------------------------------------------------------------------------------------
+struct MmtLongAttentionBackward : public Node {
+  mmt_long_attention a;
+  SavedVariable out, lse, low, q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets;
+  std::string name() const override { return "MmtLongAttentionBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable *s : {&out, &lse, &low, &q, &k, &v, &prefix, &q_doc, &k_doc, &kv_len, &slopes, &rel_bias, &rel_buckets}) s->reset_data();
+  }
+  variable_list apply(variable_list &&grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    Tensor dout = grads[0], dlse = grads[1];
+    if (!dout.defined() && !dlse.defined()) return variable_list(4);
+    const auto self = shared_from_this();
+    const Tensor o = out.unpack(self), l = lse.unpack(self), lo = low.unpack(), pf = prefix.unpack(), qd = q_doc.unpack(), kd = k_doc.unpack(),
+                 kl = kv_len.unpack(), sl = slopes.unpack(), rb = rel_bias.unpack(), ru = rel_buckets.unpack();
+    Tensor qt = q.unpack(), kt = k.unpack(), vt = v.unpack();
+    variable_list g(4);
+    {
+      c10::DeviceGuard device(qt.device());
+      at::AutoDispatchBelowADInplaceOrView below;
+      // (saved tensors may come back at other addresses)
+      const Rows rq = rows(qt), rk = rows(kt), rv = rows(vt);
+      a.q = rq.p, a.q_bs = rq.b, a.q_rs = rq.r, a.q_hs = rq.h;
+      a.k = rk.p, a.k_bs = rk.b, a.k_rs = rk.r, a.k_hs = rk.h;
+      a.v = rv.p, a.v_bs = rv.b, a.v_rs = rv.r, a.v_hs = rv.h;
+      a.prefix = address<int32_t>(pf), a.q_doc = address<int32_t>(qd), a.k_doc = address<int32_t>(kd), a.kv_len = address<int32_t>(kl);
+      a.slopes = address<float>(sl), a.rel_bias = address<float>(rb), a.rel_buckets = address<int32_t>(ru);
+      if (!dout.defined()) dout = at::zeros_like(o);
+      const Rows rd = rows(dout);
+      if (dlse.defined()) dlse = dlse.contiguous();
+      g[0] = like(qt), g[1] = like(kt), g[2] = like(vt);
+      if (rb.defined()) g[3] = like(rb);
+      if ((int64_t)a.B * a.Lq * a.Lk == 0) {
+        for (Tensor &t : g)
+          if (t.defined()) t.zero_();
+      } else {
+        const size_t n = lib.attention_workspace(&a, 1);
+        const Tensor ws = bytes(n, qt);
+        check(lib.attention_bwd(&a, o.const_data_ptr(), lo.defined() ? lo.const_data_ptr() : nullptr, (const float *)l.const_data_ptr(), rd.p, rd.b, rd.r,
+                                rd.h, address<float>(dlse), g[0].mutable_data_ptr(), g[1].mutable_data_ptr(), g[2].mutable_data_ptr(),
+                                rb.defined() ? (float *)g[3].mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), n, stream_of(qt)));
+      }
+    }
+    return final_grads(std::move(g), "long_attention");
+  }
+};
+
+// `args`: address of a checked mmt_long_attention that describes the tensors
+std::tuple<Tensor, Tensor> long_attention(uintptr_t args, const Tensor &q, const Tensor &k, const Tensor &v, const Maybe &prefix, const Maybe &q_doc,
+                                          const Maybe &k_doc, const Maybe &kv_len, const Maybe &slopes, const Maybe &rel_bias, const Maybe &rel_buckets) {
+  const mmt_long_attention &a = *(const mmt_long_attention *)args;
+  const Tensor table = rel_bias.value_or(Tensor());
+  supported({q, k, v, table});
+  const bool wanted = torch::autograd::compute_requires_grad(q, k, v, table);
+  c10::DeviceGuard device(q.device());
+  Tensor out, lse, low;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = like(q);
+    lse = at::empty({a.B, a.H, a.Lq}, at::TensorOptions().dtype(at::kFloat).device(q.device()));
+    if (wanted && a.dtype != MMT_F32) low = like(q);
+    if (!a.Lk) {
+      out.zero_(), lse.fill_(-INFINITY);
+      if (low.defined()) low.zero_();
+    } else if (a.B && a.Lq) {
+      const size_t n = lib.attention_workspace(&a, 0);
+      const Tensor ws = n ? bytes(n, q) : Tensor();
+      check(lib.attention_fwd(&a, out.mutable_data_ptr(), low.defined() ? low.mutable_data_ptr() : nullptr, (float *)lse.mutable_data_ptr(),
+                              n ? ws.mutable_data_ptr() : nullptr, n, stream_of(q)));
+    }
+  }
+  if (wanted) {
+    auto node = node_for<MmtLongAttentionBackward>({q, k, v, table});
+    node->a = a;
+    torch::autograd::set_history({out, lse}, node);
+    node->out = SavedVariable(out, true), node->lse = SavedVariable(lse, true), node->low = SavedVariable(low, false);
+    node->q = SavedVariable(q, false), node->k = SavedVariable(k, false), node->v = SavedVariable(v, false);
+    node->prefix = SavedVariable(prefix, false), node->q_doc = SavedVariable(q_doc, false), node->k_doc = SavedVariable(k_doc, false);
+    node->kv_len = SavedVariable(kv_len, false), node->slopes = SavedVariable(slopes, false);
+    node->rel_bias = SavedVariable(table, false), node->rel_buckets = SavedVariable(rel_buckets, false);
+  }
+  return {out, lse};
+}
+
+// ---- norm + rotation of queries and keys -----------------------------------------------------------------------------------
+struct MmtQkNormRopeBackward : public Node {
+  mmt_qk_norm_rope a;
+  SavedVariable q, k, q_weight, k_weight, inv_freq, positions;
+  std::string name() const override { return "MmtQkNormRopeBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable *s : {&q, &k, &q_weight, &k_weight, &inv_freq, &positions}) s->reset_data();
+  }
+  variable_list apply(variable_list &&grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    Tensor dqo = grads[0], dko = grads[1];
+    if (!dqo.defined() && !dko.defined()) return variable_list(4);
+    Tensor qt = q.unpack(), kt = k.unpack();
+    const Tensor qw = q_weight.unpack(), kw = k_weight.unpack(), fr = inv_freq.unpack(), ps = positions.unpack();
+    variable_list g(4);
+    {
+      c10::DeviceGuard device(qt.device());
+      at::AutoDispatchBelowADInplaceOrView below;
+      const Rows rq = rows(qt), rk = rows(kt);
+      a.q = rq.p, a.q_bs = rq.b, a.q_rs = rq.r, a.q_hs = rq.h;
+      a.k = rk.p, a.k_bs = rk.b, a.k_rs = rk.r, a.k_hs = rk.h;
+      a.q_weight = qw.const_data_ptr(), a.k_weight = kw.const_data_ptr();
+      a.inv_freq = address<double>(fr), a.positions = address<int64_t>(ps);
+      if (!dqo.defined()) dqo = at::zeros_like(qt);
+      if (!dko.defined()) dko = at::zeros_like(kt);
+      const Rows rdq = rows(dqo), rdk = rows(dko);
+      g[0] = like(qt), g[1] = like(kt), g[2] = like(qw), g[3] = like(kw);
+      if ((int64_t)a.B * a.L == 0) {
+        g[2].zero_(), g[3].zero_();
+      } else {
+        const size_t n = lib.rope_workspace(&a);
+        const Tensor ws = bytes(n, qt);
+        check(lib.rope_bwd(&a, rdq.p, rdq.b, rdq.r, rdq.h, rdk.p, rdk.b, rdk.r, rdk.h, g[0].mutable_data_ptr(), g[1].mutable_data_ptr(),
+                           g[2].mutable_data_ptr(), g[3].mutable_data_ptr(), ws.mutable_data_ptr(), n, stream_of(qt)));
+      }
+    }
+    return final_grads(std::move(g), "qk_norm_rope");
+  }
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rope(uintptr_t args, const Tensor &q, const Tensor &k, const Tensor &q_weight, const Tensor &k_weight,
+                                        const Tensor &inv_freq, const Maybe &positions) {
+  const mmt_qk_norm_rope &a = *(const mmt_qk_norm_rope *)args;
+  supported({q, k, q_weight, k_weight});
+  const bool wanted = torch::autograd::compute_requires_grad(q, k, q_weight, k_weight);
+  c10::DeviceGuard device(q.device());
+  Tensor qo, ko;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    qo = like(q), ko = like(k);
+    if (a.B && a.L) check(lib.rope_fwd(&a, qo.mutable_data_ptr(), ko.mutable_data_ptr(), stream_of(q)));
+  }
+  if (wanted) {
+    auto node = node_for<MmtQkNormRopeBackward>({q, k, q_weight, k_weight});
+    node->a = a;
+    torch::autograd::set_history({qo, ko}, node);
+    node->q = SavedVariable(q, false), node->k = SavedVariable(k, false), node->q_weight = SavedVariable(q_weight, false);
+    node->k_weight = SavedVariable(k_weight, false), node->inv_freq = SavedVariable(inv_freq, false), node->positions = SavedVariable(positions, false);
+  }
+  return {qo, ko};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_autograd, m) {
+  // entries: addresses in the order of struct Entries; error: the exception that a failed call raises
+  // sizes: what the caller takes the argument structs' sizes for
+  m.def("bind", [](const std::vector<uintptr_t> &entries, std::pair<size_t, size_t> sizes, py::object error) {
+    TORCH_CHECK(sizes.first == sizeof(mmt_long_attention) && sizes.second == sizeof(mmt_qk_norm_rope), "bind: other argument structs");
+    TORCH_CHECK(entries.size() * sizeof(uintptr_t) == sizeof(Entries), "bind: ", sizeof(Entries) / sizeof(uintptr_t), " entry points are needed");
+    std::memcpy((void *)&lib, entries.data(), sizeof(Entries));
+    static PyObject *raised = nullptr;
+    if (!raised)
+      py::register_exception_translator([](std::exception_ptr p) {
+        try {
+          if (p) std::rethrow_exception(p);
+        } catch (const Failure &e) {
+          PyErr_SetString(raised, e.what());
+        }
+      });
+    raised = error.release().ptr();
+  });
+  m.def("long_attention", &long_attention, py::call_guard<py::gil_scoped_release>());
+  m.def("qk_norm_rope", &qk_norm_rope, py::call_guard<py::gil_scoped_release>());
+}

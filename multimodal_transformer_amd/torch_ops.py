@@ -10,12 +10,13 @@ integer handle (``handle_of``), which stays valid while the descriptor is alive.
 """
 from __future__ import annotations
 
+import ctypes
 import weakref
 
 import torch
 
 from . import ops
-from ._lib import MmtError
+from ._lib import MmtError, native as _native
 
 _HANDLES: "weakref.WeakValueDictionary[int, object]" = weakref.WeakValueDictionary()
 
@@ -155,25 +156,6 @@ for _name, _fn, _meta in (
     _lib.impl(_name, _meta, "Meta")
 
 
-class _LongAttention(torch.autograd.Function):
-    """Differentiable in q, k, v and rel_bias; the arguments of ``mmt::long_attention`` in order."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets):
-        _constant(slopes, "long_attention: the slopes of the distance bias")
-        out, lse, low = ops.long_attention(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets,
-                                           keep_low=True)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(out, lse, low, q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets)
-        ctx.plain = scale, causal, softcap
-        return out, lse
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, dlse):
-        return _long_attention_grads(ctx, dout, dlse, ops.long_attention_backward)
-
-
 def _constant(t, what):
     if t is not None and t.requires_grad:
         raise MmtError(f"{what} are constants, they get no gradient")
@@ -191,23 +173,7 @@ def _long_attention_grads(ctx, dout, dlse, bwd):
     return (dq, dk, dv) + (None,) * 8 + (dbias if rel_bias is not None else None, None)
 
 
-class _QkNormRope(torch.autograd.Function):
-    """Differentiable in q, k and the weights; the arguments of ``mmt::qk_norm_rope`` in order."""
-
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved):
-        _constant(inv_freq, "qk_norm_rope: the frequencies")
-        ctx.save_for_backward(q, k, q_weight, k_weight, inv_freq, positions)
-        ctx.plain = eps, interleaved
-        return ops.qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dqo, dko):
-        return ops.qk_norm_rope_backward(dqo, dko, *ctx.saved_tensors, *ctx.plain) + (None,) * 4
-
-
-# The same through the dispatcher, for callers of torch.ops.mmt.* and for tracing
+# gradients of the dispatcher's ops, for callers of torch.ops.mmt.* and for tracing
 def _long_attention_ctx(ctx, inputs, output):
     q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets = inputs
     _constant(slopes, "long_attention: the slopes of the distance bias")
@@ -242,7 +208,7 @@ torch.library.register_autograd("mmt::qk_norm_rope_bwd", _no_second("qk_norm_rop
 
 def _traced(t):
     """The call is being traced (fake tensors, a dispatch mode, torch.compile): it has to go through the dispatcher.  Otherwise the
-    wrappers below go straight to the kernels, which saves the dispatcher's way through Python (some 50 us per call)."""
+    wrappers below go straight to the kernels."""
     return type(t) not in (torch.Tensor, torch.nn.Parameter) or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
 
 
@@ -301,13 +267,14 @@ def long_attention(q, k, v, *, scale=None, causal=False, prefix=None, q_doc=None
     slopes     (H) float32: -slopes[h] * distance is added         rel_bias  (H,n) float32, learned, at rel_buckets (2 reach + 1) int32 of
                                                                              the clamped distance (``ops.relative_buckets``)
     Rows that see nothing give zeros (and an lse of -inf).  Returns out (B,Lq,H,dh), with ``return_lse`` also the log-sums (B,H,Lq)."""
-    args = (q, k, v, scale, bool(causal), prefix, q_doc, k_doc, kv_len, float(softcap), slopes, rel_bias, rel_buckets)
     if _traced(q):
-        out, lse = torch.ops.mmt.long_attention(*args)[:2]
-    elif torch.is_grad_enabled():
-        out, lse = _LongAttention.apply(*args)
+        out, lse = torch.ops.mmt.long_attention(q, k, v, scale, bool(causal), prefix, q_doc, k_doc, kv_len, float(softcap), slopes,
+                                                rel_bias, rel_buckets)[:2]
     else:
-        out, lse = ops.long_attention(*args)
+        if torch.is_grad_enabled():
+            _constant(slopes, "long_attention: the slopes of the distance bias")
+        a, q, k, v = ops._attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets)
+        out, lse = _native().long_attention(ctypes.addressof(a), q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets)
     return (out, lse) if return_lse else out
 
 
@@ -315,7 +282,9 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps=1e-6
     """RMS norm of queries (B,L,H,dh) and keys (B,L,Hk,dh) per head, times the weights (dh), and the rotation of their first
     2 * len(inv_freq) elements by position * inv_freq (float64, ``ops.rotary_frequencies``) in the same pass; differentiable in q, k
     and the weights.  ``positions`` (B,L) int64, None: 0..L-1.  Pairs are (m, m + rot/2), with ``interleaved`` (2m, 2m + 1)."""
-    args = (q, k, q_weight, k_weight, inv_freq, positions, float(eps), bool(interleaved))
     if _traced(q):
-        return torch.ops.mmt.qk_norm_rope(*args)
-    return _QkNormRope.apply(*args) if torch.is_grad_enabled() else ops.qk_norm_rope(*args)
+        return torch.ops.mmt.qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, float(eps), bool(interleaved))
+    if torch.is_grad_enabled():
+        _constant(inv_freq, "qk_norm_rope: the frequencies")
+    a, q, k = ops._rope_args(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
+    return _native().qk_norm_rope(ctypes.addressof(a), q, k, q_weight, k_weight, inv_freq, positions)
