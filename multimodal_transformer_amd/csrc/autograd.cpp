@@ -53,7 +53,8 @@ Rows rows(Tensor &t) {
   for (int copies = 0;; ++copies) {
     const int64_t odd = 15 / t.element_size();
     const Rows s = {t.const_data_ptr(), t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0, t.size(2) > 1 ? t.stride(2) : 0};
-    if (!(t.stride(3) != 1 && t.size(3) > 1) && !((uintptr_t)s.p & 15) && !((s.b | s.r | s.h) & odd) && s.r < (1 << 24)) return s;
+    if (!(t.stride(3) != 1 && t.size(3) > 1) && !((uintptr_t)s.p & 15) && !((s.b | s.r | s.h) & odd) && s.r * t.element_size() < (1 << 25))
+      return s;
     TORCH_CHECK(copies < 2, "rows cannot be laid out for the kernels");
     t = copies ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
   }

@@ -22,8 +22,10 @@ static int check(const mmt_long_attention *a, const char *who) {
     return mmt_set_error(MMT_EINVAL, "%s: B, H, Hk, Lq and Lk have to be positive", who);
   if (a->H % a->Hk) return mmt_set_error(MMT_EINVAL, "%s: %d query heads are no multiple of %d key heads", who, a->H, a->Hk);
   if (a->dh < 8 || a->dh > 128 || a->dh % 8) return mmt_set_error(MMT_EINVAL, "%s: head size %d, need a multiple of 8 up to 128", who, a->dh);
-  if (!(a->scale > 0.f) || !isfinite(a->scale)) return mmt_set_error(MMT_EINVAL, "%s: the scale has to be positive and finite", who);
-  if (!(a->softcap >= 0.f) || !isfinite(a->softcap)) return mmt_set_error(MMT_EINVAL, "%s: the cap has to be finite and not negative", who);
+  // (also in units of log 2, and divided by one another)
+  if (!(a->scale > 0.f) || !isfinite(2.f * a->scale)) return mmt_set_error(MMT_EINVAL, "%s: the scale has to be positive and finite", who);
+  if (!(a->softcap >= 0.f) || !isfinite(2.f * a->softcap) || (a->softcap > 0.f && !isfinite(a->scale / a->softcap)))
+    return mmt_set_error(MMT_EINVAL, "%s: the cap has to be finite, not negative and not far below the scale", who);
   if (a->prefix && !a->causal) return mmt_set_error(MMT_EINVAL, "%s: a prefix is an exception from the causal mask", who);
   if (!a->q_doc != !a->k_doc) return mmt_set_error(MMT_EINVAL, "%s: documents need ids for the queries and the keys", who);
   if (!a->rel_bias != !a->rel_buckets) return mmt_set_error(MMT_EINVAL, "%s: a learned bias needs its table and its buckets", who);
@@ -36,9 +38,10 @@ static int check(const mmt_long_attention *a, const char *who) {
     return mmt_set_error(MMT_EINVAL, "%s: rows of q, k and v have to start at multiples of 16 bytes", who);
   const int64_t far = ((int64_t)1 << 31) / 64 / elem_size(a->dtype);       // 64 rows are addressed with 32 bits
   if (a->q_rs >= far || a->k_rs >= far || a->v_rs >= far || a->q_rs < 0 || a->k_rs < 0 || a->v_rs < 0)
-    return mmt_set_error(MMT_EINVAL, "%s: token strides have to stay below 2^24 elements", who);
+    return mmt_set_error(MMT_EINVAL, "%s: token strides have to stay below 2^25 bytes", who);
+  // (a launch has fewer than 2^32 threads, 512 to a workgroup)
   const double items = (double)a->B * a->H * (((double)a->Lq + ROWS - 1) / ROWS) + (double)a->B * a->Hk * (((double)a->Lk + ROWS - 1) / ROWS);
-  if (items > 3e7 || (double)a->B * a->H * a->Lq > 2e9) return mmt_set_error(MMT_EINVAL, "%s: too many rows for one call", who);
+  if (items > 8e6 || (double)a->B * a->H * a->Lq > 2e9) return mmt_set_error(MMT_EINVAL, "%s: too many rows for one call", who);
   return MMT_OK;
 }
 
@@ -146,7 +149,7 @@ extern "C" int mmt_long_attention_bwd(const mmt_long_attention *a, const void *o
     return mmt_set_error(MMT_EINVAL, "mmt_long_attention_bwd: null pointer");
   if (((uintptr_t)out | (uintptr_t)out_low | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15 ||
       (do_bs | do_rs | do_hs) % (16 / elem_size(a->dtype)) || do_rs < 0 || do_rs >= ((int64_t)1 << 31) / 64 / elem_size(a->dtype))
-    return mmt_set_error(MMT_EINVAL, "mmt_long_attention_bwd: rows have to start at multiples of 16 bytes, token strides to stay below 2^24 elements");
+    return mmt_set_error(MMT_EINVAL, "mmt_long_attention_bwd: rows have to start at multiples of 16 bytes, token strides to stay below 2^25 bytes");
   Args g = {};
   g.a = *a;
   plan(g, true);

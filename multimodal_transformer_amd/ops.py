@@ -771,7 +771,7 @@ _ELEM = {torch.float32: _lib.MMT_F32, torch.bfloat16: _lib.MMT_BF16, torch.float
 
 def _head_rows(t, name, shape, dtype, device):
     """A (B, L, heads, dh) tensor whose rows (head slices) the kernels can read where they are: contiguous elements, every row at a
-    multiple of 16 bytes; anything else (a transposed last axis, an odd offset) is copied once.  Strides of 0 (broadcast) are fine.
+    multiple of 16 bytes, the next token's less than 2^25 bytes away; anything else (a transposed last axis, an odd offset) is copied once.  Strides of 0 (broadcast) are fine.
     -> the tensor and its address, batch, token and head stride (0 for an axis of length 1, whose stride means nothing)."""
     if not isinstance(t, torch.Tensor):
         raise MmtError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
@@ -786,11 +786,12 @@ def _head_rows(t, name, shape, dtype, device):
         raise MmtError(f"{name}: tensor is on {t.device}, expected {device}")
     b, r, h, one = t.stride()
     p = t.data_ptr()
-    odd = 15 // t.element_size()
-    if one != 1 or (p & 15) or ((b | r | h) & odd) or r >= 1 << 24:
+    size = t.element_size()
+    odd, far = 15 // size, (1 << 25) // size
+    if one != 1 or (p & 15) or ((b | r | h) & odd) or r >= far:
         n0, n1, n2, n3 = t.shape
         b, r, h = b if n0 > 1 else 0, r if n1 > 1 else 0, h if n2 > 1 else 0
-        if (one != 1 and n3 > 1) or (p & 15) or ((b | r | h) & odd) or r >= 1 << 24:
+        if (one != 1 and n3 > 1) or (p & 15) or ((b | r | h) & odd) or r >= far:
             t = t.contiguous()
             if t.data_ptr() & 15:          # contiguous all along, but cut out of a larger buffer at an odd place
                 t = t.clone()
@@ -862,6 +863,8 @@ def _rope_args(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved):
     q, qp, qb, qr, qh = _head_rows(q, "q", None, q.dtype, dev)
     k, kp, kb, kr, kh = _head_rows(k, "k", None, q.dtype, dev)
     B, L, H, dh = q.shape
+    if max(B, L, H, k.shape[2]) > 1 << 30:
+        raise MmtError("qk_norm_rope: too many rows for one call")
     if k.shape[0] != B or k.shape[1] != L or k.shape[3] != dh or k.shape[2] < 1 or H < 1:
         raise MmtError(f"qk_norm_rope: q {tuple(q.shape)} and k {tuple(k.shape)} do not line up")
     if not isinstance(q_weight, torch.Tensor) or q_weight.dtype not in (q.dtype, torch.float32):
@@ -923,6 +926,8 @@ def _attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softca
     v, vp, vb, vr, vh = _head_rows(v, "v", k.shape, q.dtype, dev)
     B, Lq, H, dh = q.shape
     kB, Lk, Hk, kd = k.shape
+    if max(B, Lq, Lk, H) > 1 << 30:
+        raise MmtError("long_attention: too many rows for one call")
     if kB != B or kd != dh or Hk < 1 or H < 1 or H % Hk:
         raise MmtError(f"long_attention: q {tuple(q.shape)} and k {tuple(k.shape)} do not line up (batch, head size, heads a "
                        "multiple of the key heads)")

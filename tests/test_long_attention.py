@@ -623,3 +623,214 @@ def test_a_block_of_scene_attention(dtype):
     for n, x, y in zip(("out", "dqkv", "dq_weight", "dk_weight", "dbias"), got, want):
         rel = float((x.detach().cpu().double() - y).norm() / y.norm())
         assert rel <= 16 * long_rows.unit(dtype) + 2e-6, (n, rel)
+
+
+# ----------------------------------------------------------------------------------------------------------- further CPU checks
+@pytest.mark.parametrize("bad,word", [
+    (dict(scale=3e38), b"scale"), (dict(softcap=3e38), b"cap"), (dict(scale=1.0, softcap=1e-39), b"cap"),
+    (dict(B=9000, Lq=128000, Lk=128), b"too many"), (dict(Lk=(1 << 30) + 1), b"2^30"), (dict(k_rs=1 << 24), b"2^25"),
+    (dict(dtype=_lib.MMT_F32, v_rs=1 << 23), b"2^25")])
+def test_attention_refuses_what_would_overflow(bad, word):
+    lib = _lib.load()
+    a = _desc(**bad)
+    assert lib.mmt_long_attention_workspace_bytes(ctypes.byref(a), 0) == 0
+    assert lib.mmt_long_attention_fwd(ctypes.byref(a), 0x1000, None, None, 0x1000, 1 << 40, None) == -1 and word in lib.mmt_last_error()
+
+
+def test_native_nodes_refuse_another_library():
+    """The nodes are bound to entry points by address: another number of them, or structs of other sizes, is an error."""
+    n = _lib.native()
+    sizes = ctypes.sizeof(_lib.LongAttention), ctypes.sizeof(_lib.QkNormRope)
+    for entries, s in (([0] * 6, sizes), ([0] * 7, (sizes[0] + 8, sizes[1])), ([0] * 7, (sizes[0], sizes[1] - 8))):
+        with pytest.raises(RuntimeError):
+            n.bind(entries, s, MmtError)
+
+
+# ----------------------------------------------------------------------------------------------------------- further GPU checks
+PACKED = {   # Lq, Lk, H, Hk, dh: rows of all heads of a key head fill fewer tiles of 128 together, and are more than 32
+    "slopes": ((20, 300, 8, 2, 64), dict(slopes=True)), "cap": ((40, 700, 4, 1, 128), dict()), "three": ((33, 90, 6, 2, 80), dict(slopes=True, cache=True)),
+    "docs": ((33, 150, 6, 2, 32), dict(docs=[[(4, 50), (1, 80), (-1, 20)], [(0, 150)]])), "prefix": ((15, 64, 8, 2, 96), dict(prefix=True, slopes=True))}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", sorted(PACKED))
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_rows_of_several_heads_in_a_tile(dtype, name):
+    shape, f = PACKED[name]
+    t, kw = _case(dtype, 2, *shape, seed=17, **f)
+    _check(t, kw, dtype, causal=True, softcap=2.0 if name == "cap" else 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [(BF16, 64), (F16, 128), (F32, 64)], ids=lambda c: f"{IDS[c[0]]}x{c[1]}")
+def test_gradients_in_parts_over_heads_and_queries(case):
+    """Few key tiles: dK and dV in parts over the four query heads of a key head and over the queries; with a gradient of the log-sum."""
+    dtype, dh = case
+    t, kw = _case(dtype, 1, 1100, 200, 4, 1, dh, seed=23, slopes=True)
+    _check(t, kw, dtype, with_lse_grad=True)
+    t, kw = _case(dtype, 1, 1100, 1100, 4, 1, dh, seed=24, buckets=8, reach=70)
+    _check(t, kw, dtype, causal=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Lk", [512, 513])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+def test_around_the_longest_row_of_two_passes(dtype, Lk):
+    t, kw = _case(dtype, 1, 130, Lk, 2, 1, 64, seed=Lk, docs=[[(0, Lk - 90), (1, 80), (-1, 10)]])
+    _check(t, kw, dtype, causal=True)
+
+
+def _run(t, kw, **plain):
+    q, k, v = (t[n].clone().requires_grad_() for n in "qkv")
+    kw = dict(kw)
+    leaves = [q, k, v]
+    if "rel_bias" in kw:
+        kw["rel_bias"] = kw["rel_bias"].clone().requires_grad_()
+        leaves.append(kw["rel_bias"])
+    out, lse = torch_ops.long_attention(q, k, v, return_lse=True, **kw, **plain)
+    return [out, lse] + list(torch.autograd.grad(out, leaves, t["go"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Lq", [1, 40])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_numbers_out_of_range_are_clamped(dtype, Lq):
+    """Cache lengths below 0 and above Lk, bucket numbers outside the table, prefixes beyond the row: as the nearest that is inside."""
+    t, kw = _case(dtype, 4, Lq, 90, 4, 2, 64, seed=29, buckets=8, reach=16, both=True)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    lut = kw["rel_buckets"].clone()
+    lut[3], lut[20] = -7, 1000
+    far = _run(t, dict(kw, kv_len=i32([-5, 1 << 30, 3, 90]), rel_buckets=lut, prefix=i32([-(1 << 30), 1 << 30, 200, 5])), causal=True)
+    near = _run(t, dict(kw, kv_len=i32([0, 90, 3, 90]), rel_buckets=lut.clamp(0, 7), prefix=i32([0, 90, 90, 5])), causal=True)
+    assert all(torch.equal(a, b) for a, b in zip(far, near))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_any_document_ids(dtype):
+    """Ids are only compared: the largest ones, in alternation within a tile, give the bits of small ones; so do queries whose ids
+    are in another order than the keys'."""
+    t, kw = _case(dtype, 2, 140, 140, 2, 1, 64, seed=33)
+    small = (torch.arange(140, dtype=torch.int32, device=DEV) % 3).expand(2, 140).contiguous()
+    large = small * ((1 << 30) - 1) + 1                     # 1, 2^30, 2^31 - 1
+    _check(t, dict(q_doc=small, k_doc=small), dtype, causal=True)
+    for q_small in (small, small.flip(1).contiguous()):
+        a = _run(t, dict(q_doc=q_small, k_doc=small), causal=True)
+        b = _run(t, dict(q_doc=q_small * ((1 << 30) - 1) + 1, k_doc=large), causal=True)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=IDS.get)
+def test_tokens_far_apart(dtype):
+    """Token strides at and beyond 2^25 bytes are copied, below it read in place; head and batch strides may be of any size."""
+    far = (1 << 25) // dtype.itemsize
+    flat = torch.zeros(3 * far + 64, dtype=dtype, device=DEV)
+    g = torch.Generator().manual_seed(2)
+    for stride in (far - 64, far):                        # (2 x 2 heads at distinct multiples of the stride)
+        for st in ((0, stride, 16, 1), (2 * stride, 32, stride, 1)):
+            k = torch.as_strided(flat, (1, 3, 2, 16) if st[0] == 0 else (2, 1, 2, 16), st)
+            x = torch.randn(k.shape, generator=g).to(dtype).to(DEV)
+            k.copy_(x)
+            q = torch.randn(k.shape, generator=g).to(dtype).to(DEV)
+            a = _run({"q": k, "k": q, "v": q, "go": q}, {})
+            b = _run({"q": x, "k": q, "v": q, "go": q}, {})
+            assert all(torch.equal(u, w) for u, w in zip(a, b))
+            out = [torch_ops.long_attention(q, kk, kk) for kk in (k, x)]
+            assert torch.equal(*out)
+    with pytest.raises(MmtError):
+        torch_ops.long_attention(q, q.new_zeros(2, 1, 2, 16).expand(2, (1 << 30) + 1, 2, 16), q.new_zeros(2, 1, 2, 16).expand(2, (1 << 30) + 1, 2, 16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_the_graph_keeps_autograds_rules(dtype):
+    """Saved tensors that come back from elsewhere, a graph kept and walked twice, recomputation, some leaves only; inputs changed in
+    place, a graph walked after its end, forward-mode and functional transforms are errors."""
+    t, kw = _case(dtype, 2, 50, 50, 4, 2, 32, seed=41, buckets=8, reach=16)
+    w, f = torch.ones(32, dtype=dtype, device=DEV), ops.rotary_frequencies(32, device=DEV)
+    leaves = [x.clone().requires_grad_() for x in (t["q"], t["k"], t["v"], kw["rel_bias"], w)]
+
+    def call(q, k, v, b, ww):
+        x, y = torch_ops.qk_norm_rope(q, k, ww, w, f)
+        return torch_ops.long_attention(x, y, v.transpose(1, 2).contiguous().transpose(1, 2), causal=True, rel_bias=b, rel_buckets=kw["rel_buckets"])
+    out = call(*leaves)
+    want = torch.autograd.grad(out, leaves, t["go"], retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(out, leaves, t["go"])))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, leaves, t["go"])
+    with torch.autograd.graph.save_on_cpu():
+        out = call(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(out, leaves, t["go"])))
+    out = torch.utils.checkpoint.checkpoint(call, *leaves, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(out, leaves, t["go"])))
+    for n in range(5):
+        some = [x if i == n else x.detach() for i, x in enumerate(leaves)]
+        assert torch.equal(torch.autograd.grad(call(*some), leaves[n], t["go"])[0], want[n])
+    assert not call(*[x.detach() for x in leaves]).requires_grad
+    with torch.no_grad():
+        assert not call(*leaves).requires_grad
+    with torch.inference_mode():
+        assert torch.equal(call(*leaves), out)
+    q = leaves[0] * 1
+    o = torch_ops.long_attention(q, leaves[1], leaves[2])
+    q.zero_()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(o, leaves[1], t["go"])
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(t["q"], t["go"])
+        for fn in (lambda: torch_ops.long_attention(dual, t["k"], t["v"]), lambda: torch_ops.qk_norm_rope(dual, t["k"], w, w, f)):
+            with pytest.raises((MmtError, RuntimeError)):
+                fn()
+    with pytest.raises((MmtError, RuntimeError)):
+        torch.func.grad(lambda q: torch_ops.long_attention(q, t["k"], t["v"]).float().sum())(t["q"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+def test_a_training_step_in_a_graph(dtype):
+    """Forward and backward through the differentiable entry points, captured together on leaves of their own; every replay equals the
+    eager step on the inputs of its turn."""
+    t, kw = _case(dtype, 2, 140, 140, 4, 2, 64, seed=43, buckets=8, reach=30)
+    w, f = torch.ones(64, dtype=dtype, device=DEV), ops.rotary_frequencies(64, device=DEV)
+
+    def step():
+        q, k, v, b, ww = (x.detach().requires_grad_() for x in (t["q"], t["k"], t["v"], kw["rel_bias"], w))
+        x, y = torch_ops.qk_norm_rope(q, k, ww, w, f)
+        o = torch_ops.long_attention(x, y, v, causal=True, rel_bias=b, rel_buckets=kw["rel_buckets"])
+        return [o.detach()] + list(torch.autograd.grad(o, (q, k, v, b, ww), t["go"]))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for turn in range(3):
+        for x in (t["q"], t["k"], t["go"]):
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(200 + turn)).to(dtype))
+        want = [x.clone() for x in step()]
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), turn
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh,rot", [(256, 256), (128, 32), (96, 48), (256, 80), (32, 32), (16, 16), (64, 24), (64, 6)])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_norm_rope_pairs(dtype, dh, rot):
+    """Every distance between the two of a pair: 1, 2, 4, 8, 16 lanes, other numbers of whole lanes, halves that end inside a lane."""
+    g = torch.Generator().manual_seed(dh + rot)
+    q, k = (torch.randn(2, 11, n, dh, generator=g).to(dtype).to(DEV).requires_grad_() for n in (3, 1))
+    w = (1 + 0.3 * torch.randn(dh, generator=g)).to(dtype).to(DEV).requires_grad_()
+    f = ops.rotary_frequencies(rot, 100.0, DEV)
+    gq, gk = (torch.randn(x.shape, generator=g).to(dtype).to(DEV) for x in (q, k))
+    for inter in (False, True):
+        yq, yk = torch_ops.qk_norm_rope(q, k, w, w.detach(), f, interleaved=inter)
+        dq, dk, dw = torch.autograd.grad((yq, yk), (q, k, w), (gq, gk))
+        for x, gy, y, dx, dwx in ((q, gq, yq, dq, dw), (k, gk, yk, dk, None)):
+            val, tol = long_rows.norm_rope(x, w, f, None, 1e-6, inter, gy)
+            _near(y, val["y"], tol["y"], "y")
+            _near(dx, val["dx"], tol["dx"], "dx")
+            if dwx is not None:
+                _near(dwx, val["dw"], tol["dw"], "dw")
