@@ -149,16 +149,22 @@ template <typename T, int D> __device__ __forceinline__ typename Elem<T>::V8 col
   }
 }
 
-// row operand straight from memory (the tile that stays in registers); elements at and beyond dh, and dead rows, are zero
-template <typename T> __device__ __forceinline__ typename Elem<T>::V8 mem_frag(const T *row, int c, int h, int dh, bool live) {
-  typedef typename Elem<T>::V8 V8;
-  V8 r = {};
+// Row operand straight from memory (the tile that stays in registers), whatever the row holds: requested before it is known which rows
+// are live, so that a workgroup's first loads wait for nothing.  `live_frag` zeroes dead rows, and elements at and beyond dh, and is where
+// the operand has to be here.
+template <typename T> __device__ __forceinline__ typename Elem<T>::V8 mem_frag(const T *row, int c, int h, int dh) {
   const int d = 16 * c + 8 * h;
-  if (live && d < dh) r = *(const V8 *)(row + d);
-  return r;
+  return *(const typename Elem<T>::V8 *)(row + (d < dh ? d : 0));
 }
+template <typename V> __device__ __forceinline__ void live_frag(V &v, int c, int h, int dh, bool live) {
+  const bool in = live && 16 * c + 8 * h < dh;
+  v = in ? v : V{};
+  asm volatile("" : "+v"(v));
+}
+// a value that all lanes share and no kernel of this call writes
+template <typename V> __device__ __forceinline__ V scalar_load(const V *p) { return *(const __attribute__((address_space(4))) V *)(uintptr_t)p; }
 
-// What was loaded ahead of a loop has arrived here.  Otherwise the compiler waits for it at its first use inside the loop, every time
+// What was loaded ahead of a loop has arrived here (live_frag does the same).  Otherwise the compiler waits for it at its first use inside the loop, every time
 // around - and with it, requests being counted in order, for the tile that has just been asked for.
 template <typename V> __device__ __forceinline__ void settle(V &v) { asm volatile("" : "+v"(v)); }
 
@@ -321,12 +327,17 @@ struct TileIter {
   unsigned long long mask;
   DocRange mine;
   int cur_lo, cur_hi, cur_dead;                      // of the tile that next() returned
-  __device__ __forceinline__ void start(const DocRange *r, int l, int h, int t0, int t1) {
-    rng = r, lo = l, hi = h, base = t0, end = t1;
-    mine = DocRange{0, 0, 0, 0};
-    cur_lo = cur_hi = cur_dead = 0;
-    fill();
+  // `ready`: the ranges of tiles t0 .. t0 + 63, one per lane, where they have been loaded already
+  static __device__ __forceinline__ DocRange ahead(const DocRange *r, int t0, int n_tiles) {
+    return r ? r[min(t0 + (int)(threadIdx.x & 63), n_tiles - 1)] : DocRange{0, 0, 0, 0};
   }
+  __device__ __forceinline__ void start(const DocRange *r, int l, int h, int t0, int t1, DocRange ready) {
+    rng = r, lo = l, hi = h, base = t0, end = t1;
+    mine = ready;
+    cur_lo = cur_hi = cur_dead = 0;
+    mask = __ballot(base + (int)(threadIdx.x & 63) < end && (!rng || (mine.lo <= hi && mine.hi >= lo)));
+  }
+  __device__ __forceinline__ void here() { settle(mine.lo), settle(mine.hi), settle(mine.dead); }     // (ahead of a loop: see settle)
   __device__ __forceinline__ void fill() {
     const int t = base + (threadIdx.x & 63);
     bool ok = t < end;

@@ -14,10 +14,15 @@ struct Row {
 };
 
 template <typename A> __device__ __forceinline__ int row_len(const A &a, int b) {
-  return a.kv_len ? max(0, min(a.kv_len[b], a.Lk)) : a.Lk;
+  return a.kv_len ? max(0, min(scalar_load(a.kv_len + b), a.Lk)) : a.Lk;
 }
 
-__device__ __forceinline__ Row make_row(const Args &g, int b, int head0, int r, int len) {
+// first invisible key of position p, before documents
+__device__ __forceinline__ int visible_end(const mmt_long_attention &a, int len, int prefix, int p) {
+  return a.causal ? min(len, max(p + 1, prefix)) : len;
+}
+// (the document and the slope are only on their way: dead rows, and settle(slope), where they are needed)
+__device__ __forceinline__ Row make_row(const Args &g, int b, int head0, int r, int len, int prefix) {
   const mmt_long_attention &a = g.a;
   Row w;
   w.i = r / g.pack;
@@ -25,12 +30,10 @@ __device__ __forceinline__ Row make_row(const Args &g, int b, int head0, int r, 
   w.valid = w.i < a.Lq;
   w.p = len - a.Lq + w.i;
   w.doc = 0;
-  if (a.q_doc && w.valid) w.doc = a.q_doc[(int64_t)b * a.Lq + w.i];
+  if (a.q_doc) w.doc = a.q_doc[(int64_t)b * a.Lq + min(w.i, a.Lq - 1)];
+  w.slope = a.slopes ? a.slopes[w.h] * LOG2E : 0.f;
   w.live = w.valid && w.doc >= 0;
-  w.hi = len;
-  if (a.causal) w.hi = min(len, max(w.p + 1, a.prefix ? a.prefix[b] : 0));
-  w.slope = a.slopes && w.valid ? a.slopes[w.h] * LOG2E : 0.f;
-  settle(w.slope);
+  w.hi = visible_end(a, len, prefix, w.p);
   return w;
 }
 
@@ -47,6 +50,13 @@ __device__ __forceinline__ Bounds wave_bounds(const Row &w) {
   b.d_min = wave_min(w.live ? w.doc : 0x7fffffff);
   b.d_max = wave_max(w.live ? w.doc : -1);
   return b;
+}
+// without documents they follow from the first and the last of rows r0 .. r0 + n - 1
+__device__ __forceinline__ Bounds range_bounds(const Args &g, int r0, int n, int len, int prefix) {
+  const mmt_long_attention &a = g.a;
+  const int i0 = r0 / g.pack, i1 = min(a.Lq - 1, (r0 + n - 1) / g.pack), off = len - a.Lq;
+  if (i0 > i1) return Bounds{0x7fffffff, 0, 0x7fffffff, -0x7fffffff, 0x7fffffff, -1};
+  return Bounds{visible_end(a, len, prefix, off + i0), max(0, visible_end(a, len, prefix, off + i1)), off + i0, off + i1, 0, 0};
 }
 __device__ __forceinline__ Bounds group_bounds(const Bounds &w, int *s, int wave) {      // s: 6 * WAVES ints of LDS
   if ((threadIdx.x & 63) == 0) {
@@ -340,29 +350,23 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   const int kh = grp % a.Hk, b = grp / a.Hk;
   const int head0 = kh * g.G + gi;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
-  const int len = row_len(a, b);
-  const Row w = make_row(g, b, head0, qt * ROWS + wave * 32 + col, len);
-  const Bounds wb = wave_bounds(w);
-  const Bounds gb = group_bounds(wb, sB, wave);
-  if (MOD && a.rel_bias) lut.fill(a, head0);
-
+  const int len = row_len(a, b), prefix = a.prefix ? scalar_load(a.prefix + b) : 0;
+  // what does not depend on one another is requested before any of it is waited for: the time of a short row is these waits
+  Row w = make_row(g, b, head0, qt * ROWS + wave * 32 + col, len, prefix);
   const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)w.h * a.q_hs;
   V8 fq[NC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
-#pragma unroll
-  for (int c = 0; c < NC; ++c) settle(fq[c]);
-
-  FwdState<T, D> st;
-#pragma unroll
-  for (int d = 0; d < D / 32; ++d) st.acc[d] = f32x16{};
-  st.m = -INFINITY, st.l = 0.f;
-  const ScoreCtx sc = score_ctx(a);
-
-  const int tiles = (gb.hi_max + BK - 1) / BK, per = (tiles + g.nsplit - 1) / g.nsplit;
-  TileIter it;
-  it.start(g.krng ? g.krng + (int64_t)b * g.nkt : nullptr, gb.d_min, gb.d_max, split * per, min(tiles, (split + 1) * per));
+  for (int c = 0; c < NC; ++c) fq[c] = mem_frag<T>(qrow, c, h, a.dh);
+  const DocRange *rng = g.krng ? g.krng + (int64_t)b * g.nkt : nullptr;
   const int *kdoc = a.k_doc ? a.k_doc + (int64_t)b * a.Lk : nullptr;
+  DocRange ready = TileIter::ahead(rng, 0, g.nkt);
+  Bounds wb, gb;
+  if (rng) wb = wave_bounds(w), gb = group_bounds(wb, sB, wave);
+  else wb = range_bounds(g, qt * ROWS + wave * 32, 32, len, prefix), gb = range_bounds(g, qt * ROWS, ROWS, len, prefix);
+  const int tiles = (gb.hi_max + BK - 1) / BK, per = (tiles + g.nsplit - 1) / g.nsplit;
+  if (split) ready = TileIter::ahead(rng, split * per, g.nkt);
+  TileIter it;
+  it.start(rng, gb.d_min, gb.d_max, split * per, min(tiles, (split + 1) * per), ready);
   Dma<T, D> dk, dv;
   dk.init((const T *)a.k + (int64_t)b * a.k_bs + (int64_t)kh * a.k_hs, a.k_rs, a.Lk, a.dh);
   dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
@@ -374,6 +378,16 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     dv.load(lds + L::BYTES, t * BK);
     if (kdoc) ids = kdoc[min(t * BK + lane, a.Lk - 1)];
   }
+  if (MOD && a.rel_bias) lut.fill(a, head0);
+  FwdState<T, D> st;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) st.acc[d] = f32x16{};
+  st.m = -INFINITY, st.l = 0.f;
+  const ScoreCtx sc = score_ctx(a);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) live_frag(fq[c], c, h, a.dh, w.live);
+  settle(w.slope), settle(w.doc);
+  it.here();
   // (the buffer is a constant of the step: every LDS address of the loop is one register and an immediate)
   auto step = [&](auto buffer) {
     constexpr int buf = decltype(buffer)::value;
@@ -434,25 +448,13 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   bias.bucket = (unsigned char *)(bias.table + (MOD && a.rel_bias ? g.pack * a.n_buckets : 0));
   const int grp = blockIdx.x % g.groups, split = blockIdx.x / g.groups, kh = grp % a.Hk, b = grp / a.Hk, head0 = kh * g.G;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
-  const int len = row_len(a, b);
-  const Row w = make_row(g, b, head0, col, len);
-  const Bounds wb = wave_bounds(w);
-  if (MOD && a.rel_bias) {
-    bias.fill(a, head0, g.pack);
-    __syncthreads();
-  }
-  const float *tab = bias.table + (w.valid ? w.h - head0 : 0) * a.n_buckets;
+  const int len = row_len(a, b), prefix = a.prefix ? scalar_load(a.prefix + b) : 0;
+  Row w = make_row(g, b, head0, col, len, prefix);
   const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)w.h * a.q_hs;
   V8 fq[NC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
-#pragma unroll
-  for (int c = 0; c < NC; ++c) settle(fq[c]);
-  FwdState<T, D> st;
-#pragma unroll
-  for (int d = 0; d < ND; ++d) st.acc[d] = f32x16{};
-  st.m = -INFINITY, st.l = 0.f;
-  const ScoreCtx sc = score_ctx(a);
+  for (int c = 0; c < NC; ++c) fq[c] = mem_frag<T>(qrow, c, h, a.dh);
+  const Bounds wb = a.q_doc ? wave_bounds(w) : range_bounds(g, 0, 32, len, prefix);
   const int tiles = (wb.hi_max + BK - 1) / BK, workers = g.nsplit * WAVES;
   const int *kdoc = a.k_doc ? a.k_doc + (int64_t)b * a.Lk : nullptr;
   Dma<T, D, BK, 64> dk, dv;
@@ -466,6 +468,19 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     dk.load(lds, t * BK);
     dv.load(lds + TILE, t * BK);
   }
+  if (MOD && a.rel_bias) {
+    bias.fill(a, head0, g.pack);
+    __syncthreads();
+  }
+  const float *tab = bias.table + (w.valid ? w.h - head0 : 0) * a.n_buckets;
+  FwdState<T, D> st;
+#pragma unroll
+  for (int d = 0; d < ND; ++d) st.acc[d] = f32x16{};
+  st.m = -INFINITY, st.l = 0.f;
+  const ScoreCtx sc = score_ctx(a);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) live_frag(fq[c], c, h, a.dh, w.live);
+  settle(w.slope), settle(w.doc);
   while (t < tiles) {
     const int k0 = t * BK, tn = t + workers;
     const int doc = kdoc && lane < BK && k0 + lane < a.Lk ? kdoc[k0 + lane] : -1;
@@ -676,11 +691,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   if (a.causal) qt = g.nqt - 1 - qt;
   const int kh = grp % a.Hk, b = grp / a.Hk, head = kh * g.G + gi;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
-  const int len = row_len(a, b);
-  const Row w = make_row(g, b, head, qt * ROWS + wave * 32 + col, len);
-  const Bounds wb = wave_bounds(w);
-  const Bounds gb = group_bounds(wb, sB, wave);
-  if (MOD && a.rel_bias) lut.fill(a, head);
+  const int len = row_len(a, b), prefix = a.prefix ? scalar_load(a.prefix + b) : 0;
+  Row w = make_row(g, b, head, qt * ROWS + wave * 32 + col, len, prefix);
   const int64_t r = ((int64_t)b * a.H + head) * a.Lq + min(w.i, a.Lq - 1);
   const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)head * a.q_hs;
   const T *drow = (const T *)g.dout + (int64_t)b * g.do_bs + (int64_t)min(w.i, a.Lq - 1) * g.do_rs + (int64_t)head * g.do_hs;
@@ -689,21 +701,47 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   float delta = 0.f;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
-    fd[c] = mem_frag<T>(drow, c, h, a.dh, w.live);
-    const V8 o = mem_frag<T>((const T *)g.out + orow, c, h, a.dh, w.live);
-    V8 lo = {};
-    if (g.low) lo = mem_frag<T>((const T *)g.low + orow, c, h, a.dh, w.live);
+    fq[c] = mem_frag<T>(qrow, c, h, a.dh);
+    fd[c] = mem_frag<T>(drow, c, h, a.dh);
+  }
+  float dl = g.dlse ? g.dlse[r] : 0.f, lse = g.lse[r];
+  const DocRange *rng = g.krng ? g.krng + (int64_t)b * g.nkt : nullptr;
+  const int *kdoc = a.k_doc ? a.k_doc + (int64_t)b * a.Lk : nullptr;
+  const DocRange ranges = TileIter::ahead(rng, 0, g.nkt);
+  Bounds wb, gb;
+  if (rng) wb = wave_bounds(w), gb = group_bounds(wb, sB, wave);
+  else wb = range_bounds(g, qt * ROWS + wave * 32, 32, len, prefix), gb = range_bounds(g, qt * ROWS, ROWS, len, prefix);
+  const int tiles = (gb.hi_max + BK - 1) / BK;
+  const unsigned lds = lds_address(smem);
+  Dma<T, D> dk, dv;
+  dk.init((const T *)a.k + (int64_t)b * a.k_bs + (int64_t)kh * a.k_hs, a.k_rs, a.Lk, a.dh);
+  dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
+  TileIter it;
+  int t, ids = 0;                                        // ids: the document of the tile's key `lane`
+  auto first = [&](DocRange ready) {
+    it.start(rng, gb.d_min, gb.d_max, 0, tiles, ready);
+    t = it.next();
+    if (t >= 0) {
+      dk.load(lds, t * BK);
+      dv.load(lds + L::BYTES, t * BK);
+      if (kdoc) ids = kdoc[min(t * BK + lane, a.Lk - 1)];
+    }
+  };
+  first(ranges);
+  if (MOD && a.rel_bias) lut.fill(a, head);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    V8 o = mem_frag<T>((const T *)g.out + orow, c, h, a.dh), lo = {};
+    if (g.low) lo = mem_frag<T>((const T *)g.low + orow, c, h, a.dh);
+    live_frag(fq[c], c, h, a.dh, w.live), live_frag(fd[c], c, h, a.dh, w.live);
 #pragma unroll
     for (int e = 0; e < 8; ++e) delta = fmaf((float)o[e] + (float)lo[e], (float)fd[c][e], delta);
   }
-#pragma unroll
-  for (int c = 0; c < NC; ++c) settle(fq[c]), settle(fd[c]);
-  const float dl = g.dlse && w.live ? g.dlse[r] : 0.f;
-  delta = half_sum(delta) - dl;
-  float lse = w.live ? g.lse[r] : -INFINITY;
-  lse = lse == -INFINITY ? INFINITY : lse * LOG2E;
-  settle(lse);
+  dl = w.live ? dl : 0.f;
+  delta = w.live ? half_sum(delta) - dl : 0.f;
+  lse = !w.live || lse == -INFINITY ? INFINITY : lse * LOG2E;
+  settle(lse), settle(w.slope), settle(w.doc);
+  it.here();
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
@@ -715,22 +753,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   }
   float all_u = 0.f, far_u[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f};
 
-  const int tiles = (gb.hi_max + BK - 1) / BK;
-  const int *kdoc = a.k_doc ? a.k_doc + (int64_t)b * a.Lk : nullptr;
-  Dma<T, D> dk, dv;
-  dk.init((const T *)a.k + (int64_t)b * a.k_bs + (int64_t)kh * a.k_hs, a.k_rs, a.Lk, a.dh);
-  dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
-  const unsigned lds = lds_address(smem);
   for (int pass = sizeof(T) == 2 && a.Lk <= TWICE ? 0 : 1; pass < 2; ++pass) {
-    TileIter it;
-    it.start(g.krng ? g.krng + (int64_t)b * g.nkt : nullptr, gb.d_min, gb.d_max, 0, tiles);
-    int t = it.next();
-    int ids = 0;                                           // the document of the tile's key `lane`
-    if (t >= 0) {
-      dk.load(lds, t * BK);
-      dv.load(lds + L::BYTES, t * BK);
-      if (kdoc) ids = kdoc[min(t * BK + lane, a.Lk - 1)];
-    }
     auto step = [&](auto buffer) {
       constexpr int buf = decltype(buffer)::value;
       const int k0 = t * BK;
@@ -815,6 +838,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
       delta += all_u;
       all_u = 0.f;
       __syncthreads();                                      // (the buffers are filled anew)
+      first(TileIter::ahead(rng, 0, g.nkt));
     }
   }
   if (w.valid && h == 0) g.stat[r] = make_float2(lse, delta + all_u);
@@ -870,42 +894,45 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
   const int kh = grp % a.Hk, b = grp / a.Hk, head0 = kh * g.G;
   const int g_per = (g.G + g.zh - 1) / g.zh, g0 = zh * g_per, g1 = min(g.G, g0 + g_per);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
-  const int len = row_len(a, b), off = len - a.Lq, prefix = a.prefix ? a.prefix[b] : 0;
+  const int len = row_len(a, b), off = len - a.Lq, prefix = a.prefix ? scalar_load(a.prefix + b) : 0;
   const int j = kt * ROWS + wave * 32 + col;
-  const int kdoc = a.k_doc && j < a.Lk ? a.k_doc[(int64_t)b * a.Lk + j] : 0;
-  const bool live = j < len && kdoc >= 0;
-  const int j_lo = kt * ROWS + wave * 32;                 // first key of the wave
-  const int d_min = wave_min(live ? kdoc : 0x7fffffff), d_max = wave_max(live ? kdoc : -1);
-  const bool all_live = __all(live);
-  if (lane == 0) sB[2 * wave] = d_min, sB[2 * wave + 1] = d_max;
-  __syncthreads();
-  int gd_min = 0x7fffffff, gd_max = -1;
-  for (int v = 0; v < WAVES; ++v) gd_min = min(gd_min, sB[2 * v]), gd_max = max(gd_max, sB[2 * v + 1]);
-  gd_min = __builtin_amdgcn_readfirstlane(gd_min), gd_max = __builtin_amdgcn_readfirstlane(gd_max);
-
+  const int kdoc = a.k_doc ? a.k_doc[(int64_t)b * a.Lk + min(j, a.Lk - 1)] : 0;
   const T *krow = (const T *)a.k + (int64_t)b * a.k_bs + (int64_t)min(j, a.Lk - 1) * a.k_rs + (int64_t)kh * a.k_hs;
   const T *vrow = (const T *)a.v + (int64_t)b * a.v_bs + (int64_t)min(j, a.Lk - 1) * a.v_rs + (int64_t)kh * a.v_hs;
   V8 fk[NC], fv[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    fk[c] = mem_frag<T>(krow, c, h, a.dh, live);
-    fv[c] = mem_frag<T>(vrow, c, h, a.dh, live);
+    fk[c] = mem_frag<T>(krow, c, h, a.dh);
+    fv[c] = mem_frag<T>(vrow, c, h, a.dh);
   }
-#pragma unroll
-  for (int c = 0; c < NC; ++c) settle(fk[c]), settle(fv[c]);
+  // queries that may see a key of this workgroup: position >= its first key, unless the prefix reaches into it
+  const int i_first = a.causal && prefix <= kt * ROWS ? max(0, kt * ROWS - off) : 0;
+  const int all0 = min(i_first, a.Lq) / BQ, all1 = kt * ROWS < len ? (a.Lq + BQ - 1) / BQ : 0;
+  const int t_per = (max(0, all1 - all0) + g.zq - 1) / g.zq, t0 = all0 + zq * t_per, t1 = min(all1, t0 + t_per);
+  const int n_qt = (a.Lq + BQ - 1) / BQ;
+  const DocRange *rng = g.qrng ? g.qrng + (int64_t)b * n_qt : nullptr;
+  const DocRange ranges = TileIter::ahead(rng, t0, n_qt);
+  const bool live = j < len && kdoc >= 0;
+  const int j_lo = kt * ROWS + wave * 32;                 // first key of the wave
+  const bool all_live = __all(live);
+  int gd_min = 0, gd_max = 0;
+  if (rng) {
+    const int d_min = wave_min(live ? kdoc : 0x7fffffff), d_max = wave_max(live ? kdoc : -1);
+    if (lane == 0) sB[2 * wave] = d_min, sB[2 * wave + 1] = d_max;
+    __syncthreads();
+    gd_min = 0x7fffffff, gd_max = -1;
+    for (int v = 0; v < WAVES; ++v) gd_min = min(gd_min, sB[2 * v]), gd_max = max(gd_max, sB[2 * v + 1]);
+    gd_min = __builtin_amdgcn_readfirstlane(gd_min), gd_max = __builtin_amdgcn_readfirstlane(gd_max);
+  }
+
   f32x16 acck[ND], accv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acck[d] = f32x16{}, accv[d] = f32x16{};
   const ScoreCtx sc = score_ctx(a);
   // fp16: P is rounded times 2^PSHIFT; the surplus is taken out of dS again together with its own scaling
-  const float dscale = Elem<T>::PSHIFT != 0.f ? *g.dscale : 1.f;
+  const float dscale = Elem<T>::PSHIFT != 0.f ? scalar_load(g.dscale) : 1.f;
   const float ds_mul = dscale * ex2(-Elem<T>::PSHIFT);
 
-  // queries that may see a key of this workgroup: position >= its first key, unless the prefix reaches into it
-  const int i_first = a.causal && prefix <= kt * ROWS ? max(0, kt * ROWS - off) : 0;
-  const int all0 = min(i_first, a.Lq) / BQ, all1 = kt * ROWS < len ? (a.Lq + BQ - 1) / BQ : 0;
-  const int t_per = (max(0, all1 - all0) + g.zq - 1) / g.zq, t0 = all0 + zq * t_per, t1 = min(all1, t0 + t_per);
-  const DocRange *rng = g.qrng ? g.qrng + (int64_t)b * ((a.Lq + BQ - 1) / BQ) : nullptr;
   const int *qdoc = a.q_doc ? a.q_doc + (int64_t)b * a.Lq : nullptr;
   const unsigned lds = lds_address(smem);
   Dma<T, D> dmq, dmo;
@@ -920,17 +947,14 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
   float2 st_next = make_float2(INFINITY, 0.f);
   float slope_next = 0.f;
   int doc_next = -1;
-  auto advance = [&]() {                                  // next tile, over head ends; -1 at the end
+  auto advance = [&](auto at_start) {                                  // next tile, over head ends; -1 at the end
     int n = gi < g0 ? -1 : it.next();
     while (n < 0 && ++gi < g1) {
       stat = g.stat + ((int64_t)b * a.H + head0 + gi) * a.Lq;
       dmq.base = qbase + (int64_t)gi * a.q_hs * (int64_t)sizeof(T);
       dmo.base = obase + (int64_t)gi * g.do_hs * (int64_t)sizeof(T);
-      if (MOD && a.slopes) {
-        slope_next = a.slopes[head0 + gi] * LOG2E;
-        settle(slope_next);
-      }
-      it.start(rng, gd_min, gd_max, t0, t1);
+      if (MOD && a.slopes) slope_next = scalar_load(a.slopes + head0 + gi) * LOG2E;
+      it.start(rng, gd_min, gd_max, t0, t1, decltype(at_start)::value && gi == g0 ? ranges : TileIter::ahead(rng, t0, n_qt));
       n = it.next();
     }
     return n;
@@ -945,8 +969,11 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
       st_next = stat[i];
     }
   };
-  t = advance();
+  t = advance(Const<1>());
   if (t >= 0) fetch(t, 0);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) live_frag(fk[c], c, h, a.dh, live), live_frag(fv[c], c, h, a.dh, live);
+  it.here();
   auto step = [&](auto buffer) {
     constexpr int buf = decltype(buffer)::value;
     const int q0 = t * BQ, head = head0 + gi;
@@ -973,7 +1000,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
       zero_rows<T, D>(sO, a.Lq - q0, sDoc);
       __syncthreads();
     }
-    const int tn = advance();
+    const int tn = advance(Const<0>());
     if (tn >= 0) fetch(tn, buf ^ 1);
     const int p0 = off + q0;
     // the last row of the tile sees the most
@@ -1090,29 +1117,36 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
   const int kh = grp % a.Hk, b = grp / a.Hk, head0 = kh * g.G;
   const int g_per = (g.G + g.zh - 1) / g.zh, g0 = zh * g_per, g1 = min(g.G, g0 + g_per);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
-  const int len = row_len(a, b), off = len - a.Lq, prefix = a.prefix ? a.prefix[b] : 0;
+  const int len = row_len(a, b), off = len - a.Lq, prefix = a.prefix ? scalar_load(a.prefix + b) : 0;
   const int qh = wave & 1, kb = wave >> 1;                // first step: half of the queries, block of 32 keys
   const int j_lo = kt * ROWS + kb * 32, j = j_lo + col;
-  const int kdoc = a.k_doc && j < a.Lk ? a.k_doc[(int64_t)b * a.Lk + j] : 0;
-  const bool live = j < len && kdoc >= 0;
-  const int d_min = wave_min(live ? kdoc : 0x7fffffff), d_max = wave_max(live ? kdoc : -1);
-  const bool all_live = __all(live);
-  if (lane == 0) sB[2 * wave] = d_min, sB[2 * wave + 1] = d_max;
-  __syncthreads();
-  int gd_min = 0x7fffffff, gd_max = -1;
-  for (int v = 0; v < 8; ++v) gd_min = min(gd_min, sB[2 * v]), gd_max = max(gd_max, sB[2 * v + 1]);
-  gd_min = __builtin_amdgcn_readfirstlane(gd_min), gd_max = __builtin_amdgcn_readfirstlane(gd_max);
-
+  const int kdoc = a.k_doc ? a.k_doc[(int64_t)b * a.Lk + min(j, a.Lk - 1)] : 0;
   const T *krow = (const T *)a.k + (int64_t)b * a.k_bs + (int64_t)min(j, a.Lk - 1) * a.k_rs + (int64_t)kh * a.k_hs;
   const T *vrow = (const T *)a.v + (int64_t)b * a.v_bs + (int64_t)min(j, a.Lk - 1) * a.v_rs + (int64_t)kh * a.v_hs;
   V8 fk[NC], fv[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    fk[c] = mem_frag<T>(krow, c, h, a.dh, live);
-    fv[c] = mem_frag<T>(vrow, c, h, a.dh, live);
+    fk[c] = mem_frag<T>(krow, c, h, a.dh);
+    fv[c] = mem_frag<T>(vrow, c, h, a.dh);
   }
-#pragma unroll
-  for (int c = 0; c < NC; ++c) settle(fk[c]), settle(fv[c]);
+  const int i_first = a.causal && prefix <= kt * ROWS ? max(0, kt * ROWS - off) : 0;
+  const int all0 = min(i_first, a.Lq) / BQ, all1 = kt * ROWS < len ? (a.Lq + BQ - 1) / BQ : 0;
+  const int t_per = (max(0, all1 - all0) + g.zq - 1) / g.zq, t0 = all0 + zq * t_per, t1 = min(all1, t0 + t_per);
+  const int n_qt = (a.Lq + BQ - 1) / BQ;
+  const DocRange *rng = g.qrng ? g.qrng + (int64_t)b * n_qt : nullptr;
+  const DocRange ranges = TileIter::ahead(rng, t0, n_qt);
+  const bool live = j < len && kdoc >= 0;
+  const bool all_live = __all(live);
+  int gd_min = 0, gd_max = 0;
+  if (rng) {
+    const int d_min = wave_min(live ? kdoc : 0x7fffffff), d_max = wave_max(live ? kdoc : -1);
+    if (lane == 0) sB[2 * wave] = d_min, sB[2 * wave + 1] = d_max;
+    __syncthreads();
+    gd_min = 0x7fffffff, gd_max = -1;
+    for (int v = 0; v < 8; ++v) gd_min = min(gd_min, sB[2 * v]), gd_max = max(gd_max, sB[2 * v + 1]);
+    gd_min = __builtin_amdgcn_readfirstlane(gd_min), gd_max = __builtin_amdgcn_readfirstlane(gd_max);
+  }
+
   // second step: which output, which keys (blocks kb2, kb2 + 1, ..), which dimension tiles (dt2, ..)
   const bool to_k = wave & 1;
   const int part = wave >> 1, kb2 = KB == 2 ? 2 * (part & 1) : part, dt2 = KB == 2 ? NT * (part >> 1) : 0;
@@ -1122,13 +1156,9 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
 #pragma unroll
     for (int d = 0; d < NT; ++d) acc[k][d] = f32x16{};
   const ScoreCtx sc = score_ctx(a);
-  const float dscale = Elem<T>::PSHIFT != 0.f ? *g.dscale : 1.f;
+  const float dscale = Elem<T>::PSHIFT != 0.f ? scalar_load(g.dscale) : 1.f;
   const float ds_mul = dscale * ex2(-Elem<T>::PSHIFT);
 
-  const int i_first = a.causal && prefix <= kt * ROWS ? max(0, kt * ROWS - off) : 0;
-  const int all0 = min(i_first, a.Lq) / BQ, all1 = kt * ROWS < len ? (a.Lq + BQ - 1) / BQ : 0;
-  const int t_per = (max(0, all1 - all0) + g.zq - 1) / g.zq, t0 = all0 + zq * t_per, t1 = min(all1, t0 + t_per);
-  const DocRange *rng = g.qrng ? g.qrng + (int64_t)b * ((a.Lq + BQ - 1) / BQ) : nullptr;
   const int *qdoc = a.q_doc ? a.q_doc + (int64_t)b * a.Lq : nullptr;
   const unsigned lds = lds_address(smem);
   Dma<T, D, BQ, 512> dmq, dmo;
@@ -1143,17 +1173,14 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
   float2 st_next = make_float2(INFINITY, 0.f);
   float slope_next = 0.f;
   int doc_next = -1;
-  auto advance = [&]() {
+  auto advance = [&](auto at_start) {
     int n = gi < g0 ? -1 : it.next();
     while (n < 0 && ++gi < g1) {
       stat = g.stat + ((int64_t)b * a.H + head0 + gi) * a.Lq;
       dmq.base = qbase + (int64_t)gi * a.q_hs * (int64_t)sizeof(T);
       dmo.base = obase + (int64_t)gi * g.do_hs * (int64_t)sizeof(T);
-      if (MOD && a.slopes) {
-        slope_next = a.slopes[head0 + gi] * LOG2E;
-        settle(slope_next);
-      }
-      it.start(rng, gd_min, gd_max, t0, t1);
+      if (MOD && a.slopes) slope_next = scalar_load(a.slopes + head0 + gi) * LOG2E;
+      it.start(rng, gd_min, gd_max, t0, t1, decltype(at_start)::value && gi == g0 ? ranges : TileIter::ahead(rng, t0, n_qt));
       n = it.next();
     }
     return n;
@@ -1168,8 +1195,11 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
       st_next = stat[i];
     }
   };
-  t = advance();
+  t = advance(Const<1>());
   if (t >= 0) fetch(t, 0);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) live_frag(fk[c], c, h, a.dh, live), live_frag(fv[c], c, h, a.dh, live);
+  it.here();
   while (t >= 0) {
     const int q0 = t * BQ, head = head0 + gi, cur_gi = gi;
     char *sQ = smem + buf * 2 * L::BYTES, *sO = sQ + L::BYTES;
@@ -1194,7 +1224,7 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
       zero_rows<T, D, BQ, 512>(sO, a.Lq - q0, sDoc);
       __syncthreads();
     }
-    const int tn = advance();
+    const int tn = advance(Const<0>());
     if (tn >= 0) fetch(tn, buf ^ 1);
     {
       const int p0 = off + q0 + 32 * qh;                  // position of the first of this wave's queries
@@ -1324,26 +1354,21 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   const int grp = blockIdx.x % g.groups, n = blockIdx.x / g.groups, gi = n % g.G, qt = n / g.G;
   const int kh = grp % a.Hk, b = grp / a.Hk, head = kh * g.G + gi;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
-  const int len = row_len(a, b);
-  const Row w = make_row(g, b, head, qt * ROWS + wave * 32 + col, len);
-  const Bounds wb = wave_bounds(w);
-  const Bounds gb = group_bounds(wb, sB, wave);
-  lut.fill(a, head, bucket);
-  float *mine = hist + (int64_t)wave * a.n_buckets * 64 + lane;
-  for (int k = 0; k < a.n_buckets; ++k) mine[k * 64] = 0.f;
+  const int len = row_len(a, b), prefix = a.prefix ? scalar_load(a.prefix + b) : 0;
+  Row w = make_row(g, b, head, qt * ROWS + wave * 32 + col, len, prefix);
   const int64_t r = ((int64_t)b * a.H + head) * a.Lq + min(w.i, a.Lq - 1);
-  const float2 rs = w.live ? g.stat[r] : make_float2(INFINITY, 0.f);
-  const float lse2 = rs.x, delta = rs.y;
+  float2 rs = g.stat[r];
   const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)head * a.q_hs;
   const T *drow = (const T *)g.dout + (int64_t)b * g.do_bs + (int64_t)min(w.i, a.Lq - 1) * g.do_rs + (int64_t)head * g.do_hs;
   V8 fq[NC], fd[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    fq[c] = mem_frag<T>(qrow, c, h, a.dh, w.live);
-    fd[c] = mem_frag<T>(drow, c, h, a.dh, w.live);
+    fq[c] = mem_frag<T>(qrow, c, h, a.dh);
+    fd[c] = mem_frag<T>(drow, c, h, a.dh);
   }
-#pragma unroll
-  for (int c = 0; c < NC; ++c) settle(fq[c]), settle(fd[c]);
+  Bounds wb, gb;
+  if (g.krng) wb = wave_bounds(w), gb = group_bounds(wb, sB, wave);
+  else wb = range_bounds(g, qt * ROWS + wave * 32, 32, len, prefix), gb = range_bounds(g, qt * ROWS, ROWS, len, prefix);
   const ScoreCtx sc = score_ctx(a);
   const int tiles = (gb.hi_max + BK - 1) / BK;
   const DocRange *rng = g.krng ? g.krng + (int64_t)b * g.nkt : nullptr;
@@ -1371,8 +1396,14 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   };
   int t = next(t0);
   int *ids = sDoc, *ids_next = sDoc + BK;
-  __syncthreads();                                        // (the tables are filled)
   if (t < t1) request(t, ids);
+  lut.fill(a, head, bucket);
+  float *mine = hist + (int64_t)wave * a.n_buckets * 64 + lane;
+  for (int k = 0; k < a.n_buckets; ++k) mine[k * 64] = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) live_frag(fq[c], c, h, a.dh, w.live), live_frag(fd[c], c, h, a.dh, w.live);
+  const float lse2 = w.live ? rs.x : INFINITY, delta = w.live ? rs.y : 0.f;
+  settle(w.slope), settle(w.doc);
   while (t < t1) {
     const int k0 = t * BK;
     dma_wait<0>();
@@ -1510,7 +1541,7 @@ template <typename T> static void docs(const Args &g, DocRange *out, bool querie
 
 template <typename T> void forward(Args &g, DocRange *ranges, hipStream_t st) {
   const mmt_long_attention &a = g.a;
-  if (ranges) docs<T>(g, ranges, false, st), g.krng = ranges;
+  if (ranges && !g.few) docs<T>(g, ranges, false, st), g.krng = ranges;
   if (a.dh <= 32) fwd_size<T, 32>(g, st);
   else if (a.dh <= 64) fwd_size<T, 64>(g, st);
   else if (a.dh <= 96) fwd_size<T, 96>(g, st);
