@@ -366,4 +366,24 @@ struct TileIter {
   __device__ __forceinline__ bool mixed() const { return rng && !(cur_dead == 0 && cur_lo == cur_hi && lo == hi && lo == cur_lo); }
 };
 
+// The tiles of an iterator dealt to the teams of a workgroup, one each at a time.  All of it is the same in all waves but for what is
+// this team's: its tile (-1: none this time), whether that needs document masks, whether it holds rows that have to be zeroed.
+template <int TEAMS> struct Deal {
+  TileIter it;
+  int lead, t;                       // the first team's tile: -1 ends the loop for all
+  bool mixed, zero, any_zero;        // any_zero: some team zeroes rows, all meet once more
+  __device__ __forceinline__ bool zeroes(int tile, int bk, int len) const { return tile * bk + bk > len || (it.mixed() && it.cur_dead != 0); }
+  __device__ __forceinline__ void next(int team, int bk, int len) {
+    lead = t = it.next();
+    mixed = it.mixed(), any_zero = zero = zeroes(t, bk, len);
+    if constexpr (TEAMS == 2) {
+      if (lead < 0) return;
+      const int other = it.next();
+      const bool z = other >= 0 && zeroes(other, bk, len);
+      any_zero = zero || z;
+      if (team) t = other, mixed = it.mixed(), zero = z;
+    }
+  }
+};
+
 }  // namespace la

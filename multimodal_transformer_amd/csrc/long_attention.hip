@@ -45,6 +45,12 @@ static int check(const mmt_long_attention *a, const char *who) {
   return MMT_OK;
 }
 
+// One workgroup of 128 rows per CU leaves each SIMD one wave, which waits for most of its time: two teams then share its keys.  Where
+// that many rows are causal, the workgroups that remain for a second turn are the shortest.
+static int teams(const mmt_long_attention &a, int64_t items) {
+  return a.dtype != MMT_F32 && items < (a.causal ? 512 : 257) && a.Lk > 192 ? 2 : 1;
+}
+
 // Forward: splits of the keys where there are fewer workgroups than CUs, enough for two on each of the 256, at least four tiles each.
 // Backward: parts of dK / dV over the query heads, then over the queries; causal rows are uneven, so twice as many.
 static void plan(Args &g, bool backward) {
@@ -63,11 +69,14 @@ static void plan(Args &g, bool backward) {
   if (!backward) {
     const int64_t base = (int64_t)g.groups * (g.G / g.pack) * g.nqt;
     const int64_t tiles = g.few ? (a.Lk + 127) / 128 : g.nkt;               // a step of all waves
-    if (base < 256) g.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>((512 + base - 1) / base, tiles / 4));
+    g.teams = g.few ? 1 : teams(a, base);
+    const int64_t want = 512 / g.teams;
+    if (base < want / 2) g.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>((want + base - 1) / base, tiles / (4 * g.teams)));
     g.items = (int)(base * g.nsplit);
   } else {
     const int64_t base = (int64_t)g.groups * ((a.Lk + ROWS - 1) / ROWS), want = ((a.causal ? 1024 : 512) + base - 1) / base;
     g.zh = (int)std::min<int64_t>(g.G, want);
+    g.teams = teams(a, (int64_t)a.B * a.H * g.nqt);
     g.zq = (int)std::max<int64_t>(1, std::min<int64_t>(want / g.zh, (a.Lq + bk - 1) / bk / 8));
   }
 }

@@ -23,6 +23,7 @@ struct Args {                      // mmt_long_attention plus what the launcher 
   int G, pack;                     // query heads per key head; heads whose rows share a tile (1 or G)
   int few;                         // all rows of a key head fit into 32: the waves split the keys instead
   int nqt, nkt, nsplit, items;     // row tiles, key tiles, splits of the keys, workgroups
+  int teams;                       // forward, dQ: 1, or 2 teams of four waves that deal the key tiles among themselves
   int groups;                      // workgroups n, n + groups, .. share keys and values
   int zh, zq;                      // dK / dV: parts over the query heads of a key head, over the queries
   float *part_dk, *part_dv;        // (zh * zq, B, Lk, Hk, dh) when there are several parts

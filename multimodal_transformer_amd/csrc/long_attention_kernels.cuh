@@ -331,14 +331,14 @@ __device__ __forceinline__ void fwd_store(const Args &g, const FwdState<T, D> &s
 // share a key head - against a range of key tiles.  K and V tiles go straight from memory to LDS, one
 // tile ahead of the products (two buffers, one barrier per tile).  MOD: the scores are capped or biased; without it they go from the
 // product into the exponential as they are.
-template <typename T, int D, bool MOD>
-__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_fwd_kernel(const Args g) {
+template <typename T, int D, bool MOD, int TEAMS>
+__global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_fwd_kernel(const Args g) {
   typedef Tile<T, D> L;
   typedef typename Elem<T>::V8 V8;
   constexpr int BK = L::BK, NC = D / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
-  int *sDoc2 = (int *)(smem + 4 * L::BYTES), *sB = sDoc2 + 2 * BK;
+  int *sDoc2 = (int *)(smem + TEAMS * 4 * L::BYTES), *sB = sDoc2 + TEAMS * 2 * BK;
   const Lut lut = {(float *)(sB + 6 * WAVES) + a.reach + PAD};
   const int grp = blockIdx.x % g.groups;
   int n = blockIdx.x / g.groups;
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   if (a.causal) qt = g.nqt - 1 - qt;                     // the tiles with the most keys first
   const int kh = grp % a.Hk, b = grp / a.Hk;
   const int head0 = kh * g.G + gi;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+  const int lane = threadIdx.x & 63, w_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = w_all % WAVES, team = w_all / WAVES, h = lane >> 5, col = lane & 31;
   const int len = row_len(a, b), prefix = a.prefix ? scalar_load(a.prefix + b) : 0;
   // what does not depend on one another is requested before any of it is waited for: the time of a short row is these waits
   Row w = make_row(g, b, head0, qt * ROWS + wave * 32 + col, len, prefix);
@@ -365,20 +365,21 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   else wb = range_bounds(g, qt * ROWS + wave * 32, 32, len, prefix), gb = range_bounds(g, qt * ROWS, ROWS, len, prefix);
   const int tiles = (gb.hi_max + BK - 1) / BK, per = (tiles + g.nsplit - 1) / g.nsplit;
   if (split) ready = TileIter::ahead(rng, split * per, g.nkt);
-  TileIter it;
-  it.start(rng, gb.d_min, gb.d_max, split * per, min(tiles, (split + 1) * per), ready);
+  Deal<TEAMS> deal;
+  deal.it.start(rng, gb.d_min, gb.d_max, split * per, min(tiles, (split + 1) * per), ready);
   Dma<T, D> dk, dv;
   dk.init((const T *)a.k + (int64_t)b * a.k_bs + (int64_t)kh * a.k_hs, a.k_rs, a.Lk, a.dh);
   dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
-  const unsigned lds = lds_address(smem);
-  int t = it.next();
+  char *const tiles_at = smem + team * 4 * L::BYTES;
+  const unsigned lds = lds_address(tiles_at);
+  deal.next(team, BK, len);
   int ids = 0;                                           // the document of the tile's key `lane`
-  if (t >= 0) {
-    dk.load(lds, t * BK);
-    dv.load(lds + L::BYTES, t * BK);
-    if (kdoc) ids = kdoc[min(t * BK + lane, a.Lk - 1)];
+  if (deal.t >= 0) {
+    dk.load(lds, deal.t * BK);
+    dv.load(lds + L::BYTES, deal.t * BK);
+    if (kdoc) ids = kdoc[min(deal.t * BK + lane, a.Lk - 1)];
   }
-  if (MOD && a.rel_bias) lut.fill(a, head0);
+  if (MOD && a.rel_bias) lut.fill<TEAMS * THREADS>(a, head0);
   FwdState<T, D> st;
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) st.acc[d] = f32x16{};
@@ -387,28 +388,28 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
 #pragma unroll
   for (int c = 0; c < NC; ++c) live_frag(fq[c], c, h, a.dh, w.live);
   settle(w.slope), settle(w.doc);
-  it.here();
+  deal.it.here();
   // (the buffer is a constant of the step: every LDS address of the loop is one register and an immediate)
   auto step = [&](auto buffer) {
     constexpr int buf = decltype(buffer)::value;
-    const int k0 = t * BK;
-    const bool mixed = it.mixed(), dead = it.cur_dead != 0;
-    char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
-    int *sDoc = sDoc2 + buf * BK;
+    const int k0 = deal.t * BK;
+    const bool mine = TEAMS == 1 || deal.t >= 0, mixed = deal.mixed, zero = deal.zero, any_zero = deal.any_zero;
+    char *sK = tiles_at + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
+    int *sDoc = sDoc2 + (TEAMS == 1 ? buf : team * 2 + buf) * BK;
     if (kdoc && wave == 0 && lane < BK) sDoc[lane] = ids;
     dma_wait<0>();
     __syncthreads();                                     // the tile is here, and nobody reads the other buffer any more
-    if (k0 + BK > len || (mixed && dead)) {              // (a key row only reaches scores that are masked: V alone)
-      zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
+    if (any_zero) {                                      // (a key row only reaches scores that are masked: V alone)
+      if (zero) zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
       __syncthreads();
     }
-    const int tn = it.next();
-    if (tn >= 0) {
-      dk.load(lds + (buf ^ 1) * 2 * L::BYTES, tn * BK);
-      dv.load(lds + (buf ^ 1) * 2 * L::BYTES + L::BYTES, tn * BK);
-      if (kdoc) ids = kdoc[min(tn * BK + lane, a.Lk - 1)];
+    deal.next(team, BK, len);
+    if (deal.t >= 0) {
+      dk.load(lds + (buf ^ 1) * 2 * L::BYTES, deal.t * BK);
+      dv.load(lds + (buf ^ 1) * 2 * L::BYTES + L::BYTES, deal.t * BK);
+      if (kdoc) ids = kdoc[min(deal.t * BK + lane, a.Lk - 1)];
     }
-    if (k0 < wb.hi_max) {
+    if (mine && k0 < wb.hi_max) {
       const bool need_mask = k0 + BK > wb.hi_min || mixed;
       const Place at = place(a, k0 - wb.p_max, k0 + BK - 1 - wb.p_min);
       // modified scores: 32 keys at a time (the modification needs the registers); else all of the tile
@@ -421,12 +422,30 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
         fwd_values<T, D, NK>(st, x, sV + kt * 32 * L::NS * 16, lane);
       }
     }
-    t = tn;
-  };
-  while (t >= 0) {
+    };
+  while (deal.lead >= 0) {
     step(Const<0>());
-    if (t < 0) break;
+    if (deal.lead < 0) break;
     step(Const<1>());
+  }
+  if constexpr (TEAMS == 2) {                             // the second team's part of every row, through LDS (the tiles are done with)
+    float *s = (float *)smem + threadIdx.x % THREADS;
+    __syncthreads();
+    if (team) {
+      s[0] = st.m, s[THREADS] = st.l;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[(2 + 16 * d + i) * THREADS] = st.acc[d][i];
+    }
+    __syncthreads();
+    if (team) return;
+    const float m = fmaxf(st.m, s[0]), ms = m == -INFINITY ? 0.f : m, f0 = ex2(st.m - ms), f1 = ex2(s[0] - ms);
+    st.m = m, st.l = fmaf(st.l, f0, s[THREADS] * f1);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.acc[d][i] = fmaf(st.acc[d][i], f0, s[(2 + 16 * d + i) * THREADS] * f1);
   }
   fwd_store(g, st, w, b, split, h);
 }
@@ -677,20 +696,20 @@ __device__ __forceinline__ float score_grad_scale(const f32x4 *maxima, int parts
 // probability's rounding does not average out, and such calls are short (8 us for 128 rows of 21 keys and 8 heads, with one pass 7).
 // With a learned bias the kernel also sums dU over the tiles that lie wholly beyond the reach on either side.
 constexpr int TWICE = 512;
-template <typename T, int D, bool MOD>
-__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_dq_kernel(const Args g) {
+template <typename T, int D, bool MOD, int TEAMS>
+__global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_dq_kernel(const Args g) {
   typedef Tile<T, D> L;
   typedef typename Elem<T>::V8 V8;
   constexpr int BK = L::BK, NK = BK / 32, NC = D / 16, ND = D / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
-  int *sDoc2 = (int *)(smem + 4 * L::BYTES), *sB = sDoc2 + 2 * BK;
+  int *sDoc2 = (int *)(smem + TEAMS * 4 * L::BYTES), *sB = sDoc2 + TEAMS * 2 * BK;
   const Lut lut = {(float *)(sB + 6 * WAVES) + a.reach + PAD};
   const int grp = blockIdx.x % g.groups, n = blockIdx.x / g.groups, gi = n % g.G;
   int qt = n / g.G;
   if (a.causal) qt = g.nqt - 1 - qt;
   const int kh = grp % a.Hk, b = grp / a.Hk, head = kh * g.G + gi;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+  const int lane = threadIdx.x & 63, w_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = w_all % WAVES, team = w_all / WAVES, h = lane >> 5, col = lane & 31;
   const int len = row_len(a, b), prefix = a.prefix ? scalar_load(a.prefix + b) : 0;
   Row w = make_row(g, b, head, qt * ROWS + wave * 32 + col, len, prefix);
   const int64_t r = ((int64_t)b * a.H + head) * a.Lq + min(w.i, a.Lq - 1);
@@ -712,23 +731,24 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   if (rng) wb = wave_bounds(w), gb = group_bounds(wb, sB, wave);
   else wb = range_bounds(g, qt * ROWS + wave * 32, 32, len, prefix), gb = range_bounds(g, qt * ROWS, ROWS, len, prefix);
   const int tiles = (gb.hi_max + BK - 1) / BK;
-  const unsigned lds = lds_address(smem);
+  char *const tiles_at = smem + team * 4 * L::BYTES;
+  const unsigned lds = lds_address(tiles_at);
   Dma<T, D> dk, dv;
   dk.init((const T *)a.k + (int64_t)b * a.k_bs + (int64_t)kh * a.k_hs, a.k_rs, a.Lk, a.dh);
   dv.init((const T *)a.v + (int64_t)b * a.v_bs + (int64_t)kh * a.v_hs, a.v_rs, a.Lk, a.dh);
-  TileIter it;
-  int t, ids = 0;                                        // ids: the document of the tile's key `lane`
+  Deal<TEAMS> deal;
+  int ids = 0;                                           // ids: the document of the tile's key `lane`
   auto first = [&](DocRange ready) {
-    it.start(rng, gb.d_min, gb.d_max, 0, tiles, ready);
-    t = it.next();
-    if (t >= 0) {
-      dk.load(lds, t * BK);
-      dv.load(lds + L::BYTES, t * BK);
-      if (kdoc) ids = kdoc[min(t * BK + lane, a.Lk - 1)];
+    deal.it.start(rng, gb.d_min, gb.d_max, 0, tiles, ready);
+    deal.next(team, BK, len);
+    if (deal.t >= 0) {
+      dk.load(lds, deal.t * BK);
+      dv.load(lds + L::BYTES, deal.t * BK);
+      if (kdoc) ids = kdoc[min(deal.t * BK + lane, a.Lk - 1)];
     }
   };
   first(ranges);
-  if (MOD && a.rel_bias) lut.fill(a, head);
+  if (MOD && a.rel_bias) lut.fill<TEAMS * THREADS>(a, head);
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     V8 o = mem_frag<T>((const T *)g.out + orow, c, h, a.dh), lo = {};
@@ -741,7 +761,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   delta = w.live ? half_sum(delta) - dl : 0.f;
   lse = !w.live || lse == -INFINITY ? INFINITY : lse * LOG2E;
   settle(lse), settle(w.slope), settle(w.doc);
-  it.here();
+  deal.it.here();
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
@@ -756,25 +776,27 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   for (int pass = sizeof(T) == 2 && a.Lk <= TWICE ? 0 : 1; pass < 2; ++pass) {
     auto step = [&](auto buffer) {
       constexpr int buf = decltype(buffer)::value;
-      const int k0 = t * BK;
-      const bool mixed = it.mixed(), dead = it.cur_dead != 0;
-      char *sK = smem + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
-      int *sDoc = sDoc2 + buf * BK;
+      const int k0 = deal.t * BK;
+      const bool mine = TEAMS == 1 || deal.t >= 0, mixed = deal.mixed, zero = deal.zero, any_zero = deal.any_zero;
+      char *sK = tiles_at + buf * 2 * L::BYTES, *sV = sK + L::BYTES;
+      int *sDoc = sDoc2 + (TEAMS == 1 ? buf : team * 2 + buf) * BK;
       if (kdoc && wave == 0 && lane < BK) sDoc[lane] = ids;
       dma_wait<0>();
       __syncthreads();
-      if (k0 + BK > len || (mixed && dead)) {
-        zero_rows<T, D>(sK, len - k0, mixed ? sDoc : nullptr);
-        zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
+      if (any_zero) {
+        if (zero) {
+          zero_rows<T, D>(sK, len - k0, mixed ? sDoc : nullptr);
+          zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
+        }
         __syncthreads();
       }
-      const int tn = it.next();
-      if (tn >= 0) {
-        dk.load(lds + (buf ^ 1) * 2 * L::BYTES, tn * BK);
-        dv.load(lds + (buf ^ 1) * 2 * L::BYTES + L::BYTES, tn * BK);
-        if (kdoc) ids = kdoc[min(tn * BK + lane, a.Lk - 1)];
+      deal.next(team, BK, len);
+      if (deal.t >= 0) {
+        dk.load(lds + (buf ^ 1) * 2 * L::BYTES, deal.t * BK);
+        dv.load(lds + (buf ^ 1) * 2 * L::BYTES + L::BYTES, deal.t * BK);
+        if (kdoc) ids = kdoc[min(deal.t * BK + lane, a.Lk - 1)];
       }
-      if (k0 < wb.hi_max) {
+      if (mine && k0 < wb.hi_max) {
         const bool need_mask = k0 + BK > wb.hi_min || mixed;
         // by the whole workgroup's rows: the table kernel takes the tiles that are left with the same rule
         const Place at = place(a, k0 - gb.p_max, k0 + BK - 1 - gb.p_min);
@@ -825,15 +847,22 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
           }
         }
       }
-      t = tn;
-    };
-    while (t >= 0) {
+        };
+    while (deal.lead >= 0) {
       step(Const<0>());
-      if (t < 0) break;
+      if (deal.lead < 0) break;
       step(Const<1>());
     }
     // the sum of dU over a row is dlse (0 without it) by definition: what it is instead is the error of delta
-    all_u = lse == INFINITY ? 0.f : half_sum(all_u) - dl;
+    all_u = half_sum(all_u);
+    if constexpr (TEAMS == 2) {
+      float *s = (float *)smem;
+      __syncthreads();                                      // (the tiles are done with)
+      s[threadIdx.x] = all_u;
+      __syncthreads();
+      all_u = s[threadIdx.x % THREADS] + s[THREADS + threadIdx.x % THREADS];
+    }
+    all_u = lse == INFINITY ? 0.f : all_u - dl;
     if (pass == 0) {
       delta += all_u;
       all_u = 0.f;
@@ -841,20 +870,36 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
       first(TileIter::ahead(rng, 0, g.nkt));
     }
   }
-  if (w.valid && h == 0) g.stat[r] = make_float2(lse, delta + all_u);
+  if (w.valid && h == 0 && team == 0) g.stat[r] = make_float2(lse, delta + all_u);
   if (MOD && a.rel_bias) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) far_u[s] = wave_sum(w.live ? far_u[s] - all_u * far_p[s] : 0.f);
     __syncthreads();
     float *sF = (float *)sB;
-    if (lane == 0) sF[2 * wave] = far_u[0], sF[2 * wave + 1] = far_u[1];
+    if (lane == 0) sF[2 * w_all] = far_u[0], sF[2 * w_all + 1] = far_u[1];
     __syncthreads();
     if (threadIdx.x < 2) {
       float v = 0.f;
-      for (int u = 0; u < WAVES; ++u) v += sF[2 * u + threadIdx.x];
+      for (int u = 0; u < TEAMS * WAVES; ++u) v += sF[2 * u + threadIdx.x];
       // item order (b, qt, head) for the reduction, whatever order the workgroups ran in
       g.far_part[(((int64_t)b * g.nqt + qt) * a.H + head) * 2 + threadIdx.x] = v;
     }
+  }
+  if constexpr (TEAMS == 2) {
+    float *s = (float *)smem + threadIdx.x % THREADS;
+    __syncthreads();
+    if (team) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[(16 * d + i) * THREADS] = acc[d][i];
+    }
+    __syncthreads();
+    if (team) return;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] += s[(16 * d + i) * THREADS];
   }
   if (!w.valid) return;
   T *o = (T *)g.dq + (((int64_t)b * a.Lq + w.i) * a.H + head) * a.dh;
@@ -1501,9 +1546,22 @@ template <typename T, int D> static void fwd_size(const Args &g, hipStream_t st)
     else launch(mmt_long_attn_few_kernel<T, D, false>, g.items, lds, st, g);
     return;
   }
-  const size_t lds = 4 * Tile<T, D>::BYTES + 8 * Tile<T, D>::BK + 24 * WAVES + 4 * Lut::floats(g.a);
-  if (modified(g.a)) launch(mmt_long_attn_fwd_kernel<T, D, true>, g.items, lds, st, g);
-  else launch(mmt_long_attn_fwd_kernel<T, D, false>, g.items, lds, st, g);
+  const size_t tiles = 4 * Tile<T, D>::BYTES + 8 * Tile<T, D>::BK, rest = 24 * WAVES + 4 * Lut::floats(g.a);
+  if constexpr (sizeof(T) == 2) {
+    if (g.teams == 2) {
+      if (modified(g.a)) launch(mmt_long_attn_fwd_kernel<T, D, true, 2>, g.items, 2 * tiles + rest, st, g, 2 * THREADS);
+      else launch(mmt_long_attn_fwd_kernel<T, D, false, 2>, g.items, 2 * tiles + rest, st, g, 2 * THREADS);
+      return;
+    }
+  }
+  if (modified(g.a)) launch(mmt_long_attn_fwd_kernel<T, D, true, 1>, g.items, tiles + rest, st, g);
+  else launch(mmt_long_attn_fwd_kernel<T, D, false, 1>, g.items, tiles + rest, st, g);
+}
+
+template <typename T, int D, int TEAMS> static void dq_launch(const Args &g, int64_t items, hipStream_t st) {
+  const size_t lds = TEAMS * (4 * Tile<T, D>::BYTES + 8 * Tile<T, D>::BK) + 24 * WAVES + 4 * Lut::floats(g.a);
+  if (modified(g.a)) launch(mmt_long_attn_dq_kernel<T, D, true, TEAMS>, items, lds, st, g, TEAMS * THREADS);
+  else launch(mmt_long_attn_dq_kernel<T, D, false, TEAMS>, items, lds, st, g, TEAMS * THREADS);
 }
 
 template <typename T, int D> static void bwd_size(Args &g, hipStream_t st, float *table_part, float *dtable) {
@@ -1512,9 +1570,12 @@ template <typename T, int D> static void bwd_size(Args &g, hipStream_t st, float
   const bool mod = modified(a);
   const size_t small = 24 * WAVES;
   const int64_t qitems = (int64_t)a.B * a.H * g.nqt;
-  const size_t lds_q = 4 * L::BYTES + 8 * L::BK + small + 4 * Lut::floats(a);
-  if (mod) launch(mmt_long_attn_dq_kernel<T, D, true>, qitems, lds_q, st, g);
-  else launch(mmt_long_attn_dq_kernel<T, D, false>, qitems, lds_q, st, g);
+  if constexpr (sizeof(T) == 2) {
+    if (g.teams == 2) dq_launch<T, D, 2>(g, qitems, st);
+    else dq_launch<T, D, 1>(g, qitems, st);
+  } else {
+    dq_launch<T, D, 1>(g, qitems, st);
+  }
   if (a.rel_bias) {
     const size_t lds = 2 * L::BYTES + 8 * L::BK + small + 4 * Lut::floats(a) + ((Lut::floats(a) + 15) & ~15) + (size_t)WAVES * a.n_buckets * 256;
     (void)hipFuncSetAttribute((const void *)mmt_long_attn_table_kernel<T, D>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

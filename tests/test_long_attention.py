@@ -834,3 +834,24 @@ def test_norm_rope_pairs(dtype, dh, rot):
             _near(dx, val["dx"], tol["dx"], "dx")
             if dwx is not None:
                 _near(dwx, val["dw"], tol["dw"], "dw")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", sorted(FEATURES))
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+def test_features_of_rows_that_two_teams_share(dtype, name):
+    """16-bit calls of few workgroups and more than three tiles of keys: an odd number of tiles, tiles that only one team has."""
+    f = dict(FEATURES[name])
+    plain = f.pop("plain", {})
+    t, kw = _case(dtype, 6 if f.get("cache") else 1, 70, 290, 2, 1, 64, seed=len(name), **f)
+    _check(t, kw, dtype, **plain)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh", [32, 96, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+def test_documents_of_rows_that_two_teams_share(dtype, dh):
+    docs = [[(0, 70), (-1, 3), (1, 130), (2, 40), (-1, 77), (3, 280)], [(-1, 200), (5, 1), (4, 399)], [(0, 600)]]
+    t, kw = _case(dtype, 3, 600, 600, 2, 1, dh, seed=dh, docs=docs, buckets=8, reach=40, both=True, slopes=True)
+    _check(t, kw, dtype, causal=True, softcap=4.0)
+    _check(t, kw, dtype)
