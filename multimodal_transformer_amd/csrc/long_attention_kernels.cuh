@@ -331,6 +331,12 @@ __device__ __forceinline__ void fwd_store(const Args &g, const FwdState<T, D> &s
 // share a key head - against a range of key tiles.  K and V tiles go straight from memory to LDS, one
 // tile ahead of the products (two buffers, one barrier per tile).  MOD: the scores are capped or biased; without it they go from the
 // product into the exponential as they are.
+// S is computed transposed (the accumulator's rows are keys, its columns the wave's queries), so that a lane owns one query: maximum and
+// sum need one exchange between the two lane halves, and the rounded P is already the operand of the second product.
+// Measured, bf16 causal 8192 tokens x 16 heads of 128 over 4, learned bias: 376 us, 730 TFLOP/s of the 1156 that a large library product
+// reaches; non-causal 2 x 2048 x 16 heads of 64: 70 us, 490.  Bound by the vector instructions of the softmax (54 % busy) between the
+// matrix instructions (34 %), with two waves per SIMD to overlap them; LDS is at a quarter of its rate, without bank conflicts.
+// TEAMS = 2: eight waves, two per 32 rows, which deal the key tiles among themselves and join at the end (rule and figures at teams()).
 template <typename T, int D, bool MOD, int TEAMS>
 __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_fwd_kernel(const Args g) {
   typedef Tile<T, D> L;
@@ -453,7 +459,9 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
 // Few queries (all rows that share a key head fit into 32): the rows are the same for all four waves, which deal the keys among
 // themselves, 32 at a time, and meet at the end, where their maxima, sums and accumulators are joined.  Each has one buffer for K and
 // one for V: the next keys are requested as soon as the products have been taken from the buffer, the next values after theirs, so
-// that up to 32 KiB per wave and, with two workgroups, 128 KiB per CU are on their way.  Bound by reading the cache.
+// that 16 KiB per wave at a head size of 128 and, with two workgroups, 128 KiB per CU are on their way.  Bound by reading the cache: 16
+// requests of up to 32768 tokens (1.36 GB) x 8 key heads of 128 in bf16 take 288 us, 4.7 TB/s where a copy reaches 4.9 (the
+// general kernel: 712 us, three of its four waves without rows).
 template <typename T, int D, bool MOD>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_few_kernel(const Args g) {
   typedef Tile<T, D> L;
@@ -558,7 +566,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
 }
 
 // Joins the splits of a row: weights 2^(m_s - max m).  One wave per row: four groups of 16 lanes (8 elements each) take every fourth
-// split and are added in a fixed order.
+// split and are added in a fixed order.  Bound by the latency of a few loads: 7 us for 2048 rows of 128 and 16 splits (17 MB).
 template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_join_kernel(const Args g) {
   const mmt_long_attention &a = g.a;
   const int64_t rows = (int64_t)a.B * a.H * a.Lq, r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -693,7 +701,9 @@ __device__ __forceinline__ float score_grad_scale(const f32x4 *maxima, int parts
 // dQ, and the statistics of the rows for the other kernels: log-sum in units of log 2 (+inf for a row without keys: its probabilities
 // are 0) and the corrected delta.  The forward's geometry; K is read twice from LDS (as rows for the scores, transposed for
 // dQ^T += K^T dS^T), V once.  16-bit types with rows of at most TWICE keys go over them twice, the first time for delta alone: there a
-// probability's rounding does not average out, and such calls are short (8 us for 128 rows of 21 keys and 8 heads, with one pass 7).
+// probability's rounding does not average out, and such calls are short (128 x 21 tokens x 8 heads of 32: 16.5 us, with one pass 12.2;
+// 8 x 500 x 8 heads of 64: 31 and 21).  fp32 rounds no probability and always makes one.  Bound like the forward: 515 us for its causal
+// case of 8192 tokens (800 TFLOP/s), 88 us for the one of 2048.
 // With a learned bias the kernel also sums dU over the tiles that lie wholly beyond the reach on either side.
 constexpr int TWICE = 512;
 template <typename T, int D, bool MOD, int TEAMS>
@@ -921,9 +931,12 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
 // dK, dV.  A wave owns 32 keys (the accumulator's columns; their rows of K and V stay in registers as operands), the queries of the
 // heads that share the key head go by in LDS tiles, as rows for S and dP and transposed for dV^T += dO^T P and dK^T += Q^T dS.
 // With few key tiles the query heads and the queries are dealt over zh x zq parts, which a second kernel adds up in order.
-// K, V, dK and dV of 32 keys take 192 registers at a head size of 128: one wave per SIMD there, its 512 registers against the latency.
+// For fp32, and 16-bit types up to a head size of 64: K, V, dK and dV of 32 keys take 192 registers at 128, which leaves room for one wave
+// per SIMD (8192 causal tokens x 16 heads: 1380 us, the next kernel's 715).  Up to 64 this one is: bf16
+// 2 x 2048 x 16 heads of 64 98 us, the next one 129; 2 x 4096 tokens in packed scenes 85, the next one 98.  Bound by vector instructions
+// and the latency between them, at two waves per SIMD: 700 TFLOP/s in the first case.
 template <typename T, int D, bool MOD>
-__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt_long_attn_dkv_kernel(const Args g) {
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_dkv_kernel(const Args g) {
   typedef Tile<T, D> L;
   typedef typename Elem<T>::V8 V8;
   constexpr int BQ = L::BK, NQ = BQ / 32, NC = D / 16, ND = D / 32;
@@ -1143,7 +1156,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 || D > 64 ? 1 : 2) mmt
 //   1. wave w computes P and dS of 32 queries x 32 keys (its K and V rows stay in registers) and leaves them in LDS in the order of
 //      the accumulator, which is the order of the second step's operand: 16 bytes per lane, no rearrangement;
 //   2. wave w adds up one of the two outputs for KB x 32 keys and a part of the dimensions, with dO or Q read transposed.
-// Bound by LDS: about 290 KiB go through it per tile, at 128 bytes a cycle a little more than the tile's matrix instructions take.
+// 8192 causal tokens x 16 heads of 128 over 4: 715 us, 770 TFLOP/s for the four products.  About 290 KiB go through LDS per tile, half of
+// the time of its matrix instructions; bound by the steps' order, with two barriers per tile and one workgroup per CU.
 template <typename T, int D, bool MOD>
 __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g) {
   typedef Tile<T, D> L;
@@ -1365,7 +1379,7 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
   }
 }
 
-// the parts of dK and dV, in order
+// the parts of dK and dV, in order; bound by memory (4 parts of 2 x 16.8 MB: 23 us, 6.5 TB/s, part of it still cached)
 template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_dkv_sum_kernel(const Args g) {
   const int64_t n = (int64_t)g.a.B * g.a.Lk * g.a.Hk * g.a.dh, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;
@@ -1379,7 +1393,7 @@ template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_dkv_s
 }
 
 // The gradient of the learned bias over the tiles within the reach (the dQ kernel has summed the others).  Sums of millions of
-// signed terms that have to come out right to fp32: dU is recomputed with the exact delta of each row, and every lane adds into
+// signed terms that have to come out right to fp32 (31 us for 2 x 2048 x 16 heads of 64 and a reach of 128): dU is recomputed with the exact delta of each row, and every lane adds into
 // a column of its own of a [bucket][lane] array in LDS, so that the order of the additions is the program's.  Bound by the latency of
 // these load - add - store chains (LDS additions that return nothing took four times as long): four elements at a time are loaded
 // together, each of the four then adds all those of its bucket, so that equal buckets store equal sums.  The next tile is on its way

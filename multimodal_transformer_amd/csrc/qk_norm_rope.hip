@@ -6,7 +6,8 @@
 // The angles of a token are shared by all its heads: a workgroup forms them once per token, in 64 bits (position * frequency reaches
 // 10^6 turns, of which fp32 would keep 2 digits), reduces them to a fraction of a turn, and a lane keeps the cosines and sines of its 8
 // elements in registers while it walks over the token's heads.  Bound by memory: every element is read once and written once
-// (backwards: two read, one written).
+// (backwards: two read, one written).  bf16, 4 x 4096 tokens x 20 heads of 128: 42 us forward, 4.0 TB/s, 67 us backward, 3.8 TB/s, and 6 for the
+// sum of the weights' gradients, where a large copy reaches 4.9.  32 single tokens of 20 heads: 6 us, the launch and three waits for memory.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -20,7 +21,9 @@ int mmt_set_error(int code, const char *fmt, ...);   // transformer.hip
 
 namespace {
 
-constexpr int NT = 256, MAX_PARTS = 2048;
+constexpr int NT = 256;
+// workgroups backwards, each with a part of the weights' gradients: 1024 take 74 us and 4 for their sum in the case above, 2048 67 and 6
+constexpr int MAX_PARTS = 2048;
 
 template <typename T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
 
@@ -238,7 +241,8 @@ int check(const mmt_qk_norm_rope *a, const char *who) {
   return MMT_OK;
 }
 
-// lane groups per token: one, unless there are too few tokens for 2048 workgroups that way (more than there are heads is no use)
+// lane groups per token: one, unless there are too few tokens for 2048 workgroups that way (more than there are heads is no use); always
+// one takes 18 us instead of 6 for 32 tokens of 20 heads of 128, 14 and 17 instead of 8 and 12 for 3111 of 16 heads of 32 in fp32
 int lanes_per_head(const mmt_qk_norm_rope *a) { return a->dh <= 32 ? 4 : a->dh <= 64 ? 8 : a->dh <= 128 ? 16 : 32; }
 int groups_per_token(const mmt_qk_norm_rope *a) {
   const int groups = NT / lanes_per_head(a);
