@@ -42,12 +42,13 @@ template <int N> struct Const {
 // BK: keys (queries, in the key-gradient kernel) per LDS tile; fp32 elements are twice as large, so half as many.
 // PSHIFT: probabilities are multiplied by 2^PSHIFT before they are rounded to the element type (and the sums with them): fp16 has
 // 5 exponent bits, so that without it every probability under 2^-14 would lose digits and every one under 2^-25 vanish.
+// SLACK: by so much, in units of log 2, a score may exceed what its exponential refers to; in fp16 2^(PSHIFT + SLACK) has to stay finite.
 template <typename T> struct Elem;
 template <> struct Elem<__bf16> {
   typedef bf16x8 V8;
   typedef bf16x4 V4;
   static constexpr int BK = 64;
-  static constexpr float PSHIFT = 0.f;
+  static constexpr float PSHIFT = 0.f, SLACK = 8.f;
   static __device__ __forceinline__ f32x16 mma(const V8 &a, const V8 &b, const f32x16 &c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -56,7 +57,7 @@ template <> struct Elem<_Float16> {
   typedef f16x8 V8;
   typedef f16x4 V4;
   static constexpr int BK = 64;
-  static constexpr float PSHIFT = 14.f;
+  static constexpr float PSHIFT = 14.f, SLACK = 1.f;
   static __device__ __forceinline__ f32x16 mma(const V8 &a, const V8 &b, const f32x16 &c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -65,7 +66,7 @@ template <> struct Elem<float> {
   typedef f32x8 V8;
   typedef f32x4 V4;
   static constexpr int BK = 32;
-  static constexpr float PSHIFT = 0.f;
+  static constexpr float PSHIFT = 0.f, SLACK = 8.f;
   // eight 2-deep steps; step e pairs element e of the two lane halves, which is what the 16-bit instruction sums too
   static __device__ __forceinline__ f32x16 mma(const V8 &a, const V8 &b, f32x16 c) {
 #pragma unroll

@@ -92,7 +92,7 @@ static void plan(Args &g, bool backward) {
 static size_t align64(size_t n) { return (n + 63) & ~(size_t)63; }
 
 struct Workspace {                 // one piece after another, each a multiple of 64 bytes
-  size_t docs, part_o, part_ml, stat, maxima, far, table, part_dk, part_dv, total;
+  size_t docs, part_o, part_ml, stat, maxima, norm, far, table, part_dk, part_dv, total;
 };
 static Workspace layout(const Args &g, bool backward) {
   const mmt_long_attention &a = g.a;
@@ -110,6 +110,7 @@ static Workspace layout(const Args &g, bool backward) {
     if (a.dtype == MMT_F16) w.maxima = n, n += 16 * (STAT_PARTS + 4);
     if (a.rel_bias) {
       const size_t tiles = (size_t)a.B * g.nqt * a.H;
+      w.norm = n, n += align64(4 * rows);
       w.far = n, n += align64(8 * tiles);
       w.table = n, n += align64(4 * tiles * a.n_buckets);
     }
@@ -178,7 +179,7 @@ extern "C" int mmt_long_attention_bwd(const mmt_long_attention *a, const void *o
   g.dout = dout, g.do_bs = do_bs, g.do_rs = do_rs, g.do_hs = do_hs;
   g.dq = dq, g.dk = dk, g.dv = dv, g.dlse = dlse;
   g.stat = (float2 *)(ws + w.stat);
-  if (a->rel_bias) g.far_part = (float *)(ws + w.far);
+  if (a->rel_bias) g.norm = (float *)(ws + w.norm), g.far_part = (float *)(ws + w.far);
   if (g.zh * g.zq > 1) g.part_dk = (float *)(ws + w.part_dk), g.part_dv = (float *)(ws + w.part_dv);
   DocRange *ranges = a->q_doc ? (DocRange *)(ws + w.docs) : nullptr;
   float *table = a->rel_bias ? (float *)(ws + w.table) : nullptr;

@@ -41,6 +41,7 @@ struct Args {                      // mmt_long_attention plus what the launcher 
   float *dscale;                   // fp16: power of two the score gradients are multiplied by before they are rounded
   void *dq, *dk, *dv;              // (B, Lq, H, dh), (B, Lk, Hk, dh)
   const float *dlse;               // (B, H, Lq) gradient of the log-sum, or NULL
+  float *norm;                     // learned bias: (B, H, Lq) 1 / sum of the probabilities as the backward forms them
   float *far_part;                 // (items, 2)
 };
 

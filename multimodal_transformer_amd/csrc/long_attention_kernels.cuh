@@ -219,7 +219,7 @@ __device__ __forceinline__ void mask_keys(float *x, int key0, int hi, const int 
 
 // ---------------------------------------------------------------------------------------------------------------- forward
 // One wave's 32 rows against NK x 32 keys of a tile in LDS: products, modification, masks, running maximum and sum, o^T += v^T P^T.
-// The running maximum is kept in units of log 2.
+// The running maximum (FwdState::m, or up to SLACK less than it) is in units of log 2.
 template <typename T, int D> struct FwdState {
   f32x16 acc[D / 32];
   float m, l;
@@ -252,10 +252,13 @@ __device__ __forceinline__ void fwd_softmax(FwdState<T, D> &st, float *x, int ke
   float mx = x[0];
 #pragma unroll
   for (int i = 1; i < NK * 16; ++i) mx = fmaxf(mx, x[i]);
+  // What the exponentials refer to follows the maximum only where that has gone SLACK ahead: sums and accumulators are rescaled in the
+  // first tiles of a row, not in every one that raises the maximum of one of 32 rows.
   const float m_new = fmaxf(st.m, fmaf(half_max(mx), f.mul, f.add));
-  const float ms = m_new == -INFINITY ? 0.f : m_new;
-  const float alpha = ex2(st.m - ms);
-  st.m = m_new;
+  const bool moved = m_new - st.m > Elem<T>::SLACK;
+  const float ref = moved ? m_new : st.m, ms = ref == -INFINITY ? 0.f : ref;
+  const float alpha = moved ? ex2(st.m - ms) : 1.f;
+  st.m = ref;
   const float off = Elem<T>::PSHIFT + (f.add - ms);
   float sum = 0.f;
 #pragma unroll
@@ -264,7 +267,7 @@ __device__ __forceinline__ void fwd_softmax(FwdState<T, D> &st, float *x, int ke
     sum += x[i];
   }
   st.l = fmaf(st.l, alpha, sum);
-  if (__any(alpha != 1.f)) {
+  if (__any(moved)) {
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -307,7 +310,7 @@ __device__ __forceinline__ void fwd_store(const Args &g, const FwdState<T, D> &s
   }
   const bool some = w.live && l != 0.f;                   // (a NaN sum is "some")
   const float inv = some ? 1.f / l : 0.f;
-  if (g.lse && h == 0) g.lse[r] = some ? (st.m + log2f(l) - Elem<T>::PSHIFT) * LN2 : -INFINITY;
+  if (g.lse && h == 0) g.lse[r] = some ? (st.m + log2f(l * ex2(-Elem<T>::PSHIFT))) * LN2 : -INFINITY;
   const int64_t o = (((int64_t)b * a.Lq + w.i) * a.H + w.h) * a.dh;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -597,7 +600,7 @@ template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_join_
   const bool some = l != 0.f;
   const float inv = some ? 1.f / l : 0.f;
   const int64_t i = r % a.Lq, bh = r / a.Lq, hd = bh % a.H, b = bh / a.H;
-  if (g.lse && lane == 0) g.lse[r] = some ? (m + log2f(l) - Elem<T>::PSHIFT) * LN2 : -INFINITY;
+  if (g.lse && lane == 0) g.lse[r] = some ? (m + log2f(l * ex2(-Elem<T>::PSHIFT))) * LN2 : -INFINITY;
   if (sub == 0 && d0 < a.dh) {
     typename Elem<T>::V8 v, lo;
 #pragma unroll
@@ -700,12 +703,13 @@ __device__ __forceinline__ float score_grad_scale(const f32x4 *maxima, int parts
 
 // dQ, and the statistics of the rows for the other kernels: log-sum in units of log 2 (+inf for a row without keys: its probabilities
 // are 0) and the corrected delta.  The forward's geometry; K is read twice from LDS (as rows for the scores, transposed for
-// dQ^T += K^T dS^T), V once.  16-bit types with rows of at most TWICE keys go over them twice, the first time for delta alone: there a
-// probability's rounding does not average out, and such calls are short (128 x 21 tokens x 8 heads of 32: 16.5 us, with one pass 12.2;
-// 8 x 500 x 8 heads of 64: 31 and 21).  fp32 rounds no probability and always makes one.  Bound like the forward: 515 us for its causal
-// case of 8192 tokens (800 TFLOP/s), 88 us for the one of 2048.
+// dQ^T += K^T dS^T), V once. Where a workgroup's rows see at most TWICE tiles (the beginnings of causal rows and of documents, short
+// rows), 16-bit types go over them twice, the first time for delta alone: a probability's rounding does not average out over few keys.
+// Packed scenes of 300 to 800 tokens (2 x 4096, 16 heads of 64): dQ is 0.0025 off with one pass for all, in 70 us, 0.0024 with two up to 8
+// tiles, in 87, and with two for all, in 122; 0.0023 is what the roundings of dS and of dQ itself make.  fp32 rounds no probability.
+// Bound like the forward: 515 us for its causal case of 8192 tokens (800 TFLOP/s), 86 us for the one of 2048.
 // With a learned bias the kernel also sums dU over the tiles that lie wholly beyond the reach on either side.
-constexpr int TWICE = 512;
+constexpr int TWICE = 8;
 template <typename T, int D, bool MOD, int TEAMS>
 __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_dq_kernel(const Args g) {
   typedef Tile<T, D> L;
@@ -781,9 +785,10 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
     dscale = score_grad_scale(g.maxima, g.stat_parts);
     if (blockIdx.x == 0 && threadIdx.x == 0) *g.dscale = dscale;
   }
-  float all_u = 0.f, far_u[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f};
+  float all_u = 0.f, all_p = 0.f, far_u[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f};
 
-  for (int pass = sizeof(T) == 2 && a.Lk <= TWICE ? 0 : 1; pass < 2; ++pass) {
+  const bool twice = sizeof(T) == 2 && deal.lead >= 0 && __popcll(deal.it.mask) + TEAMS <= TWICE;      // (the tiles of a lookup at least)
+  for (int pass = twice ? 0 : 1; pass < 2; ++pass) {
     auto step = [&](auto buffer) {
       constexpr int buf = decltype(buffer)::value;
       const int k0 = deal.t * BK;
@@ -836,6 +841,7 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
           }
           all_u += su;
           if (pass == 0) continue;
+          if (MOD) all_p += sp;
           if (MOD && a.rel_bias) {
             if (at.far < 0) far_u[0] += su, far_p[0] += sp;
             if (at.far > 0) far_u[1] += su, far_p[1] += sp;
@@ -880,10 +886,21 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
       first(TileIter::ahead(rng, 0, g.nkt));
     }
   }
+  if (MOD && a.rel_bias) {                                  // what the probabilities sum to, instead of 1: lse is rounded at its own size
+    all_p = half_sum(all_p);
+    if constexpr (TEAMS == 2) {
+      float *s = (float *)smem + 2 * THREADS;
+      s[threadIdx.x] = all_p;
+      __syncthreads();
+      all_p = s[threadIdx.x % THREADS] + s[THREADS + threadIdx.x % THREADS];
+    }
+    all_p = all_p > 0.f ? 1.f / all_p : 1.f;
+    if (w.valid && h == 0 && team == 0) g.norm[r] = all_p;
+  }
   if (w.valid && h == 0 && team == 0) g.stat[r] = make_float2(lse, delta + all_u);
   if (MOD && a.rel_bias) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) far_u[s] = wave_sum(w.live ? far_u[s] - all_u * far_p[s] : 0.f);
+    for (int s = 0; s < 2; ++s) far_u[s] = wave_sum(w.live ? (far_u[s] - all_u * far_p[s]) * all_p : 0.f);
     __syncthreads();
     float *sF = (float *)sB;
     if (lane == 0) sF[2 * w_all] = far_u[0], sF[2 * w_all + 1] = far_u[1];
@@ -1417,6 +1434,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   Row w = make_row(g, b, head, qt * ROWS + wave * 32 + col, len, prefix);
   const int64_t r = ((int64_t)b * a.H + head) * a.Lq + min(w.i, a.Lq - 1);
   float2 rs = g.stat[r];
+  float norm = g.norm[r];
   const T *qrow = (const T *)a.q + (int64_t)b * a.q_bs + (int64_t)min(w.i, a.Lq - 1) * a.q_rs + (int64_t)head * a.q_hs;
   const T *drow = (const T *)g.dout + (int64_t)b * g.do_bs + (int64_t)min(w.i, a.Lq - 1) * g.do_rs + (int64_t)head * g.do_hs;
   V8 fq[NC], fd[NC];
@@ -1462,7 +1480,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
 #pragma unroll
   for (int c = 0; c < NC; ++c) live_frag(fq[c], c, h, a.dh, w.live), live_frag(fd[c], c, h, a.dh, w.live);
   const float lse2 = w.live ? rs.x : INFINITY, delta = w.live ? rs.y : 0.f;
-  settle(w.slope), settle(w.doc);
+  settle(w.slope), settle(w.doc), settle(norm);
   while (t < t1) {
     const int k0 = t * BK;
     dma_wait<0>();
@@ -1505,7 +1523,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] = mine[n[e] * 64];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) u[e] = ex2(x[4 * q + e] - lse2) * (dp[kt][4 * q + e] - delta);
+          for (int e = 0; e < 4; ++e) u[e] = ex2(x[4 * q + e] - lse2) * norm * (dp[kt][4 * q + e] - delta);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float sum = n[0] == n[e] ? u[0] : 0.f;

@@ -673,7 +673,7 @@ def test_gradients_in_parts_over_heads_and_queries(case):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("Lk", [512, 513])
+@pytest.mark.parametrize("Lk", [192, 256, 257, 320, 512, 513])
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
 def test_around_the_longest_row_of_two_passes(dtype, Lk):
     t, kw = _case(dtype, 1, 130, Lk, 2, 1, 64, seed=Lk, docs=[[(0, Lk - 90), (1, 80), (-1, 10)]])
