@@ -775,6 +775,7 @@ __global__ __launch_bounds__(256) void mmt_ln_fwd_kernel(const float *__restrict
                                                          int M, int N, const float *__restrict__ g,
                                                          const float *__restrict__ b, int relu, float *__restrict__ y,
                                                          float *__restrict__ xhat, float *__restrict__ rstd_out) {
+#pragma clang fp contract(off)
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= M) return;
   const float *xr = x + (size_t)row * N, *rr = res ? res + (size_t)row * N : nullptr;
@@ -786,14 +787,14 @@ __global__ __launch_bounds__(256) void mmt_ln_fwd_kernel(const float *__restrict
   float v = 0.f;
   for (int c = lane; c < N; c += 64) {
     const float d = xr[c] + (rr ? rr[c] : 0.f) - mu;
-    v += d * d;
+    v = fmaf(d, d, v);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   const float rstd = 1.0f / sqrtf(v / (float)N + 1e-5f);
   for (int c = lane; c < N; c += 64) {
     const float h = (xr[c] + (rr ? rr[c] : 0.f) - mu) * rstd;
-    float o = h * g[c] + b[c];
+    float o = fmaf(h, g[c], b[c]);
     if (relu) o = fmaxf(o, 0.f);
     y[(size_t)row * N + c] = o;
     xhat[(size_t)row * N + c] = h;
@@ -804,10 +805,10 @@ __global__ __launch_bounds__(256) void mmt_ln_fwd_kernel(const float *__restrict
 // The same two kernels with the row in registers (N = 64 * NPL columns): every load of a row is requested at once and the row is
 // read once instead of three times (the generic forms above walk it per pass: three dependent memory round trips in a kernel
 // that 31 + 24 launches of a training step sit behind).  Same element-to-lane assignment, same order of additions: same bits.
-// Contraction is switched off in both and every fused multiply-add is written out, in the places where the compiler fuses in the
-// generic forms: a contraction the compiler is free to pick differently here (it did: d0*d0 + d1*d1 fused the other way round, the
-// constant 1/N folded into the subtraction) moves a result by an ulp, and the full-size gradient test against the reference's
-// autograd sits on exactly those ulps after 12 feedback steps.
+// Contraction is switched off in all four and every fused multiply-add is written out: a contraction the compiler is free to pick
+// differently (it did: d0*d0 + d1*d1 fused the other way round, the constant 1/N folded into the subtraction; without packed fp32
+// instructions the sum of dg * xhat) moves a result by an ulp, and the full-size gradient test against the reference's autograd sits on
+// exactly those ulps after 12 feedback steps.
 template <int NPL>
 __global__ __launch_bounds__(256) void mmt_ln_fwd_regs_kernel(const float *__restrict__ x, const float *__restrict__ res, int M,
                                                               const float *__restrict__ g, const float *__restrict__ b, int relu,
@@ -917,6 +918,7 @@ __global__ __launch_bounds__(256) void mmt_ln_bwd_kernel(const float *__restrict
                                                          float *__restrict__ dx, int accumulate,
                                                          float *__restrict__ dy_masked, const uint8_t *__restrict__ drop,
                                                          float drop_scale, float *__restrict__ dxm) {
+#pragma clang fp contract(off)
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= M) return;
   const size_t o = (size_t)row * N;
@@ -938,7 +940,7 @@ __global__ __launch_bounds__(256) void mmt_ln_bwd_kernel(const float *__restrict
   for (int c = lane; c < N; c += 64) {
     float d = dy_masked ? dy_masked[o + c] : dy[o + c];
     if (!dy_masked && y_relu && !(y_relu[o + c] > 0.f)) d = 0.f;
-    const float v = rs * (d * g[c] - m1 - xhat[o + c] * m2);
+    const float v = rs * fmaf(-xhat[o + c], m2, fmaf(d, g[c], -m1));
     dx[o + c] = accumulate ? dx[o + c] + v : v;
     if (drop) dxm[o + c] = drop[o + c] ? v * drop_scale : 0.f;
   }
