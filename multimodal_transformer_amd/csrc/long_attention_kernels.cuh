@@ -336,9 +336,10 @@ __device__ __forceinline__ void fwd_store(const Args &g, const FwdState<T, D> &s
 // product into the exponential as they are.
 // S is computed transposed (the accumulator's rows are keys, its columns the wave's queries), so that a lane owns one query: maximum and
 // sum need one exchange between the two lane halves, and the rounded P is already the operand of the second product.
-// Measured, bf16 causal 8192 tokens x 16 heads of 128 over 4, learned bias: 376 us, 730 TFLOP/s of the 1156 that a large library product
-// reaches; non-causal 2 x 2048 x 16 heads of 64: 70 us, 490.  Bound by the vector instructions of the softmax (54 % busy) between the
-// matrix instructions (34 %), with two waves per SIMD to overlap them; LDS is at a quarter of its rate, without bank conflicts.
+// Measured, bf16 causal 8192 tokens x 16 heads of 128 over 4, learned bias: 345 us, 800 TFLOP/s of the 1156 that a large library product
+// reaches; non-causal 2 x 2048 x 16 heads of 64: 68 us, 510.  Bound by the vector instructions of the softmax (48 and 55 % of the cycles)
+// between the matrix instructions (40 and 24 %) at the two waves per SIMD that the registers allow; LDS is at 32 and 21 %, without bank
+// conflicts.
 // TEAMS = 2: eight waves, two per 32 rows, which deal the key tiles among themselves and join at the end (rule and figures at teams()).
 template <typename T, int D, bool MOD, int TEAMS>
 __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_fwd_kernel(const Args g) {
@@ -1174,7 +1175,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
 //      the accumulator, which is the order of the second step's operand: 16 bytes per lane, no rearrangement;
 //   2. wave w adds up one of the two outputs for KB x 32 keys and a part of the dimensions, with dO or Q read transposed.
 // 8192 causal tokens x 16 heads of 128 over 4: 715 us, 770 TFLOP/s for the four products.  About 290 KiB go through LDS per tile, half of
-// the time of its matrix instructions; bound by the steps' order, with two barriers per tile and one workgroup per CU.
+// the time of its matrix instructions (LDS 41 % of the cycles, matrix 37 %, vector 30 %); bound by the steps' order: two barriers per
+// tile, one workgroup per CU, and its waves wait for 47 % of the time.
 template <typename T, int D, bool MOD>
 __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g) {
   typedef Tile<T, D> L;
