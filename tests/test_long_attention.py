@@ -855,3 +855,45 @@ def test_documents_of_rows_that_two_teams_share(dtype, dh):
     t, kw = _case(dtype, 3, 600, 600, 2, 1, dh, seed=dh, docs=docs, buckets=8, reach=40, both=True, slopes=True)
     _check(t, kw, dtype, causal=True, softcap=4.0)
     _check(t, kw, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_many_short_rows(dtype):
+    """A batch beyond 2^16: first, middle and last rows, forward and backward, within the bounds of 64 bits (dK and dV of shared heads are
+    added in parts that depend on the size of the call: not the bits of a batch of one)."""
+    B, L, H, dh = 70000, 3, 2, 8
+    g = torch.Generator().manual_seed(47)
+    q, k, v, go = (torch.randn(B, L, n, dh, generator=g).to(dtype).to(DEV) for n in (H, 1, 1, H))
+    got = _run({"q": q, "k": k, "v": v, "go": go}, {}, causal=True)
+    rot = torch_ops.qk_norm_rope(q, k, torch.ones(dh, dtype=dtype, device=DEV), torch.ones(dh, dtype=dtype, device=DEV), ops.rotary_frequencies(dh, device=DEV))
+    for b in (0, 34999, 65536, B - 1):
+        s = slice(b, b + 1)
+        val, tol = long_rows.attention(q[s], k[s], v[s], dout=go[s], causal=True, dtype=dtype)
+        for n, x in zip(("out", "lse", "dq", "dk", "dv"), got):
+            _near(x[s], val[n], tol[n], f"{n} of batch row {b}")
+        r = torch_ops.qk_norm_rope(q[s], k[s], torch.ones(dh, dtype=dtype, device=DEV), torch.ones(dh, dtype=dtype, device=DEV), ops.rotary_frequencies(dh, device=DEV))
+        assert all(torch.equal(x[s], y) for x, y in zip(rot, r)), b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_a_row_of_forty_thousand_tokens(dtype):
+    """Single rows of a long causal call against 64 bits, and its gradients against a call of the last tokens alone over the same keys:
+    a gradient of zero in all other rows makes the two the same sums."""
+    L, H, dh = 40000, 2, 32
+    t, kw = _case(dtype, 1, L, L, H, 1, dh, seed=53, slopes=True, buckets=16, reach=200)
+    t["go"][:, :-70] = 0
+    got = _run(t, kw, causal=True)
+    for i in (0, 12345, 33333, L - 1):
+        val, tol = long_rows.attention(t["q"][:, i:i + 1], t["k"][:, :i + 1], t["v"][:, :i + 1], causal=True, dtype=dtype, **kw)
+        _near(got[0][:, i:i + 1], val["out"], tol["out"], f"row {i}")
+        _near(got[1][:, :, i:i + 1], val["lse"], tol["lse"], f"lse of row {i}")
+    val, tol = long_rows.attention(t["q"][:, -70:], t["k"], t["v"], dout=t["go"][:, -70:], causal=True, dtype=dtype, **kw)
+    _near(got[2][:, -70:], val["dq"], tol["dq"], "dq")
+    assert (got[2][:, :-70] == 0).all()
+    # keys so far away that their probability is under 2^-126 get none at all (fp32 holds no smaller normal number): each of the 70 x 2 rows
+    # then misses at most 2^-126 |dP - delta| scale |q| of a dK and 2^-126 |dO| of a dV, with |dP|, |delta| <= 32 max|dO| max|v| < 2^10 and
+    # scale |q|, |dO| < 2^3: less than 140 * 2^-126 * 2^11 * 2^3 < 2^-104 together
+    for n, x in zip(("dk", "dv", "dbias"), got[3:]):
+        _near(x, val[n], tol[n] + (2.0 ** -104 if n != "dbias" else 0.0), n)
