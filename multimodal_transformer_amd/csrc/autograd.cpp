@@ -2,8 +2,10 @@
 // keys (no counterpart in the reference).  torch runs a node's backward on a thread of its own.  A Python function has to be entered
 // there, with the interpreter's lock handed over twice, and runs on a core that has not seen it: with 128 rows of 21 tokens and 8
 // heads (fp32) a step of forward and backward took 147 us, of which the kernels are busy for 46.  These nodes do the same without the
-// interpreter: 70 us, and 12 instead of 16 for a call without gradients.  Arguments are checked in Python (ops.py), which also fills the argument struct; the C entry points of libmmt_amd.so are
-// handed over as addresses, so that this file needs torch's headers and nothing of the library's.
+// interpreter: 70 us.  Arguments are checked in Python (ops.py), which also fills the argument struct; the C entry points of
+// libmmt_amd.so are handed over as addresses, so that this file needs torch's headers and nothing of the library's.
+// The entry points `plain_*` fill the struct themselves where nothing has to be said or copied, and return None otherwise, upon which the
+// caller goes through the checks: a single token's call takes 8 us, 12 through the checks in Python, 16 with the node in Python too.
 #include <ATen/FuncTorchTLS.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -49,16 +51,32 @@ struct Rows {
   const void *p;
   int64_t b, r, h;
 };
+bool in_place(const Tensor &t, Rows &s) {
+  const int64_t odd = 15 / t.element_size();
+  s = {t.const_data_ptr(), t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0, t.size(2) > 1 ? t.stride(2) : 0};
+  return !(t.stride(3) != 1 && t.size(3) > 1) && !((uintptr_t)s.p & 15) && !((s.b | s.r | s.h) & odd) && s.r * t.element_size() < (1 << 25);
+}
 Rows rows(Tensor &t) {
-  for (int copies = 0;; ++copies) {
-    const int64_t odd = 15 / t.element_size();
-    const Rows s = {t.const_data_ptr(), t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0, t.size(2) > 1 ? t.stride(2) : 0};
-    if (!(t.stride(3) != 1 && t.size(3) > 1) && !((uintptr_t)s.p & 15) && !((s.b | s.r | s.h) & odd) && s.r * t.element_size() < (1 << 25))
-      return s;
+  Rows s;
+  for (int copies = 0; !in_place(t, s); ++copies) {
     TORCH_CHECK(copies < 2, "rows cannot be laid out for the kernels");
     t = copies ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
   }
+  return s;
 }
+// (0: none of them)
+int element_type(const Tensor &t, int &type) {
+  const auto s = t.scalar_type();
+  type = s == at::kFloat ? MMT_F32 : s == at::kBFloat16 ? MMT_BF16 : MMT_F16;
+  return s == at::kFloat || s == at::kBFloat16 || s == at::kHalf;
+}
+constexpr int64_t MOST = 1 << 30;
+bool beside(const Tensor &t, const Tensor &q) { return t.defined() && t.is_cuda() && t.device() == q.device() && t.layout() == at::kStrided; }
+// an optional contiguous tensor beside q
+bool side(const Maybe &t, const Tensor &q, at::ScalarType type, at::IntArrayRef shape) {
+  return !t || (beside(*t, q) && t->scalar_type() == type && t->sizes() == shape && t->is_contiguous());
+}
+template <typename T> const T *address(const Maybe &t) { return t ? (const T *)t->const_data_ptr() : nullptr; }
 
 // what these nodes do not support has to be an error, as with any other function of torch that does not
 void supported(std::initializer_list<Tensor> inputs) {
@@ -169,6 +187,38 @@ std::tuple<Tensor, Tensor> long_attention(uintptr_t args, const Tensor &q, const
   return {out, lse};
 }
 
+std::optional<std::tuple<Tensor, Tensor>> plain_long_attention(const Tensor &q, const Tensor &k, const Tensor &v, std::optional<double> scale, bool causal,
+                                                               const Maybe &prefix, const Maybe &q_doc, const Maybe &k_doc, const Maybe &kv_len,
+                                                               double softcap, const Maybe &slopes, const Maybe &rel_bias, const Maybe &rel_buckets) {
+  mmt_long_attention a = {};
+  if (!q.defined() || !q.is_cuda() || !element_type(q, a.dtype) || q.dim() != 4 || !beside(k, q) || !beside(v, q) || k.dim() != 4 ||
+      k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() || k.sizes() != v.sizes())
+    return std::nullopt;
+  const int64_t B = q.size(0), Lq = q.size(1), H = q.size(2), dh = q.size(3), Lk = k.size(1), Hk = k.size(2);
+  if (k.size(0) != B || k.size(3) != dh || Hk < 1 || H < 1 || H % Hk || std::max({B, Lq, Lk, H}) > MOST) return std::nullopt;
+  if ((prefix && !causal) || !q_doc != !k_doc || !rel_bias != !rel_buckets) return std::nullopt;
+  if (slopes && slopes->requires_grad() && at::GradMode::is_enabled()) return std::nullopt;
+  Rows rq, rk, rv;
+  if (!in_place(q, rq) || !in_place(k, rk) || !in_place(v, rv)) return std::nullopt;
+  if (!side(prefix, q, at::kInt, {B}) || !side(kv_len, q, at::kInt, {B}) || !side(q_doc, q, at::kInt, {B, Lq}) || !side(k_doc, q, at::kInt, {B, Lk}) ||
+      !side(slopes, q, at::kFloat, {H}))
+    return std::nullopt;
+  if (rel_bias) {
+    if (!beside(*rel_bias, q) || rel_bias->dim() != 2 || !beside(*rel_buckets, q) || rel_buckets->dim() != 1 || rel_buckets->numel() < 3 ||
+        rel_buckets->numel() % 2 == 0 || rel_buckets->numel() > MOST || rel_bias->size(1) > MOST || !side(rel_bias, q, at::kFloat, {H, rel_bias->size(1)}) ||
+        !side(rel_buckets, q, at::kInt, {rel_buckets->numel()}))
+      return std::nullopt;
+    a.n_buckets = (int)rel_bias->size(1), a.reach = (int)(rel_buckets->numel() / 2);
+  }
+  a.q = rq.p, a.k = rk.p, a.v = rv.p;
+  a.q_bs = rq.b, a.q_rs = rq.r, a.q_hs = rq.h, a.k_bs = rk.b, a.k_rs = rk.r, a.k_hs = rk.h, a.v_bs = rv.b, a.v_rs = rv.r, a.v_hs = rv.h;
+  a.B = (int)B, a.Lq = (int)Lq, a.Lk = (int)Lk, a.H = (int)H, a.Hk = (int)Hk, a.dh = (int)std::min(dh, MOST), a.causal = causal;
+  a.scale = (float)(scale ? *scale : 1. / std::sqrt((double)dh)), a.softcap = (float)softcap;
+  a.prefix = address<int32_t>(prefix), a.kv_len = address<int32_t>(kv_len), a.q_doc = address<int32_t>(q_doc), a.k_doc = address<int32_t>(k_doc);
+  a.slopes = address<float>(slopes), a.rel_bias = address<float>(rel_bias), a.rel_buckets = address<int32_t>(rel_buckets);
+  return long_attention((uintptr_t)&a, q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets);
+}
+
 // ---- norm + rotation of queries and keys -----------------------------------------------------------------------------------
 struct MmtQkNormRopeBackward : public Node {
   mmt_qk_norm_rope a;
@@ -232,6 +282,28 @@ std::tuple<Tensor, Tensor> qk_norm_rope(uintptr_t args, const Tensor &q, const T
   return {qo, ko};
 }
 
+std::optional<std::tuple<Tensor, Tensor>> plain_qk_norm_rope(const Tensor &q, const Tensor &k, const Tensor &q_weight, const Tensor &k_weight,
+                                                             const Tensor &inv_freq, const Maybe &positions, double eps, bool interleaved) {
+  mmt_qk_norm_rope a = {};
+  if (!q.defined() || !q.is_cuda() || !element_type(q, a.dtype) || q.dim() != 4 || !beside(k, q) || k.dim() != 4 || k.scalar_type() != q.scalar_type())
+    return std::nullopt;
+  const int64_t B = q.size(0), L = q.size(1), H = q.size(2), dh = q.size(3), Hk = k.size(2);
+  if (k.size(0) != B || k.size(1) != L || k.size(3) != dh || Hk < 1 || H < 1 || std::max({B, L, H, Hk}) > MOST) return std::nullopt;
+  if (!beside(q_weight, q) || !element_type(q_weight, a.w_dtype) || (a.w_dtype != a.dtype && a.w_dtype != MMT_F32)) return std::nullopt;
+  if (!side(q_weight, q, q_weight.scalar_type(), {dh}) || !side(k_weight, q, q_weight.scalar_type(), {dh})) return std::nullopt;
+  if (!beside(inv_freq, q) || inv_freq.dim() != 1 || inv_freq.numel() > MOST / 2 || !side(inv_freq, q, at::kDouble, {inv_freq.numel()}) ||
+      !side(positions, q, at::kLong, {B, L}) || (inv_freq.requires_grad() && at::GradMode::is_enabled()))
+    return std::nullopt;
+  Rows rq, rk;
+  if (!in_place(q, rq) || !in_place(k, rk)) return std::nullopt;
+  a.q = rq.p, a.k = rk.p, a.q_weight = q_weight.const_data_ptr(), a.k_weight = k_weight.const_data_ptr();
+  a.q_bs = rq.b, a.q_rs = rq.r, a.q_hs = rq.h, a.k_bs = rk.b, a.k_rs = rk.r, a.k_hs = rk.h;
+  a.inv_freq = address<double>(inv_freq), a.positions = address<int64_t>(positions);
+  a.B = (int)B, a.L = (int)L, a.H = (int)H, a.Hk = (int)Hk, a.dh = (int)std::min(dh, MOST), a.rot = (int)(2 * inv_freq.numel());
+  a.interleaved = interleaved, a.eps = (float)eps;
+  return qk_norm_rope((uintptr_t)&a, q, k, q_weight, k_weight, inv_freq, positions);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
@@ -254,4 +326,6 @@ PYBIND11_MODULE(_autograd, m) {
   });
   m.def("long_attention", &long_attention, py::call_guard<py::gil_scoped_release>());
   m.def("qk_norm_rope", &qk_norm_rope, py::call_guard<py::gil_scoped_release>());
+  m.def("plain_long_attention", &plain_long_attention, py::call_guard<py::gil_scoped_release>());
+  m.def("plain_qk_norm_rope", &plain_qk_norm_rope, py::call_guard<py::gil_scoped_release>());
 }

@@ -157,7 +157,7 @@ for _name, _fn, _meta in (
 
 
 def _constant(t, what):
-    if t is not None and t.requires_grad:
+    if isinstance(t, torch.Tensor) and t.requires_grad:
         raise MmtError(f"{what} are constants, they get no gradient")
 
 
@@ -210,6 +210,14 @@ def _traced(t):
     """The call is being traced (fake tensors, a dispatch mode, torch.compile): it has to go through the dispatcher.  Otherwise the
     wrappers below go straight to the kernels."""
     return type(t) not in (torch.Tensor, torch.nn.Parameter) or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+
+
+def _plain(fn, *args):
+    """The native call that checks for itself; None where an argument is not what it expects."""
+    try:
+        return fn(*args)
+    except TypeError:
+        return None
 
 
 # ---- what the module classes call: the same ops through the dispatcher, with this package's error for host tensors ------------
@@ -271,10 +279,13 @@ def long_attention(q, k, v, *, scale=None, causal=False, prefix=None, q_doc=None
         out, lse = torch.ops.mmt.long_attention(q, k, v, scale, bool(causal), prefix, q_doc, k_doc, kv_len, float(softcap), slopes,
                                                 rel_bias, rel_buckets)[:2]
     else:
-        if torch.is_grad_enabled():
-            _constant(slopes, "long_attention: the slopes of the distance bias")
-        a, q, k, v = ops._attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets)
-        out, lse = _native().long_attention(ctypes.addressof(a), q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets)
+        both = _plain(_native().plain_long_attention, q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets)
+        if both is None:                                  # something to copy, or to complain about
+            if torch.is_grad_enabled():
+                _constant(slopes, "long_attention: the slopes of the distance bias")
+            a, q, k, v = ops._attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets)
+            both = _native().long_attention(ctypes.addressof(a), q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets)
+        out, lse = both
     return (out, lse) if return_lse else out
 
 
@@ -284,7 +295,10 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps=1e-6
     and the weights.  ``positions`` (B,L) int64, None: 0..L-1.  Pairs are (m, m + rot/2), with ``interleaved`` (2m, 2m + 1)."""
     if _traced(q):
         return torch.ops.mmt.qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, float(eps), bool(interleaved))
-    if torch.is_grad_enabled():
-        _constant(inv_freq, "qk_norm_rope: the frequencies")
-    a, q, k = ops._rope_args(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
-    return _native().qk_norm_rope(ctypes.addressof(a), q, k, q_weight, k_weight, inv_freq, positions)
+    both = _plain(_native().plain_qk_norm_rope, q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
+    if both is None:
+        if torch.is_grad_enabled():
+            _constant(inv_freq, "qk_norm_rope: the frequencies")
+        a, q, k = ops._rope_args(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
+        both = _native().qk_norm_rope(ctypes.addressof(a), q, k, q_weight, k_weight, inv_freq, positions)
+    return both

@@ -897,3 +897,34 @@ def test_a_row_of_forty_thousand_tokens(dtype):
     # scale |q|, |dO| < 2^3: less than 140 * 2^-126 * 2^11 * 2^3 < 2^-104 together
     for n, x in zip(("dk", "dv", "dbias"), got[3:]):
         _near(x, val[n], tol[n] + (2.0 ** -104 if n != "dbias" else 0.0), n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_plain_calls_equal_the_checked_ones(dtype, monkeypatch):
+    """Calls that need no copy are filled in natively: the same bits as through the checks, with every option; what the native call does
+    not take (a list for a tensor, a view to copy) goes through them."""
+    t, kw = _case(dtype, 3, 60, 200, 4, 2, 64, seed=59, docs=[[(0, 150), (-1, 50)], [(1, 80), (2, 120)], [(3, 200)]], prefix=True, cache=True,
+                  slopes=True, buckets=16, reach=40)
+    w, f = torch.ones(64, dtype=dtype, device=DEV, requires_grad=True), ops.rotary_frequencies(64, device=DEV)
+    pos = torch.arange(60, device=DEV).expand(3, 60).contiguous() * 3
+
+    def both():
+        x, y = torch_ops.qk_norm_rope(t["q"], t["k"][:, :60], w, w, f, pos, eps=1e-5, interleaved=True)
+        return _run(t, kw, causal=True, softcap=6.0, scale=0.3) + [x, y] + list(torch.autograd.grad(x.float().sum() + y.float().sum(), w))
+    plain = both()
+    monkeypatch.setattr(torch_ops, "_plain", lambda *a: None)
+    assert all(torch.equal(a, b) for a, b in zip(plain, both()))
+    monkeypatch.undo()
+    seen = []
+    take = torch_ops._plain
+    monkeypatch.setattr(torch_ops, "_plain", lambda *a: seen.append(take(*a)) or seen[-1])
+    torch_ops.long_attention(t["q"], t["k"], t["v"])
+    torch_ops.long_attention(t["q"].transpose(2, 3).contiguous().transpose(2, 3), t["k"], t["v"])
+    assert seen[0] is not None and seen[1] is None
+    for bad in (dict(kv_len=[1, 2, 3]), dict(q_doc=3, k_doc=3), dict(rel_bias=1.0, rel_buckets=kw["rel_buckets"])):
+        with pytest.raises(MmtError):
+            torch_ops.long_attention(t["q"], t["k"], t["v"], **bad)
+    for bad in ((None, t["k"], w, w, f), (t["q"], t["k"][:, :60], w, None, f), (t["q"], t["k"][:, :60], w, w, [1.0])):
+        with pytest.raises(MmtError):
+            torch_ops.qk_norm_rope(*bad)
