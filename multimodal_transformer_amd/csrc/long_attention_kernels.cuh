@@ -715,7 +715,7 @@ template <typename T, int D, bool MOD, int TEAMS>
 __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_dq_kernel(const Args g) {
   typedef Tile<T, D> L;
   typedef typename Elem<T>::V8 V8;
-  constexpr int BK = L::BK, NK = BK / 32, NC = D / 16, ND = D / 32;
+  constexpr int BK = L::BK, NK = BK / 32, NC = D / 16, ND = D / 32, AT_ONCE = D > 64 ? 1 : NK;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
   int *sDoc2 = (int *)(smem + TEAMS * 4 * L::BYTES), *sB = sDoc2 + TEAMS * 2 * BK;
@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
         const bool need_mask = k0 + BK > wb.hi_min || mixed;
         // by the whole workgroup's rows: the table kernel takes the tiles that are left with the same rule
         const Place at = place(a, k0 - gb.p_max, k0 + BK - 1 - gb.p_min);
-#pragma unroll(D > 64 ? 1 : NK)
+#pragma unroll AT_ONCE
         for (int kt = 0; kt < NK; ++kt) {
           // (the two products one after the other where registers are short: what is live grows with how far the compiler pulls them together)
           f32x16 s = {}, dp = {};
@@ -1106,7 +1106,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
         if (need_mask) {
           const int lo = a.causal ? (j < prefix ? 0 : j - off - q0 - 32 * qt) : -(1 << 30);      // first row of the sub-tile that sees key j
 #pragma unroll
-          for (int i = 0; i < 16; ++i) p[i] = live & (acc_row(i, h) >= lo) ? p[i] : 0.f;
+          for (int i = 0; i < 16; ++i) p[i] = (live & (acc_row(i, h) >= lo)) ? p[i] : 0.f;
           if (mixed) {
             int id[16];
 #pragma unroll
@@ -1325,7 +1325,7 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
       if (need_mask) {
         const int lo = a.causal ? (j < prefix ? 0 : j - p0) : -(1 << 30);      // first of the queries that sees key j
 #pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = live & (acc_row(i, h) >= lo) ? p[i] : 0.f;
+        for (int i = 0; i < 16; ++i) p[i] = (live & (acc_row(i, h) >= lo)) ? p[i] : 0.f;
         if (mixed) {
           int id[16];
 #pragma unroll
