@@ -928,3 +928,32 @@ def test_plain_calls_equal_the_checked_ones(dtype, monkeypatch):
     for bad in ((None, t["k"], w, w, f), (t["q"], t["k"][:, :60], w, None, f), (t["q"], t["k"][:, :60], w, w, [1.0])):
         with pytest.raises(MmtError):
             torch_ops.qk_norm_rope(*bad)
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once():
+    """Training steps of two Python threads (the calls let go of the interpreter), each on a stream of its own: the bits of one alone."""
+    import threading
+    cases = [_case(BF16, 2, 150, 150, 4, 2, 64, seed=n, buckets=8, reach=20) for n in (61, 62)]
+    want = [_run(t, kw, causal=True) for t, kw in cases]
+    torch.cuda.synchronize()
+    got, failed = [[], []], []
+
+    def work(n):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[n].append(_run(*cases[n], causal=True))
+                with pytest.raises(MmtError):
+                    torch_ops.long_attention(cases[n][0]["q"], cases[n][0]["k"], cases[n][0]["v"], scale=-1.0)
+        except BaseException as e:
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for n in range(2):
+        assert len(got[n]) == 20 and all(torch.equal(a, b) for run in got[n] for a, b in zip(want[n], run))
