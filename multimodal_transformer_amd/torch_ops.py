@@ -207,9 +207,10 @@ torch.library.register_autograd("mmt::qk_norm_rope_bwd", _no_second("qk_norm_rop
 
 
 def _traced(t):
-    """The call is being traced (fake tensors, a dispatch mode, torch.compile): it has to go through the dispatcher.  Otherwise the
-    wrappers below go straight to the kernels."""
-    return type(t) not in (torch.Tensor, torch.nn.Parameter) or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+    """The call is being traced (fake tensors, a dispatch mode, torch.compile, torch.jit.trace): it has to go through the dispatcher.
+    Otherwise the wrappers below go straight to the kernels."""
+    return type(t) not in (torch.Tensor, torch.nn.Parameter) or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0 or \
+        torch._C._is_tracing()
 
 
 def _plain(fn, *args):
