@@ -46,6 +46,16 @@ Tensor like(const Tensor &t) { return at::empty(t.sizes(), at::TensorOptions().d
 Tensor bytes(size_t n, const Tensor &beside) { return at::empty({(int64_t)n}, at::TensorOptions().dtype(at::kByte).device(beside.device())); }
 template <typename T> const T *address(const Tensor &t) { return t.defined() ? (const T *)t.const_data_ptr() : nullptr; }
 
+// What a tensor subclass, a lazily negated view or a lazy zero stands for is not what lies at its address (or it has none): such arguments
+// go through the dispatcher, which turns them into plain ones
+bool has_memory(const Tensor &t) { return !t.unsafeGetTensorImpl()->is_python_dispatch() && !t.is_neg() && !t._is_zerotensor(); }
+// a gradient, or what saved-tensor hooks gave back, as plain memory
+Tensor in_memory(const Tensor &t) {
+  if (has_memory(t)) return t;
+  if (t.unsafeGetTensorImpl()->is_python_dispatch()) throw Failure("a tensor subclass without memory of its own arrived in the backward pass");
+  return t._is_zerotensor() ? at::zeros(t.sizes(), at::TensorOptions().dtype(t.scalar_type()).device(t.device())) : t.resolve_neg();
+}
+
 // Row strides of a (B, L, heads, dh) tensor as the kernels read them where it lies, of a copy where they cannot (ops._head_rows)
 struct Rows {
   const void *p;
@@ -58,6 +68,7 @@ bool in_place(const Tensor &t, Rows &s) {
 }
 Rows rows(Tensor &t) {
   Rows s;
+  t = in_memory(t);
   for (int copies = 0; !in_place(t, s); ++copies) {
     TORCH_CHECK(copies < 2, "rows cannot be laid out for the kernels");
     t = copies ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
@@ -71,7 +82,7 @@ int element_type(const Tensor &t, int &type) {
   return s == at::kFloat || s == at::kBFloat16 || s == at::kHalf;
 }
 constexpr int64_t MOST = 1 << 30;
-bool beside(const Tensor &t, const Tensor &q) { return t.defined() && t.is_cuda() && t.device() == q.device() && t.layout() == at::kStrided; }
+bool beside(const Tensor &t, const Tensor &q) { return t.defined() && t.is_cuda() && t.device() == q.device() && t.layout() == at::kStrided && has_memory(t); }
 // an optional contiguous tensor beside q
 bool side(const Maybe &t, const Tensor &q, at::ScalarType type, at::IntArrayRef shape) {
   return !t || (beside(*t, q) && t->scalar_type() == type && t->sizes() == shape && t->is_contiguous());
@@ -132,7 +143,7 @@ struct MmtLongAttentionBackward : public Node {
       a.slopes = address<float>(sl), a.rel_bias = address<float>(rb), a.rel_buckets = address<int32_t>(ru);
       if (!dout.defined()) dout = at::zeros_like(o);
       const Rows rd = rows(dout);
-      if (dlse.defined()) dlse = dlse.contiguous();
+      if (dlse.defined()) dlse = in_memory(dlse).contiguous();
       g[0] = like(qt), g[1] = like(kt), g[2] = like(vt);
       if (rb.defined()) g[3] = like(rb);
       if ((int64_t)a.B * a.Lq * a.Lk == 0) {
@@ -191,7 +202,7 @@ std::optional<std::tuple<Tensor, Tensor>> plain_long_attention(const Tensor &q, 
                                                                const Maybe &prefix, const Maybe &q_doc, const Maybe &k_doc, const Maybe &kv_len,
                                                                double softcap, const Maybe &slopes, const Maybe &rel_bias, const Maybe &rel_buckets) {
   mmt_long_attention a = {};
-  if (!q.defined() || !q.is_cuda() || !element_type(q, a.dtype) || q.dim() != 4 || !beside(k, q) || !beside(v, q) || k.dim() != 4 ||
+  if (!beside(q, q) || !element_type(q, a.dtype) || q.dim() != 4 || !beside(k, q) || !beside(v, q) || k.dim() != 4 ||
       k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() || k.sizes() != v.sizes())
     return std::nullopt;
   const int64_t B = q.size(0), Lq = q.size(1), H = q.size(2), dh = q.size(3), Lk = k.size(1), Hk = k.size(2);
@@ -285,7 +296,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope(uintptr_t args, const Tensor &q, const T
 std::optional<std::tuple<Tensor, Tensor>> plain_qk_norm_rope(const Tensor &q, const Tensor &k, const Tensor &q_weight, const Tensor &k_weight,
                                                              const Tensor &inv_freq, const Maybe &positions, double eps, bool interleaved) {
   mmt_qk_norm_rope a = {};
-  if (!q.defined() || !q.is_cuda() || !element_type(q, a.dtype) || q.dim() != 4 || !beside(k, q) || k.dim() != 4 || k.scalar_type() != q.scalar_type())
+  if (!beside(q, q) || !element_type(q, a.dtype) || q.dim() != 4 || !beside(k, q) || k.dim() != 4 || k.scalar_type() != q.scalar_type())
     return std::nullopt;
   const int64_t B = q.size(0), L = q.size(1), H = q.size(2), dh = q.size(3), Hk = k.size(2);
   if (k.size(0) != B || k.size(1) != L || k.size(3) != dh || Hk < 1 || H < 1 || std::max({B, L, H, Hk}) > MOST) return std::nullopt;

@@ -769,6 +769,15 @@ def finalize(pred_st, node_pos=None, gt=None, metres=True, want_pred=True, want_
 _ELEM = {torch.float32: _lib.MMT_F32, torch.bfloat16: _lib.MMT_BF16, torch.float16: _lib.MMT_F16}
 
 
+def _address(t, name):
+    """Where the tensor's elements lie.  A subclass without memory, a lazily negated view, a lazy zero have no such place (the dispatcher,
+    torch.ops.mmt.*, resolves them)."""
+    p = t.data_ptr()
+    if (p == 0 and t.numel()) or t.is_neg():
+        raise MmtError(f"{name}: not a tensor with memory of its own (a lazy view or a subclass)")
+    return p
+
+
 def _head_rows(t, name, shape, dtype, device):
     """A (B, L, heads, dh) tensor whose rows (head slices) the kernels can read where they are: contiguous elements, every row at a
     multiple of 16 bytes, the next token's less than 2^25 bytes away; anything else (a transposed last axis, an odd offset) is copied once.  Strides of 0 (broadcast) are fine.
@@ -785,7 +794,7 @@ def _head_rows(t, name, shape, dtype, device):
             raise MmtError(f"{name}: dtype {t.dtype}, expected {dtype}")
         raise MmtError(f"{name}: tensor is on {t.device}, expected {device}")
     b, r, h, one = t.stride()
-    p = t.data_ptr()
+    p = _address(t, name)
     size = t.element_size()
     odd, far = 15 // size, (1 << 25) // size
     if one != 1 or (p & 15) or ((b | r | h) & odd) or r >= far:
@@ -807,7 +816,7 @@ def _side(t, name, shape, dtype, device):
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.device == device):
         _chk(t, name, shape, dtype)
         raise MmtError(f"{name}: tensor is on {t.device}, expected {device}")
-    return t.data_ptr()
+    return _address(t, name)
 
 
 def _on_device(fn):

@@ -213,6 +213,18 @@ def _traced(t):
         torch._C._is_tracing()
 
 
+def _lazy(*args):
+    """Some argument is not the memory at its address (a tensor subclass, a lazily negated view, a lazy zero): the dispatcher turns it
+    into what the kernels read."""
+    return any(isinstance(t, torch.Tensor) and (type(t) not in (torch.Tensor, torch.nn.Parameter) or t.is_neg() or t._is_zerotensor())
+               for t in args)
+
+
+def _dispatched(op, *args):
+    """(a lazy zero would become an expanded one, which the kernels' tables must not be: it is written out)"""
+    return op(*(t.clone() if isinstance(t, torch.Tensor) and t._is_zerotensor() else t for t in args))
+
+
 def _plain(fn, *args):
     """The native call that checks for itself; None where an argument is not what it expects."""
     try:
@@ -276,17 +288,19 @@ def long_attention(q, k, v, *, scale=None, causal=False, prefix=None, q_doc=None
     slopes     (H) float32: -slopes[h] * distance is added         rel_bias  (H,n) float32, learned, at rel_buckets (2 reach + 1) int32 of
                                                                              the clamped distance (``ops.relative_buckets``)
     Rows that see nothing give zeros (and an lse of -inf).  Returns out (B,Lq,H,dh), with ``return_lse`` also the log-sums (B,H,Lq)."""
-    if _traced(q):
-        out, lse = torch.ops.mmt.long_attention(q, k, v, scale, bool(causal), prefix, q_doc, k_doc, kv_len, float(softcap), slopes,
-                                                rel_bias, rel_buckets)[:2]
-    else:
-        both = _plain(_native().plain_long_attention, q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets)
-        if both is None:                                  # something to copy, or to complain about
+    traced = _traced(q)
+    both = None if traced else _plain(_native().plain_long_attention, q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes,
+                                      rel_bias, rel_buckets)
+    if both is None:                                      # something to trace, to copy, or to complain about
+        if traced or _lazy(q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets):
+            both = _dispatched(torch.ops.mmt.long_attention, q, k, v, scale, bool(causal), prefix, q_doc, k_doc, kv_len, float(softcap),
+                               slopes, rel_bias, rel_buckets)[:2]
+        else:
             if torch.is_grad_enabled():
                 _constant(slopes, "long_attention: the slopes of the distance bias")
             a, q, k, v = ops._attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets)
             both = _native().long_attention(ctypes.addressof(a), q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets)
-        out, lse = both
+    out, lse = both
     return (out, lse) if return_lse else out
 
 
@@ -294,10 +308,11 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps=1e-6
     """RMS norm of queries (B,L,H,dh) and keys (B,L,Hk,dh) per head, times the weights (dh), and the rotation of their first
     2 * len(inv_freq) elements by position * inv_freq (float64, ``ops.rotary_frequencies``) in the same pass; differentiable in q, k
     and the weights.  ``positions`` (B,L) int64, None: 0..L-1.  Pairs are (m, m + rot/2), with ``interleaved`` (2m, 2m + 1)."""
-    if _traced(q):
-        return torch.ops.mmt.qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, float(eps), bool(interleaved))
-    both = _plain(_native().plain_qk_norm_rope, q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
+    traced = _traced(q)
+    both = None if traced else _plain(_native().plain_qk_norm_rope, q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
     if both is None:
+        if traced or _lazy(q, k, q_weight, k_weight, inv_freq, positions):
+            return _dispatched(torch.ops.mmt.qk_norm_rope, q, k, q_weight, k_weight, inv_freq, positions, float(eps), bool(interleaved))
         if torch.is_grad_enabled():
             _constant(inv_freq, "qk_norm_rope: the frequencies")
         a, q, k = ops._rope_args(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)

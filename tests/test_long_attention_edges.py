@@ -49,3 +49,79 @@ def test_a_traced_call_computes_on_new_inputs(dtype):
     traced = torch.jit.trace(block, tuple(first[n] for n in "qkv"), check_trace=False)
     for t in (then, first):
         assert all(torch.equal(a, b) for a, b in zip(traced(*(t[n] for n in "qkv")), block(*(t[n] for n in "qkv"))))
+
+
+# ------------------------------------------------------------------------------------------- tensors that are not plain memory
+class _Held(torch.Tensor):
+    """A subclass without memory of its own: every operator that meets it gets the tensor it holds."""
+
+    @staticmethod
+    def __new__(cls, held):
+        return torch.Tensor._make_wrapper_subclass(cls, held.shape, strides=held.stride(), dtype=held.dtype, device=held.device)
+
+    def __init__(self, held):
+        self.held = held
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        give = lambda x: x.held if isinstance(x, _Held) else x
+        return func(*(give(x) for x in args), **{n: give(x) for n, x in (kwargs or {}).items()})
+
+
+def test_tensors_without_memory_are_refused_by_the_plain_calls():
+    """ops.* reads addresses: a tensor that has none is an error, not an argument that was left out."""
+    held = _Held(torch.empty(4, device="meta"))
+    assert held.data_ptr() == 0
+    on = torch.Tensor._make_wrapper_subclass(_Held, (1, 3, 4, 8), dtype=F32, device="cuda:0")
+    for call in (lambda: ops._side(on, "slopes", on.shape, F32, on.device),
+                 lambda: ops._head_rows(on, "q", None, F32, on.device)):
+        with pytest.raises(MmtError, match="memory"):
+            call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_subclasses_and_lazy_views_count_like_what_they_stand_for(dtype):
+    """A tensor subclass, a lazily negated view, a lazy zero in place of any argument: the bits of the plain tensor."""
+    t, kw = _case(dtype, 2, 50, 90, 4, 2, 32, seed=71, prefix=True, cache=True, slopes=True, buckets=8, reach=16,
+                  docs=[[(0, 60), (1, 30)], [(0, 90)]])
+    args = dict(kw, **{n: t[n] for n in "qkv"})
+    call = lambda **a: torch_ops.long_attention(a.pop("q"), a.pop("k"), a.pop("v"), causal=True, return_lse=True, **a)
+    want = call(**args)
+    for name, x in args.items():
+        ways = [_Held(x)]
+        if x.is_floating_point():
+            ways.append(torch._neg_view(-x))
+        for way in ways:
+            assert all(torch.equal(a, b) for a, b in zip(call(**dict(args, **{name: way})), want)), name
+    zero = torch._efficientzerotensor((4,), dtype=F32, device=DEV)
+    got = call(**dict(args, slopes=zero)), call(**dict(args, slopes=torch.zeros(4, device=DEV)))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    w, f = torch.linspace(0.5, 2, 32, device=DEV), ops.rotary_frequencies(32, device=DEV)
+    pos = torch.arange(50, device=DEV).expand(2, 50).contiguous() * 7
+    args = dict(q=t["q"], k=t["k"][:, :50].contiguous(), q_weight=w, k_weight=2 * w, inv_freq=f, positions=pos)
+    want = torch_ops.qk_norm_rope(**args)
+    for name, x in args.items():
+        for way in [_Held(x)] + ([torch._neg_view(-x)] if x.is_floating_point() else []):
+            assert all(torch.equal(a, b) for a, b in zip(torch_ops.qk_norm_rope(**dict(args, **{name: way})), want)), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_gradients_that_come_as_lazy_views(dtype):
+    t, _ = _case(dtype, 2, 40, 40, 4, 2, 32, seed=73)
+    w, f = torch.ones(32, dtype=dtype, device=DEV), ops.rotary_frequencies(32, device=DEV)
+    q, k, v = (t[n].clone().requires_grad_() for n in "qkv")
+    dlse = torch.randn(2, 4, 40, generator=torch.Generator().manual_seed(1)).to(DEV)
+    lazy = lambda x: torch._neg_view(-x)
+    zeros = lambda x: torch._efficientzerotensor(x.shape, dtype=x.dtype, device=x.device)
+
+    def grads(how_out, how_lse):
+        x, y = torch_ops.qk_norm_rope(q, k, w, w, f)
+        both = torch_ops.long_attention(x, y, v, causal=True, return_lse=True)
+        first = torch.autograd.grad(both, (x, y, v), (how_out(t["go"]), how_lse(dlse)), retain_graph=True)
+        return list(first) + list(torch.autograd.grad((x, y), (q, k), (how_out(first[0]), how_out(first[1]))))
+    plain = grads(lambda x: x, lambda x: x)
+    assert all(torch.equal(a, b) for a, b in zip(plain, grads(lazy, lazy)))
+    assert all(torch.equal(a, b) for a, b in zip(grads(lambda x: x, torch.zeros_like), grads(lambda x: x, zeros)))
+    assert all(torch.equal(a, b) for a, b in zip(grads(torch.zeros_like, lambda x: x), grads(zeros, lambda x: x)))
