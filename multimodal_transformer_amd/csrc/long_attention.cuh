@@ -240,6 +240,18 @@ __device__ __forceinline__ void zero_rows(char *lds, int end, const int *doc) {
   }
 }
 
+// The same for rows of queries, by their log-sums (+inf: missing, padding, or a row that sees nothing)
+template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS>
+__device__ __forceinline__ void zero_blind_rows(char *lds, const float *lse) {
+  typedef Tile<T, D> L;
+  const int tid = rare_tid() % NT;
+#pragma unroll
+  for (int n = 0; n < R * L::NS / NT; ++n) {
+    const int idx = tid + n * NT;
+    if (lse[idx / L::NS] == INFINITY) *(u32x4 *)(lds + idx * 16) = u32x4{};
+  }
+}
+
 // ---- lanes ----------------------------------------------------------------------------------------------------------------
 // the two halves of the wave hold complementary parts of a row: v[lane] op v[lane ^ 32]
 // (s_nop: the distance from a VALU write to the lane swap, which the compiler does not see inside asm)

@@ -663,8 +663,10 @@ template <typename T> __global__ void __launch_bounds__(STAT_THREADS) mmt_long_a
   for (int64_t r = (int64_t)blockIdx.x * STAT_ROWS + (threadIdx.x >> 4); r < rows; r += (int64_t)gridDim.x * STAT_ROWS) {
     const int64_t hd = r % a.H, bi = r / a.H, i = bi % a.Lq, b = bi / a.Lq;
     if (a.q_doc && a.q_doc[b * a.Lq + i] < 0) continue;
-    m[0] = fmaxf(m[0], square((const T *)g.dout + b * g.do_bs + i * g.do_rs + hd * g.do_hs));
-    const float dl = g.dlse ? fabsf(g.dlse[(b * a.H + hd) * a.Lq + i]) : 0.f;
+    const float dl = g.dlse ? fabsf(g.dlse[(b * a.H + hd) * a.Lq + i]) : 0.f, lse = g.lse[(b * a.H + hd) * a.Lq + i];
+    const float norm = square((const T *)g.dout + b * g.do_bs + i * g.do_rs + hd * g.do_hs);
+    if (lse == -INFINITY) continue;                       // (sees nothing: takes no part)
+    m[0] = fmaxf(m[0], norm);
     if (isfinite(dl)) m[2] = fmaxf(m[2], dl);
   }
   for (int64_t r = (int64_t)blockIdx.x * STAT_ROWS + (threadIdx.x >> 4); r < vrows; r += (int64_t)gridDim.x * STAT_ROWS) {
@@ -772,9 +774,14 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
 #pragma unroll
     for (int e = 0; e < 8; ++e) delta = fmaf((float)o[e] + (float)lo[e], (float)fd[c][e], delta);
   }
+  // A row that sees nothing takes no part, whatever arrives as its gradient (a squared log-sum's is -inf).  The dK / dV kernels read here
+  // which of their tiles hold such rows: 0 x inf would reach all keys.
+  const bool sees = lse != -INFINITY, blind = __any(w.valid && !sees);
+  if (lane == 0 && team == 0) g.blind[(((int64_t)b * a.H + head) * g.nqt + qt) * WAVES + wave] = blind;
+  w.live = w.live && sees;
   dl = w.live ? dl : 0.f;
   delta = w.live ? half_sum(delta) - dl : 0.f;
-  lse = !w.live || lse == -INFINITY ? INFINITY : lse * LOG2E;
+  lse = w.live ? lse * LOG2E : INFINITY;
   settle(lse), settle(w.slope), settle(w.doc);
   deal.it.here();
   f32x16 acc[ND];
@@ -1020,6 +1027,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   TileIter it;
   int gi = g0 - 1, t = -1, lut_gi = -1;
   const float2 *stat = nullptr;
+  const int *blind = nullptr;
+  int blind_next = 0;
   float2 st_next = make_float2(INFINITY, 0.f);
   float slope_next = 0.f;
   int doc_next = -1;
@@ -1027,6 +1036,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     int n = gi < g0 ? -1 : it.next();
     while (n < 0 && ++gi < g1) {
       stat = g.stat + ((int64_t)b * a.H + head0 + gi) * a.Lq;
+      blind = g.blind + ((int64_t)b * a.H + head0 + gi) * g.nqt * WAVES;
       dmq.base = qbase + (int64_t)gi * a.q_hs * (int64_t)sizeof(T);
       dmo.base = obase + (int64_t)gi * g.do_hs * (int64_t)sizeof(T);
       if (MOD && a.slopes) slope_next = scalar_load(a.slopes + head0 + gi) * LOG2E;
@@ -1038,6 +1048,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   auto fetch = [&](int tile, int to) {
     dmq.load(lds + to * 2 * L::BYTES, tile * BQ);
     dmo.load(lds + to * 2 * L::BYTES + L::BYTES, tile * BQ);
+    blind_next = blind[tile * (BQ / 32) + (lane & (BQ / 32 - 1))];       // (a lane's own: a scalar load would hold up the reads from LDS)
     if (threadIdx.x < BQ) {
       // (neither waits for the other, or for the tile: rows that are missing or dead are sorted out when the tile is here)
       const int i = min(tile * BQ + (int)threadIdx.x, a.Lq - 1);
@@ -1071,9 +1082,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
       lut_gi = cur_gi;
       __syncthreads();
     }
-    if (q0 + BQ > a.Lq || dead) {
-      zero_rows<T, D>(sQ, a.Lq - q0, sDoc);
-      zero_rows<T, D>(sO, a.Lq - q0, sDoc);
+    if (q0 + BQ > a.Lq || dead || __any(blind_next)) {
+      zero_blind_rows<T, D>(sQ, sStat);
+      zero_blind_rows<T, D>(sO, sStat);
       __syncthreads();
     }
     const int tn = advance(Const<0>());
@@ -1248,6 +1259,8 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
   TileIter it;
   int gi = g0 - 1, t = -1, buf = 0, lut_gi = -1;
   const float2 *stat = nullptr;
+  const int *blind = nullptr;
+  int blind_next = 0;
   float2 st_next = make_float2(INFINITY, 0.f);
   float slope_next = 0.f;
   int doc_next = -1;
@@ -1255,6 +1268,7 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
     int n = gi < g0 ? -1 : it.next();
     while (n < 0 && ++gi < g1) {
       stat = g.stat + ((int64_t)b * a.H + head0 + gi) * a.Lq;
+      blind = g.blind + ((int64_t)b * a.H + head0 + gi) * g.nqt * WAVES;
       dmq.base = qbase + (int64_t)gi * a.q_hs * (int64_t)sizeof(T);
       dmo.base = obase + (int64_t)gi * g.do_hs * (int64_t)sizeof(T);
       if (MOD && a.slopes) slope_next = scalar_load(a.slopes + head0 + gi) * LOG2E;
@@ -1266,6 +1280,7 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
   auto fetch = [&](int tile, int to) {
     dmq.load(lds + to * 2 * L::BYTES, tile * BQ);
     dmo.load(lds + to * 2 * L::BYTES + L::BYTES, tile * BQ);
+    blind_next = blind[tile * (BQ / 32) + (lane & (BQ / 32 - 1))];       // (a lane's own: a scalar load would hold up the reads from LDS)
     if (threadIdx.x < BQ) {
       // (neither waits for the other, or for the tile: rows that are missing or dead are sorted out when the tile is here)
       const int i = min(tile * BQ + (int)threadIdx.x, a.Lq - 1);
@@ -1297,9 +1312,9 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
       lut_gi = cur_gi;
       __syncthreads();
     }
-    if (q0 + BQ > a.Lq || dead) {
-      zero_rows<T, D, BQ, 512>(sQ, a.Lq - q0, sDoc);
-      zero_rows<T, D, BQ, 512>(sO, a.Lq - q0, sDoc);
+    if (q0 + BQ > a.Lq || dead || __any(blind_next)) {
+      zero_blind_rows<T, D, BQ, 512>(sQ, sStat);
+      zero_blind_rows<T, D, BQ, 512>(sO, sStat);
       __syncthreads();
     }
     const int tn = advance(Const<0>());
@@ -1479,6 +1494,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   lut.fill(a, head, bucket);
   float *mine = hist + (int64_t)wave * a.n_buckets * 64 + lane;
   for (int k = 0; k < a.n_buckets; ++k) mine[k * 64] = 0.f;
+  w.live = w.live && rs.x != INFINITY;                    // (a row that sees nothing)
 #pragma unroll
   for (int c = 0; c < NC; ++c) live_frag(fq[c], c, h, a.dh, w.live), live_frag(fd[c], c, h, a.dh, w.live);
   const float lse2 = w.live ? rs.x : INFINITY, delta = w.live ? rs.y : 0.f;

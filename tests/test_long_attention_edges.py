@@ -125,3 +125,48 @@ def test_gradients_that_come_as_lazy_views(dtype):
     assert all(torch.equal(a, b) for a, b in zip(plain, grads(lazy, lazy)))
     assert all(torch.equal(a, b) for a, b in zip(grads(lambda x: x, torch.zeros_like), grads(lambda x: x, zeros)))
     assert all(torch.equal(a, b) for a, b in zip(grads(torch.zeros_like, lambda x: x), grads(zeros, lambda x: x)))
+
+
+# --------------------------------------------------------------------------------------------------------- rows that see nothing
+def _blind(case, dtype, dh):
+    """A case in which some rows see no key: (tensors, masks, plain arguments)."""
+    f = {"cache": dict(cache=True), "docs": dict(docs=[[(0, 60), (1, 140)], [(2, 200)]]), "bias": dict(buckets=8, reach=16, both=True),
+         "table": dict(buckets=8, reach=16, both=True, docs=[[(0, 60), (1, 140)], [(2, 200)]])}[case]
+    t, kw = _case(dtype, 2, 150, 200, 4, 2, dh, seed=81, **f)
+    if case == "cache":                                   # positions before the first key; a cache that holds nothing
+        kw["kv_len"] = torch.tensor([61, 0], dtype=torch.int32, device=DEV)
+    elif case == "bias":                                  # what lies ahead, and the row itself, are hidden: the first row sees nothing
+        t, kw = _case(dtype, 2, 150, 150, 4, 2, dh, seed=81, **f)
+        kw["rel_bias"][:, 4:] = -math.inf
+        kw["rel_bias"][:, 0] = -math.inf
+    else:                                                 # ids without keys, in the middle and at the end of a tile
+        kw["q_doc"][0, 37:90:3] = 77
+        kw["q_doc"][1, 120:] = 78
+    return t, kw, dict(causal=case != "bias", softcap=3.0 if case == "table" else 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf], ids=str)
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("case", ["cache", "docs", "bias", "table"])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_gradients_of_rows_that_see_nothing_reach_nothing(dtype, case, dh, bad):
+    """A row that sees nothing has an output of 0 and a log-sum of -inf whatever the inputs are: gradients that arrive there, such as the
+    -inf of a squared log-sum, count as none."""
+    t, kw, plain = _blind(case, dtype, dh)
+    q, k, v = (t[n].clone().requires_grad_() for n in "qkv")
+    kw = dict(kw)
+    leaves = [q, k, v]
+    if "rel_bias" in kw:
+        leaves.append(kw["rel_bias"].requires_grad_())
+    out, lse = torch_ops.long_attention(q, k, v, return_lse=True, **kw, **plain)
+    none = (lse == -math.inf).transpose(1, 2)
+    assert none.any() and not none.all() and (out[none] == 0).all()
+    dlse = torch.randn(lse.shape, generator=torch.Generator().manual_seed(5)).to(DEV)
+    clean_o, clean_l = t["go"].masked_fill(none[..., None], 0), dlse.masked_fill(none.transpose(1, 2), 0)
+    val, tol = long_rows.attention(t["q"], t["k"], t["v"], dout=clean_o, dlse=clean_l, dtype=dtype, **kw, **plain)
+    for go, dl in ((clean_o, clean_l.masked_fill(none.transpose(1, 2), bad)), (clean_o.masked_fill(none[..., None], bad), clean_l)):
+        got = torch.autograd.grad((out, lse), leaves, (go, dl), retain_graph=True)
+        assert (got[0][none] == 0).all()
+        for name, x in zip(("dq", "dk", "dv", "dbias"), got):
+            _near(x, val[name], tol[name], name)
