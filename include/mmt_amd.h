@@ -606,7 +606,10 @@ int mmt_lane_gather(const double *table, const double *lanes, const int64_t *row
  *   u += -slopes[h] |p - j| + rel_bias[h][rel_buckets[clamp(j - p, -reach, reach) + reach]]
  *   visible: equal ids in q_doc / k_doc, neither negative, and (not causal, or j <= p, or j < prefix[b])
  *   out_i = sum_j softmax(u)_j v_j over the visible keys;  lse_i = log sum exp u.  A row that sees nothing: out 0, lse -inf,
- *   gradients 0, and what arrives as its dout and dlse (which may be inf or NaN) reaches nothing.  An entry of -inf in rel_bias hides its bucket like a mask.
+ *   gradients 0, and what arrives as its dout and dlse (which may be inf or NaN) reaches nothing.
+ *   rel_bias entries count as clamped to -2^14 .. 2^14 (a constant such as -1e9 masks its bucket where another key is visible; a row all
+ *   of whose keys carry it has the softmax of its other terms); an entry at or below -2^100, that is -inf or the lowest value of fp32 or
+ *   bf16, hides its bucket like a mask: a row all of whose keys carry such entries sees nothing.
  * Heads: query head h reads key head h / (H / Hk).  q / k / v rows (head slices) are dh contiguous elements at any batch / token /
  * head stride (elements) that keeps them at multiples of 16 bytes, token strides below 2^25 bytes; a stride of 0 broadcasts.  out (B,Lq,H,dh) and lse (B,H,Lq; may
  * be NULL) contiguous.  Keys at j >= n and keys and queries with a negative id are never multiplied with anything: they may hold

@@ -75,12 +75,13 @@ __device__ __forceinline__ Bounds group_bounds(const Bounds &w, int *s, int wave
   return b;
 }
 
-// The learned bias in LDS, in units of log 2.  Bucket numbers outside the table are clamped into it.  An entry at or below -2^100 (the
-// lowest value of a type, used as a mask) is taken for -inf: next to it a score vanishes in rounding, and the saved log-sum of a row
-// of such entries could not tell them apart.
+// The learned bias in LDS, in units of log 2.  Bucket numbers outside the table are clamped into it.  Entries count as clamped to
+// -2^14 .. 2^14: next to another visible key e^-2^14 is 0 all the same, and of a row all of whose keys carry a mask's constant such as
+// -1e9 fp32 would keep no digit of the scores, nor the log-sum enough to form the probabilities again (gradients 20 times too large at
+// -1e9, 2 % off at -1e6).  At or below -2^100 (-inf, the lowest value of fp32 and bf16) an entry hides its bucket like a mask.
 __device__ __forceinline__ float bias_entry(const mmt_long_attention &a, int head, int bucket) {
   const float v = a.rel_bias[(int64_t)head * a.n_buckets + bucket];
-  return v <= -0x1p100f ? -INFINITY : v * LOG2E;
+  return (v <= -0x1p100f ? -INFINITY : v < -0x1p14f ? -0x1p14f : v > 0x1p14f ? 0x1p14f : v) * LOG2E;      // (NaN stays)
 }
 __device__ __forceinline__ int bias_bucket(const mmt_long_attention &a, int d) {
   return max(0, min(a.rel_buckets[max(-a.reach, min(a.reach, d)) + a.reach], a.n_buckets - 1));

@@ -286,7 +286,8 @@ def long_attention(q, k, v, *, scale=None, causal=False, prefix=None, q_doc=None
     kv_len     (B) int32: keys at and beyond it do not exist       q_doc, k_doc  (B,Lq), (B,Lk) int32: only equal ids see each other;
                                                                              negative: padding, sees and is seen by nothing
     slopes     (H) float32: -slopes[h] * distance is added         rel_bias  (H,n) float32, learned, at rel_buckets (2 reach + 1) int32 of
-                                                                             the clamped distance (``ops.relative_buckets``)
+                                                                             the clamped distance (``ops.relative_buckets``);
+               entries count as clamped to -2^14 .. 2^14, at or below -2^100 (-inf, a type's lowest value) they hide their bucket
     Rows that see nothing give zeros (and an lse of -inf).  Returns out (B,Lq,H,dh), with ``return_lse`` also the log-sums (B,H,Lq)."""
     traced = _traced(q)
     both = None if traced else _plain(_native().plain_long_attention, q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes,

@@ -76,8 +76,10 @@ def attention(q, k, v, scale=None, causal=False, prefix=None, q_doc=None, k_doc=
                 x = x - float(slopes[h]) * apart.abs().double()
                 e = e + 4 * F32 * float(slopes[h]) * apart.abs().double()
             if rel_bias is not None:
-                x = x + rel_bias[h].double()[bucket]
-                e = e + 4 * F32 * rel_bias[h].double().abs()[bucket].clamp_max(1e6)
+                entry = rel_bias[h].double()             # clamped to +-2^14; at or below -2^100: a mask
+                entry = torch.where(entry <= -2.0 ** 100, -math.inf, entry.clamp(-2.0 ** 14, 2.0 ** 14))
+                x = x + entry[bucket]
+                e = e + 4 * F32 * entry.abs()[bucket].clamp_max(2.0 ** 14)
             x = x.masked_fill(~see, -math.inf)
             lse = torch.logsumexp(x, -1) if Lk else torch.full((Lq,), -math.inf, dtype=torch.float64)
             some = lse > -math.inf

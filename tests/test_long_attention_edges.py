@@ -170,3 +170,22 @@ def test_gradients_of_rows_that_see_nothing_reach_nothing(dtype, case, dh, bad):
         assert (got[0][none] == 0).all()
         for name, x in zip(("dq", "dk", "dv", "dbias"), got):
             _near(x, val[name], tol[name], name)
+
+
+# ------------------------------------------------------------------------------------------------- masks' constants in the bias table
+LOWEST = {"-1e4": -1e4, "fp16": -65504.0, "-1e9": -1e9, "-2^99": -2.0 ** 99, "bf16": torch.finfo(BF16).min, "fp32": torch.finfo(F32).min,
+          "-inf": -math.inf, "1e9": 1e9}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 130, 130, 2, 2), (2, 1, 70, 4, 1), (1, 40, 300, 4, 2)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("name", list(LOWEST))
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_mask_constants_in_the_bias_table(dtype, name, shape):
+    """The constants that serve as masks, in some buckets and in all of a head's: buckets they hide next to other keys, rows that see
+    nothing else (the first token of a causal row, whose own bucket is masked; a head with all buckets masked)."""
+    t, kw = _case(dtype, *shape, 64, seed=4, buckets=8, reach=16)
+    kw["rel_bias"][0, 0] = kw["rel_bias"][0, 3] = LOWEST[name]
+    kw["rel_bias"][1, :] = LOWEST[name]
+    _check(t, kw, dtype, causal=True)
+    _check(t, kw, dtype, causal=True, softcap=5.0)
