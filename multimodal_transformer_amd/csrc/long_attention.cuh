@@ -189,7 +189,8 @@ __device__ __forceinline__ unsigned lds_address(const void *p) {
 
 // Tiles of a (rows, dh) matrix on their way to LDS.  A lane's byte offset inside a tile is the same for every tile; the tile's own
 // part is a scalar.  Slots at and beyond dh repeat slot 0 and rows at and beyond n_rows the last row (nothing outside the tensor is
-// read); the operands these elements meet are zero, or results nobody stores.
+// read); their results are masked or nobody stores them, but for row operands, where the slots beyond dh meet zeros (0 x inf is not 0):
+// `clear_pads` makes them zero.
 // NT threads (the workgroup, or one wave) move tiles of R rows, NT / NS rows at a time; where the exclusive or of a row repeats after
 // as many rows, the steps differ by a scalar and one offset serves them all.
 template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS> struct Dma {
@@ -225,6 +226,24 @@ template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS> struct Dm
       }
     }
   }
+  // The tile's own requests have arrived (dma_wait): each lane clears those of its pieces that lie beyond dh, ahead of the barrier that
+  // publishes the tile.
+  static __device__ __forceinline__ void clear_pads(char *tile, int dh) {
+    const int tid = rare_tid() % NT;
+    auto beyond = [&](int idx) {
+      const int d = L::swz(idx / L::NS, idx % L::NS) * L::EPS;
+      return d >= dh && d < D;
+    };
+    if constexpr (ONE) {
+      if (!beyond(tid)) return;
+#pragma unroll
+      for (int n = 0; n < N; ++n) *(u32x4 *)(tile + (tid + n * NT) * 16) = u32x4{};
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (beyond(tid + n * NT)) *(u32x4 *)(tile + (tid + n * NT) * 16) = u32x4{};
+    }
+  }
 };
 
 // Rows of a tile that must not take part become zeros (whatever they hold: 0 x NaN would reach every other row): at and beyond `end`
@@ -237,18 +256,6 @@ __device__ __forceinline__ void zero_rows(char *lds, int end, const int *doc) {
   for (int n = 0; n < R * L::NS / NT; ++n) {
     const int idx = tid + n * NT, row = idx / L::NS;
     if (row >= end || (doc && doc[row] < 0)) *(u32x4 *)(lds + idx * 16) = u32x4{};
-  }
-}
-
-// The same for rows of queries, by their log-sums (+inf: missing, padding, or a row that sees nothing)
-template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS>
-__device__ __forceinline__ void zero_blind_rows(char *lds, const float *lse) {
-  typedef Tile<T, D> L;
-  const int tid = rare_tid() % NT;
-#pragma unroll
-  for (int n = 0; n < R * L::NS / NT; ++n) {
-    const int idx = tid + n * NT;
-    if (lse[idx / L::NS] == INFINITY) *(u32x4 *)(lds + idx * 16) = u32x4{};
   }
 }
 

@@ -342,7 +342,7 @@ __device__ __forceinline__ void fwd_store(const Args &g, const FwdState<T, D> &s
 // between the matrix instructions (40 and 24 %) at the two waves per SIMD that the registers allow; LDS is at 32 and 21 %, without bank
 // conflicts.
 // TEAMS = 2: eight waves, two per 32 rows, which deal the key tiles among themselves and join at the end (rule and figures at teams()).
-template <typename T, int D, bool MOD, int TEAMS>
+template <typename T, int D, bool GAPS, bool MOD, int TEAMS>
 __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_fwd_kernel(const Args g) {
   typedef Tile<T, D> L;
   typedef typename Elem<T>::V8 V8;
@@ -409,6 +409,7 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
     int *sDoc = sDoc2 + (TEAMS == 1 ? buf : team * 2 + buf) * BK;
     if (kdoc && wave == 0 && lane < BK) sDoc[lane] = ids;
     dma_wait<0>();
+    if constexpr (GAPS) dk.clear_pads(sK, a.dh);
     __syncthreads();                                     // the tile is here, and nobody reads the other buffer any more
     if (any_zero) {                                      // (a key row only reaches scores that are masked: V alone)
       if (zero) zero_rows<T, D>(sV, len - k0, mixed ? sDoc : nullptr);
@@ -519,6 +520,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     const Place at = place(a, k0 - wb.p_max, k0 + BK - 1 - wb.p_min);
     // requests complete in order: all but the newest tile (the values asked for after these keys, the keys asked for after these values)
     dma_wait<dv.N>();
+    if (a.dh < D) dk.clear_pads(sK, a.dh);
     float x[16];
     fwd_products<T, D, 1>(x, fq, sK, lane);
     wave_sync();                                          // the keys have been read
@@ -714,7 +716,7 @@ __device__ __forceinline__ float score_grad_scale(const f32x4 *maxima, int parts
 // Bound like the forward: 515 us for its causal case of 8192 tokens (800 TFLOP/s), 86 us for the one of 2048.
 // With a learned bias the kernel also sums dU over the tiles that lie wholly beyond the reach on either side.
 constexpr int TWICE = 8;
-template <typename T, int D, bool MOD, int TEAMS>
+template <typename T, int D, bool GAPS, bool MOD, int TEAMS>
 __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_dq_kernel(const Args g) {
   typedef Tile<T, D> L;
   typedef typename Elem<T>::V8 V8;
@@ -806,6 +808,7 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
       int *sDoc = sDoc2 + (TEAMS == 1 ? buf : team * 2 + buf) * BK;
       if (kdoc && wave == 0 && lane < BK) sDoc[lane] = ids;
       dma_wait<0>();
+      if constexpr (GAPS) dk.clear_pads(sK, a.dh), dv.clear_pads(sV, a.dh);
       __syncthreads();
       if (any_zero) {
         if (zero) {
@@ -961,7 +964,7 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
 // per SIMD (8192 causal tokens x 16 heads: 1380 us, the next kernel's 715).  Up to 64 this one is: bf16
 // 2 x 2048 x 16 heads of 64 98 us, the next one 129; 2 x 4096 tokens in packed scenes 85, the next one 98.  Bound by vector instructions
 // and the latency between them, at two waves per SIMD: 700 TFLOP/s in the first case.
-template <typename T, int D, bool MOD>
+template <typename T, int D, bool GAPS, bool MOD>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_dkv_kernel(const Args g) {
   typedef Tile<T, D> L;
   typedef typename Elem<T>::V8 V8;
@@ -1068,24 +1071,27 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     char *sQ = smem + buf * 2 * L::BYTES, *sO = sQ + L::BYTES;
     float *sStat = sStat2 + buf * 2 * BQ;
     int *sDoc = sDoc2 + buf * BQ;
-    const bool mixed = it.mixed(), dead = it.cur_dead != 0;
+    const bool docs = it.mixed(), dead = it.cur_dead != 0;
     const int cur_gi = gi;
     const float slope = slope_next;
     if (threadIdx.x < BQ) {
-      const int doc = q0 + (int)threadIdx.x < a.Lq ? doc_next : -1;
+      const int doc = q0 + (int)threadIdx.x < a.Lq && st_next.x != INFINITY ? doc_next : -1;      // negative: takes no part
       sDoc[threadIdx.x] = doc;
       sStat[threadIdx.x] = doc >= 0 ? st_next.x : INFINITY, sStat[BQ + threadIdx.x] = doc >= 0 ? st_next.y : 0.f;
     }
     dma_wait<0>();
+    if constexpr (GAPS) dmq.clear_pads(sQ, a.dh), dmo.clear_pads(sO, a.dh);
     __syncthreads();
     if (MOD && a.rel_bias && lut_gi != cur_gi) {          // another head's bias
       lut.fill(a, head);
       lut_gi = cur_gi;
       __syncthreads();
     }
-    if (q0 + BQ > a.Lq || dead || __any(blind_next)) {
-      zero_blind_rows<T, D>(sQ, sStat);
-      zero_blind_rows<T, D>(sO, sStat);
+    // where not all rows take part, those that do not are cleared and masked (a cleared row's product with an infinite key is NaN)
+    const bool part = q0 + BQ > a.Lq || dead || __any(blind_next), mixed = docs || part;
+    if (part) {
+      zero_rows<T, D>(sQ, BQ, sDoc);
+      zero_rows<T, D>(sO, BQ, sDoc);
       __syncthreads();
     }
     const int tn = advance(Const<0>());
@@ -1189,7 +1195,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
 // 8192 causal tokens x 16 heads of 128 over 4: 715 us, 770 TFLOP/s for the four products.  About 290 KiB go through LDS per tile, half of
 // the time of its matrix instructions (LDS 41 % of the cycles, matrix 37 %, vector 30 %); bound by the steps' order: two barriers per
 // tile, one workgroup per CU, and its waves wait for 47 % of the time.
-template <typename T, int D, bool MOD>
+template <typename T, int D, bool GAPS, bool MOD>
 __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g) {
   typedef Tile<T, D> L;
   typedef typename Elem<T>::V8 V8;
@@ -1299,23 +1305,26 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
     char *sQ = smem + buf * 2 * L::BYTES, *sO = sQ + L::BYTES;
     float *sStat = sStat2 + buf * 2 * BQ;
     int *sDoc = sDoc2 + buf * BQ;
-    const bool mixed = it.mixed(), dead = it.cur_dead != 0;
+    const bool docs = it.mixed(), dead = it.cur_dead != 0;
     const float slope = slope_next;
     if (threadIdx.x < BQ) {
-      const int doc = q0 + (int)threadIdx.x < a.Lq ? doc_next : -1;
+      const int doc = q0 + (int)threadIdx.x < a.Lq && st_next.x != INFINITY ? doc_next : -1;      // negative: takes no part
       sDoc[threadIdx.x] = doc;
       sStat[threadIdx.x] = doc >= 0 ? st_next.x : INFINITY, sStat[BQ + threadIdx.x] = doc >= 0 ? st_next.y : 0.f;
     }
     dma_wait<0>();
+    if constexpr (GAPS) dmq.clear_pads(sQ, a.dh), dmo.clear_pads(sO, a.dh);
     __syncthreads();                                      // the tile is here; the last one's second step is done everywhere
     if (MOD && a.rel_bias && lut_gi != cur_gi) {          // another head's bias
       lut.fill<512>(a, head);
       lut_gi = cur_gi;
       __syncthreads();
     }
-    if (q0 + BQ > a.Lq || dead || __any(blind_next)) {
-      zero_blind_rows<T, D, BQ, 512>(sQ, sStat);
-      zero_blind_rows<T, D, BQ, 512>(sO, sStat);
+    // where not all rows take part, those that do not are cleared and masked (a cleared row's product with an infinite key is NaN)
+    const bool part = q0 + BQ > a.Lq || dead || __any(blind_next), mixed = docs || part;
+    if (part) {
+      zero_rows<T, D, BQ, 512>(sQ, BQ, sDoc);
+      zero_rows<T, D, BQ, 512>(sO, BQ, sDoc);
       __syncthreads();
     }
     const int tn = advance(Const<0>());
@@ -1498,11 +1507,13 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   w.live = w.live && rs.x != INFINITY;                    // (a row that sees nothing)
 #pragma unroll
   for (int c = 0; c < NC; ++c) live_frag(fq[c], c, h, a.dh, w.live), live_frag(fd[c], c, h, a.dh, w.live);
+  if (!w.live) w.hi = 0;                                  // (every score masked: a cleared row's product with an infinite key is NaN)
   const float lse2 = w.live ? rs.x : INFINITY, delta = w.live ? rs.y : 0.f;
   settle(w.slope), settle(w.doc), settle(norm);
   while (t < t1) {
     const int k0 = t * BK;
     dma_wait<0>();
+    if (a.dh < D) dk.clear_pads(sK, a.dh), dv.clear_pads(sV, a.dh);
     __syncthreads();
     if (k0 + BK > len || kdoc) {
       zero_rows<T, D>(sK, len - k0, kdoc ? ids : nullptr);
@@ -1589,7 +1600,7 @@ template <typename K> static void launch(K kernel, int64_t grid, size_t lds, hip
 
 static inline bool modified(const mmt_long_attention &a) { return a.softcap > 0.f || a.slopes || a.rel_bias; }
 
-template <typename T, int D> static void fwd_size(const Args &g, hipStream_t st) {
+template <typename T, int D, bool GAPS> static void fwd_size(const Args &g, hipStream_t st) {
   if (g.few) {
     const size_t tiles = 2 * WAVES * 32 * Tile<T, D>::NS * 16 + 4 * 32 * WAVES + PackedBias::bytes(g.a, g.pack);
     const size_t join = 4 * 64 * WAVES * (2 + D / 2), lds = tiles > join ? tiles : join;
@@ -1600,32 +1611,32 @@ template <typename T, int D> static void fwd_size(const Args &g, hipStream_t st)
   const size_t tiles = 4 * Tile<T, D>::BYTES + 8 * Tile<T, D>::BK, rest = 24 * WAVES + 4 * Lut::floats(g.a);
   if constexpr (sizeof(T) == 2) {
     if (g.teams == 2) {
-      if (modified(g.a)) launch(mmt_long_attn_fwd_kernel<T, D, true, 2>, g.items, 2 * tiles + rest, st, g, 2 * THREADS);
-      else launch(mmt_long_attn_fwd_kernel<T, D, false, 2>, g.items, 2 * tiles + rest, st, g, 2 * THREADS);
+      if (modified(g.a)) launch(mmt_long_attn_fwd_kernel<T, D, GAPS, true, 2>, g.items, 2 * tiles + rest, st, g, 2 * THREADS);
+      else launch(mmt_long_attn_fwd_kernel<T, D, GAPS, false, 2>, g.items, 2 * tiles + rest, st, g, 2 * THREADS);
       return;
     }
   }
-  if (modified(g.a)) launch(mmt_long_attn_fwd_kernel<T, D, true, 1>, g.items, tiles + rest, st, g);
-  else launch(mmt_long_attn_fwd_kernel<T, D, false, 1>, g.items, tiles + rest, st, g);
+  if (modified(g.a)) launch(mmt_long_attn_fwd_kernel<T, D, GAPS, true, 1>, g.items, tiles + rest, st, g);
+  else launch(mmt_long_attn_fwd_kernel<T, D, GAPS, false, 1>, g.items, tiles + rest, st, g);
 }
 
-template <typename T, int D, int TEAMS> static void dq_launch(const Args &g, int64_t items, hipStream_t st) {
+template <typename T, int D, bool GAPS, int TEAMS> static void dq_launch(const Args &g, int64_t items, hipStream_t st) {
   const size_t lds = TEAMS * (4 * Tile<T, D>::BYTES + 8 * Tile<T, D>::BK) + 24 * WAVES + 4 * Lut::floats(g.a);
-  if (modified(g.a)) launch(mmt_long_attn_dq_kernel<T, D, true, TEAMS>, items, lds, st, g, TEAMS * THREADS);
-  else launch(mmt_long_attn_dq_kernel<T, D, false, TEAMS>, items, lds, st, g, TEAMS * THREADS);
+  if (modified(g.a)) launch(mmt_long_attn_dq_kernel<T, D, GAPS, true, TEAMS>, items, lds, st, g, TEAMS * THREADS);
+  else launch(mmt_long_attn_dq_kernel<T, D, GAPS, false, TEAMS>, items, lds, st, g, TEAMS * THREADS);
 }
 
-template <typename T, int D> static void bwd_size(Args &g, hipStream_t st, float *table_part, float *dtable) {
+template <typename T, int D, bool GAPS> static void bwd_size(Args &g, hipStream_t st, float *table_part, float *dtable) {
   typedef Tile<T, D> L;
   const mmt_long_attention &a = g.a;
   const bool mod = modified(a);
   const size_t small = 24 * WAVES;
   const int64_t qitems = (int64_t)a.B * a.H * g.nqt;
   if constexpr (sizeof(T) == 2) {
-    if (g.teams == 2) dq_launch<T, D, 2>(g, qitems, st);
-    else dq_launch<T, D, 1>(g, qitems, st);
+    if (g.teams == 2) dq_launch<T, D, GAPS, 2>(g, qitems, st);
+    else dq_launch<T, D, GAPS, 1>(g, qitems, st);
   } else {
-    dq_launch<T, D, 1>(g, qitems, st);
+    dq_launch<T, D, GAPS, 1>(g, qitems, st);
   }
   if (a.rel_bias) {
     const size_t lds = 2 * L::BYTES + 8 * L::BK + small + 4 * Lut::floats(a) + ((Lut::floats(a) + 15) & ~15) + (size_t)WAVES * a.n_buckets * 256;
@@ -1638,11 +1649,11 @@ template <typename T, int D> static void bwd_size(Args &g, hipStream_t st, float
   const int64_t kitems = (int64_t)g.groups * ((a.Lk + ROWS - 1) / ROWS) * g.zh * g.zq;
   if constexpr (sizeof(T) == 2 && D > 64) {
     const size_t lds2 = 4 * L::BYTES + 2 * 128 * 64 * 2 + 24 * 64 + 64 + 4 * Lut::floats(a);
-    if (mod) launch(mmt_long_attn_dkv2_kernel<T, D, true>, kitems, lds2, st, g, 512);
-    else launch(mmt_long_attn_dkv2_kernel<T, D, false>, kitems, lds2, st, g, 512);
+    if (mod) launch(mmt_long_attn_dkv2_kernel<T, D, GAPS, true>, kitems, lds2, st, g, 512);
+    else launch(mmt_long_attn_dkv2_kernel<T, D, GAPS, false>, kitems, lds2, st, g, 512);
   } else {
-    if (mod) launch(mmt_long_attn_dkv_kernel<T, D, true>, kitems, lds_k, st, g);
-    else launch(mmt_long_attn_dkv_kernel<T, D, false>, kitems, lds_k, st, g);
+    if (mod) launch(mmt_long_attn_dkv_kernel<T, D, GAPS, true>, kitems, lds_k, st, g);
+    else launch(mmt_long_attn_dkv_kernel<T, D, GAPS, false>, kitems, lds_k, st, g);
   }
 }
 
@@ -1651,13 +1662,23 @@ template <typename T> static void docs(const Args &g, DocRange *out, bool querie
   hipLaunchKernelGGL(mmt_long_attn_docs_kernel<T>, dim3((total + 3) / 4), dim3(256), 0, st, g, bk, nk, total, out);
 }
 
+// The instantiation of a head size: the next of 32, 64, 96, 128, and whether it leaves slots empty that have to be cleared (as a question
+// of every step this cost the kernels 2 to 4 % at the head sizes that leave none)
+template <typename F> static void by_size(int dh, F f) {
+  if (dh < 32) f(Const<32>(), Const<1>());
+  else if (dh == 32) f(Const<32>(), Const<0>());
+  else if (dh < 64) f(Const<64>(), Const<1>());
+  else if (dh == 64) f(Const<64>(), Const<0>());
+  else if (dh < 96) f(Const<96>(), Const<1>());
+  else if (dh == 96) f(Const<96>(), Const<0>());
+  else if (dh < 128) f(Const<128>(), Const<1>());
+  else f(Const<128>(), Const<0>());
+}
+
 template <typename T> void forward(Args &g, DocRange *ranges, hipStream_t st) {
   const mmt_long_attention &a = g.a;
   if (ranges && !g.few) docs<T>(g, ranges, false, st), g.krng = ranges;
-  if (a.dh <= 32) fwd_size<T, 32>(g, st);
-  else if (a.dh <= 64) fwd_size<T, 64>(g, st);
-  else if (a.dh <= 96) fwd_size<T, 96>(g, st);
-  else fwd_size<T, 128>(g, st);
+  by_size(a.dh, [&](auto size, auto gaps) { fwd_size<T, decltype(size)::value, decltype(gaps)::value != 0>(g, st); });
   if (g.nsplit > 1) {
     const int64_t rows = (int64_t)a.B * a.H * a.Lq;
     hipLaunchKernelGGL(mmt_long_attn_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, g);
@@ -1674,10 +1695,7 @@ template <typename T> void backward(Args &g, DocRange *ranges, f32x4 *maxima, fl
     g.dscale = (float *)(maxima + STAT_PARTS);
     hipLaunchKernelGGL(mmt_long_attn_maxima_kernel<T>, dim3(g.stat_parts), dim3(STAT_THREADS), 0, st, g, maxima);
   }
-  if (a.dh <= 32) bwd_size<T, 32>(g, st, table_part, dtable);
-  else if (a.dh <= 64) bwd_size<T, 64>(g, st, table_part, dtable);
-  else if (a.dh <= 96) bwd_size<T, 96>(g, st, table_part, dtable);
-  else bwd_size<T, 128>(g, st, table_part, dtable);
+  by_size(a.dh, [&](auto size, auto gaps) { bwd_size<T, decltype(size)::value, decltype(gaps)::value != 0>(g, st, table_part, dtable); });
   if (g.part_dk) {
     const int64_t n = (int64_t)a.B * a.Lk * a.Hk * a.dh;
     hipLaunchKernelGGL(mmt_long_attn_dkv_sum_kernel<T>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, g);

@@ -189,3 +189,25 @@ def test_mask_constants_in_the_bias_table(dtype, name, shape):
     kw["rel_bias"][1, :] = LOWEST[name]
     _check(t, kw, dtype, causal=True)
     _check(t, kw, dtype, causal=True, softcap=5.0)
+
+
+# ------------------------------------------------------------------------------------------- head sizes inside a tile's padded one
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", [False, True], ids=["plain", "bias"])
+@pytest.mark.parametrize("shape", [(1, 1, 70, 2, 1), (2, 21, 21, 4, 2), (1, 150, 200, 2, 1), (1, 130, 600, 2, 2)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dh", [8, 24, 32, 40, 56, 72, 80, 88, 104, 120, 128])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_infinite_keys_at_every_head_size(dtype, dh, shape, bias):
+    """A key with an infinite element whose products are -inf weighs nothing, forward and in every gradient but the infinite element's
+    own, at head sizes that fill a tile and at those that do not."""
+    B, Lq, Lk, H, Hk = shape
+    t, kw = _case(dtype, B, Lq, Lk, H, Hk, dh, seed=dh, **(dict(buckets=8, reach=20) if bias else {}))
+    t["q"][..., 3] = t["q"][..., 3].abs() + 0.25
+    t["k"][:, 5, :, 3] = -math.inf
+    t["k"][:, Lk - 2, 0, 3] = -math.inf
+    got = _run(t, kw, causal=bias)
+    val, tol = long_rows.attention(t["q"], t["k"], t["v"], dout=t["go"], dtype=dtype, causal=bias, **kw)
+    others = [d for d in range(dh) if d != 3]
+    got[2], val["dq"], tol["dq"] = (x[..., others] for x in (got[2], val["dq"], tol["dq"]))
+    for name, x in zip(("out", "lse", "dq", "dk", "dv", "dbias"), got):
+        _near(x, val[name], tol[name], name)
