@@ -89,7 +89,7 @@ bool side(const Maybe &t, const Tensor &q, at::ScalarType type, at::IntArrayRef 
 }
 template <typename T> const T *address(const Maybe &t) { return t ? (const T *)t->const_data_ptr() : nullptr; }
 
-// what these nodes do not support has to be an error, as with any other function of torch that does not
+// what these nodes do not support, of constants either, has to be an error, as with any other function of torch that does not
 void supported(std::initializer_list<Tensor> inputs) {
   const auto &functorch = at::functorch::functorchTLSAccessor();
   if (functorch) functorch->checkSupportsCppAutogradFunction();
@@ -166,7 +166,7 @@ std::tuple<Tensor, Tensor> long_attention(uintptr_t args, const Tensor &q, const
                                           const Maybe &k_doc, const Maybe &kv_len, const Maybe &slopes, const Maybe &rel_bias, const Maybe &rel_buckets) {
   const mmt_long_attention &a = *(const mmt_long_attention *)args;
   const Tensor table = rel_bias.value_or(Tensor());
-  supported({q, k, v, table});
+  supported({q, k, v, table, slopes.value_or(Tensor())});
   const bool wanted = torch::autograd::compute_requires_grad(q, k, v, table);
   c10::DeviceGuard device(q.device());
   Tensor out, lse, low;
@@ -274,7 +274,7 @@ struct MmtQkNormRopeBackward : public Node {
 std::tuple<Tensor, Tensor> qk_norm_rope(uintptr_t args, const Tensor &q, const Tensor &k, const Tensor &q_weight, const Tensor &k_weight,
                                         const Tensor &inv_freq, const Maybe &positions) {
   const mmt_qk_norm_rope &a = *(const mmt_qk_norm_rope *)args;
-  supported({q, k, q_weight, k_weight});
+  supported({q, k, q_weight, k_weight, inv_freq});
   const bool wanted = torch::autograd::compute_requires_grad(q, k, q_weight, k_weight);
   c10::DeviceGuard device(q.device());
   Tensor qo, ko;

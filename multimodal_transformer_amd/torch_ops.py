@@ -14,6 +14,7 @@ import ctypes
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 from ._lib import MmtError, native as _native
@@ -110,11 +111,22 @@ def _ade_fde(pred, gt):
 
 
 # ---- attention over long rows, norm + rotation: differentiable ------------------------------------------------------------------
+def _no_tangents(fn):
+    """An operator without forward-mode gradients: a tangent that arrives is an error, it would vanish."""
+    def call(*args):
+        if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in args):
+            raise MmtError("forward-mode gradients are not supported")
+        return fn(*args)
+    return call
+
+
+@_no_tangents
 def _long_attention(*args):
     out, lse, low = ops.long_attention(*args, keep_low=True)
     return out, lse, low if low is not None else out.new_empty(0)
 
 
+@_no_tangents
 def _long_attention_bwd(*args):
     dq, dk, dv, dbias = ops.long_attention_backward(*args)
     return dq, dk, dv, dbias if dbias is not None else dq.new_empty(0, dtype=torch.float32)
@@ -142,8 +154,8 @@ def _qk_norm_rope_bwd_meta(dqo, dko, q, k, q_weight, k_weight, *rest):
 for _name, _fn, _meta in (
         ("long_attention", _long_attention, _long_attention_meta),
         ("long_attention_bwd", _long_attention_bwd, _long_attention_bwd_meta),
-        ("qk_norm_rope", ops.qk_norm_rope, _qk_norm_rope_meta),
-        ("qk_norm_rope_bwd", ops.qk_norm_rope_backward, _qk_norm_rope_bwd_meta),
+        ("qk_norm_rope", _no_tangents(ops.qk_norm_rope), _qk_norm_rope_meta),
+        ("qk_norm_rope_bwd", _no_tangents(ops.qk_norm_rope_backward), _qk_norm_rope_bwd_meta),
         ("encoder_fwd", _encoder_fwd, _encoder_fwd_meta),
         ("decoder_ar_fwd", _decoder_ar_fwd, _decoder_ar_fwd_meta),
         ("decoder_tf_fwd", _decoder_tf_fwd, _decoder_tf_fwd_meta),

@@ -211,3 +211,32 @@ def test_infinite_keys_at_every_head_size(dtype, dh, shape, bias):
     got[2], val["dq"], tol["dq"] = (x[..., others] for x in (got[2], val["dq"], tol["dq"]))
     for name, x in zip(("out", "lse", "dq", "dk", "dv", "dbias"), got):
         _near(x, val[name], tol[name], name)
+
+
+# --------------------------------------------------------------------------------------------------------------- forward mode
+def test_a_tangent_under_the_dispatcher_is_refused():
+    """Below autograd the dispatcher's op still sees the tangent of an argument: an error, whatever else is wrong with the call."""
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(torch.ones(1, 2, 2, 8), torch.ones(1, 2, 2, 8))
+        for fn in (torch_ops._long_attention, torch_ops._long_attention_bwd):
+            with pytest.raises(MmtError, match="forward-mode"):
+                fn(dual, dual, dual)
+
+
+@pytest.mark.gpu
+def test_tangents_of_constants_are_refused():
+    """Forward-mode gradients are not supported, of the constants as little as of q, k and v: an error, not a tangent that vanishes."""
+    t, kw = _case(F32, 1, 20, 20, 2, 2, 32, seed=91, slopes=True)
+    w, f = torch.ones(32, device=DEV), ops.rotary_frequencies(32, device=DEV)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda x: torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for fn in (lambda: torch_ops.long_attention(t["q"], t["k"], t["v"], slopes=dual(kw["slopes"])),
+                   lambda: torch_ops.long_attention(t["q"].transpose(2, 3).contiguous().transpose(2, 3), t["k"], t["v"], slopes=dual(kw["slopes"])),
+                   lambda: torch_ops.qk_norm_rope(t["q"], t["k"], w, w, dual(f)),
+                   lambda: torch_ops.qk_norm_rope(t["q"], t["k"], dual(w), w, f),
+                   lambda: torch.ops.mmt.qk_norm_rope(t["q"], t["k"], w, w, dual(f), None, 1e-6, False),
+                   lambda: torch.ops.mmt.long_attention(dual(t["q"]), t["k"], t["v"], None, False, None, None, None, None, 0.0, None, None, None),
+                   lambda: torch.ops.mmt.long_attention(t["q"], t["k"], t["v"], None, False, None, None, None, None, 0.0, dual(kw["slopes"]),
+                                                        None, None)):
+            with pytest.raises((MmtError, RuntimeError)):
+                fn()
