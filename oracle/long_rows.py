@@ -47,6 +47,14 @@ def attention(q, k, v, scale=None, causal=False, prefix=None, q_doc=None, k_doc=
     cpu = lambda t: None if t is None else t.detach().cpu()
     prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets = map(cpu, (prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets))
     j = torch.arange(Lk)
+    if back and dtype == torch.float16:
+        # What bounds the score gradients of the whole call: the largest |dout|, |v| and |dlse| of live rows and keys.  They are scaled by the
+        # power of two that takes 2 max|dout| max|v| + max|dlse| into (2^14, 2^15]; the smallest step is then 2^-24.
+        lens = torch.full((B, 1), Lk) if kv_len is None else kv_len.long().clamp(0, Lk)[:, None]
+        live_q = torch.ones(B, Lq, dtype=torch.bool) if q_doc is None else q_doc >= 0
+        live_k = (j[None] < lens) & (True if k_doc is None else k_doc >= 0)
+        most = lambda rows, live: float(torch.where(live & torch.isfinite(rows), rows, torch.zeros((), dtype=torch.float64)).max()) if rows.numel() else 0.0
+        glob = 2 * most(do.norm(dim=-1), live_q[..., None]) * most(v.norm(dim=-1), live_k[..., None]) + most(dl.abs(), live_q[:, None])
     for b in range(B):
         n = Lk if kv_len is None else max(0, min(int(kv_len[b]), Lk))
         p = n - Lq + torch.arange(Lq)
@@ -110,12 +118,9 @@ def attention(q, k, v, scale=None, causal=False, prefix=None, q_doc=None, k_doc=
                 slope = 1 - t * t
                 dS = dU * slope
                 eS = eU * slope + dU.abs() * (2 * t.abs() * e / softcap + 8 * F32)
-            # fp16: score gradients are scaled by a power of two 2^s with bound * 2^s in (2^14, 2^15], their smallest step is 2^-24
-            bound = 2 * float(D.norm(dim=-1).max()) * float(V.norm(dim=-1).max()) + float(dl_row.abs().max()) if Lq and Lk else 0.0
             e_in = eS + up * (dS.abs() + eS)
             if dtype == torch.float16:
-                glob = 2 * float(torch.nan_to_num(do).norm(dim=-1).max()) * float(torch.nan_to_num(v).norm(dim=-1).max()) + float(dl.abs().max())
-                e_in = e_in + torch.where(P > 0, 2.0 ** -38 * max(glob, bound), 0.0)
+                e_in = e_in + torch.where(P > 0, 2.0 ** -38 * glob, 0.0)
             val["dq"][b, :, h] = scale * (dS @ K)
             w = scale * (e_in + n32 * dS.abs())
             tol["dq"][b, :, h] = w @ K.abs()
@@ -135,6 +140,8 @@ def attention(q, k, v, scale=None, causal=False, prefix=None, q_doc=None, k_doc=
             tol[name] = tol[name] + u * (val[name].abs() + tol[name]) + fl
         if rel_bias is not None:
             tol["dbias"] = tol["dbias"] + F32 * val["dbias"].abs()
+    for name in val:
+        assert not (torch.isfinite(val[name]) & ~torch.isfinite(tol[name])).any(), f"the bound on {name} would pass anything"
     return val, tol
 
 

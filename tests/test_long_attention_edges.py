@@ -240,3 +240,34 @@ def test_tangents_of_constants_are_refused():
                                                         None, None)):
             with pytest.raises((MmtError, RuntimeError)):
                 fn()
+
+
+# ------------------------------------------------------------------------------------------------------------- the bounds themselves
+@pytest.mark.parametrize("bad", [0.0, math.nan, math.inf, -math.inf], ids=str)
+@pytest.mark.parametrize("cache", [False, True], ids=["docs", "cache"])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_the_bounds_do_not_depend_on_what_padding_holds(dtype, cache, bad):
+    """The oracle's bounds with anything in padding and behind the cache's end: those of zeros there, and finite."""
+    g = torch.Generator().manual_seed(8)
+    q, k, v, go = (torch.randn(2, 60, n, 16, generator=g).to(dtype) for n in (4, 2, 2, 4))
+    if cache:
+        kw = dict(kv_len=torch.tensor([60, 33], dtype=torch.int32))
+        dead, dead_q = torch.arange(60)[None] >= kw["kv_len"][:, None], torch.zeros(2, 60, dtype=torch.bool)
+    else:
+        ids = torch.tensor([[0] * 30 + [-1] * 9 + [1] * 21, [-1] * 3 + [2] * 50 + [-1] * 7], dtype=torch.int32)
+        kw = dict(q_doc=ids, k_doc=ids)
+        dead = dead_q = ids < 0
+    res = []
+    for hold in (0.0, bad):
+        k[dead], v[dead] = hold, hold
+        q[dead_q], go[dead_q] = hold, hold
+        res.append(long_rows.attention(q, k, v, dout=go, causal=True, dtype=dtype, **kw))
+    for name, x in res[0][1].items():
+        assert torch.isfinite(x).all(), name
+        assert torch.equal(x, res[1][1][name]), name
+
+
+def test_a_bound_that_would_pass_anything_is_an_error():
+    x = torch.rand(1, 3, 1, 8) + 0.5
+    with pytest.raises(AssertionError, match="bound"):
+        long_rows.attention(x, torch.full_like(x, math.inf), x, softcap=1.0, dtype=F32)
