@@ -271,3 +271,73 @@ def test_a_bound_that_would_pass_anything_is_an_error():
     x = torch.rand(1, 3, 1, 8) + 0.5
     with pytest.raises(AssertionError, match="bound"):
         long_rows.attention(x, torch.full_like(x, math.inf), x, softcap=1.0, dtype=F32)
+
+
+# ------------------------------------------------------------------------------------- precision of the rows' correction (delta)
+def _rounded_gradients(q, k, v, go, dtype, causal, delta):
+    """dq and dk in 64 bits but for the roundings that the backward makes: of P and dS to the element type where they enter a product, and
+    of the results.  ``delta`` = rowsum(dO o) comes from o itself ("exact"), from the rounded output and what its rounding took ("low": P was
+    rounded on its way there), or from the rounded output alone ("out")."""
+    scale = q.shape[-1] ** -0.5
+    # powers of two ahead of the roundings keep fp16's exponent range out of this
+    rnd = lambda x: ((x * (up := 2.0 ** (14 - math.ceil(math.log2(float(x.abs().max())))))).to(dtype).double() / up)
+    heads = lambda x: x.double().transpose(1, 2)
+    Q, K, V, D = map(heads, (q, k, v, go))
+    s = scale * Q @ K.transpose(2, 3)
+    if causal:
+        s = s.masked_fill(~torch.ones(s.shape[-2:], dtype=torch.bool).tril(), -math.inf)
+    P = s.softmax(-1)
+    out = P @ V if delta == "exact" else rnd(P) @ V
+    if delta != "exact":
+        kept = out.to(dtype).double()
+        out = kept + (out - kept).to(dtype).double() if delta == "low" else kept
+    dS = rnd(P * (D @ V.transpose(2, 3) - (D * out).sum(-1, keepdim=True)))
+    return (scale * dS @ K).transpose(1, 2), (scale * dS.transpose(2, 3) @ Q).transpose(1, 2)
+
+
+def _offset_case(dtype, L, H=2, dh=64):
+    """Values around a common offset: all of a row's dP lie near delta, of which little may be lost."""
+    g = torch.Generator().manual_seed(L)
+    q, k, v, go = (torch.randn(1, L, H, dh, generator=g) for _ in range(4))
+    return [x.to(dtype) for x in (q, k, 4 + v / 4, go)]
+
+
+def _off(x, y):
+    return float((x.double().cpu() - y).norm() / y.norm())
+
+
+# (length, causal): up to 512 keys every row of dQ sees its corrected delta, beyond that the one from the output and its low part; dK always
+# the corrected one.  Bound: twice what the roundings of P and dS alone do, which the next worse delta exceeds.
+PRECISION = [(140, True, "exact", "low"), (400, True, "exact", "low"), (2304, False, "low", "out")]
+
+
+@pytest.mark.parametrize("L,causal,has,worse", PRECISION, ids=lambda x: str(x))
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+def test_what_the_precision_of_delta_is_worth(dtype, L, causal, has, worse):
+    """The next test's bounds fail without what it tests: with the next worse delta dQ, and with the rounded output's dK, are beyond them."""
+    t = _offset_case(dtype, L)
+    want = _rounded_gradients(*t, torch.float64, causal, "exact")
+    got = {d: [_off(x.to(dtype), y) for x, y in zip(_rounded_gradients(*t, dtype, causal, d), want)] for d in ("exact", "low", "out")}
+    assert got[worse][0] > 2 * got[has][0] and got["out"][1] > 2 * got["exact"][1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L,causal,has,worse", PRECISION, ids=lambda x: str(x))
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+def test_precision_of_delta(dtype, L, causal, has, worse):
+    t = _offset_case(dtype, L)
+    want = _rounded_gradients(*t, torch.float64, causal, "exact")
+    allowed = [2 * _off(_rounded_gradients(*t, dtype, causal, d)[n].to(dtype), want[n]) for n, d in enumerate((has, "exact"))]
+    dev = dict(zip(("q", "k", "v", "go"), (x.to(DEV) for x in t)))
+    got = _run(dev, {}, causal=causal)
+    for name, x, y, most in zip(("dq", "dk"), got[2:], want, allowed):
+        assert _off(x, y) <= most, (name, _off(x, y), most)
+    if L > 512:
+        return
+    # the same as scenes of one row: what counts is how many keys a row sees
+    row = {n: torch.cat((x, x.flip(1), x), 1) for n, x in dev.items()}
+    ids = torch.arange(3, dtype=torch.int32, device=DEV).repeat_interleave(L)[None].contiguous()
+    got = _run(row, dict(q_doc=ids, k_doc=ids), causal=causal)
+    for name, x, y, most in zip(("dq", "dk"), got[2:], want, allowed):
+        for at in (0, 2 * L):
+            assert _off(x[:, at:at + L], y) <= most, (name, at, _off(x[:, at:at + L], y), most)
