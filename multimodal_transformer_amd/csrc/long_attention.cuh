@@ -382,6 +382,20 @@ struct TileIter {
     }
     return __builtin_amdgcn_readfirstlane(base + n);
   }
+  // at most `most` tiles are left, those that have not been looked up yet among them (256 at a time: one wait for memory)
+  __device__ __forceinline__ bool at_most(int most) const {
+    int n = __popcll(mask);
+    for (int t0 = base + 64; n <= most && t0 < end; t0 += 256) {
+      if (!rng) return false;                            // (a whole lookup, and more behind it)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int t = t0 + 64 * u + (int)(threadIdx.x & 63);
+        const DocRange r = rng[min(t, end - 1)];
+        n += __popcll(__ballot(t < end && r.lo <= hi && r.hi >= lo));
+      }
+    }
+    return n <= most;
+  }
   // not a single document that all rows of [lo, hi] share: masks are needed
   __device__ __forceinline__ bool mixed() const { return rng && !(cur_dead == 0 && cur_lo == cur_hi && lo == hi && lo == cur_lo); }
 };

@@ -798,7 +798,7 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
   }
   float all_u = 0.f, all_p = 0.f, far_u[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f};
 
-  const bool twice = sizeof(T) == 2 && deal.lead >= 0 && __popcll(deal.it.mask) + TEAMS <= TWICE;      // (the tiles of a lookup at least)
+  const bool twice = sizeof(T) == 2 && deal.lead >= 0 && deal.it.at_most(TWICE - TEAMS);
   for (int pass = twice ? 0 : 1; pass < 2; ++pass) {
     auto step = [&](auto buffer) {
       constexpr int buf = decltype(buffer)::value;

@@ -341,3 +341,21 @@ def test_precision_of_delta(dtype, L, causal, has, worse):
     for name, x, y, most in zip(("dq", "dk"), got[2:], want, allowed):
         for at in (0, 2 * L):
             assert _off(x[:, at:at + L], y) <= most, (name, at, _off(x[:, at:at + L], y), most)
+
+
+# ------------------------------------------------------------------------------------------------------------ two passes of dQ
+@pytest.mark.gpu
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=IDS.get)
+def test_a_scene_has_the_same_gradient_wherever_it_starts(dtype, dh):
+    """A scene of 4352 tokens behind another one, across token 4096, and at the start of its row: the same tiles in the same order, so the
+    same bits (what a workgroup does depends on all the tiles it sees, not on how they are looked up)."""
+    L, n = 8704, 4352
+    a, _ = _case(dtype, 1, L, L, 2, 1, dh, seed=97)
+    ids = lambda *s: torch.tensor([i for i, m in s for _ in range(m)], dtype=torch.int32, device=DEV)[None]
+    first, late = ids((0, n), (1, L - n)), ids((1, 3840), (0, n), (2, L - n - 3840))
+    b = {x: torch.cat((y[:, n:n + 3840], y[:, :n], y[:, n + 3840:]), 1) for x, y in a.items()}
+    res = [_run(t, dict(q_doc=d, k_doc=d), causal=True) for t, d in ((a, first), (b, late))]
+    cut = lambda x, at: x[:, at:at + n] if x.dim() == 4 else x[:, :, at:at + n]
+    for name, x, y in zip(("out", "lse", "dq"), *res):
+        assert torch.equal(cut(x, 0), cut(y, 3840)), name
