@@ -615,7 +615,9 @@ int mmt_lane_gather(const double *table, const double *lanes, const int64_t *row
  * be NULL) contiguous.  Keys at j >= n and keys and queries with a negative id are never multiplied with anything: they may hold
  * NaN.  Bucket numbers are clamped to 0..n_buckets-1, lengths to 0..Lk.  Limits: dh a multiple of 8 up to 128, n_buckets <= 64,
  * reach <= 1024.  Sums, statistics and the products' accumulators are fp32; the probabilities and the
- * score gradients are rounded to the element type where they enter the second product.
+ * score gradients are rounded to the element type where they enter the second product; fp16 score gradients are scaled for it by one power
+ * of two per call, taken from the largest |dout|, |v| and |dlse|: what is 2^-38 of 2 max|dout| max|v| + max|dlse| is lost.
+ * The backward forms the probabilities again from lse, whose rounding makes them off by 2^-22 |lse| of their value.
  * fwd: out_low (like out, may be NULL) receives what rounding took from out, rounded to the element type itself: with it the
  * backward forms rowsum(dout out) to twice the digits, which rows that see few keys need.
  * bwd: `out`, `out_low` (may be NULL) and `lse` are the forward's, dout rows like q, dlse (B,H,Lq) may be NULL; dq (B,Lq,H,dh), dk, dv (B,Lk,Hk,dh)

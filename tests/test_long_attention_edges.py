@@ -359,3 +359,17 @@ def test_a_scene_has_the_same_gradient_wherever_it_starts(dtype, dh):
     cut = lambda x, at: x[:, at:at + n] if x.dim() == 4 else x[:, :, at:at + n]
     for name, x, y in zip(("out", "lse", "dq"), *res):
         assert torch.equal(cut(x, 0), cut(y, 3840)), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("factor", [2.0 ** -14, 2.0 ** -20], ids=["2^-14", "2^-20"])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_gradients_of_very_different_size_in_one_call(dtype, factor):
+    """One row's gradient a million times the others': each keeps what its own type keeps of it (fp16 scales the score gradients of a call
+    by one power of two, and what that costs the small ones is in the bound: 2^-38 of the largest)."""
+    t, kw = _case(dtype, 2, 140, 140, 4, 2, 64, seed=101, buckets=8, reach=16)
+    small = torch.full((2, 140, 1, 1), factor, device=DEV)
+    small[0, 77] = 1.0
+    t["go"] = (t["go"].float() * small).to(dtype)
+    _check(t, kw, dtype, causal=True)
+    _check(t, kw, dtype)
