@@ -207,7 +207,7 @@ std::optional<std::tuple<Tensor, Tensor>> plain_long_attention(const Tensor &q, 
     return std::nullopt;
   const int64_t B = q.size(0), Lq = q.size(1), H = q.size(2), dh = q.size(3), Lk = k.size(1), Hk = k.size(2);
   if (k.size(0) != B || k.size(3) != dh || Hk < 1 || H < 1 || H % Hk || std::max({B, Lq, Lk, H}) > MOST) return std::nullopt;
-  if ((prefix && !causal) || !q_doc != !k_doc || !rel_bias != !rel_buckets) return std::nullopt;
+  if ((prefix && !causal) || (softcap != 0. && (float)softcap == 0.f) || !q_doc != !k_doc || !rel_bias != !rel_buckets) return std::nullopt;
   if (slopes && slopes->requires_grad() && at::GradMode::is_enabled()) return std::nullopt;
   Rows rq, rk, rv;
   if (!in_place(q, rq) || !in_place(k, rk) || !in_place(v, rv)) return std::nullopt;

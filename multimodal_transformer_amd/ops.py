@@ -941,6 +941,8 @@ def _attention_args(q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softca
         raise MmtError(f"long_attention: q {tuple(q.shape)} and k {tuple(k.shape)} do not line up (batch, head size, heads a "
                        "multiple of the key heads)")
     i32, f32, n, reach = torch.int32, torch.float32, 0, 0
+    if softcap != 0 and C.c_float(softcap).value == 0:
+        raise MmtError(f"long_attention: a cap of {softcap} is 0 in fp32, which stands for none")
     if prefix is not None and not causal:
         raise MmtError("long_attention: a prefix is an exception from the causal mask")
     if (q_doc is None) != (k_doc is None):

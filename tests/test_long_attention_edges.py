@@ -373,3 +373,22 @@ def test_gradients_of_very_different_size_in_one_call(dtype, factor):
     t["go"] = (t["go"].float() * small).to(dtype)
     _check(t, kw, dtype, causal=True)
     _check(t, kw, dtype)
+
+
+# ------------------------------------------------------------------------------------------------- numbers that fp32 cannot hold
+def test_a_cap_that_vanishes_in_fp32_is_refused(monkeypatch):
+    """1e-50 is a cap, 0 is none: a cap that fp32 rounds to 0 must not switch the cap off."""
+    monkeypatch.setattr(ops, "_head_rows", lambda t, *a: (t, 0x1000, 0, 16, 16))
+    q = torch.zeros(1, 2, 1, 8)
+    for cap in (1e-50, 5e-324):
+        with pytest.raises(MmtError, match="cap"):
+            ops._attention_args(q, q, q, None, False, None, None, None, None, cap, None, None, None)
+    ops._attention_args(q, q, q, None, False, None, None, None, None, 0.0, None, None, None)
+
+
+@pytest.mark.gpu
+def test_a_cap_that_vanishes_in_fp32_is_refused_by_the_native_call():
+    t, _ = _case(F32, 1, 8, 8, 2, 2, 32)
+    for cap in (1e-50, 1e-42):
+        with pytest.raises(MmtError, match="cap"):
+            torch_ops.long_attention(t["q"], t["k"], t["v"], softcap=cap)
