@@ -41,7 +41,8 @@ static int check(const mmt_long_attention *a, const char *who) {
     return mmt_set_error(MMT_EINVAL, "%s: token strides have to stay below 2^25 bytes", who);
   // (a launch has fewer than 2^32 threads, 512 to a workgroup)
   const double items = (double)a->B * a->H * (((double)a->Lq + ROWS - 1) / ROWS) + (double)a->B * a->Hk * (((double)a->Lk + ROWS - 1) / ROWS);
-  if (items > 8e6 || (double)a->B * a->H * a->Lq > 2e9) return mmt_set_error(MMT_EINVAL, "%s: too many rows for one call", who);
+  const double sums = a->rel_bias ? 64. * a->H * a->n_buckets : 0.;                 // one wave for each entry of the table
+  if (items > 8e6 || (double)a->B * a->H * a->Lq > 2e9 || sums >= 4294967296.) return mmt_set_error(MMT_EINVAL, "%s: too many rows for one call", who);
   return MMT_OK;
 }
 

@@ -1,14 +1,15 @@
 """Edges of attention over long rows and of the norm + rotation in front of it: calls under torch's tracer, tensors that are not plain
 memory, rows that see nothing, lowest-value biases, head sizes inside a tile, precision of the corrected backward pass."""
+import ctypes
 import math
 
 import pytest
 import torch
 
-from multimodal_transformer_amd import ops, torch_ops
+from multimodal_transformer_amd import _lib, ops, torch_ops
 from multimodal_transformer_amd._lib import MmtError
 from oracle import long_rows
-from test_long_attention import BF16, DEV, F16, F32, IDS, TYPES, _case, _check, _near, _run
+from test_long_attention import BF16, DEV, F16, F32, IDS, TYPES, _case, _check, _desc, _near, _run
 
 
 # ------------------------------------------------------------------------------------------------------------------ under the tracer
@@ -392,3 +393,12 @@ def test_a_cap_that_vanishes_in_fp32_is_refused_by_the_native_call():
     for cap in (1e-50, 1e-42):
         with pytest.raises(MmtError, match="cap"):
             torch_ops.long_attention(t["q"], t["k"], t["v"], softcap=cap)
+
+
+def test_a_table_of_too_many_entries_is_refused():
+    """One wave sums each entry of the bias gradient: a launch has fewer than 2^32 threads."""
+    lib = _lib.load()
+    a = _desc(B=1, Lq=1, Lk=1, H=1 << 21, Hk=1 << 21, rel_bias=0x1000, rel_buckets=0x1000, n_buckets=32, reach=8)
+    assert lib.mmt_long_attention_workspace_bytes(ctypes.byref(a), 1) == 0 and b"too many" in lib.mmt_last_error()
+    a.n_buckets = 31
+    assert lib.mmt_long_attention_workspace_bytes(ctypes.byref(a), 1) > 0
