@@ -402,3 +402,42 @@ def test_a_table_of_too_many_entries_is_refused():
     assert lib.mmt_long_attention_workspace_bytes(ctypes.byref(a), 1) == 0 and b"too many" in lib.mmt_last_error()
     a.n_buckets = 31
     assert lib.mmt_long_attention_workspace_bytes(ctypes.byref(a), 1) > 0
+
+
+# ------------------------------------------------------------------------------------------------------------- captured training steps
+@pytest.mark.gpu
+def test_leaves_of_a_graph_that_lives_elsewhere_are_refused_while_capturing():
+    """A leaf whose accumulator an eager graph of another stream holds: the forward call of a captured step is an error.  Without that graph,
+    or on leaves made inside, the step is captured and replays."""
+    t, kw = _case(BF16, 1, 70, 70, 2, 2, 64, seed=103, buckets=8, reach=16)
+    w, f = torch.ones(64, device=DEV, requires_grad=True), ops.rotary_frequencies(64, device=DEV)
+    table = kw["rel_bias"].requires_grad_()
+
+    def step(table, w, v):
+        a, b = torch_ops.qk_norm_rope(t["q"], t["k"], w, w.detach(), f)
+        return torch_ops.long_attention(a, b, v, causal=True, rel_bias=table, rel_buckets=kw["rel_buckets"])
+    for leaf in (dict(table=table, w=w.detach(), v=t["v"]), dict(table=table.detach(), w=w, v=t["v"]),
+                 dict(table=table.detach(), w=w.detach(), v=t["v"].clone().requires_grad_())):
+        alive = step(**leaf)                                # an eager graph of the leaf, on the eager stream
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with pytest.raises(MmtError, match="capture"):
+            with torch.cuda.graph(g):
+                step(**leaf)
+        torch.cuda.synchronize()
+        of = [x for x in leaf.values() if x.requires_grad]
+        want, = torch.autograd.grad(alive, of, t["go"])     # the eager graph is as it was
+        del alive
+
+        def captured():
+            own = {n: x.detach().requires_grad_(x.requires_grad) for n, x in leaf.items()}
+            return torch.autograd.grad(step(**own), [x for x in own.values() if x.requires_grad], t["go"])[0]
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = captured()
+        for _ in range(3):
+            got.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+            assert torch.equal(captured(), want)
