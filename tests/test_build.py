@@ -18,3 +18,10 @@ def test_the_library_needs_no_torch():
     assert "libmmt_amd.so" in with_torch and "_autograd.so" in with_torch
     assert "libmmt_amd.so" in without and "_autograd.so" not in without
     assert "_autograd.so" in _would_run("PYTHON=/bin/false", "autograd")
+
+
+def test_build_compiles_what_is_built_already(monkeypatch):
+    seen = []
+    monkeypatch.setattr(subprocess, "check_call", lambda cmd: seen.append(cmd))
+    entry.build()
+    assert seen and "-B" in seen[0] and {"all", "autograd"} <= set(seen[0])
