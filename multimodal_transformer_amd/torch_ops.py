@@ -301,11 +301,13 @@ def long_attention(q, k, v, *, scale=None, causal=False, prefix=None, q_doc=None
                                                                              the clamped distance (``ops.relative_buckets``);
                entries count as clamped to -2^14 .. 2^14, at or below -2^100 (-inf, a type's lowest value) they hide their bucket
     Rows that see nothing give zeros (and an lse of -inf).  Returns out (B,Lq,H,dh), with ``return_lse`` also the log-sums (B,H,Lq)."""
-    traced = _traced(q)
-    both = None if traced else _plain(_native().plain_long_attention, q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes,
-                                      rel_bias, rel_buckets)
-    if both is None:                                      # something to trace, to copy, or to complain about
-        if traced or _lazy(q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets):
+    if _traced(q):
+        out, lse = torch.ops.mmt.long_attention(q, k, v, scale, bool(causal), prefix, q_doc, k_doc, kv_len, float(softcap), slopes,
+                                                rel_bias, rel_buckets)[:2]
+        return (out, lse) if return_lse else out
+    both = _plain(_native().plain_long_attention, q, k, v, scale, causal, prefix, q_doc, k_doc, kv_len, softcap, slopes, rel_bias, rel_buckets)
+    if both is None:                                      # something to copy, or to complain about
+        if _lazy(q, k, v, prefix, q_doc, k_doc, kv_len, slopes, rel_bias, rel_buckets):
             both = _dispatched(torch.ops.mmt.long_attention, q, k, v, scale, bool(causal), prefix, q_doc, k_doc, kv_len, float(softcap),
                                slopes, rel_bias, rel_buckets)[:2]
         else:
@@ -321,10 +323,11 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps=1e-6
     """RMS norm of queries (B,L,H,dh) and keys (B,L,Hk,dh) per head, times the weights (dh), and the rotation of their first
     2 * len(inv_freq) elements by position * inv_freq (float64, ``ops.rotary_frequencies``) in the same pass; differentiable in q, k
     and the weights.  ``positions`` (B,L) int64, None: 0..L-1.  Pairs are (m, m + rot/2), with ``interleaved`` (2m, 2m + 1)."""
-    traced = _traced(q)
-    both = None if traced else _plain(_native().plain_qk_norm_rope, q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
+    if _traced(q):
+        return torch.ops.mmt.qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, float(eps), bool(interleaved))
+    both = _plain(_native().plain_qk_norm_rope, q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
     if both is None:
-        if traced or _lazy(q, k, q_weight, k_weight, inv_freq, positions):
+        if _lazy(q, k, q_weight, k_weight, inv_freq, positions):
             return _dispatched(torch.ops.mmt.qk_norm_rope, q, k, q_weight, k_weight, inv_freq, positions, float(eps), bool(interleaved))
         if torch.is_grad_enabled():
             _constant(inv_freq, "qk_norm_rope: the frequencies")

@@ -441,3 +441,37 @@ def test_leaves_of_a_graph_that_lives_elsewhere_are_refused_while_capturing():
             torch.cuda.synchronize()
             assert torch.equal(got, want)
             assert torch.equal(captured(), want)
+
+
+# ------------------------------------------------------------------------------------------------------------------ under the compiler
+def test_a_compiled_call_is_one_graph():
+    """torch.compile takes the wrappers into its graph as the operators, without a break."""
+    with torch.library._scoped_library("mmt", "IMPL") as lib:
+        lib.impl("long_attention", _host_attention, "CPU")
+        lib.impl("qk_norm_rope", lambda q, k, *rest: (q * 2, k * 3), "CPU")
+
+        def block(q, k, v, w, f):
+            a, b = torch_ops.qk_norm_rope(q, k, w, w, f)
+            return torch_ops.long_attention(a, b, v, return_lse=True)
+        g = torch.Generator().manual_seed(0)
+        q, k, v = (torch.randn(1, 5, 2, 8, generator=g) for _ in range(3))
+        got = torch.compile(block, backend="aot_eager", fullgraph=True)(q, k, v, torch.ones(8), ops.rotary_frequencies(8))
+        assert all(torch.equal(x, y) for x, y in zip(got, _host_attention(q * 2, k * 3, v)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_a_compiled_step_has_the_same_bits(dtype):
+    t, kw = _case(dtype, 2, 50, 50, 4, 2, 32, seed=107, buckets=8, reach=16, slopes=True, prefix=True)
+    w, f = torch.ones(32, dtype=dtype, device=DEV), ops.rotary_frequencies(32, device=DEV)
+    table = kw.pop("rel_bias")
+
+    def block(q, k, v, table, w):
+        a, b = torch_ops.qk_norm_rope(q, k, w, w, f)
+        return torch_ops.long_attention(a, b, v, causal=True, softcap=5.0, rel_bias=table, **kw)
+    res = []
+    for fn in (block, torch.compile(block, backend="aot_eager", fullgraph=True)):
+        leaves = [x.clone().requires_grad_() for x in (t["q"], t["k"], t["v"], table, w)]
+        out = fn(*leaves)
+        res.append([out] + list(torch.autograd.grad(out, leaves, t["go"])))
+    assert all(torch.equal(x, y) for x, y in zip(*res))
