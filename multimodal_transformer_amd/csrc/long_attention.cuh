@@ -227,12 +227,13 @@ template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS> struct Dm
     }
   }
   // The tile's own requests have arrived (dma_wait): each lane clears those of its pieces that lie beyond dh, ahead of the barrier that
-  // publishes the tile.
+  // publishes the tile.  Only half of a chunk of 16 elements: chunks wholly beyond dh are not read (has_chunk).
   static __device__ __forceinline__ void clear_pads(char *tile, int dh) {
+    if (dh % 16 == 0) return;
     const int tid = rare_tid() % NT;
     auto beyond = [&](int idx) {
       const int d = L::swz(idx / L::NS, idx % L::NS) * L::EPS;
-      return d >= dh && d < D;
+      return d >= dh && d < dh + 8;
     };
     if constexpr (ONE) {
       if (!beyond(tid)) return;
@@ -245,6 +246,9 @@ template <typename T, int D, int R = Tile<T, D>::BK, int NT = THREADS> struct Dm
     }
   }
 };
+
+// Whether chunk c of an operand's 16 elements holds any of the head's: where dh leaves slots empty (GAPS) the last chunk may not
+template <bool GAPS, int NC> __device__ __forceinline__ bool has_chunk(int c, int dh) { return !GAPS || c < NC - 1 || 16 * c < dh; }
 
 // Rows of a tile that must not take part become zeros (whatever they hold: 0 x NaN would reach every other row): at and beyond `end`
 // (tile row), or with a negative document id

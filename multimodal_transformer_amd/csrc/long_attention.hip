@@ -93,7 +93,7 @@ static void plan(Args &g, bool backward) {
 static size_t align64(size_t n) { return (n + 63) & ~(size_t)63; }
 
 struct Workspace {                 // one piece after another, each a multiple of 64 bytes
-  size_t docs, part_o, part_ml, stat, blind, maxima, norm, far, table, part_dk, part_dv, total;
+  size_t docs, part_o, part_ml, stat, maxima, norm, far, table, part_dk, part_dv, total;
 };
 static Workspace layout(const Args &g, bool backward) {
   const mmt_long_attention &a = g.a;
@@ -108,7 +108,6 @@ static Workspace layout(const Args &g, bool backward) {
     }
   } else {
     w.stat = n, n += align64(8 * rows);
-    w.blind = n, n += align64(sizeof(int) * a.B * a.H * (size_t)g.nqt * WAVES);
     if (a.dtype == MMT_F16) w.maxima = n, n += 16 * (STAT_PARTS + 4);
     if (a.rel_bias) {
       const size_t tiles = (size_t)a.B * g.nqt * a.H;
@@ -180,7 +179,7 @@ extern "C" int mmt_long_attention_bwd(const mmt_long_attention *a, const void *o
   g.out = const_cast<void *>(out), g.low = const_cast<void *>(out_low), g.lse = const_cast<float *>(lse);
   g.dout = dout, g.do_bs = do_bs, g.do_rs = do_rs, g.do_hs = do_hs;
   g.dq = dq, g.dk = dk, g.dv = dv, g.dlse = dlse;
-  g.stat = (float2 *)(ws + w.stat), g.blind = (int *)(ws + w.blind);
+  g.stat = (float2 *)(ws + w.stat);
   if (a->rel_bias) g.norm = (float *)(ws + w.norm), g.far_part = (float *)(ws + w.far);
   if (g.zh * g.zq > 1) g.part_dk = (float *)(ws + w.part_dk), g.part_dv = (float *)(ws + w.part_dv);
   DocRange *ranges = a->q_doc ? (DocRange *)(ws + w.docs) : nullptr;

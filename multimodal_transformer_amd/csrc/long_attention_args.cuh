@@ -43,7 +43,6 @@ struct Args {                      // mmt_long_attention plus what the launcher 
   const float *dlse;               // (B, H, Lq) gradient of the log-sum, or NULL
   float *norm;                     // learned bias: (B, H, Lq) 1 / sum of the probabilities as the backward forms them
   float *far_part;                 // (items, 2)
-  int *blind;                      // (B, H, nqt, WAVES): some of these 32 rows see nothing
 };
 
 template <typename T> void forward(Args &g, DocRange *ranges, hipStream_t st);

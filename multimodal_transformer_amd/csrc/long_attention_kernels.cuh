@@ -225,13 +225,14 @@ template <typename T, int D> struct FwdState {
   f32x16 acc[D / 32];
   float m, l;
 };
-template <typename T, int D, int NK>
-__device__ __forceinline__ void fwd_products(float *x, const typename Elem<T>::V8 *fq, const char *sK, int lane) {
+template <typename T, int D, bool GAPS, int NK>
+__device__ __forceinline__ void fwd_products(float *x, const typename Elem<T>::V8 *fq, const char *sK, int lane, int dh) {
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt) {
     f32x16 s = {};
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + (lane & 31), c, lane >> 5), fq[c], s);
+    for (int c = 0; c < D / 16; ++c)
+      if (has_chunk<GAPS, D / 16>(c, dh)) s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + (lane & 31), c, lane >> 5), fq[c], s);
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[16 * kt + i] = s[i];
   }
@@ -429,7 +430,7 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
 #pragma unroll
       for (int kt = 0; kt < BK / 32; kt += NK) {
         float x[NK * 16];
-        fwd_products<T, D, NK>(x, fq, sK + kt * 32 * L::NS * 16, lane);
+        fwd_products<T, D, GAPS, NK>(x, fq, sK + kt * 32 * L::NS * 16, lane, a.dh);
         fwd_softmax<T, D, MOD, false, NK>(st, x, k0 + 32 * kt, w, a, sc, lut.mid, nullptr, at, need_mask, mixed ? sDoc + 32 * kt : nullptr, h);
         fwd_values<T, D, NK>(st, x, sV + kt * 32 * L::NS * 16, lane);
       }
@@ -520,9 +521,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     const Place at = place(a, k0 - wb.p_max, k0 + BK - 1 - wb.p_min);
     // requests complete in order: all but the newest tile (the values asked for after these keys, the keys asked for after these values)
     dma_wait<dv.N>();
-    if (a.dh < D) dk.clear_pads(sK, a.dh);
+    dk.clear_pads(sK, a.dh);
     float x[16];
-    fwd_products<T, D, 1>(x, fq, sK, lane);
+    fwd_products<T, D, true, 1>(x, fq, sK, lane, a.dh);
     wave_sync();                                          // the keys have been read
     if (tn < tiles) dk.load(lds, tn * BK);
     if (kdoc) {
@@ -777,11 +778,8 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
 #pragma unroll
     for (int e = 0; e < 8; ++e) delta = fmaf((float)o[e] + (float)lo[e], (float)fd[c][e], delta);
   }
-  // A row that sees nothing takes no part, whatever arrives as its gradient (a squared log-sum's is -inf).  The dK / dV kernels read here
-  // which of their tiles hold such rows: 0 x inf would reach all keys.
-  const bool sees = lse != -INFINITY, blind = __any(w.valid && !sees);
-  if (lane == 0 && team == 0) g.blind[(((int64_t)b * a.H + head) * g.nqt + qt) * WAVES + wave] = blind;
-  w.live = w.live && sees;
+  // A row that sees nothing takes no part, whatever arrives as its gradient (a squared log-sum's is -inf)
+  w.live = w.live && lse != -INFINITY;
   dl = w.live ? dl : 0.f;
   delta = w.live ? half_sum(delta) - dl : 0.f;
   lse = w.live ? lse * LOG2E : INFINITY;
@@ -832,7 +830,8 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
           // (the two products one after the other where registers are short: what is live grows with how far the compiler pulls them together)
           f32x16 s = {}, dp = {};
 #pragma unroll
-          for (int c = 0; c < NC; ++c) s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s);
+          for (int c = 0; c < NC; ++c)
+            if (has_chunk<GAPS, NC>(c, a.dh)) s = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s);
           float x[16], th[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = s[i];
@@ -843,7 +842,8 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
           for (int i = 0; i < 16; ++i) x[i] = ex2(fmaf(x[i], f.mul, f.add - lse));
           if constexpr (D > 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) dp = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp);
+          for (int c = 0; c < NC; ++c)
+            if (has_chunk<GAPS, NC>(c, a.dh)) dp = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp);
           float su = 0.f, sp = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -972,7 +972,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const mmt_long_attention &a = g.a;
   float *sStat2 = (float *)(smem + 4 * L::BYTES);         // [2][log-sum, delta][BQ]
-  int *sDoc2 = (int *)(sStat2 + 4 * BQ), *sB = sDoc2 + 2 * BQ;
+  int *sDoc2 = (int *)(sStat2 + 4 * BQ), *sB = sDoc2 + 2 * BQ, *sPart = sB + 2 * WAVES;      // sPart: [2], not all rows of the tile take part
   const Lut lut = {(float *)(sB + 6 * WAVES) + a.reach + PAD};
   const int grp = blockIdx.x % g.groups;
   int n = blockIdx.x / g.groups;
@@ -1031,8 +1031,6 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   TileIter it;
   int gi = g0 - 1, t = -1, lut_gi = -1;
   const float2 *stat = nullptr;
-  const int *blind = nullptr;
-  int blind_next = 0;
   float2 st_next = make_float2(INFINITY, 0.f);
   float slope_next = 0.f;
   int doc_next = -1;
@@ -1040,7 +1038,6 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     int n = gi < g0 ? -1 : it.next();
     while (n < 0 && ++gi < g1) {
       stat = g.stat + ((int64_t)b * a.H + head0 + gi) * a.Lq;
-      blind = g.blind + ((int64_t)b * a.H + head0 + gi) * g.nqt * WAVES;
       dmq.base = qbase + (int64_t)gi * a.q_hs * (int64_t)sizeof(T);
       dmo.base = obase + (int64_t)gi * g.do_hs * (int64_t)sizeof(T);
       if (MOD && a.slopes) slope_next = scalar_load(a.slopes + head0 + gi) * LOG2E;
@@ -1052,7 +1049,6 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   auto fetch = [&](int tile, int to) {
     dmq.load(lds + to * 2 * L::BYTES, tile * BQ);
     dmo.load(lds + to * 2 * L::BYTES + L::BYTES, tile * BQ);
-    blind_next = blind[tile * (BQ / 32) + (lane & (BQ / 32 - 1))];       // (a lane's own: a scalar load would hold up the reads from LDS)
     if (threadIdx.x < BQ) {
       // (neither waits for the other, or for the tile: rows that are missing or dead are sorted out when the tile is here)
       const int i = min(tile * BQ + (int)threadIdx.x, a.Lq - 1);
@@ -1071,13 +1067,15 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
     char *sQ = smem + buf * 2 * L::BYTES, *sO = sQ + L::BYTES;
     float *sStat = sStat2 + buf * 2 * BQ;
     int *sDoc = sDoc2 + buf * BQ;
-    const bool docs = it.mixed(), dead = it.cur_dead != 0;
+    const bool docs = it.mixed();
     const int cur_gi = gi;
     const float slope = slope_next;
     if (threadIdx.x < BQ) {
       const int doc = q0 + (int)threadIdx.x < a.Lq && st_next.x != INFINITY ? doc_next : -1;      // negative: takes no part
       sDoc[threadIdx.x] = doc;
       sStat[threadIdx.x] = doc >= 0 ? st_next.x : INFINITY, sStat[BQ + threadIdx.x] = doc >= 0 ? st_next.y : 0.f;
+      const bool out = __any(doc < 0);
+      if (threadIdx.x == 0) sPart[buf] = out;
     }
     dma_wait<0>();
     if constexpr (GAPS) dmq.clear_pads(sQ, a.dh), dmo.clear_pads(sO, a.dh);
@@ -1087,8 +1085,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
       lut_gi = cur_gi;
       __syncthreads();
     }
-    // where not all rows take part, those that do not are cleared and masked (a cleared row's product with an infinite key is NaN)
-    const bool part = q0 + BQ > a.Lq || dead || __any(blind_next), mixed = docs || part;
+    // rows that take no part - missing, padding, or seeing nothing - are cleared (0 x inf would reach all keys) and masked (a cleared
+    // row's product with an infinite key is NaN)
+    const bool part = __builtin_amdgcn_readfirstlane(sPart[buf]) != 0, mixed = docs || part;
     if (part) {
       zero_rows<T, D>(sQ, BQ, sDoc);
       zero_rows<T, D>(sO, BQ, sDoc);
@@ -1105,6 +1104,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
         f32x16 s = {}, dp = {};
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
+          if (!has_chunk<GAPS, NC>(c, a.dh)) continue;
           s = Elem<T>::mma(row_frag<T, D>(sQ, 32 * qt + col, c, h), fk[c], s);
           dp = Elem<T>::mma(row_frag<T, D>(sO, 32 * qt + col, c, h), fv[c], dp);
         }
@@ -1204,8 +1204,8 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
   const mmt_long_attention &a = g.a;
   char *sP = smem + 4 * L::BYTES, *sS = sP + 128 * BQ * 2;                 // [key block][16 queries][lane] x 16 bytes
   float *sStat2 = (float *)(sS + 128 * BQ * 2);                             // [2][log-sum, delta][BQ]
-  int *sDoc2 = (int *)(sStat2 + 4 * BQ), *sB = sDoc2 + 2 * BQ;
-  const Lut lut = {(float *)(sB + 16) + a.reach + PAD};
+  int *sDoc2 = (int *)(sStat2 + 4 * BQ), *sB = sDoc2 + 2 * BQ, *sPart = sB + 16;      // sPart: [2], not all rows of the tile take part
+  const Lut lut = {(float *)(sB + 20) + a.reach + PAD};
   const int grp = blockIdx.x % g.groups;
   int n = blockIdx.x / g.groups;
   const int z = n % (g.zh * g.zq), zh = z % g.zh, zq = z / g.zh;
@@ -1266,8 +1266,6 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
   TileIter it;
   int gi = g0 - 1, t = -1, buf = 0, lut_gi = -1;
   const float2 *stat = nullptr;
-  const int *blind = nullptr;
-  int blind_next = 0;
   float2 st_next = make_float2(INFINITY, 0.f);
   float slope_next = 0.f;
   int doc_next = -1;
@@ -1275,7 +1273,6 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
     int n = gi < g0 ? -1 : it.next();
     while (n < 0 && ++gi < g1) {
       stat = g.stat + ((int64_t)b * a.H + head0 + gi) * a.Lq;
-      blind = g.blind + ((int64_t)b * a.H + head0 + gi) * g.nqt * WAVES;
       dmq.base = qbase + (int64_t)gi * a.q_hs * (int64_t)sizeof(T);
       dmo.base = obase + (int64_t)gi * g.do_hs * (int64_t)sizeof(T);
       if (MOD && a.slopes) slope_next = scalar_load(a.slopes + head0 + gi) * LOG2E;
@@ -1287,7 +1284,6 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
   auto fetch = [&](int tile, int to) {
     dmq.load(lds + to * 2 * L::BYTES, tile * BQ);
     dmo.load(lds + to * 2 * L::BYTES + L::BYTES, tile * BQ);
-    blind_next = blind[tile * (BQ / 32) + (lane & (BQ / 32 - 1))];       // (a lane's own: a scalar load would hold up the reads from LDS)
     if (threadIdx.x < BQ) {
       // (neither waits for the other, or for the tile: rows that are missing or dead are sorted out when the tile is here)
       const int i = min(tile * BQ + (int)threadIdx.x, a.Lq - 1);
@@ -1305,12 +1301,14 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
     char *sQ = smem + buf * 2 * L::BYTES, *sO = sQ + L::BYTES;
     float *sStat = sStat2 + buf * 2 * BQ;
     int *sDoc = sDoc2 + buf * BQ;
-    const bool docs = it.mixed(), dead = it.cur_dead != 0;
+    const bool docs = it.mixed();
     const float slope = slope_next;
     if (threadIdx.x < BQ) {
       const int doc = q0 + (int)threadIdx.x < a.Lq && st_next.x != INFINITY ? doc_next : -1;      // negative: takes no part
       sDoc[threadIdx.x] = doc;
       sStat[threadIdx.x] = doc >= 0 ? st_next.x : INFINITY, sStat[BQ + threadIdx.x] = doc >= 0 ? st_next.y : 0.f;
+      const bool out = __any(doc < 0);
+      if (threadIdx.x == 0) sPart[buf] = out;
     }
     dma_wait<0>();
     if constexpr (GAPS) dmq.clear_pads(sQ, a.dh), dmo.clear_pads(sO, a.dh);
@@ -1320,8 +1318,9 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
       lut_gi = cur_gi;
       __syncthreads();
     }
-    // where not all rows take part, those that do not are cleared and masked (a cleared row's product with an infinite key is NaN)
-    const bool part = q0 + BQ > a.Lq || dead || __any(blind_next), mixed = docs || part;
+    // rows that take no part - missing, padding, or seeing nothing - are cleared (0 x inf would reach all keys) and masked (a cleared
+    // row's product with an infinite key is NaN)
+    const bool part = __builtin_amdgcn_readfirstlane(sPart[buf]) != 0, mixed = docs || part;
     if (part) {
       zero_rows<T, D, BQ, 512>(sQ, BQ, sDoc);
       zero_rows<T, D, BQ, 512>(sO, BQ, sDoc);
@@ -1334,7 +1333,8 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
       const bool need_mask = mixed || !all_live || (a.causal && max(p0 + 1, prefix) < j_lo + 32);
       f32x16 s = {}, dp = {};
 #pragma unroll
-      for (int c = 0; c < NC; ++c) s = Elem<T>::mma(row_frag<T, D>(sQ, 32 * qh + col, c, h), fk[c], s);
+      for (int c = 0; c < NC; ++c)
+        if (has_chunk<GAPS, NC>(c, a.dh)) s = Elem<T>::mma(row_frag<T, D>(sQ, 32 * qh + col, c, h), fk[c], s);
       float x[16], th[16], p[16];
       Linear f = {sc.c_scale, 0.f};
 #pragma unroll
@@ -1361,7 +1361,8 @@ __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g
       }
       __builtin_amdgcn_sched_barrier(0);                  // (keeps the registers of the second product out of the first one's reach)
 #pragma unroll
-      for (int c = 0; c < NC; ++c) dp = Elem<T>::mma(row_frag<T, D>(sO, 32 * qh + col, c, h), fv[c], dp);
+      for (int c = 0; c < NC; ++c)
+        if (has_chunk<GAPS, NC>(c, a.dh)) dp = Elem<T>::mma(row_frag<T, D>(sO, 32 * qh + col, c, h), fv[c], dp);
       acc_rows(st, sStat + BQ + 32 * qh, h);
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = p[i] * (dp[i] - st[i >> 2][i & 3]);
@@ -1513,7 +1514,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
   while (t < t1) {
     const int k0 = t * BK;
     dma_wait<0>();
-    if (a.dh < D) dk.clear_pads(sK, a.dh), dv.clear_pads(sV, a.dh);
+    dk.clear_pads(sK, a.dh), dv.clear_pads(sV, a.dh);
     __syncthreads();
     if (k0 + BK > len || kdoc) {
       zero_rows<T, D>(sK, len - k0, kdoc ? ids : nullptr);
@@ -1526,6 +1527,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
       s[kt] = f32x16{}, dp[kt] = f32x16{};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
+        if (!has_chunk<true, NC>(c, a.dh)) continue;
         s[kt] = Elem<T>::mma(row_frag<T, D>(sK, 32 * kt + col, c, h), fq[c], s[kt]);
         dp[kt] = Elem<T>::mma(row_frag<T, D>(sV, 32 * kt + col, c, h), fd[c], dp[kt]);
       }
@@ -1648,7 +1650,7 @@ template <typename T, int D, bool GAPS> static void bwd_size(Args &g, hipStream_
   const size_t lds_k = 4 * L::BYTES + 24 * L::BK + small + 4 * Lut::floats(a);
   const int64_t kitems = (int64_t)g.groups * ((a.Lk + ROWS - 1) / ROWS) * g.zh * g.zq;
   if constexpr (sizeof(T) == 2 && D > 64) {
-    const size_t lds2 = 4 * L::BYTES + 2 * 128 * 64 * 2 + 24 * 64 + 64 + 4 * Lut::floats(a);
+    const size_t lds2 = 4 * L::BYTES + 2 * 128 * 64 * 2 + 24 * 64 + 80 + 4 * Lut::floats(a);
     if (mod) launch(mmt_long_attn_dkv2_kernel<T, D, GAPS, true>, kitems, lds2, st, g, 512);
     else launch(mmt_long_attn_dkv2_kernel<T, D, GAPS, false>, kitems, lds2, st, g, 512);
   } else {
