@@ -162,7 +162,7 @@ template <typename V> __device__ __forceinline__ void live_frag(V &v, int c, int
   v = in ? v : V{};
   asm volatile("" : "+v"(v));
 }
-// a value that all lanes share and no kernel of this call writes
+// a value that all lanes share and that this kernel does not write
 template <typename V> __device__ __forceinline__ V scalar_load(const V *p) { return *(const __attribute__((address_space(4))) V *)(uintptr_t)p; }
 
 // What was loaded ahead of a loop has arrived here (live_frag does the same).  Otherwise the compiler waits for it at its first use inside the loop, every time
@@ -302,8 +302,10 @@ __device__ __forceinline__ void acc_rows(f32x4 *v, const float *s, int h) {
 }
 
 // ---- score transform ------------------------------------------------------------------------------------------------------
-// tanh without cancellation.  |y| <= 3/8: odd series to y^11, remainder < 21844/6081075 y^13 = 3e-8 of y.  Beyond: 1 - 2 / (1 + e^2y),
-// whose absolute error of an ulp of 1 is then below 2e-7 of the value.
+// tanh without cancellation.  |y| <= 3/8: odd series to y^11, remainder < 21844/6081075 y^13 = 3e-8 of y; over all floats of that range it
+// is off by at most 7.5e-8 of the value.  Beyond: 1 - 2 / (1 + e^2y).  With an ulp each of the exponential and the reciprocal, and the
+// roundings of the argument and the sums, arithmetic allows 6.3e-7 of the value at 3/8; over all floats up to 10 it is at most 2.3e-7 (at
+// 0.552), and falls off from there.
 __device__ __forceinline__ float tanh_series(float y) {
   const float z = y * y;
   float p = fmaf(z, -8.86323552990219657e-3f, 2.18694885361552028e-2f);

@@ -48,8 +48,8 @@ static int check(const mmt_long_attention *a, const char *who) {
 
 // One workgroup of 128 rows per CU leaves each SIMD one wave, which waits for most of its time: two teams of waves then share its keys.
 // Where that many rows are causal, the workgroups that remain for a second turn are the shortest.  Measured with one team and two: bf16
-// causal 2 x 1024 x 16 heads of 64 (256 workgroups) forward 36 and 29 us, dQ 41 and 33; fp16 causal 3 x 1333 x 8 heads of 80 (264) 45 and
-// 38, 66 and 52.  fp32 needs the registers of both.
+// causal 2 x 1024 x 16 heads of 64 (256 workgroups) forward 23 and 21 us, dQ 27 and 24; fp16 causal 3 x 1333 x 8 heads of 80 (264) with a
+// learned bias 47 and 37, 63 and 50.  fp32 needs the registers of both.
 static int teams(const mmt_long_attention &a, int64_t items) {
   return a.dtype != MMT_F32 && items < (a.causal ? 512 : 257) && a.Lk > 192 ? 2 : 1;
 }
@@ -59,10 +59,10 @@ static void plan(Args &g, bool backward) {
   const int bk = tile_keys(a.dtype);
   g.G = a.H / a.Hk;
   // few queries: the rows of all heads that share a key head go into one tile of 32, which reads the cache once (32768 tokens, one query
-  // of 4 heads per key head: 294 us instead of 712)
+  // of 4 heads per key head: 285 us instead of 914)
   g.few = !backward && (int64_t)a.Lq * g.G <= 32;
-  // else packed where rows of one head would leave more of the tiles of 128 empty (64 queries of 4 heads over 16384 tokens: 39 us instead
-  // of 55); a learned bias is laid out for one head
+  // else packed where rows of one head would leave more of the tiles of 128 empty (64 queries of 4 heads over 16384 tokens: 38 us instead
+  // of 56); a learned bias is laid out for one head
   const bool fewer = ((int64_t)a.Lq * g.G + ROWS - 1) / ROWS < (int64_t)g.G * ((a.Lq + ROWS - 1) / ROWS);
   g.pack = g.few || (!backward && !a.rel_bias && fewer) ? g.G : 1;
   g.nqt = (int)(((int64_t)a.Lq * g.pack + ROWS - 1) / ROWS);
@@ -73,16 +73,17 @@ static void plan(Args &g, bool backward) {
     const int64_t base = (int64_t)g.groups * (g.G / g.pack) * g.nqt;
     const int64_t tiles = g.few ? (a.Lk + 127) / 128 : g.nkt;               // a step of all waves
     g.teams = g.few ? 1 : teams(a, base);
-    // the keys are split where that leaves half of the CUs' places empty, two workgroups of four waves per CU: 39 + 10 us with the joining
-    // kernel for the chunk above with one team, with one workgroup per CU 47 + 7; at least four tiles to a team (264 workgroups split in
-    // two: 32 + 18 us, whole 46)
+    // the keys are split where that leaves half of the CUs' places empty, two workgroups of four waves per CU or one of two teams: 37 + 10 us
+    // with the joining kernel for the chunk above with one team, 38 + 7 with two, with half as many workgroups 57 + 5; at least four tiles to a
+    // team, and no split above half (264 workgroups of one team split in two: 32 + 18 us, whole 46)
     const int64_t want = 512 / g.teams;
     if (base < want / 2) g.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>((want + base - 1) / base, tiles / (4 * g.teams)));
     g.items = (int)(base * g.nsplit);
   } else {
     // parts of dK / dV over the query heads, then over the queries, for 512 workgroups, for causal rows, which are uneven, 1024 (bf16 8192 x
-    // 16 heads of 128 over 4: 682 us and 23 for the sum of the parts, for 512 705 and 14, for 256 1153; packed scenes of 2 x 4096 tokens 85 and
-    // 12, for 512 105 and 8); at least eight tiles of queries each (fp16 3 x 1333 x 8 heads of 80 over 2: 50 and 8 us, with four 67 and 13)
+    // 16 heads of 128 over 4: 618 us and 23 for the sum of the parts, for 512 609 and 14, for 256 1113; packed scenes of 2 x 4096 tokens 79 and
+    // 13, for 512 99 and 8, for 256 187); at least eight tiles of queries each (fp16 3 x 1333 x 8 heads of 80 over 2: 48 and 8 us, with four 64
+    // and 13).  All of these were chosen on 16-bit types; fp32 takes them as they are.
     const int64_t base = (int64_t)g.groups * ((a.Lk + ROWS - 1) / ROWS), want = ((a.causal ? 1024 : 512) + base - 1) / base;
     g.zh = (int)std::min<int64_t>(g.G, want);
     g.teams = teams(a, (int64_t)a.B * a.H * g.nqt);

@@ -338,8 +338,8 @@ __device__ __forceinline__ void fwd_store(const Args &g, const FwdState<T, D> &s
 // product into the exponential as they are.
 // S is computed transposed (the accumulator's rows are keys, its columns the wave's queries), so that a lane owns one query: maximum and
 // sum need one exchange between the two lane halves, and the rounded P is already the operand of the second product.
-// Measured, bf16 causal 8192 tokens x 16 heads of 128 over 4, learned bias: 345 us, 800 TFLOP/s of the 1156 that a large library product
-// reaches; non-causal 2 x 2048 x 16 heads of 64: 68 us, 510.  Bound by the vector instructions of the softmax (48 and 55 % of the cycles)
+// Measured, bf16 causal 8192 tokens x 16 heads of 128 over 4, learned bias: 319 us, 860 TFLOP/s of the 1156 that a large library product
+// reaches; non-causal 2 x 2048 x 16 heads of 64: 61 us, 570; unmodified, causal 2 x 4096 x 16 heads of 128 over 4: 159 us, 860.  Bound by the vector instructions of the softmax (48 and 55 % of the cycles)
 // between the matrix instructions (40 and 24 %) at the two waves per SIMD that the registers allow; LDS is at 32 and 21 %, without bank
 // conflicts.
 // TEAMS = 2: eight waves, two per 32 rows, which deal the key tiles among themselves and join at the end (rule and figures at teams()).
@@ -467,8 +467,9 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
 // themselves, 32 at a time, and meet at the end, where their maxima, sums and accumulators are joined.  Each has one buffer for K and
 // one for V: the next keys are requested as soon as the products have been taken from the buffer, the next values after theirs, so
 // that 16 KiB per wave at a head size of 128 and, with two workgroups, 128 KiB per CU are on their way.  Bound by reading the cache: 16
-// requests of up to 32768 tokens (1.36 GB) x 8 key heads of 128 in bf16 take 288 us, 4.7 TB/s where a copy reaches 4.9 (the
-// general kernel: 712 us, three of its four waves without rows).
+// requests of up to 32768 tokens (1.36 GB) x 8 key heads of 128 in bf16 take 285 us, 4.8 TB/s where a copy reaches 4.9 (the
+// general kernel: 914 us, three of its four waves without rows).  At a head size of 128 all 256 registers are taken and 48 bytes per lane
+// live in scratch.
 template <typename T, int D, bool MOD>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_few_kernel(const Args g) {
   typedef Tile<T, D> L;
@@ -712,9 +713,9 @@ __device__ __forceinline__ float score_grad_scale(const f32x4 *maxima, int parts
 // are 0) and the corrected delta.  The forward's geometry; K is read twice from LDS (as rows for the scores, transposed for
 // dQ^T += K^T dS^T), V once. Where a workgroup's rows see at most TWICE tiles (the beginnings of causal rows and of documents, short
 // rows), 16-bit types go over them twice, the first time for delta alone: a probability's rounding does not average out over few keys.
-// Packed scenes of 300 to 800 tokens (2 x 4096, 16 heads of 64): dQ is 0.0025 off with one pass for all, in 70 us, 0.0024 with two up to 8
-// tiles, in 87, and with two for all, in 122; 0.0023 is what the roundings of dS and of dQ itself make.  fp32 rounds no probability.
-// Bound like the forward: 515 us for its causal case of 8192 tokens (800 TFLOP/s), 86 us for the one of 2048.
+// Packed scenes of 300 to 800 tokens (2 x 4096, 16 heads of 64): dQ is 0.0025 off with one pass for all, in 65 us, 0.0024 with two up to 8
+// tiles, in 82, and with two for all, in 112; 0.0023 is what the roundings of dS and of dQ itself make.  fp32 rounds no probability.
+// Bound like the forward: 472 us for its causal case of 8192 tokens (870 TFLOP/s), 81 us for the one of 2048.
 // With a learned bias the kernel also sums dU over the tiles that lie wholly beyond the reach on either side.
 constexpr int TWICE = 8;
 template <typename T, int D, bool GAPS, bool MOD, int TEAMS>
@@ -961,9 +962,9 @@ __global__ void __launch_bounds__(TEAMS * THREADS, sizeof(T) == 4 ? 1 : 2) mmt_l
 // heads that share the key head go by in LDS tiles, as rows for S and dP and transposed for dV^T += dO^T P and dK^T += Q^T dS.
 // With few key tiles the query heads and the queries are dealt over zh x zq parts, which a second kernel adds up in order.
 // For fp32, and 16-bit types up to a head size of 64: K, V, dK and dV of 32 keys take 192 registers at 128, which leaves room for one wave
-// per SIMD (8192 causal tokens x 16 heads: 1380 us, the next kernel's 715).  Up to 64 this one is: bf16
-// 2 x 2048 x 16 heads of 64 98 us, the next one 129; 2 x 4096 tokens in packed scenes 85, the next one 98.  Bound by vector instructions
-// and the latency between them, at two waves per SIMD: 700 TFLOP/s in the first case.
+// per SIMD (8192 causal tokens x 16 heads: 1380 us with one, 2470 with two and spills, the next kernel's 618).  Up to 64 this one is: bf16
+// 2 x 2048 x 16 heads of 64 93 us, the next one 118; 2 x 4096 tokens in packed scenes 79, the next one 91.  Bound by vector instructions
+// and the latency between them, at two waves per SIMD: 740 TFLOP/s in the first case.
 template <typename T, int D, bool GAPS, bool MOD>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn_dkv_kernel(const Args g) {
   typedef Tile<T, D> L;
@@ -1192,9 +1193,10 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 1 : 2) mmt_long_attn
 //   1. wave w computes P and dS of 32 queries x 32 keys (its K and V rows stay in registers) and leaves them in LDS in the order of
 //      the accumulator, which is the order of the second step's operand: 16 bytes per lane, no rearrangement;
 //   2. wave w adds up one of the two outputs for KB x 32 keys and a part of the dimensions, with dO or Q read transposed.
-// 8192 causal tokens x 16 heads of 128 over 4: 715 us, 770 TFLOP/s for the four products.  About 290 KiB go through LDS per tile, half of
+// 8192 causal tokens x 16 heads of 128 over 4: 618 us, 890 TFLOP/s for the four products.  About 290 KiB go through LDS per tile, half of
 // the time of its matrix instructions (LDS 41 % of the cycles, matrix 37 %, vector 30 %); bound by the steps' order: two barriers per
-// tile, one workgroup per CU, and its waves wait for 47 % of the time.
+// tile, one workgroup per CU, and its waves wait for 47 % of the time.  With modified scores at 128, 20 bytes per lane live in scratch (all 256
+// registers are taken).
 template <typename T, int D, bool GAPS, bool MOD>
 __global__ void __launch_bounds__(512, 2) mmt_long_attn_dkv2_kernel(const Args g) {
   typedef Tile<T, D> L;
@@ -1438,7 +1440,7 @@ template <typename T> __global__ void __launch_bounds__(256) mmt_long_attn_dkv_s
 }
 
 // The gradient of the learned bias over the tiles within the reach (the dQ kernel has summed the others).  Sums of millions of
-// signed terms that have to come out right to fp32 (31 us for 2 x 2048 x 16 heads of 64 and a reach of 128): dU is recomputed with the exact delta of each row, and every lane adds into
+// signed terms that have to come out right to fp32 (30 us for 2 x 2048 x 16 heads of 64 and a reach of 128): dU is recomputed with the exact delta of each row, and every lane adds into
 // a column of its own of a [bucket][lane] array in LDS, so that the order of the additions is the program's.  Bound by the latency of
 // these load - add - store chains (LDS additions that return nothing took four times as long): four elements at a time are loaded
 // together, each of the four then adds all those of its bucket, so that equal buckets store equal sums.  The next tile is on its way

@@ -6,7 +6,7 @@
 // The angles of a token are shared by all its heads: a workgroup forms them once per token, in 64 bits (position * frequency reaches
 // 10^6 turns, of which fp32 would keep 2 digits), reduces them to a fraction of a turn, and a lane keeps the cosines and sines of its 8
 // elements in registers while it walks over the token's heads.  Bound by memory: every element is read once and written once
-// (backwards: two read, one written).  bf16, 4 x 4096 tokens x 20 heads of 128: 42 us forward, 4.0 TB/s, 67 us backward, 3.8 TB/s, and 6 for the
+// (backwards: two read, one written).  bf16, 4 x 4096 tokens x 20 heads of 128: 39 us forward, 4.3 TB/s, 64 us backward, 3.9 TB/s, and 6 for the
 // sum of the weights' gradients, where a large copy reaches 4.9.  32 single tokens of 20 heads: 6 us, the launch and three waits for memory.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -22,7 +22,7 @@ int mmt_set_error(int code, const char *fmt, ...);   // transformer.hip
 namespace {
 
 constexpr int NT = 256;
-// workgroups backwards, each with a part of the weights' gradients: 1024 take 74 us and 4 for their sum in the case above, 2048 67 and 6
+// workgroups backwards, each with a part of the weights' gradients: half as many take a tenth longer in the case above, and their sum 4 us instead of 6
 constexpr int MAX_PARTS = 2048;
 
 template <typename T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
