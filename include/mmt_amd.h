@@ -613,8 +613,8 @@ int mmt_lane_gather(const double *table, const double *lanes, const int64_t *row
  * Heads: query head h reads key head h / (H / Hk).  q / k / v rows (head slices) are dh contiguous elements at any batch / token /
  * head stride (elements) that keeps them at multiples of 16 bytes, token strides below 2^25 bytes; a stride of 0 broadcasts.  out (B,Lq,H,dh) and lse (B,H,Lq; may
  * be NULL) contiguous.  Keys at j >= n and keys and queries with a negative id are never multiplied with anything: they may hold
- * NaN.  Keys that only their position or another document hides may be multiplied by a probability of 0: they have to be finite.  Bucket numbers are clamped to 0..n_buckets-1, lengths to 0..Lk.  Limits: dh a multiple of 8 up to 128, n_buckets <= 64,
- * reach <= 1024.  Sums, statistics and the products' accumulators are fp32; the probabilities and the
+ * NaN.  Keys that only their position or another document hides may be multiplied by a probability of 0: they have to be finite.  Bucket
+ * numbers are clamped to 0..n_buckets-1, lengths to 0..Lk.  Limits: dh a multiple of 8 up to 128, n_buckets <= 64, reach <= 1024.  Sums, statistics and the products' accumulators are fp32; the probabilities and the
  * score gradients are rounded to the element type where they enter the second product; fp16 score gradients are scaled for it by one power
  * of two per call, taken from the largest |dout|, |v| and |dlse|: what is 2^-38 of 2 max|dout| max|v| + max|dlse| is lost.
  * The backward forms the probabilities again from lse, whose rounding makes them off by 2^-22 |lse| of their value.
